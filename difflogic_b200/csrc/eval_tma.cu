@@ -174,6 +174,7 @@ eval_tma_kernel(const SplitRows x, const int64_t *__restrict__ a, const int64_t 
 int groupbitsum_async_error();       // groupbitsum_tma.cu
 int eval_groupbitsum_async_error();  // eval_groupbitsum.cu
 int forward_tma_async_error();       // forward_tma.cu
+int matmul_async_error();            // matmul.cu
 
 static int sm_count() {
     static int cached[64] = {0};
@@ -276,5 +277,7 @@ extern "C" DL_API int dl_async_error(void) {
     if (fused < 0) return fused;
     const int fwd = dl::forward_tma_async_error();
     if (fwd < 0) return fwd;
-    return flag | other | fused | fwd;
+    const int products = dl::matmul_async_error();
+    if (products < 0) return products;
+    return flag | other | fused | fwd | products;
 }

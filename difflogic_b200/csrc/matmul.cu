@@ -1,0 +1,772 @@
+// Dense layers and the orthogonalisation of matrices: the matrix products of matmul.cuh with their epilogues, what lays out their
+// operands, and the entry points.
+#include "matmul.cuh"
+#include "matmul_plan.h"
+
+namespace dl {
+
+int matmul_async_error() {
+    int flag = 0;
+    if (cudaMemcpyFromSymbol(&flag, g_matmul_async_error, sizeof(int)) != cudaSuccess) {
+        cudaGetLastError();
+        return -1;
+    }
+    return flag;
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+bool make_tile_map(CUtensorMap *map, const void *base, bool bfloat, int64_t inner, int64_t rows, int64_t planes, int64_t row_bytes,
+                   int64_t plane_bytes) {
+    const EncodeTiled encode = encode_tiled();
+    if (encode == nullptr) return false;
+    if (planes == 1) plane_bytes = row_bytes * rows;   // not used, but looked at
+    const cuuint64_t sizes[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t pitches[2] = {(cuuint64_t)row_bytes, (cuuint64_t)plane_bytes};
+    const cuuint32_t box[3] = {kChunk, kChunk, 1}, steps[3] = {1, 1, 1};
+    return encode(map, bfloat ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), sizes,
+                  pitches, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// -- launching a product --------------------------------------------------------------------------------------------------------
+
+struct Product {
+    Operand a, b;
+    int64_t m, n, k, batch;
+    int planes;
+    bool bfloat, symmetric;
+};
+
+static bool map_operand(CUtensorMap *map, const Operand &o, const Product &p, int64_t rows) {
+    const int64_t inner = o.mn ? rows : p.k, outer = o.mn ? p.k : rows;
+    return make_tile_map(map, o.base, p.bfloat, inner, outer, p.planes * p.batch, o.pitch * 2, o.plane * 2);
+}
+
+template <int PLANES, int COLUMNS, class Epilogue>
+static int launch_tiles(const Product &p, const MatmulShape &shape, const CUtensorMap &a, const CUtensorMap &b, const Epilogue &epilogue,
+                        int sms, cudaStream_t st, const char *what) {
+    auto kernel = matmul_kernel<PLANES, COLUMNS, Epilogue>;
+    constexpr int kShared = MatmulConfig<PLANES, COLUMNS>::kSharedBytes;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared) != cudaSuccess) return launch_status(what);
+    launch_dependent(true, kernel, dim3((unsigned)(shape.tiles < sms ? shape.tiles : sms)), dim3(kMatmulThreads), kShared, st, a, b, shape,
+                     epilogue);
+    return launch_status(what);
+}
+
+template <int PLANES, class Epilogue>
+static int launch_columns(const Product &p, const MatmulPlan &plan, const Epilogue &epilogue, int sms, cudaStream_t st, const char *what) {
+    CUtensorMap a, b;
+    if (!map_operand(&a, p.a, p, p.m) || !map_operand(&b, p.b, p, p.n))
+        return fail(DL_ERR_CUDA, "%s: the driver refuses the map of an operand", what);
+    MatmulShape s = {};
+    s.m = (int32_t)p.m;
+    s.n = (int32_t)p.n;
+    s.batch = (int32_t)p.batch;
+    s.planes_z = p.planes;
+    s.tiles_m = (int32_t)ceil_div(p.m, kMatmulRows);
+    s.tiles_n = (int32_t)ceil_div(p.n, plan.columns);
+    s.splits = plan.splits;
+    s.k_steps = (int32_t)ceil_div(p.k, kChunk);
+    s.steps_per_split = plan.steps_per_split;
+    s.symmetric = p.symmetric;
+    int64_t per_matrix = (int64_t)s.tiles_m * s.tiles_n;
+    if (p.symmetric) {
+        per_matrix = 0;
+        for (int64_t mi = 0; mi < s.tiles_m; ++mi) {
+            const int64_t across = ceil_div((mi + 1) * kMatmulRows, plan.columns);
+            per_matrix += across < s.tiles_n ? across : s.tiles_n;
+        }
+    }
+    const int64_t tiles = per_matrix * s.splits * p.batch;
+    if (tiles > INT32_MAX / 2) return fail(DL_ERR_TOO_LARGE, "%s: too many tiles", what);
+    s.per_matrix = (int32_t)per_matrix;
+    s.tiles = (int32_t)tiles;
+    s.a_mn = p.a.mn;
+    s.b_mn = p.b.mn;
+    s.instruction = instruction_descriptor(p.bfloat, p.a.mn, p.b.mn, plan.columns);
+    if (plan.columns == 64) return launch_tiles<PLANES, 64>(p, s, a, b, epilogue, sms, st, what);
+    if (plan.columns == 128) return launch_tiles<PLANES, 128>(p, s, a, b, epilogue, sms, st, what);
+    if constexpr (PLANES < 3) return launch_tiles<PLANES, 256>(p, s, a, b, epilogue, sms, st, what);
+    return fail(DL_ERR_INVALID_ARG, "%s: no such tile", what);
+}
+
+// One product with its epilogue; `partial`: plan.partial_bytes.
+template <int PLANES, class Epilogue>
+static int launch_product(const Product &p, const MatmulPlan &plan, const Epilogue &epilogue, float *partial, int sms, cudaStream_t st,
+                          const char *what) {
+    if (plan.splits == 1) return launch_columns<PLANES>(p, plan, epilogue, sms, st, what);
+    const int status = launch_columns<PLANES>(p, plan, StorePartial{partial, p.n, p.m * p.n}, sms, st, what);
+    if (status != DL_OK) return status;
+    const int64_t quads = ceil_div(p.n, 4) * p.m * p.batch;
+    int64_t blocks = ceil_div(quads, kThreads);
+    if (blocks > 8 * sms) blocks = 8 * sms;
+    launch_dependent(true, matmul_join_kernel<Epilogue>, dim3((unsigned)blocks), dim3(kThreads), 0, st, (const float *)partial, plan.splits,
+                     (int)p.batch, (int)p.m, (int)p.n, (int)p.symmetric, epilogue);
+    return launch_status(what);
+}
+
+// Values of a row of planes that the library lays out: whole units of 16 bytes.
+static int64_t padded(int64_t n) { return ceil_div(n, 8) * 8; }
+static int64_t padded_bytes(int64_t n) { return ceil_div(n, 256) * 256; }
+
+// ============================================================== dense layers ====================================================
+
+// Derivatives of the activation are kept for the backward pass, in fp32 or -- 16-bit layers -- in fp16 times 2^14: 11 bits, where the
+// layer's own type may have 8, and down to 4e-12, where sigmoids saturate.
+constexpr float kSlopeScale = 16384.f;
+
+__device__ __forceinline__ float activate(float z, int act, float &slope) {
+    if (act == DL_ACT_NONE) {
+        slope = 1.f;
+        return z;
+    }
+    if (act == DL_ACT_RELU) {
+        slope = z > 0.f ? 1.f : 0.f;
+        return z > 0.f || z != z ? z : 0.f;
+    }
+    if (act == DL_ACT_GELU) {
+        const float phi = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+        // far out z times an exp(-z^2 / 2) of zero is zero, infinity times it would not be
+        slope = phi + (fabsf(z) > 15.f ? 0.f : z * expf(-0.5f * z * z) * 0.39894228040143268f);
+        return z == -INFINITY ? 0.f : z * phi;
+    }
+    const float s = 1.f / (1.f + expf(-z));
+    if (act == DL_ACT_SIGMOID) {
+        slope = s * (1.f - s);
+        return s;
+    }
+    // expf(-z) overflows below -88.7: s is zero there, and so is the product with a finite z
+    slope = s * (1.f + (s == 0.f || s == 1.f ? 0.f : z * (1.f - s)));
+    return z == -INFINITY ? 0.f : z * s;
+}
+
+// y = act(sum + bias) + residual.  rows_are_features: the rows of the product are the layer's outputs, else its columns are; the result
+// lies [batch][feature] or, feature_major, [feature][batch].
+struct DenseEpilogue {
+    void *y;
+    const void *bias, *residual;
+    void *slope;
+    int64_t y_pitch, residual_batch, residual_feature;   // of the residual: values to the next sample, to the next feature
+    int type, act;
+    bool rows_are_features, feature_major;
+
+    // Neighbouring columns of the product are neighbours in memory, or neighbouring rows are.
+    __device__ __forceinline__ bool across() const { return rows_are_features == feature_major; }
+    __device__ __forceinline__ bool by_column(int, int) const { return !across(); }
+    __device__ __forceinline__ bool by_row(int, int) const { return across(); }
+
+    __device__ __forceinline__ float value(int64_t sample, int64_t feature, float z, float &slope_of) const {
+        if (bias != nullptr) z += load_as_float(bias, feature, type);
+        float v = activate(z, act, slope_of);
+        if (residual != nullptr) v += load_as_float(residual, sample * residual_batch + feature * residual_feature, type);
+        return v;
+    }
+    __device__ __forceinline__ void one(int, int row, int col, float sum) const {
+        const int64_t sample = rows_are_features ? col : row, feature = rows_are_features ? row : col;
+        float d;
+        const float v = value(sample, feature, sum, d);
+        const int64_t i = feature_major ? feature * y_pitch + sample : sample * y_pitch + feature;
+        if (type == kFloat32) {
+            reinterpret_cast<float *>(y)[i] = v;
+            if (slope != nullptr) reinterpret_cast<float *>(slope)[i] = d;
+        } else {
+            reinterpret_cast<uint16_t *>(y)[i] = to_16bit(v, type);
+            if (slope != nullptr) reinterpret_cast<uint16_t *>(slope)[i] = to_16bit(d * kSlopeScale, kFloat16);
+        }
+    }
+    __device__ __forceinline__ void four(int, int row, int col, const float (&sum)[4], int valid) const {
+        float v[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < valid)
+                v[j] = value(rows_are_features ? col + j : row, rows_are_features ? row : col + j, sum[j], d[j]);
+        const int64_t i = (int64_t)row * y_pitch + col;
+        store4(y, i, type, valid, v);
+        if (slope != nullptr) {
+            if (type != kFloat32) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[j] *= kSlopeScale;
+            }
+            store4(slope, i, type == kFloat32 ? kFloat32 : kFloat16, valid, d);
+        }
+    }
+};
+
+// Gradients: the sums as they are, in the layer's type.
+struct PlainEpilogue {
+    void *out;
+    int64_t pitch;
+    int type;
+    __device__ __forceinline__ bool by_column(int, int) const { return false; }
+    __device__ __forceinline__ bool by_row(int, int) const { return true; }
+    __device__ __forceinline__ void one(int, int, int, float) const {}
+    __device__ __forceinline__ void four(int, int row, int col, const float (&sum)[4], int valid) const {
+        store4(out, row * pitch + col, type, valid, sum);
+    }
+};
+
+// rows x cols values, `pitch` apart, into planes of padded rows: 16-bit types as they are, fp32 as triples.
+__global__ void __launch_bounds__(kThreads)
+lay_out_kernel(const void *__restrict__ src, int64_t rows, int64_t cols, int64_t pitch, int type, uint16_t *__restrict__ dst, int64_t dst_pitch,
+               int64_t plane) {
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const int64_t quads = (cols + 3) / 4, total = rows * quads;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t row = i / quads, col = (i - row * quads) * 4, to = row * dst_pitch + col;
+        const int valid = (int)(cols - col < 4 ? cols - col : 4);
+        float v[4];
+        load4(src, row * pitch + col, type, valid, v);
+        uint16_t p[3][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (type == kFloat32) split_triple(v[j], p[0][j], p[1][j], p[2][j]);
+            else p[0][j] = to_16bit(v[j], type);   // the value itself
+        }
+        // padded rows: the last quad of a row may write its whole unit
+        *reinterpret_cast<ushort4 *>(dst + to) = make_ushort4(p[0][0], p[0][1], p[0][2], p[0][3]);
+        if (type == kFloat32) {
+            *reinterpret_cast<ushort4 *>(dst + plane + to) = make_ushort4(p[1][0], p[1][1], p[1][2], p[1][3]);
+            *reinterpret_cast<ushort4 *>(dst + 2 * plane + to) = make_ushort4(p[2][0], p[2][1], p[2][2], p[2][3]);
+        }
+    }
+}
+
+// gz = gy * slope into planes (none where the gradient of y can be used as it is: dst null), and the sums of its columns (sum_rows: of
+// its rows) over a strip of rows.  A block takes 128 columns (32 lanes of 4) and a strip; 8 row groups.
+__global__ void __launch_bounds__(kThreads)
+pre_gradient_kernel(const void *__restrict__ gy, const void *__restrict__ slope, int64_t rows, int64_t cols, int type,
+                    uint16_t *__restrict__ dst, int64_t dst_pitch, int64_t plane, int64_t strip, float *__restrict__ partial, int sum_rows) {
+    __shared__ float s_sum[kThreads / 32][128];
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+    const int64_t col = (int64_t)blockIdx.x * 128 + lane * 4, first = (int64_t)blockIdx.y * strip, last = first + strip < rows ? first + strip : rows;
+    const int valid = (int)(cols - col < 4 ? cols - col : 4);
+    float total[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int64_t row = first + group; row < last; row += kThreads / 32) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (valid > 0) {
+            load4(gy, row * cols + col, type, valid, v);
+            if (slope != nullptr) {
+                float d[4];
+                load4(slope, row * cols + col, type == kFloat32 ? kFloat32 : kFloat16, valid, d);
+                const float scale = type == kFloat32 ? 1.f : 1.f / kSlopeScale;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] *= d[j] * scale;
+            }
+            if (dst != nullptr) {
+                const int64_t to = row * dst_pitch + col;
+                uint16_t p[3][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (type == kFloat32) split_triple(v[j], p[0][j], p[1][j], p[2][j]);
+                    else p[0][j] = to_16bit(v[j], type);
+                }
+                *reinterpret_cast<ushort4 *>(dst + to) = make_ushort4(p[0][0], p[0][1], p[0][2], p[0][3]);
+                if (type == kFloat32) {
+                    *reinterpret_cast<ushort4 *>(dst + plane + to) = make_ushort4(p[1][0], p[1][1], p[1][2], p[1][3]);
+                    *reinterpret_cast<ushort4 *>(dst + 2 * plane + to) = make_ushort4(p[2][0], p[2][1], p[2][2], p[2][3]);
+                }
+            }
+        }
+        if (partial != nullptr && sum_rows) {   // the features are rows: this row's share of 128 samples
+            float r = v[0] + v[1] + v[2] + v[3];
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) r += __shfl_xor_sync(0xffffffffu, r, off);
+            if (lane == 0) partial[(int64_t)blockIdx.x * rows + row] = r;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) total[j] += v[j];
+    }
+    if (partial == nullptr || sum_rows) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s_sum[group][lane * 4 + j] = total[j];
+    __syncthreads();
+    const int64_t c = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    if (threadIdx.x < 128 && c < cols) {
+        float r = 0.f;
+#pragma unroll
+        for (int g = 0; g < kThreads / 32; ++g) r += s_sum[g][threadIdx.x];
+        partial[blockIdx.y * cols + c] = r;
+    }
+}
+
+// Adds the partial sums up, in their order.
+__global__ void __launch_bounds__(kThreads)
+bias_gradient_kernel(const float *__restrict__ partial, int64_t parts, int64_t features, void *__restrict__ out, int type) {
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= features) return;
+    float r = 0.f;
+    for (int64_t p = 0; p < parts; ++p) r += partial[p * features + i];
+    if (type == kFloat32) reinterpret_cast<float *>(out)[i] = r;
+    else reinterpret_cast<uint16_t *>(out)[i] = to_16bit(r, type);
+}
+
+// What of an operand the copies can read in place: 16-bit values whose base and rows lie on units of 16 bytes.
+static bool in_place(const void *p, int64_t pitch, int type) { return type != kFloat32 && aligned_to(p, 16) && pitch % 8 == 0; }
+
+struct DenseLayout {
+    int planes;
+    int64_t x_rows, x_cols, x_pitch;   // as it lies in memory
+    bool lay_x, lay_w;
+    int64_t x_plane_pitch, x_plane, w_plane_pitch, w_plane;   // of the planes that the library lays out
+    int64_t x_bytes, w_bytes;
+};
+
+static DenseLayout dense_layout(int64_t batch, int64_t inner, int64_t outer, int64_t x_pitch, bool x_feature_major, int type, const void *x,
+                                const void *w) {
+    DenseLayout l = {};
+    l.planes = type == kFloat32 ? 3 : 1;
+    l.x_rows = x_feature_major ? inner : batch;
+    l.x_cols = x_feature_major ? batch : inner;
+    l.x_pitch = x_pitch;
+    l.lay_x = !in_place(x, x_pitch, type);
+    l.lay_w = !in_place(w, inner, type);
+    l.x_plane_pitch = padded(l.x_cols);
+    l.x_plane = l.x_rows * l.x_plane_pitch;
+    l.w_plane_pitch = padded(inner);
+    l.w_plane = outer * l.w_plane_pitch;
+    l.x_bytes = l.lay_x ? padded_bytes(l.planes * l.x_plane * 2) : 0;
+    l.w_bytes = l.lay_w ? padded_bytes(l.planes * l.w_plane * 2) : 0;
+    return l;
+}
+
+static int lay_out(const void *src, int64_t rows, int64_t cols, int64_t pitch, int type, void *dst, int64_t dst_pitch, int64_t plane, int sms,
+                   cudaStream_t st, const char *what) {
+    int64_t blocks = ceil_div(rows * ceil_div(cols, 4), kThreads);
+    if (blocks > 16 * sms) blocks = 16 * sms;
+    launch_dependent(true, lay_out_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, src, rows, cols, pitch, type,
+                     reinterpret_cast<uint16_t *>(dst), dst_pitch, plane);
+    return launch_status(what);
+}
+
+template <class Epilogue>
+static int launch_planes(const Product &p, const MatmulPlan &plan, const Epilogue &e, float *partial, int sms, cudaStream_t st, const char *what) {
+    return p.planes == 3 ? launch_product<3>(p, plan, e, partial, sms, st, what) : launch_product<1>(p, plan, e, partial, sms, st, what);
+}
+
+// The layer's outputs are the rows of the product where that leaves fewer of a tile's 128 rows and 64 columns empty.
+static bool features_as_rows(int64_t batch, int64_t outer) { return batch < outer && batch < 256; }
+
+static MatmulPlan plan_forward(int64_t batch, int64_t inner, int64_t outer, int planes, int sms) {
+    return features_as_rows(batch, outer) ? plan_matmul(outer, batch, inner, 1, planes, false, sms) : plan_matmul(batch, outer, inner, 1, planes, false, sms);
+}
+
+// Strips of rows of a pre-activation gradient, enough for whole SMs.
+static int64_t strips_of(int64_t rows, int64_t cols, int sms, int64_t *strip) {
+    int64_t strips = ceil_div(4 * sms, ceil_div(cols, 128));
+    if (strips > ceil_div(rows, 8)) strips = ceil_div(rows, 8);
+    if (strips > 65535) strips = 65535;
+    *strip = ceil_div(rows, strips);
+    return ceil_div(rows, *strip);
+}
+
+static bool dense_sizes(int64_t batch, int64_t inner, int64_t outer, int type, const char *what, int *status) {
+    *status = DL_OK;
+    if (batch < 0 || inner <= 0 || outer <= 0 || batch > INT32_MAX / 2 || inner > INT32_MAX / 2 || outer > INT32_MAX / 2)
+        *status = fail(DL_ERR_INVALID_ARG, "%s: bad size", what);
+    else if (type < kFloat32 || type > kFloat16)
+        *status = fail(DL_ERR_INVALID_ARG, "%s: unknown type %d", what, type);
+    return *status == DL_OK;
+}
+
+}  // namespace dl
+
+using namespace dl;
+
+extern "C" DL_API int64_t dl_dense_planes_bytes(const void *p, int64_t rows, int64_t cols, int64_t pitch, int type) {
+    if (rows <= 0 || cols <= 0 || in_place(p, pitch, type)) return 0;
+    return padded_bytes((type == kFloat32 ? 3 : 1) * rows * padded(cols) * 2);
+}
+
+extern "C" DL_API int64_t dl_dense_forward_workspace_bytes(int64_t batch, int64_t inner, int64_t outer, int type) {
+    if (batch <= 0 || inner <= 0 || outer <= 0) return 0;
+    return plan_forward(batch, inner, outer, type == kFloat32 ? 3 : 1, current_sms()).partial_bytes;
+}
+
+extern "C" DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_feature_major, const void *w, const void *bias, const void *residual,
+                                       int64_t residual_batch, int64_t residual_feature, int act, void *y, int y_feature_major, void *slope,
+                                       void *x_planes, void *w_planes, void *workspace, int64_t batch, int64_t inner, int64_t outer, int type,
+                                       void *stream) {
+    const char *what = "dl_dense_forward";
+    int status;
+    if (!dense_sizes(batch, inner, outer, type, what, &status)) return status;
+    DL_REQUIRE(act >= DL_ACT_NONE && act <= DL_ACT_GELU, DL_ERR_INVALID_ARG, "%s: unknown activation %d", what, act);
+    if (batch == 0) return DL_OK;
+    DL_REQUIRE(x && w && y, DL_ERR_INVALID_ARG, "%s: null pointer", what);
+    DL_REQUIRE(x_pitch >= (x_feature_major ? batch : inner), DL_ERR_INVALID_ARG, "%s: rows of x overlap", what);
+    const DenseLayout l = dense_layout(batch, inner, outer, x_pitch, x_feature_major != 0, type, x, w);
+    const int sms = current_sms();
+    const MatmulPlan plan = plan_forward(batch, inner, outer, l.planes, sms);
+    DL_REQUIRE((!l.lay_x || x_planes) && (!l.lay_w || w_planes) && (plan.partial_bytes == 0 || workspace), DL_ERR_INVALID_ARG,
+               "%s: a workspace is missing", what);
+    DL_REQUIRE(aligned_to(x_planes, 16) && aligned_to(w_planes, 16) && aligned_to(workspace, 16), DL_ERR_INVALID_ARG,
+               "%s: workspaces must be 16-byte aligned", what);
+    cudaStream_t st = as_stream(stream);
+    if (l.lay_x && (status = lay_out(x, l.x_rows, l.x_cols, x_pitch, type, x_planes, l.x_plane_pitch, l.x_plane, sms, st, what)) != DL_OK) return status;
+    if (l.lay_w && (status = lay_out(w, outer, inner, inner, type, w_planes, l.w_plane_pitch, l.w_plane, sms, st, what)) != DL_OK) return status;
+    const Operand ox = {l.lay_x ? x_planes : x, l.lay_x ? l.x_plane_pitch : x_pitch, l.x_plane, 0, x_feature_major != 0};
+    const Operand ow = {l.lay_w ? w_planes : w, l.lay_w ? l.w_plane_pitch : inner, l.w_plane, 0, false};
+    const bool rows_are_features = features_as_rows(batch, outer);
+    Product p = {};
+    p.a = rows_are_features ? ow : ox;
+    p.b = rows_are_features ? ox : ow;
+    p.m = rows_are_features ? outer : batch;
+    p.n = rows_are_features ? batch : outer;
+    p.k = inner;
+    p.batch = 1;
+    p.planes = l.planes;
+    p.bfloat = type != kFloat16;
+    const DenseEpilogue e = {y, bias, residual, slope, y_feature_major ? batch : outer, residual_batch, residual_feature, type, act,
+                             rows_are_features, y_feature_major != 0};
+    return launch_planes(p, plan, e, reinterpret_cast<float *>(workspace), sms, st, what);
+}
+
+namespace dl {
+
+struct DenseBackward {
+    int planes;
+    bool lay_gz;
+    int64_t g_rows, g_cols, g_pitch, g_plane, strips, strip, parts;
+    MatmulPlan to_x, to_w;
+    int64_t g_bytes, bias_bytes, x_bytes, w_bytes;   // workspace: gz planes, partial bias sums, splits of the two products
+};
+
+static DenseBackward plan_backward(int64_t batch, int64_t inner, int64_t outer, bool g_feature_major, int type, bool act, const void *gy, int sms) {
+    DenseBackward b = {};
+    b.planes = type == kFloat32 ? 3 : 1;
+    b.g_rows = g_feature_major ? outer : batch;
+    b.g_cols = g_feature_major ? batch : outer;
+    b.lay_gz = act || !in_place(gy, b.g_cols, type);
+    b.g_pitch = padded(b.g_cols);
+    b.g_plane = b.g_rows * b.g_pitch;
+    b.g_bytes = b.lay_gz ? padded_bytes(b.planes * b.g_plane * 2) : 0;
+    b.strips = strips_of(b.g_rows, b.g_cols, sms, &b.strip);
+    b.parts = g_feature_major ? ceil_div(b.g_cols, 128) : b.strips;
+    b.bias_bytes = padded_bytes(b.parts * outer * 4);
+    b.to_x = plan_matmul(batch, inner, outer, 1, b.planes, false, sms);
+    b.to_w = plan_matmul(outer, inner, batch, 1, b.planes, false, sms);
+    b.x_bytes = padded_bytes(b.to_x.partial_bytes);
+    b.w_bytes = padded_bytes(b.to_w.partial_bytes);
+    return b;
+}
+
+}  // namespace dl
+
+extern "C" DL_API int64_t dl_dense_backward_workspace_bytes(int64_t batch, int64_t inner, int64_t outer, int g_feature_major, int type, int has_slope,
+                                                            const void *gy) {
+    if (batch <= 0 || inner <= 0 || outer <= 0) return 0;
+    const DenseBackward b = plan_backward(batch, inner, outer, g_feature_major != 0, type, has_slope != 0, gy, current_sms());
+    return b.g_bytes + b.bias_bytes + b.x_bytes + b.w_bytes;
+}
+
+extern "C" DL_API int dl_dense_backward(const void *gy, int g_feature_major, const void *slope, const void *x, int64_t x_pitch, int x_feature_major,
+                                        const void *w, const void *x_planes, const void *w_planes, void *gx, void *gw, void *gb, void *workspace,
+                                        int64_t batch, int64_t inner, int64_t outer, int type, void *stream) {
+    const char *what = "dl_dense_backward";
+    int status;
+    if (!dense_sizes(batch, inner, outer, type, what, &status)) return status;
+    DL_REQUIRE(batch > 0, DL_ERR_INVALID_ARG, "%s: empty batch", what);
+    DL_REQUIRE(gy && (x || !gw || x_planes) && (w || !gx || w_planes), DL_ERR_INVALID_ARG, "%s: null pointer", what);
+    DL_REQUIRE(workspace && aligned_to(workspace, 16), DL_ERR_INVALID_ARG, "%s: the workspace is missing or not 16-byte aligned", what);
+    const int sms = current_sms();
+    const DenseLayout l = dense_layout(batch, inner, outer, x_pitch, x_feature_major != 0, type, x, w);
+    const DenseBackward b = plan_backward(batch, inner, outer, g_feature_major != 0, type, slope != nullptr, gy, sms);
+    DL_REQUIRE((!gw || !l.lay_x || x_planes) && (!gx || !l.lay_w || w_planes), DL_ERR_INVALID_ARG, "%s: laid-out operands are missing", what);
+    cudaStream_t st = as_stream(stream);
+    uint8_t *at = reinterpret_cast<uint8_t *>(workspace);
+    uint16_t *gz = reinterpret_cast<uint16_t *>(at);
+    float *sums = reinterpret_cast<float *>(at + b.g_bytes), *part_x = reinterpret_cast<float *>(at + b.g_bytes + b.bias_bytes),
+          *part_w = reinterpret_cast<float *>(at + b.g_bytes + b.bias_bytes + b.x_bytes);
+    if (b.lay_gz || gb) {
+        launch_dependent(true, pre_gradient_kernel, dim3((unsigned)ceil_div(b.g_cols, 128), (unsigned)b.strips), dim3(kThreads), 0, st, gy, slope,
+                         b.g_rows, b.g_cols, type, b.lay_gz ? gz : (uint16_t *)nullptr, b.g_pitch, b.g_plane, b.strip, gb ? sums : (float *)nullptr,
+                         g_feature_major);
+        if ((status = launch_status(what)) != DL_OK) return status;
+    }
+    if (gb) {
+        launch_dependent(true, bias_gradient_kernel, dim3((unsigned)ceil_div(outer, kThreads)), dim3(kThreads), 0, st, (const float *)sums, b.parts,
+                         outer, gb, type);
+        if ((status = launch_status(what)) != DL_OK) return status;
+    }
+    Operand g = {b.lay_gz ? (const void *)gz : gy, b.lay_gz ? b.g_pitch : b.g_cols, b.g_plane, 0, false};
+    Product p = {};
+    p.batch = 1;
+    p.planes = b.planes;
+    p.bfloat = type != kFloat16;
+    if (gx) {   // gz [batch][outer] w [outer][inner], summed over the outputs
+        p.a = g;
+        p.a.mn = g_feature_major != 0;
+        p.b = {l.lay_w ? w_planes : w, l.lay_w ? l.w_plane_pitch : inner, l.w_plane, 0, true};
+        p.m = batch;
+        p.n = inner;
+        p.k = outer;
+        if ((status = launch_planes(p, b.to_x, PlainEpilogue{gx, inner, type}, part_x, sms, st, what)) != DL_OK) return status;
+    }
+    if (gw) {   // gz^T x, summed over the batch
+        p.a = g;
+        p.a.mn = g_feature_major == 0;
+        p.b = {l.lay_x ? x_planes : x, l.lay_x ? l.x_plane_pitch : x_pitch, l.x_plane, 0, x_feature_major == 0};
+        p.m = outer;
+        p.n = inner;
+        p.k = batch;
+        if ((status = launch_planes(p, b.to_w, PlainEpilogue{gw, inner, type}, part_w, sms, st, what)) != DL_OK) return status;
+    }
+    return DL_OK;
+}
+
+// =============================================================== orthogonalisation ==============================================
+
+namespace dl {
+
+// Sums of squares of a matrix, one per block, in 64 bits: fp32 values of any size fit.
+__global__ void __launch_bounds__(kThreads)
+square_sums_kernel(const void *__restrict__ g, int64_t count, int type, double *__restrict__ partial) {
+    __shared__ double s_part[kThreads / 32];
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const int64_t base = (int64_t)blockIdx.y * count, quads = (count + 3) / 4;
+    double sum = 0;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < quads; i += (int64_t)gridDim.x * kThreads) {
+        float v[4];
+        load4(g, base + i * 4, type, (int)(count - i * 4 < 4 ? count - i * 4 : 4), v);
+        sum += ((double)v[0] * v[0] + (double)v[1] * v[1]) + ((double)v[2] * v[2] + (double)v[3] * v[3]);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (threadIdx.x % 32 == 0) s_part[threadIdx.x / 32] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kThreads / 32; ++i) sum += s_part[i];
+        partial[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = sum;
+    }
+}
+
+// X = G / max(|G|, eps) as pairs.
+__global__ void __launch_bounds__(kThreads)
+normalise_kernel(const void *__restrict__ g, int64_t rows, int64_t cols, int type, const double *__restrict__ partial, int parts, double eps,
+                 uint16_t *__restrict__ x, int64_t pitch, int64_t plane) {
+    __shared__ float s_scale;
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const int64_t z = blockIdx.y;
+    if (threadIdx.x < 32) {
+        double sum = 0;
+        for (int i = threadIdx.x; i < parts; i += 32) sum += partial[z * parts + i];
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        const double norm = sqrt(sum);
+        // a scale that is not finite (an infinite or undefined entry) makes the whole result undefined
+        if (threadIdx.x == 0) s_scale = norm <= 1.7e308 ? (float)((double)kPairScale / (norm > eps ? norm : eps)) : __int_as_float(0x7fc00000);
+    }
+    __syncthreads();
+    const float scale = s_scale;
+    const int64_t quads = (cols + 3) / 4, total = rows * quads;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t row = i / quads, col = (i - row * quads) * 4;
+        float v[4];
+        load4(g, (z * rows + row) * cols + col, type, (int)(cols - col < 4 ? cols - col : 4), v);
+        uint16_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_pair(v[j] * scale, hi[j], lo[j]);
+        uint16_t *to = x + 2 * z * plane + row * pitch + col;
+        *reinterpret_cast<ushort4 *>(to) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<ushort4 *>(to + plane) = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+    }
+}
+
+// Results of the iteration as pairs: v = scale * sum (+ b * gram + a on the diagonal).
+struct PairEpilogue {
+    uint16_t *out;
+    const uint16_t *gram;   // null: none
+    int64_t pitch, plane;   // of out and gram
+    float scale, b, diagonal;
+    bool symmetric;
+
+    __device__ __forceinline__ bool by_column(int row, int col) const { return symmetric && col / kMatmulRows < row / kMatmulRows; }
+    __device__ __forceinline__ bool by_row(int row, int col) const { return !symmetric || col / kMatmulRows <= row / kMatmulRows; }
+    __device__ __forceinline__ void one(int z, int row, int col, float sum) const {   // the mirrored value
+        const int64_t i = 2 * z * plane + (int64_t)col * pitch + row;
+        float v = sum * scale;
+        if (gram != nullptr) v += b * join_pair(gram[i], gram[i + plane]);
+        uint16_t hi, lo;
+        split_pair(v, hi, lo);
+        out[i] = hi;
+        out[i + plane] = lo;
+    }
+    __device__ __forceinline__ void four(int z, int row, int col, const float (&sum)[4], int valid) const {
+        // rows are padded to whole units: the values behind the last one are written too, and read by nothing
+        const int64_t i = 2 * z * plane + (int64_t)row * pitch + col;
+        uint16_t hi[4], lo[4];
+        ushort4 gh = make_ushort4(0, 0, 0, 0), gl = gh;
+        if (gram != nullptr) {
+            gh = *reinterpret_cast<const ushort4 *>(gram + i);
+            gl = *reinterpret_cast<const ushort4 *>(gram + i + plane);
+        }
+        const uint16_t g_hi[4] = {gh.x, gh.y, gh.z, gh.w}, g_lo[4] = {gl.x, gl.y, gl.z, gl.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float v = sum[j] * scale;
+            if (gram != nullptr) v += b * join_pair(g_hi[j], g_lo[j]);
+            if (row == col + j) v += diagonal;
+            split_pair(v, hi[j], lo[j]);
+        }
+        *reinterpret_cast<ushort4 *>(out + i) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<ushort4 *>(out + i + plane) = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+    }
+};
+
+// The last product: the result itself, or the weights' update w <- decay w - rate v.
+struct OrthogonalEpilogue {
+    void *out;
+    int64_t cols, matrix;   // values of a row, of a matrix
+    int type;
+    float scale;
+    bool update;
+    float decay, rate;
+    __device__ __forceinline__ bool by_column(int, int) const { return false; }
+    __device__ __forceinline__ bool by_row(int, int) const { return true; }
+    __device__ __forceinline__ void one(int, int, int, float) const {}
+    __device__ __forceinline__ void four(int z, int row, int col, const float (&sum)[4], int valid) const {
+        const int64_t i = z * matrix + row * cols + col;
+        float v[4];
+        if (update) {
+            load4(out, i, kFloat32, valid, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = v[j] * decay - rate * (sum[j] * scale);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = sum[j] * scale;
+        }
+        store4(out, i, type, valid, v);
+    }
+};
+
+struct OrthogonalLayout {
+    int64_t side, x_pitch, x_plane, s_pitch, s_plane;   // side: the smaller one
+    bool tall;
+    int parts;
+    MatmulPlan gram, square, product;
+    int64_t x_bytes, s_bytes, norm_bytes, partial_bytes;
+    int64_t total() const { return 2 * x_bytes + 2 * s_bytes + norm_bytes + partial_bytes; }
+};
+
+static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t cols, int sms) {
+    OrthogonalLayout l = {};
+    l.tall = rows >= cols;
+    l.side = l.tall ? cols : rows;
+    l.x_pitch = padded(cols);
+    l.x_plane = rows * l.x_pitch;
+    l.s_pitch = padded(l.side);
+    l.s_plane = l.side * l.s_pitch;
+    l.parts = (int)(ceil_div(rows * cols, 4 * kThreads * 4) < 2 * sms ? ceil_div(rows * cols, 4 * kThreads * 4) : 2 * sms);
+    l.gram = plan_matmul(l.side, l.side, l.tall ? rows : cols, batch, 2, true, sms);
+    l.square = plan_matmul(l.side, l.side, l.side, batch, 2, true, sms);
+    l.product = plan_matmul(rows, cols, l.side, batch, 2, false, sms);
+    l.x_bytes = padded_bytes(batch * 2 * l.x_plane * 2);
+    l.s_bytes = padded_bytes(batch * 2 * l.s_plane * 2);
+    l.norm_bytes = padded_bytes(batch * l.parts * 8);
+    l.partial_bytes = l.gram.partial_bytes;
+    if (l.square.partial_bytes > l.partial_bytes) l.partial_bytes = l.square.partial_bytes;
+    if (l.product.partial_bytes > l.partial_bytes) l.partial_bytes = l.product.partial_bytes;
+    return l;
+}
+
+// steps times: S = X^T X (X X^T where X is wide), M = a I + b S + c S^2, X = X M (M X).  `last` takes the last product.
+static int orthogonalise(const void *g, int type, int64_t batch, int64_t rows, int64_t cols, int steps, const float *coefficients, double eps,
+                         const OrthogonalEpilogue &last, uint8_t *workspace, int sms, cudaStream_t st, const char *what) {
+    const OrthogonalLayout l = orthogonal_layout(batch, rows, cols, sms);
+    uint16_t *x = reinterpret_cast<uint16_t *>(workspace), *next = reinterpret_cast<uint16_t *>(workspace + l.x_bytes);
+    uint16_t *gram = reinterpret_cast<uint16_t *>(workspace + 2 * l.x_bytes), *poly = reinterpret_cast<uint16_t *>(workspace + 2 * l.x_bytes + l.s_bytes);
+    double *norms = reinterpret_cast<double *>(workspace + 2 * l.x_bytes + 2 * l.s_bytes);
+    float *partial = reinterpret_cast<float *>(workspace + 2 * l.x_bytes + 2 * l.s_bytes + l.norm_bytes);
+    int status;
+    launch_dependent(true, square_sums_kernel, dim3((unsigned)l.parts, (unsigned)batch), dim3(kThreads), 0, st, g, rows * cols, type, norms);
+    if ((status = launch_status(what)) != DL_OK) return status;
+    int64_t blocks = ceil_div(rows * ceil_div(cols, 4), kThreads * 2);
+    if (blocks > 16 * sms) blocks = 16 * sms;
+    launch_dependent(true, normalise_kernel, dim3((unsigned)blocks, (unsigned)batch), dim3(kThreads), 0, st, g, rows, cols, type, (const double *)norms,
+                     l.parts, eps, x, l.x_pitch, l.x_plane);
+    if ((status = launch_status(what)) != DL_OK) return status;
+    Product p = {};
+    p.batch = batch;
+    p.planes = 2;
+    const float once = 1.f / kPairScale, twice = once * once;
+    for (int i = 0; i < steps; ++i) {
+        const float a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
+        p.a = p.b = {x, l.x_pitch, l.x_plane, 0, l.tall};
+        p.m = p.n = l.side;
+        p.k = l.tall ? rows : cols;
+        p.symmetric = true;
+        if ((status = launch_product<2>(p, l.gram, PairEpilogue{gram, nullptr, l.s_pitch, l.s_plane, once, 0.f, 0.f, true}, partial, sms, st, what)) != DL_OK)
+            return status;
+        p.a = p.b = {gram, l.s_pitch, l.s_plane, 0, false};
+        p.k = l.side;
+        if ((status = launch_product<2>(p, l.square, PairEpilogue{poly, gram, l.s_pitch, l.s_plane, c * once, b, a * kPairScale, true}, partial, sms, st,
+                                        what)) != DL_OK)
+            return status;
+        const Operand m = {poly, l.s_pitch, l.s_plane, 0, false};
+        p.a = l.tall ? Operand{x, l.x_pitch, l.x_plane, 0, false} : m;
+        p.b = l.tall ? m : Operand{x, l.x_pitch, l.x_plane, 0, true};
+        p.m = rows;
+        p.n = cols;
+        p.symmetric = false;
+        if (i + 1 < steps)
+            status = launch_product<2>(p, l.product, PairEpilogue{next, nullptr, l.x_pitch, l.x_plane, once, 0.f, 0.f, false}, partial, sms, st, what);
+        else {
+            OrthogonalEpilogue e = last;
+            e.scale = twice;
+            status = launch_product<2>(p, l.product, e, partial, sms, st, what);
+        }
+        if (status != DL_OK) return status;
+        uint16_t *done = x;
+        x = next;
+        next = done;
+    }
+    return DL_OK;
+}
+
+}  // namespace dl
+
+extern "C" DL_API int64_t dl_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols) {
+    if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
+    return orthogonal_layout(batch, rows, cols, current_sms()).total();
+}
+
+extern "C" DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, int64_t rows, int64_t cols, int type, int steps,
+                                       const float *coefficients, double eps, void *workspace, void *stream) {
+    const char *what = "dl_orthogonalize";
+    DL_REQUIRE(batch >= 0 && rows >= 0 && cols >= 0 && rows <= INT32_MAX / 2 && cols <= INT32_MAX / 2, DL_ERR_INVALID_ARG, "%s: bad size", what);
+    DL_REQUIRE(batch <= 65535, DL_ERR_TOO_LARGE, "%s: more than 65535 matrices", what);
+    DL_REQUIRE(type >= kFloat32 && type <= kFloat16, DL_ERR_INVALID_ARG, "%s: unknown type %d", what, type);
+    DL_REQUIRE(steps >= 1 && steps <= 64 && coefficients, DL_ERR_INVALID_ARG, "%s: needs 1 to 64 steps and their coefficients", what);
+    DL_REQUIRE(eps > 0, DL_ERR_INVALID_ARG, "%s: eps must be positive", what);
+    if (batch == 0 || rows == 0 || cols == 0) return DL_OK;
+    DL_REQUIRE(g && out && workspace, DL_ERR_INVALID_ARG, "%s: null pointer", what);
+    DL_REQUIRE(aligned_to(workspace, 16), DL_ERR_INVALID_ARG, "%s: the workspace must be 16-byte aligned", what);
+    OrthogonalEpilogue last = {};
+    last.out = out;
+    last.cols = cols;
+    last.matrix = rows * cols;
+    last.type = type;
+    return orthogonalise(g, type, batch, rows, cols, steps, coefficients, eps, last, reinterpret_cast<uint8_t *>(workspace), current_sms(),
+                         as_stream(stream), what);
+}

@@ -1,0 +1,431 @@
+// Matrix products on the tensor cores with an epilogue: D[m][n] = sum_k A[m][k] B[n][k], per matrix of a batch.
+//
+// Operands are one to three planes of 16-bit values whose sum is the operand, so that results can be as exact as 32-bit arithmetic:
+//   1 plane   fp16 or bf16 values as they are;
+//   2 planes  fp16 pairs hi + lo, 22 bits: hi hi + (hi lo + lo hi), 3 products; for operands of known size (the value is kept
+//             times 2^12, so that lo is no subnormal for values above 2^-14);
+//   3 planes  bf16 triples, all 24 bits of an fp32 in its whole range: 6 products, those below 2^-24 left out.
+// The small products have an accumulator of their own: a running sum in the tensor cores cuts off what is below its last bit, and the
+// sum of the large products then loses no more than a plain product does.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "tensor_core.cuh"
+
+namespace dl {
+
+enum MatmulType { kFloat32 = 0, kBFloat16 = 1, kFloat16 = 2 };
+static inline int type_size(int type) { return type == kFloat32 ? 4 : 2; }
+
+struct Operand {       // rows x k, or k x rows where mn: the rows of the result are contiguous
+    const void *base;
+    int64_t pitch, plane, matrix;  // in values: between rows in memory, planes, matrices of the batch (a multiple of plane)
+    bool mn;
+};
+
+struct MatmulShape {
+    int32_t m, n, batch, planes_z;        // planes_z: planes per matrix in the maps
+    int32_t tiles_m, tiles_n, splits, k_steps, steps_per_split;
+    int32_t per_matrix;                   // tiles of a matrix (one split)
+    int32_t tiles;                        // of all matrices and splits
+    uint32_t a_mn, b_mn, instruction;
+    int32_t symmetric;                    // only tiles that reach to or below the diagonal are computed
+};
+
+#ifdef __CUDACC__
+// -- 16-bit planes --------------------------------------------------------------------------------------------------------------
+
+constexpr float kPairScale = 4096.f;
+
+__device__ __forceinline__ void split_pair(float scaled, uint16_t &hi, uint16_t &lo) {
+    const __half h = __float2half_rn(scaled);
+    hi = __half_as_ushort(h);
+    lo = __half_as_ushort(__float2half_rn(scaled - __half2float(h)));   // inf - inf: NaN, which is what the products would give
+}
+__device__ __forceinline__ float join_pair(uint16_t hi, uint16_t lo) { return __half2float(__ushort_as_half(hi)) + __half2float(__ushort_as_half(lo)); }
+
+// The nearest bf16 at each step: exact for every fp32.  Infinities and NaN go into the first plane alone; values that would round to
+// infinity are cut off.
+__device__ __forceinline__ void split_triple(float x, uint16_t &hi, uint16_t &mid, uint16_t &lo) {
+    const uint32_t bits = __float_as_uint(x);
+    if ((bits & 0x7f800000u) == 0x7f800000u) {
+        hi = (uint16_t)(bits >> 16) | (uint16_t)((bits & 0x007fffffu) ? 0x40 : 0);
+        mid = lo = 0;
+        return;
+    }
+    __nv_bfloat16 h = __float2bfloat16_rn(x);
+    hi = __bfloat16_as_ushort(h);
+    if ((hi & 0x7f80u) == 0x7f80u) hi = (uint16_t)(bits >> 16);
+    const float rest = x - __uint_as_float((uint32_t)hi << 16);
+    h = __float2bfloat16_rn(rest);
+    mid = __bfloat16_as_ushort(h);
+    lo = __bfloat16_as_ushort(__float2bfloat16_rn(rest - __bfloat162float(h)));
+}
+
+__device__ __forceinline__ float load_as_float(const void *p, int64_t i, int type) {
+    if (type == kFloat32) return reinterpret_cast<const float *>(p)[i];
+    const uint16_t v = reinterpret_cast<const uint16_t *>(p)[i];
+    return type == kBFloat16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
+}
+__device__ __forceinline__ uint16_t to_16bit(float v, int type) {
+    return type == kBFloat16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+}
+// Up to four neighbouring values, in one access where all are there and the address allows it.
+__device__ __forceinline__ void load4(const void *p, int64_t i, int type, int valid, float (&v)[4]) {
+    const char *at = reinterpret_cast<const char *>(p) + i * (type == kFloat32 ? 4 : 2);
+    if (valid == 4 && type == kFloat32 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+        const float4 f = *reinterpret_cast<const float4 *>(at);
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else if (valid == 4 && type != kFloat32 && (reinterpret_cast<uintptr_t>(at) & 7) == 0) {
+        const ushort4 u = *reinterpret_cast<const ushort4 *>(at);
+        v[0] = load_as_float(&u.x, 0, type); v[1] = load_as_float(&u.y, 0, type);
+        v[2] = load_as_float(&u.z, 0, type); v[3] = load_as_float(&u.w, 0, type);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = j < valid ? load_as_float(p, i + j, type) : 0.f;
+    }
+}
+__device__ __forceinline__ void store4(void *p, int64_t i, int type, int valid, const float (&v)[4]) {
+    char *at = reinterpret_cast<char *>(p) + i * (type == kFloat32 ? 4 : 2);
+    if (valid == 4 && type == kFloat32 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+        *reinterpret_cast<float4 *>(at) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if (valid == 4 && type != kFloat32 && (reinterpret_cast<uintptr_t>(at) & 7) == 0) {
+        *reinterpret_cast<ushort4 *>(at) = make_ushort4(to_16bit(v[0], type), to_16bit(v[1], type), to_16bit(v[2], type), to_16bit(v[3], type));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < valid) {
+                if (type == kFloat32) reinterpret_cast<float *>(p)[i + j] = v[j];
+                else reinterpret_cast<uint16_t *>(p)[i + j] = to_16bit(v[j], type);
+            }
+    }
+}
+
+// -- the kernel -----------------------------------------------------------------------------------------------------------------
+
+constexpr int kMatmulRows = 128;     // of a tile
+constexpr int kMatmulThreads = 192;  // warps 0-3: epilogue, one lane per row; warp 4: copies; warp 5: products
+constexpr int kStagePitch = 36;      // floats per row of an epilogue warp's 32 x 32 staging tile: 16-byte rows, no bank met twice
+
+template <int PLANES, int COLUMNS>
+struct MatmulConfig {
+    static constexpr int kStepBytes = PLANES * (kMatmulRows + COLUMNS) * kChunk * 2;
+    static constexpr int kFit = 196608 / kStepBytes;
+    static constexpr int kStages = kFit < 6 ? kFit : 6;
+    static constexpr int kSums = PLANES > 1 ? 2 : 1;                           // accumulators of a tile
+    static constexpr int kBuffers = 2 * kSums * COLUMNS <= 512 ? 2 : 1;        // tiles in tensor memory at a time
+    static constexpr int kTensorColumns = kSums * COLUMNS * kBuffers;
+    static constexpr int kSharedBytes = kStages * kStepBytes + 4 * 32 * kStagePitch * 4 + 1024 + 256;
+    static_assert(kStages >= 2 && kSharedBytes <= 232448, "the ring does not fit");
+    static_assert((kTensorColumns & (kTensorColumns - 1)) == 0 && kTensorColumns >= 32 && kTensorColumns <= 512, "tensor memory");
+};
+
+struct Tile {
+    int matrix, split, row, col;  // first row and column
+};
+
+template <int COLUMNS>
+__device__ __forceinline__ Tile tile_of(int id, const MatmulShape &s) {
+    Tile t;
+    const int all = s.per_matrix * s.splits;
+    t.matrix = id / all;
+    id -= t.matrix * all;
+    t.split = id / s.per_matrix;
+    id -= t.split * s.per_matrix;
+    int mi, ni;
+    if (s.symmetric) {
+        mi = 0;
+        for (;;) {
+            const int across = min(s.tiles_n, ((mi + 1) * kMatmulRows + COLUMNS - 1) / COLUMNS);
+            if (id < across) break;
+            id -= across;
+            ++mi;
+        }
+        ni = id;
+    } else {
+        // bands of 8 tiles down, so that the tiles that run at a time share operands in L2
+        const int band = 8 * s.tiles_n, first = id / band * 8, high = min(8, s.tiles_m - first), in_band = id - id / band * band;
+        mi = first + in_band % high;
+        ni = in_band / high;
+    }
+    t.row = mi * kMatmulRows;
+    t.col = ni * COLUMNS;
+    return t;
+}
+
+static __device__ int g_matmul_async_error = 0;   // set when a bounded wait ran out; read by matmul_async_error()
+
+// Persistent: every CTA takes tiles blockIdx.x, blockIdx.x + gridDim.x, ...; the copies run ahead across tiles, and the epilogue of a
+// tile runs beside the products of the next where tensor memory holds two.  All waits are bounded; when one runs out, the error flag is
+// raised and every role leaves, the copies that are in flight waited for.
+template <int PLANES, int COLUMNS, class Epilogue>
+__global__ void __launch_bounds__(kMatmulThreads, 1)
+matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MatmulShape s, const Epilogue epilogue) {
+    using Config = MatmulConfig<PLANES, COLUMNS>;
+    constexpr int kStages = Config::kStages;
+    constexpr int kPlaneA = kMatmulRows * kChunk * 2, kPlaneB = COLUMNS * kChunk * 2;
+    extern __shared__ uint8_t s_raw[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
+    float *staging = reinterpret_cast<float *>(ring + kStages * Config::kStepBytes);
+    uint64_t *full = reinterpret_cast<uint64_t *>(staging + 4 * 32 * kStagePitch), *empty = full + kStages, *sums_full = empty + kStages,
+             *sums_empty = sums_full + 2, *drained = sums_empty + 2;
+    uint32_t *s_tensor = reinterpret_cast<uint32_t *>(drained + 1);
+    volatile uint32_t *s_failed = s_tensor + 1;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(sums_full + i, 1);
+            mbar_init(sums_empty + i, 4);
+        }
+        mbar_init(drained, 1);
+        *s_failed = 0;
+        mbar_fence_init();
+    }
+    if (warp == 5) tensor_alloc(s_tensor, Config::kTensorColumns);
+    if (warp == 4 && lane == 0) {
+        map_prefetch(&map_a);
+        map_prefetch(&map_b);
+    }
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tensor = *s_tensor;
+    grid_dependency_wait();
+    grid_dependents_launch();
+
+    if (warp == 4) {
+        if (lane == 0) {
+            int stage = 0, used = 0;   // used: stages with a copy issued
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int id = blockIdx.x; id < s.tiles && ok; id += gridDim.x) {
+                const Tile t = tile_of<COLUMNS>(id, s);
+                const int first = t.split * s.steps_per_split, last = min(s.k_steps, first + s.steps_per_split);
+                for (int step = first; step < last; ++step) {
+                    ok = mbar_wait(empty + stage, phase ^ 1) && !*s_failed;
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(full + stage, Config::kStepBytes);
+                    uint8_t *at = ring + stage * Config::kStepBytes;
+                    const int k = step * kChunk;
+#pragma unroll 1
+                    for (int p = 0; p < PLANES; ++p) {
+                        const int z = t.matrix * s.planes_z + p;
+#pragma unroll
+                        for (int c = 0; c < kMatmulRows / kChunk; ++c, at += kChunkBytes) {
+                            const int row = t.row + c * kChunk;
+                            tile_load(at, &map_a, s.a_mn ? row : k, s.a_mn ? k : row, z, full + stage);
+                        }
+                    }
+#pragma unroll 1
+                    for (int p = 0; p < PLANES; ++p) {
+                        const int z = t.matrix * s.planes_z + p;
+#pragma unroll
+                        for (int c = 0; c < COLUMNS / kChunk; ++c, at += kChunkBytes) {
+                            const int col = t.col + c * kChunk;
+                            tile_load(at, &map_b, s.b_mn ? col : k, s.b_mn ? k : col, z, full + stage);
+                        }
+                    }
+                    used = max(used, stage + 1);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            if (!ok) {
+                *s_failed = 1;
+                g_matmul_async_error = 1;
+            }
+            // nothing of a CTA's copies is in flight when it ends: the latest copy into each stage
+            for (int i = 0; i < used; ++i) mbar_wait(full + i, i < stage ? phase : phase ^ 1);
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            int stage = 0, buffer = 0;
+            uint32_t phase = 0, buffer_phase = 0;
+            bool ok = true;
+            const uint32_t a_step = s.a_mn ? 2048 >> 4 : 32 >> 4, b_step = s.b_mn ? 2048 >> 4 : 32 >> 4;
+            for (int id = blockIdx.x; id < s.tiles && ok; id += gridDim.x) {
+                const Tile t = tile_of<COLUMNS>(id, s);
+                const int first = t.split * s.steps_per_split, last = min(s.k_steps, first + s.steps_per_split);
+                ok = mbar_wait(sums_empty + buffer, buffer_phase ^ 1) && !*s_failed;
+                if (!ok) break;
+                tensor_fence_after();
+                const uint32_t large = tensor + buffer * Config::kSums * COLUMNS, small = large + COLUMNS;
+                for (int step = first; step < last; ++step) {
+                    ok = mbar_wait(full + stage, phase) && !*s_failed;
+                    if (!ok) break;
+                    tensor_fence_after();
+                    const uint32_t at = smem_addr(ring + stage * Config::kStepBytes);
+                    const uint64_t a = operand_descriptor(at), b = operand_descriptor(at + PLANES * kPlaneA);
+                    const auto product = [&](int pa, int pb, uint32_t sum, bool fresh) {
+                        const uint64_t from_a = a + pa * (kPlaneA >> 4), from_b = b + pb * (kPlaneB >> 4);
+#pragma unroll
+                        for (int k = 0; k < kChunk / 16; ++k)
+                            tensor_multiply(sum, from_a + k * a_step, from_b + k * b_step, s.instruction, !(fresh && k == 0));
+                    };
+                    const bool fresh = step == first;
+                    product(0, 0, large, fresh);
+                    if (PLANES > 1) {
+                        product(0, 1, small, fresh);
+                        product(1, 0, small, false);
+                    }
+                    if (PLANES > 2) {
+                        product(1, 1, small, false);
+                        product(0, 2, small, false);
+                        product(2, 0, small, false);
+                    }
+                    tensor_commit(empty + stage);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (!ok) break;
+                tensor_commit(sums_full + buffer);
+                if (++buffer == Config::kBuffers) {
+                    buffer = 0;
+                    buffer_phase ^= 1;
+                }
+            }
+            if (!ok) {
+                *s_failed = 1;
+                g_matmul_async_error = 1;
+                tensor_commit(drained);   // tensor memory is given back when nothing writes it any more
+                mbar_wait(drained, 0);
+            }
+        }
+    } else {
+        float *mine = staging + warp * 32 * kStagePitch;
+        int buffer = 0;
+        uint32_t buffer_phase = 0;
+        for (int id = blockIdx.x; id < s.tiles; id += gridDim.x) {
+            const Tile t = tile_of<COLUMNS>(id, s);
+            if (!mbar_wait(sums_full + buffer, buffer_phase) || *s_failed) {
+                *s_failed = 1;
+                g_matmul_async_error = 1;
+                break;
+            }
+            __syncwarp();
+            tensor_fence_after();
+            const uint32_t sums = tensor + buffer * Config::kSums * COLUMNS + ((uint32_t)warp * 32 << 16);
+            const int row0 = t.row + warp * 32, slice = t.split * s.batch + t.matrix;
+#pragma unroll 1
+            for (int c0 = 0; c0 < COLUMNS && t.col + c0 < s.n; c0 += 32) {
+                uint32_t bits[32];
+                float v[32];
+                tensor_read32(sums + c0, bits);
+                tensor_read_wait();
+#pragma unroll
+                for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(bits[c]);
+                if (Config::kSums == 2) {
+                    tensor_read32(sums + COLUMNS + c0, bits);
+                    tensor_read_wait();
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) v[c] += __uint_as_float(bits[c]);
+                }
+                const int col0 = t.col + c0;
+                if (epilogue.by_column(row0, col0)) {
+                    const int row = row0 + lane;
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (row < s.m && col0 + c < s.n) epilogue.one(slice, row, col0 + c, v[c]);
+                }
+                if (epilogue.by_row(row0, col0)) {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4)
+                        *reinterpret_cast<float4 *>(mine + lane * kStagePitch + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = i * 4 + lane / 8, c = lane % 8 * 4;
+                        const float4 f = *reinterpret_cast<const float4 *>(mine + r * kStagePitch + c);
+                        const int row = row0 + r, col = col0 + c;
+                        const float four[4] = {f.x, f.y, f.z, f.w};
+                        if (row < s.m && col < s.n) epilogue.four(slice, row, col, four, min(4, s.n - col));
+                    }
+                    __syncwarp();
+                }
+            }
+            tensor_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sums_empty + buffer);
+            if (++buffer == Config::kBuffers) {
+                buffer = 0;
+                buffer_phase ^= 1;
+            }
+        }
+    }
+    __syncwarp();
+    tensor_fence_before();
+    __syncthreads();
+    if (warp == 5) tensor_free(tensor, Config::kTensorColumns);
+}
+
+// Sums of a product that was split along k: kept as they are, added up in the order of the splits by matmul_join_kernel.
+struct StorePartial {
+    float *out;
+    int64_t n, matrix;   // values of a row, of a matrix
+    __device__ __forceinline__ bool by_column(int, int) const { return false; }
+    __device__ __forceinline__ bool by_row(int, int) const { return true; }
+    __device__ __forceinline__ void one(int, int, int, float) const {}
+    __device__ __forceinline__ void four(int slice, int row, int col, const float (&v)[4], int valid) const {
+        store4(out, slice * matrix + (int64_t)row * n + col, kFloat32, valid, v);
+    }
+};
+
+template <class Epilogue>
+__global__ void __launch_bounds__(kThreads)
+matmul_join_kernel(const float *__restrict__ partial, int splits, int batch, int m, int n, int symmetric, const Epilogue epilogue) {
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const int64_t quads = (n + 3) / 4, matrix = (int64_t)m * n, total = quads * m * batch;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+        const bool columns = epilogue.by_column(0, 0) && !symmetric;
+        int64_t rest = i;
+        int row, quad;
+        if (columns) {   // neighbouring threads write neighbouring rows
+            row = (int)(rest % m);
+            rest /= m;
+            quad = (int)(rest % quads);
+            rest /= quads;
+        } else {
+            quad = (int)(rest % quads);
+            rest /= quads;
+            row = (int)(rest % m);
+            rest /= m;
+        }
+        const int z = (int)rest, col = quad * 4, valid = min(4, n - col);
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        const bool mirrored = symmetric && col / kMatmulRows > row / kMatmulRows;   // a multiple of 4 columns: all of a quad alike
+        for (int sp = 0; sp < splits; ++sp) {
+            const float *p = partial + ((int64_t)sp * batch + z) * matrix;
+            float f[4];
+            if (mirrored) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[j] = j < valid ? p[(int64_t)(col + j) * n + row] : 0.f;
+            } else {
+                load4(p, (int64_t)row * n + col, kFloat32, valid, f);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += f[j];
+        }
+        if (columns) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < valid) epilogue.one(z, row, col + j, v[j]);
+        } else {
+            epilogue.four(z, row, col, v, valid);
+        }
+    }
+}
+#endif  // __CUDACC__
+
+}  // namespace dl

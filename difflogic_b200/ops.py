@@ -8,7 +8,11 @@ Layouts: float activations are feature-major `[features, batch]` contiguous; pac
 activations are `[features, words]`; indices are int64, as LogicLayer stores them.
 """
 import collections
+import ctypes
+import functools
+import math
 
+import numpy as np
 import torch
 
 from . import _native as N
@@ -929,3 +933,62 @@ def groupsum_backward(grad_out, n, tau):
         N.check(N.lib().dl_groupsum_backward_f32(grad_out.data_ptr(), gx.data_ptr(), n, batch, k, float(tau),
                                                  N.stream_of(grad_out)))
     return gx
+
+
+# ------------------------------------------------------------------------------------------------
+# orthogonalised updates
+# ------------------------------------------------------------------------------------------------
+
+_FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)   # makes every singular value about 1 in five steps
+
+
+@functools.lru_cache(maxsize=64)
+def _newton_schulz(coefficients, steps):
+    """The coefficients of every step as the library takes them.  A singular value s becomes a s + b s^3 + c s^5; the iterates are kept
+    as numbers of up to 16, so coefficients that let values from [0, 1] grow past 8 on the way are refused."""
+    if isinstance(steps, bool) or not isinstance(steps, int) or not 1 <= steps <= 64:
+        raise ValueError("orthogonalize: steps must be a whole number from 1 to 64, got %r" % (steps,))
+    sets = coefficients if isinstance(coefficients[0], tuple) else (coefficients,) * steps
+    if len(sets) != steps or any(len(s) != 3 for s in sets):
+        raise ValueError("orthogonalize: three coefficients, or three for each of the %d steps" % steps)
+    values = np.linspace(0.0, 1.0, 4097)
+    for a, b, c in sets:
+        squares = values * values
+        values = np.abs(values * (a + squares * (b + c * squares)))
+        if not values.max() <= 8.0 or not max(abs(a), abs(b), abs(c)) <= 64.0:     # undefined ones too
+            raise ValueError("orthogonalize: with these coefficients the iteration does not stay near 1")
+    return (ctypes.c_float * (3 * steps))(*[v for s in sets for v in s])
+
+
+def _coefficients(coefficients):
+    return tuple(tuple(map(float, c)) if isinstance(c, (tuple, list)) else float(c) for c in coefficients)
+
+
+def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
+    """The nearest matrix to x with singular values near 1, by Newton-Schulz steps (the update of the Muon optimizer): X = x / max(|x|, eps)
+    in the Frobenius norm, then `steps` times X <- a X + b (X X^T) X + c (X X^T)^2 X.
+
+    x: `[..., rows, cols]` float32, bfloat16 or float16 on a CUDA device, every matrix on its own; the result has x's type.
+    coefficients: (a, b, c), or one such triple for each step.  The products run on the tensor cores with operands of 22 bits.  An entry
+    that is infinite or undefined makes its whole matrix undefined."""
+    N.require_cuda(x)
+    if x.dtype not in _FLOAT_TYPES:
+        raise ValueError("orthogonalize: float32, bfloat16 or float16, got %s" % x.dtype)
+    if x.dim() < 2:
+        raise ValueError("orthogonalize: a matrix or a batch of them, got %d dimensions" % x.dim())
+    if not 0 < eps < math.inf:
+        raise ValueError("orthogonalize: eps must be positive, got %r" % (eps,))
+    table = _newton_schulz(_coefficients(coefficients), steps)
+    x = x.detach().contiguous()
+    out = torch.empty_like(x)
+    rows, cols = x.shape[-2:]
+    if x.numel() == 0:
+        return out
+    batch = x.numel() // (rows * cols)
+    lib = N.lib()
+    with N.on_device(x):
+        work = torch.empty(lib.dl_orthogonalize_workspace_bytes(batch, rows, cols), dtype=torch.uint8, device=x.device)
+        N.check(lib.dl_orthogonalize(x.data_ptr(), out.data_ptr(), batch, rows, cols, _FLOAT_TYPES[x.dtype], steps, table, eps, work.data_ptr(),
+                                     N.stream_of(x)))
+    return out

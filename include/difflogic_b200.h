@@ -547,6 +547,46 @@ DL_API int dl_backward_w_announce_f32(const float *x, const int64_t *a, const in
                                       int32_t *block_ticket, int32_t *kernel_count, int kernels_in_bucket, int flags,
                                       void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Dense layers beside the logic layers, and the orthogonalised updates of their weights.  (The reference's own dense layers are
+ * torch.nn.Linear and its activations, experiments/main_baseline.py; it has no kernels for them.)
+ *
+ * type: 0 fp32, 1 bf16, 2 fp16.  Sums are 32-bit; fp32 operands are multiplied as exactly as 32-bit arithmetic does (three bf16
+ * planes), except that an infinite operand makes the results it enters undefined.
+ *
+ *   y = act(x w^T + bias) + residual
+ *
+ * x [batch][inner] with rows x_pitch values apart, or, x_feature_major, [inner][batch]; w [outer][inner] contiguous; bias [outer] and
+ * residual may be NULL, residual's strides in values.  y [batch][outer] or, y_feature_major, [outer][batch], contiguous.  slope (NULL:
+ * not wanted): act' in y's layout, fp32, or for 16-bit types fp16 times 2^14.  x_planes, w_planes: dl_dense_planes_bytes for x as it
+ * lies (rows, cols, pitch) and for w (outer, inner, inner); what is laid out there serves the backward pass.  The workspaces are
+ * 16-byte aligned.
+ *
+ *   gz = gy * slope;  gx = gz w [batch][inner],  gw = gz^T x [outer][inner],  gb = sum of gz over the batch
+ *
+ * gy contiguous in y's layout or the other one, slope (NULL: no activation) in gy's; gx, gw, gb NULL: not wanted.
+ * ---------------------------------------------------------------------------------------- */
+enum { DL_ACT_NONE = 0, DL_ACT_RELU = 1, DL_ACT_SIGMOID = 2, DL_ACT_SILU = 3, DL_ACT_GELU = 4 };
+DL_API int64_t dl_dense_planes_bytes(const void *p, int64_t rows, int64_t cols, int64_t pitch, int type);
+DL_API int64_t dl_dense_forward_workspace_bytes(int64_t batch, int64_t inner, int64_t outer, int type);
+DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_feature_major, const void *w, const void *bias, const void *residual,
+                            int64_t residual_batch, int64_t residual_feature, int act, void *y, int y_feature_major, void *slope,
+                            void *x_planes, void *w_planes, void *workspace, int64_t batch, int64_t inner, int64_t outer, int type,
+                            void *stream);
+DL_API int64_t dl_dense_backward_workspace_bytes(int64_t batch, int64_t inner, int64_t outer, int g_feature_major, int type, int has_slope,
+                                                 const void *gy);
+DL_API int dl_dense_backward(const void *gy, int g_feature_major, const void *slope, const void *x, int64_t x_pitch, int x_feature_major,
+                             const void *w, const void *x_planes, const void *w_planes, void *gx, void *gw, void *gb, void *workspace,
+                             int64_t batch, int64_t inner, int64_t outer, int type, void *stream);
+
+/* X = G / max(|G|_F, eps), then for each step with its (a, b, c) in `coefficients` (steps x 3, on the host)
+ *   X <- a X + b (X X^T) X + c (X X^T)^2 X
+ * for `batch` contiguous matrices rows x cols; out in G's type.  The iterates are kept to 22 bits (fp16 pairs times 2^12: values up to
+ * 16), sums in 32 bits. */
+DL_API int64_t dl_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
+DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, int64_t rows, int64_t cols, int type, int steps,
+                            const float *coefficients, double eps, void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
