@@ -20,7 +20,7 @@ DL_OK, DL_ERR_INVALID_ARG, DL_ERR_BAD_BIT_COUNT, DL_ERR_NOT_DIVISIBLE, DL_ERR_CU
 W_LOGITS, W_PROBS, W_ARGMAX = 0, 1, 2
 LAUNCH_PLAIN, LAUNCH_OVERLAP_SETUP = 0, 1
 (TUNE_NO_PDL, TUNE_EVAL_KERNEL, TUNE_EVAL_SHAPE, TUNE_GROUPBITSUM_KERNEL, TUNE_GROUPSUM_KERNEL, TUNE_FUSED_CLUSTER,
- TUNE_FORWARD_KERNEL, TUNE_WALK_KERNEL) = range(8)
+ TUNE_FORWARD_KERNEL, TUNE_WALK_KERNEL, TUNE_MATMUL_COLUMNS, TUNE_MATMUL_SPLITS) = range(10)
 
 # name -> (restype, argtypes); mirrors include/difflogic_b200.h one to one
 SIGNATURES = {
@@ -113,7 +113,7 @@ SIGNATURES = {
                                 _int, _ptr]),
     "dl_dense_backward_workspace_bytes": (_i64, [_i64, _i64, _i64, _int, _int, _int, _ptr]),
     "dl_dense_backward": (_int, [_ptr, _int, _ptr, _ptr, _i64, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _int, _ptr]),
-    "dl_orthogonalize_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "dl_orthogonalize_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
     "dl_orthogonalize": (_int, [_ptr, _ptr, _i64, _i64, _i64, _int, _int, _ptr, ctypes.c_double, _ptr, _ptr]),
     "dl_prefetch_l2": (_int, [_ptr, ctypes.c_size_t, _ptr]),
 }

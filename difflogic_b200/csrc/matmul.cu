@@ -48,13 +48,17 @@ bool make_tile_map(CUtensorMap *map, const void *base, bool bfloat, int64_t inne
 struct Product {
     Operand a, b;
     int64_t m, n, k, batch;
-    int planes;
+    int planes, planes_z;   // multiplied; per matrix in memory
     bool bfloat, symmetric;
+    int steps_per_sum;   // 0: a sum stays in tensor memory for the whole product
 };
+
+// Steps of 64 after which sums are taken out of tensor memory: results of 22 or 24 bits.
+constexpr int kExactSteps = 2;
 
 static bool map_operand(CUtensorMap *map, const Operand &o, const Product &p, int64_t rows) {
     const int64_t inner = o.mn ? rows : p.k, outer = o.mn ? p.k : rows;
-    return make_tile_map(map, o.base, p.bfloat, inner, outer, p.planes * p.batch, o.pitch * 2, o.plane * 2);
+    return make_tile_map(map, o.base, p.bfloat, inner, outer, p.planes_z * p.batch, o.pitch * 2, o.plane * 2);
 }
 
 template <int PLANES, int COLUMNS, class Epilogue>
@@ -63,7 +67,7 @@ static int launch_tiles(const Product &p, const MatmulShape &shape, const CUtens
     auto kernel = matmul_kernel<PLANES, COLUMNS, Epilogue>;
     constexpr int kShared = MatmulConfig<PLANES, COLUMNS>::kSharedBytes;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared) != cudaSuccess) return launch_status(what);
-    launch_dependent(true, kernel, dim3((unsigned)(shape.tiles < sms ? shape.tiles : sms)), dim3(kMatmulThreads), kShared, st, a, b, shape,
+    launch_dependent(true, kernel, dim3((unsigned)(shape.tiles < sms ? shape.tiles : sms)), dim3(MatmulConfig<PLANES, COLUMNS>::kThreadsAll), kShared, st, a, b, shape,
                      epilogue);
     return launch_status(what);
 }
@@ -77,12 +81,13 @@ static int launch_columns(const Product &p, const MatmulPlan &plan, const Epilog
     s.m = (int32_t)p.m;
     s.n = (int32_t)p.n;
     s.batch = (int32_t)p.batch;
-    s.planes_z = p.planes;
+    s.planes_z = p.planes_z;
     s.tiles_m = (int32_t)ceil_div(p.m, kMatmulRows);
     s.tiles_n = (int32_t)ceil_div(p.n, plan.columns);
     s.splits = plan.splits;
     s.k_steps = (int32_t)ceil_div(p.k, kChunk);
     s.steps_per_split = plan.steps_per_split;
+    s.steps_per_sum = PLANES > 1 && p.steps_per_sum > 0 ? p.steps_per_sum : s.k_steps;   // one plane: nothing adds blocks up
     s.symmetric = p.symmetric;
     int64_t per_matrix = (int64_t)s.tiles_m * s.tiles_n;
     if (p.symmetric) {
@@ -120,6 +125,13 @@ static int launch_product(const Product &p, const MatmulPlan &plan, const Epilog
     return launch_status(what);
 }
 
+// Dense layers multiply one plane or three, the iterations one or two.
+template <class Epilogue>
+static int launch_planes(const Product &p, const MatmulPlan &plan, const Epilogue &e, float *partial, int sms, cudaStream_t st, const char *what) {
+    constexpr int kMore = Epilogue::kPlanes;
+    return p.planes == 1 ? launch_product<1>(p, plan, e, partial, sms, st, what) : launch_product<kMore>(p, plan, e, partial, sms, st, what);
+}
+
 // Values of a row of planes that the library lays out: whole units of 16 bytes.
 static int64_t padded(int64_t n) { return ceil_div(n, 8) * 8; }
 static int64_t padded_bytes(int64_t n) { return ceil_div(n, 256) * 256; }
@@ -130,93 +142,141 @@ static int64_t padded_bytes(int64_t n) { return ceil_div(n, 256) * 256; }
 // layer's own type may have 8, and down to 4e-12, where sigmoids saturate.
 constexpr float kSlopeScale = 16384.f;
 
-__device__ __forceinline__ float activate(float z, int act, float &slope) {
+// act(z) in place, and its derivatives, four at a time.
+template <int N>
+__device__ __forceinline__ void activate(float (&z)[N], float (&slope)[N], int act) {
     if (act == DL_ACT_NONE) {
-        slope = 1.f;
-        return z;
+#pragma unroll
+        for (int j = 0; j < N; ++j) slope[j] = 1.f;
+    } else if (act == DL_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            slope[j] = z[j] > 0.f ? 1.f : 0.f;
+            z[j] = z[j] > 0.f || z[j] != z[j] ? z[j] : 0.f;
+        }
+    } else if (act == DL_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float phi = 0.5f * (1.f + erff(z[j] * 0.70710678118654752f));
+            // far out the density is zero, and infinity times zero would not be
+            slope[j] = phi + (fabsf(z[j]) > 15.f ? 0.f : z[j] * expf(-0.5f * z[j] * z[j]) * 0.39894228040143268f);
+            z[j] = z[j] == -INFINITY ? 0.f : z[j] * phi;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float s = __fdividef(1.f, 1.f + expf(-z[j]));   // zero below -88, where expf overflows
+            slope[j] = s * (1.f - s);
+            if (act == DL_ACT_SIGMOID) {
+                z[j] = s;
+            } else {
+                slope[j] = s + (slope[j] == 0.f ? 0.f : z[j] * slope[j]);
+                z[j] = z[j] == -INFINITY ? 0.f : z[j] * s;
+            }
+        }
     }
-    if (act == DL_ACT_RELU) {
-        slope = z > 0.f ? 1.f : 0.f;
-        return z > 0.f || z != z ? z : 0.f;
-    }
-    if (act == DL_ACT_GELU) {
-        const float phi = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-        // far out z times an exp(-z^2 / 2) of zero is zero, infinity times it would not be
-        slope = phi + (fabsf(z) > 15.f ? 0.f : z * expf(-0.5f * z * z) * 0.39894228040143268f);
-        return z == -INFINITY ? 0.f : z * phi;
-    }
-    const float s = 1.f / (1.f + expf(-z));
-    if (act == DL_ACT_SIGMOID) {
-        slope = s * (1.f - s);
-        return s;
-    }
-    // expf(-z) overflows below -88.7: s is zero there, and so is the product with a finite z
-    slope = s * (1.f + (s == 0.f || s == 1.f ? 0.f : z * (1.f - s)));
-    return z == -INFINITY ? 0.f : z * s;
 }
 
 // y = act(sum + bias) + residual.  rows_are_features: the rows of the product are the layer's outputs, else its columns are; the result
 // lies [batch][feature] or, feature_major, [feature][batch].
 struct DenseEpilogue {
+    static constexpr int kPlanes = 3;
     void *y;
     const void *bias, *residual;
     void *slope;
-    int64_t y_pitch, residual_batch, residual_feature;   // of the residual: values to the next sample, to the next feature
+    int64_t y_pitch, residual_row, residual_col;   // of the residual: values to the product's next row, to its next column
     int type, act;
     bool rows_are_features, feature_major;
 
     // Neighbouring columns of the product are neighbours in memory, or neighbouring rows are.
-    __device__ __forceinline__ bool across() const { return rows_are_features == feature_major; }
-    __device__ __forceinline__ bool by_column(int, int) const { return !across(); }
-    __device__ __forceinline__ bool by_row(int, int) const { return across(); }
+    __device__ __forceinline__ bool by_column(int, int) const { return rows_are_features != feature_major; }
+    __device__ __forceinline__ bool by_row(int, int) const { return rows_are_features == feature_major; }
 
-    __device__ __forceinline__ float value(int64_t sample, int64_t feature, float z, float &slope_of) const {
-        if (bias != nullptr) z += load_as_float(bias, feature, type);
-        float v = activate(z, act, slope_of);
-        if (residual != nullptr) v += load_as_float(residual, sample * residual_batch + feature * residual_feature, type);
-        return v;
-    }
-    __device__ __forceinline__ void one(int, int row, int col, float sum) const {
-        const int64_t sample = rows_are_features ? col : row, feature = rows_are_features ? row : col;
-        float d;
-        const float v = value(sample, feature, sum, d);
-        const int64_t i = feature_major ? feature * y_pitch + sample : sample * y_pitch + feature;
-        if (type == kFloat32) {
-            reinterpret_cast<float *>(y)[i] = v;
-            if (slope != nullptr) reinterpret_cast<float *>(slope)[i] = d;
-        } else {
-            reinterpret_cast<uint16_t *>(y)[i] = to_16bit(v, type);
-            if (slope != nullptr) reinterpret_cast<uint16_t *>(slope)[i] = to_16bit(d * kSlopeScale, kFloat16);
+    template <int N>
+    __device__ __forceinline__ void down(int, int row, int col, const float (&sum)[N], int m, int valid) const {
+        if (row >= m) return;
+        const float row_bias = bias != nullptr && rows_are_features ? load_as_float(bias, row, type) : 0.f;
+        float v[N], d[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            v[j] = sum[j] + row_bias;
+            if (bias != nullptr && !rows_are_features && j < valid) v[j] += load_as_float(bias, col + j, type);
+        }
+        activate(v, d, act);
+        if (residual != nullptr) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < valid) v[j] += load_as_float(residual, row * residual_row + (col + j) * residual_col, type);
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (j >= valid) continue;
+            const int64_t i = (col + j) * y_pitch + row;
+            if (type == kFloat32) reinterpret_cast<float *>(y)[i] = v[j];
+            else reinterpret_cast<uint16_t *>(y)[i] = to_16bit(v[j], type);
+            if (slope != nullptr) {
+                if (type == kFloat32) reinterpret_cast<float *>(slope)[i] = d[j];
+                else reinterpret_cast<uint16_t *>(slope)[i] = to_16bit(d[j] * kSlopeScale, kFloat16);
+            }
         }
     }
-    __device__ __forceinline__ void four(int, int row, int col, const float (&sum)[4], int valid) const {
-        float v[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
+    template <int N, int STEP>
+    __device__ __forceinline__ void across(int, int row, int col, const float (&sum)[N][4], int m, int valid) const {
+        float col_bias[4] = {0.f, 0.f, 0.f, 0.f}, more[N][4];
+        if (bias != nullptr && !rows_are_features) load4(bias, col, type, valid, col_bias);
+        if (residual != nullptr) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < valid)
-                v[j] = value(rows_are_features ? col + j : row, rows_are_features ? row : col + j, sum[j], d[j]);
-        const int64_t i = (int64_t)row * y_pitch + col;
-        store4(y, i, type, valid, v);
-        if (slope != nullptr) {
-            if (type != kFloat32) {
+            for (int i = 0; i < N; ++i) {
+                const int r = row + i * STEP;
+                if (residual_col == 1) {
+                    load4(residual, r * residual_row + col, type, r < m ? valid : 0, more[i]);
+                } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) d[j] *= kSlopeScale;
+                    for (int j = 0; j < 4; ++j) more[i][j] = r < m && j < valid ? load_as_float(residual, r * residual_row + (col + j) * residual_col, type) : 0.f;
+                }
             }
-            store4(slope, i, type == kFloat32 ? kFloat32 : kFloat16, valid, d);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = row + i * STEP;
+            if (r >= m) break;
+            const float row_bias = bias != nullptr && rows_are_features ? load_as_float(bias, r, type) : 0.f;
+            float v[4], d[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = sum[i][j] + (rows_are_features ? row_bias : col_bias[j]);
+            activate(v, d, act);
+            if (residual != nullptr) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += more[i][j];
+            }
+            const int64_t at = r * y_pitch + col;
+            store4(y, at, type, valid, v);
+            if (slope != nullptr) {
+                if (type != kFloat32) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) d[j] *= kSlopeScale;
+                }
+                store4(slope, at, type == kFloat32 ? kFloat32 : kFloat16, valid, d);
+            }
         }
     }
 };
 
 // Gradients: the sums as they are, in the layer's type.
 struct PlainEpilogue {
+    static constexpr int kPlanes = 3;
     void *out;
     int64_t pitch;
     int type;
     __device__ __forceinline__ bool by_column(int, int) const { return false; }
     __device__ __forceinline__ bool by_row(int, int) const { return true; }
-    __device__ __forceinline__ void one(int, int, int, float) const {}
-    __device__ __forceinline__ void four(int, int row, int col, const float (&sum)[4], int valid) const {
-        store4(out, row * pitch + col, type, valid, sum);
+    template <int N>
+    __device__ __forceinline__ void down(int, int, int, const float (&)[N], int, int) const {}
+    template <int N, int STEP>
+    __device__ __forceinline__ void across(int, int row, int col, const float (&sum)[N][4], int m, int valid) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (row + i * STEP < m) store4(out, (row + i * STEP) * pitch + col, type, valid, sum[i]);
     }
 };
 
@@ -358,11 +418,6 @@ static int lay_out(const void *src, int64_t rows, int64_t cols, int64_t pitch, i
     return launch_status(what);
 }
 
-template <class Epilogue>
-static int launch_planes(const Product &p, const MatmulPlan &plan, const Epilogue &e, float *partial, int sms, cudaStream_t st, const char *what) {
-    return p.planes == 3 ? launch_product<3>(p, plan, e, partial, sms, st, what) : launch_product<1>(p, plan, e, partial, sms, st, what);
-}
-
 // The layer's outputs are the rows of the product where that leaves fewer of a tile's 128 rows and 64 columns empty.
 static bool features_as_rows(int64_t batch, int64_t outer) { return batch < outer && batch < 256; }
 
@@ -423,8 +478,8 @@ extern "C" DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_fea
     cudaStream_t st = as_stream(stream);
     if (l.lay_x && (status = lay_out(x, l.x_rows, l.x_cols, x_pitch, type, x_planes, l.x_plane_pitch, l.x_plane, sms, st, what)) != DL_OK) return status;
     if (l.lay_w && (status = lay_out(w, outer, inner, inner, type, w_planes, l.w_plane_pitch, l.w_plane, sms, st, what)) != DL_OK) return status;
-    const Operand ox = {l.lay_x ? x_planes : x, l.lay_x ? l.x_plane_pitch : x_pitch, l.x_plane, 0, x_feature_major != 0};
-    const Operand ow = {l.lay_w ? w_planes : w, l.lay_w ? l.w_plane_pitch : inner, l.w_plane, 0, false};
+    const Operand ox = {l.lay_x ? x_planes : x, l.lay_x ? l.x_plane_pitch : x_pitch, l.x_plane, x_feature_major != 0};
+    const Operand ow = {l.lay_w ? w_planes : w, l.lay_w ? l.w_plane_pitch : inner, l.w_plane, false};
     const bool rows_are_features = features_as_rows(batch, outer);
     Product p = {};
     p.a = rows_are_features ? ow : ox;
@@ -433,10 +488,11 @@ extern "C" DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_fea
     p.n = rows_are_features ? batch : outer;
     p.k = inner;
     p.batch = 1;
-    p.planes = l.planes;
+    p.planes = p.planes_z = l.planes;
     p.bfloat = type != kFloat16;
-    const DenseEpilogue e = {y, bias, residual, slope, y_feature_major ? batch : outer, residual_batch, residual_feature, type, act,
-                             rows_are_features, y_feature_major != 0};
+    p.steps_per_sum = kExactSteps;
+    const DenseEpilogue e = {y, bias, residual, slope, y_feature_major ? batch : outer, rows_are_features ? residual_feature : residual_batch,
+                             rows_are_features ? residual_batch : residual_feature, type, act, rows_are_features, y_feature_major != 0};
     return launch_planes(p, plan, e, reinterpret_cast<float *>(workspace), sms, st, what);
 }
 
@@ -507,15 +563,16 @@ extern "C" DL_API int dl_dense_backward(const void *gy, int g_feature_major, con
                          outer, gb, type);
         if ((status = launch_status(what)) != DL_OK) return status;
     }
-    Operand g = {b.lay_gz ? (const void *)gz : gy, b.lay_gz ? b.g_pitch : b.g_cols, b.g_plane, 0, false};
+    Operand g = {b.lay_gz ? (const void *)gz : gy, b.lay_gz ? b.g_pitch : b.g_cols, b.g_plane, false};
     Product p = {};
     p.batch = 1;
-    p.planes = b.planes;
+    p.planes = p.planes_z = b.planes;
     p.bfloat = type != kFloat16;
+    p.steps_per_sum = kExactSteps;
     if (gx) {   // gz [batch][outer] w [outer][inner], summed over the outputs
         p.a = g;
         p.a.mn = g_feature_major != 0;
-        p.b = {l.lay_w ? w_planes : w, l.lay_w ? l.w_plane_pitch : inner, l.w_plane, 0, true};
+        p.b = {l.lay_w ? w_planes : w, l.lay_w ? l.w_plane_pitch : inner, l.w_plane, true};
         p.m = batch;
         p.n = inner;
         p.k = outer;
@@ -524,7 +581,7 @@ extern "C" DL_API int dl_dense_backward(const void *gy, int g_feature_major, con
     if (gw) {   // gz^T x, summed over the batch
         p.a = g;
         p.a.mn = g_feature_major == 0;
-        p.b = {l.lay_x ? x_planes : x, l.lay_x ? l.x_plane_pitch : x_pitch, l.x_plane, 0, x_feature_major == 0};
+        p.b = {l.lay_x ? x_planes : x, l.lay_x ? l.x_plane_pitch : x_pitch, l.x_plane, x_feature_major == 0};
         p.m = outer;
         p.n = inner;
         p.k = batch;
@@ -593,70 +650,111 @@ normalise_kernel(const void *__restrict__ g, int64_t rows, int64_t cols, int typ
     }
 }
 
-// Results of the iteration as pairs: v = scale * sum (+ b * gram + a on the diagonal).
+// Results of the iteration as pairs: v = scale * sum (+ factor * the pair in `more`) (+ diagonal on the diagonal).
 struct PairEpilogue {
+    static constexpr int kPlanes = 2;
     uint16_t *out;
-    const uint16_t *gram;   // null: none
-    int64_t pitch, plane;   // of out and gram
-    float scale, b, diagonal;
+    const uint16_t *more;   // laid out as `out`; null: none
+    int64_t pitch, plane;
+    float scale, factor, diagonal;
     bool symmetric;
 
     __device__ __forceinline__ bool by_column(int row, int col) const { return symmetric && col / kMatmulRows < row / kMatmulRows; }
     __device__ __forceinline__ bool by_row(int row, int col) const { return !symmetric || col / kMatmulRows <= row / kMatmulRows; }
-    __device__ __forceinline__ void one(int z, int row, int col, float sum) const {   // the mirrored value
-        const int64_t i = 2 * z * plane + (int64_t)col * pitch + row;
-        float v = sum * scale;
-        if (gram != nullptr) v += b * join_pair(gram[i], gram[i + plane]);
-        uint16_t hi, lo;
-        split_pair(v, hi, lo);
-        out[i] = hi;
-        out[i + plane] = lo;
-    }
-    __device__ __forceinline__ void four(int z, int row, int col, const float (&sum)[4], int valid) const {
-        // rows are padded to whole units: the values behind the last one are written too, and read by nothing
-        const int64_t i = 2 * z * plane + (int64_t)row * pitch + col;
-        uint16_t hi[4], lo[4];
-        ushort4 gh = make_ushort4(0, 0, 0, 0), gl = gh;
-        if (gram != nullptr) {
-            gh = *reinterpret_cast<const ushort4 *>(gram + i);
-            gl = *reinterpret_cast<const ushort4 *>(gram + i + plane);
-        }
-        const uint16_t g_hi[4] = {gh.x, gh.y, gh.z, gh.w}, g_lo[4] = {gl.x, gl.y, gl.z, gl.w};
+    template <int N>
+    __device__ __forceinline__ void down(int z, int row, int col, const float (&sum)[N], int m, int valid) const {   // the mirrored values
+        if (row >= m) return;
+        const int64_t first = 2 * z * plane + (int64_t)col * pitch + row;
+        float v[N];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float v = sum[j] * scale;
-            if (gram != nullptr) v += b * join_pair(g_hi[j], g_lo[j]);
-            if (row == col + j) v += diagonal;
-            split_pair(v, hi[j], lo[j]);
+        for (int j = 0; j < N; ++j) v[j] = sum[j] * scale;
+        if (more != nullptr) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < valid) v[j] += factor * join_pair(more[first + j * pitch], more[first + j * pitch + plane]);
         }
-        *reinterpret_cast<ushort4 *>(out + i) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<ushort4 *>(out + i + plane) = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (j < valid) split_pair(v[j], out[first + j * pitch], out[first + j * pitch + plane]);
+    }
+    template <int N, int STEP>
+    __device__ __forceinline__ void across(int z, int row, int col, const float (&sum)[N][4], int m, int) const {
+        // rows are padded to whole units: the values behind the last one are written too, and read by nothing
+        const int64_t first = 2 * z * plane + (int64_t)row * pitch + col;
+        float v[N][4];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i][j] = sum[i][j] * scale + (row + i * STEP == col + j ? diagonal : 0.f);
+        if (more != nullptr) {
+            ushort4 hi[N], lo[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (row + i * STEP >= m) continue;
+                hi[i] = *reinterpret_cast<const ushort4 *>(more + first + i * STEP * pitch);
+                lo[i] = *reinterpret_cast<const ushort4 *>(more + first + i * STEP * pitch + plane);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (row + i * STEP >= m) continue;
+                v[i][0] += factor * join_pair(hi[i].x, lo[i].x);
+                v[i][1] += factor * join_pair(hi[i].y, lo[i].y);
+                v[i][2] += factor * join_pair(hi[i].z, lo[i].z);
+                v[i][3] += factor * join_pair(hi[i].w, lo[i].w);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (row + i * STEP >= m) continue;
+            uint16_t hi[4], lo[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) split_pair(v[i][j], hi[j], lo[j]);
+            *reinterpret_cast<ushort4 *>(out + first + i * STEP * pitch) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<ushort4 *>(out + first + i * STEP * pitch + plane) = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+        }
     }
 };
 
 // The last product: the result itself, or the weights' update w <- decay w - rate v.
 struct OrthogonalEpilogue {
+    static constexpr int kPlanes = 2;
     void *out;
     int64_t cols, matrix;   // values of a row, of a matrix
+    const uint16_t *more;   // added, as in PairEpilogue
+    int64_t pitch, plane;
+    float scale, factor;
     int type;
-    float scale;
     bool update;
     float decay, rate;
     __device__ __forceinline__ bool by_column(int, int) const { return false; }
     __device__ __forceinline__ bool by_row(int, int) const { return true; }
-    __device__ __forceinline__ void one(int, int, int, float) const {}
-    __device__ __forceinline__ void four(int z, int row, int col, const float (&sum)[4], int valid) const {
-        const int64_t i = z * matrix + row * cols + col;
-        float v[4];
-        if (update) {
-            load4(out, i, kFloat32, valid, v);
+    template <int N>
+    __device__ __forceinline__ void down(int, int, int, const float (&)[N], int, int) const {}
+    template <int N, int STEP>
+    __device__ __forceinline__ void across(int z, int row, int col, const float (&sum)[N][4], int m, int valid) const {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = v[j] * decay - rate * (sum[j] * scale);
-        } else {
+        for (int i = 0; i < N; ++i) {
+            const int r = row + i * STEP;
+            if (r >= m) break;
+            const int64_t at = z * matrix + r * cols + col;
+            float v[4], w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = sum[j] * scale;
+            for (int j = 0; j < 4; ++j) v[j] = sum[i][j] * scale;
+            if (more != nullptr) {
+                const int64_t from = 2 * z * plane + r * pitch + col;
+                const ushort4 hi = *reinterpret_cast<const ushort4 *>(more + from), lo = *reinterpret_cast<const ushort4 *>(more + from + plane);
+                v[0] += factor * join_pair(hi.x, lo.x);
+                v[1] += factor * join_pair(hi.y, lo.y);
+                v[2] += factor * join_pair(hi.z, lo.z);
+                v[3] += factor * join_pair(hi.w, lo.w);
+            }
+            if (update) {
+                load4(out, at, kFloat32, valid, w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = w[j] * decay - rate * v[j];
+            }
+            store4(out, at, type, valid, v);
         }
-        store4(out, i, type, valid, v);
     }
 };
 
@@ -669,7 +767,7 @@ struct OrthogonalLayout {
     int64_t total() const { return 2 * x_bytes + 2 * s_bytes + norm_bytes + partial_bytes; }
 };
 
-static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t cols, int sms) {
+static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t cols, bool light, int sms) {
     OrthogonalLayout l = {};
     l.tall = rows >= cols;
     l.side = l.tall ? cols : rows;
@@ -678,9 +776,9 @@ static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t c
     l.s_pitch = padded(l.side);
     l.s_plane = l.side * l.s_pitch;
     l.parts = (int)(ceil_div(rows * cols, 4 * kThreads * 4) < 2 * sms ? ceil_div(rows * cols, 4 * kThreads * 4) : 2 * sms);
-    l.gram = plan_matmul(l.side, l.side, l.tall ? rows : cols, batch, 2, true, sms);
+    l.gram = plan_matmul(l.side, l.side, l.tall ? rows : cols, batch, light ? 1 : 2, true, sms);
     l.square = plan_matmul(l.side, l.side, l.side, batch, 2, true, sms);
-    l.product = plan_matmul(rows, cols, l.side, batch, 2, false, sms);
+    l.product = plan_matmul(rows, cols, l.side, batch, light ? 1 : 2, false, sms);
     l.x_bytes = padded_bytes(batch * 2 * l.x_plane * 2);
     l.s_bytes = padded_bytes(batch * 2 * l.s_plane * 2);
     l.norm_bytes = padded_bytes(batch * l.parts * 8);
@@ -690,10 +788,18 @@ static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t c
     return l;
 }
 
-// steps times: S = X^T X (X X^T where X is wide), M = a I + b S + c S^2, X = X M (M X).  `last` takes the last product.
+// steps times: S = X^T X (X X^T where X is wide), M = b S + c S^2, X = a X + X M (M X).  `last` takes the last product.
+//
+// Results of 22 bits (fp32, fp16): every product is one of pairs, and a X comes out of the product too, as the diagonal of M, since
+// the pair of a X would have to be read again.  bf16 results have 8 bits, and the steps need no more than this: S from the first planes
+// alone, which leaves the result 6e-4 off (relative, over random, low-rank and steeply falling spectra; rounding it to bf16 is
+// 1.7e-3); S^2 from pairs; X M from the first planes, a X added as the pair that it is.  That last form matters: what is rounded away
+// of X in a product with a I + b S + c S^2 grows by a factor of a in every step along directions of small singular values, 4e-2 in the
+// end where X has few large ones; M alone is next to nothing along those.  All together 1.6e-3, half the products.
 static int orthogonalise(const void *g, int type, int64_t batch, int64_t rows, int64_t cols, int steps, const float *coefficients, double eps,
                          const OrthogonalEpilogue &last, uint8_t *workspace, int sms, cudaStream_t st, const char *what) {
-    const OrthogonalLayout l = orthogonal_layout(batch, rows, cols, sms);
+    const bool light = type == kBFloat16;
+    const OrthogonalLayout l = orthogonal_layout(batch, rows, cols, light, sms);
     uint16_t *x = reinterpret_cast<uint16_t *>(workspace), *next = reinterpret_cast<uint16_t *>(workspace + l.x_bytes);
     uint16_t *gram = reinterpret_cast<uint16_t *>(workspace + 2 * l.x_bytes), *poly = reinterpret_cast<uint16_t *>(workspace + 2 * l.x_bytes + l.s_bytes);
     double *norms = reinterpret_cast<double *>(workspace + 2 * l.x_bytes + 2 * l.s_bytes);
@@ -708,33 +814,42 @@ static int orthogonalise(const void *g, int type, int64_t batch, int64_t rows, i
     if ((status = launch_status(what)) != DL_OK) return status;
     Product p = {};
     p.batch = batch;
-    p.planes = 2;
+    p.planes_z = 2;
+    p.steps_per_sum = light ? 0 : kExactSteps;
     const float once = 1.f / kPairScale, twice = once * once;
     for (int i = 0; i < steps; ++i) {
         const float a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
-        p.a = p.b = {x, l.x_pitch, l.x_plane, 0, l.tall};
+        p.a = p.b = {x, l.x_pitch, l.x_plane, l.tall};
         p.m = p.n = l.side;
         p.k = l.tall ? rows : cols;
         p.symmetric = true;
-        if ((status = launch_product<2>(p, l.gram, PairEpilogue{gram, nullptr, l.s_pitch, l.s_plane, once, 0.f, 0.f, true}, partial, sms, st, what)) != DL_OK)
-            return status;
-        p.a = p.b = {gram, l.s_pitch, l.s_plane, 0, false};
+        p.planes = light ? 1 : 2;
+        const PairEpilogue to_gram = {gram, nullptr, l.s_pitch, l.s_plane, once, 0.f, 0.f, true};
+        if ((status = launch_planes(p, l.gram, to_gram, partial, sms, st, what)) != DL_OK) return status;
+        p.a = p.b = {gram, l.s_pitch, l.s_plane, false};
         p.k = l.side;
-        if ((status = launch_product<2>(p, l.square, PairEpilogue{poly, gram, l.s_pitch, l.s_plane, c * once, b, a * kPairScale, true}, partial, sms, st,
-                                        what)) != DL_OK)
-            return status;
-        const Operand m = {poly, l.s_pitch, l.s_plane, 0, false};
-        p.a = l.tall ? Operand{x, l.x_pitch, l.x_plane, 0, false} : m;
-        p.b = l.tall ? m : Operand{x, l.x_pitch, l.x_plane, 0, true};
+        p.planes = 2;
+        const PairEpilogue to_poly = {poly, gram, l.s_pitch, l.s_plane, c * once, b, light ? 0.f : a * kPairScale, true};
+        if ((status = launch_planes(p, l.square, to_poly, partial, sms, st, what)) != DL_OK) return status;
+        const Operand m = {poly, l.s_pitch, l.s_plane, false};
+        p.a = l.tall ? Operand{x, l.x_pitch, l.x_plane, false} : m;
+        p.b = l.tall ? m : Operand{x, l.x_pitch, l.x_plane, true};
         p.m = rows;
         p.n = cols;
         p.symmetric = false;
-        if (i + 1 < steps)
-            status = launch_product<2>(p, l.product, PairEpilogue{next, nullptr, l.x_pitch, l.x_plane, once, 0.f, 0.f, false}, partial, sms, st, what);
-        else {
+        p.planes = light ? 1 : 2;
+        const uint16_t *more = light ? x : nullptr;
+        if (i + 1 < steps) {
+            const PairEpilogue to_next = {next, more, l.x_pitch, l.x_plane, once, a, 0.f, false};
+            status = launch_planes(p, l.product, to_next, partial, sms, st, what);
+        } else {
             OrthogonalEpilogue e = last;
+            e.more = more;
+            e.pitch = l.x_pitch;
+            e.plane = l.x_plane;
             e.scale = twice;
-            status = launch_product<2>(p, l.product, e, partial, sms, st, what);
+            e.factor = a * once;
+            status = launch_planes(p, l.product, e, partial, sms, st, what);
         }
         if (status != DL_OK) return status;
         uint16_t *done = x;
@@ -746,9 +861,9 @@ static int orthogonalise(const void *g, int type, int64_t batch, int64_t rows, i
 
 }  // namespace dl
 
-extern "C" DL_API int64_t dl_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols) {
+extern "C" DL_API int64_t dl_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int type) {
     if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
-    return orthogonal_layout(batch, rows, cols, current_sms()).total();
+    return orthogonal_layout(batch, rows, cols, type == kBFloat16, current_sms()).total();
 }
 
 extern "C" DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, int64_t rows, int64_t cols, int type, int steps,

@@ -5,8 +5,10 @@
 //   2 planes  fp16 pairs hi + lo, 22 bits: hi hi + (hi lo + lo hi), 3 products; for operands of known size (the value is kept
 //             times 2^12, so that lo is no subnormal for values above 2^-14);
 //   3 planes  bf16 triples, all 24 bits of an fp32 in its whole range: 6 products, those below 2^-24 left out.
-// The small products have an accumulator of their own: a running sum in the tensor cores cuts off what is below its last bit, and the
-// sum of the large products then loses no more than a plain product does.
+// A running sum in the tensor cores cuts off what is below its last bit, always towards zero: an error of about 1e-8 for every 16 values
+// (measured: 6e-7 after 800, 1.2e-6 after 2000, where 32-bit sums of rounded steps have 2e-7 and 4e-7).  So the sums of planes are
+// taken out of tensor memory every steps_per_sum steps and added up in the epilogue's registers, and the small products have a sum
+// of their own.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -21,13 +23,13 @@ static inline int type_size(int type) { return type == kFloat32 ? 4 : 2; }
 
 struct Operand {       // rows x k, or k x rows where mn: the rows of the result are contiguous
     const void *base;
-    int64_t pitch, plane, matrix;  // in values: between rows in memory, planes, matrices of the batch (a multiple of plane)
+    int64_t pitch, plane;  // in values: between rows in memory, planes
     bool mn;
 };
 
 struct MatmulShape {
     int32_t m, n, batch, planes_z;        // planes_z: planes per matrix in the maps
-    int32_t tiles_m, tiles_n, splits, k_steps, steps_per_split;
+    int32_t tiles_m, tiles_n, splits, k_steps, steps_per_split, steps_per_sum;
     int32_t per_matrix;                   // tiles of a matrix (one split)
     int32_t tiles;                        // of all matrices and splits
     uint32_t a_mn, b_mn, instruction;
@@ -106,19 +108,23 @@ __device__ __forceinline__ void store4(void *p, int64_t i, int type, int valid, 
 // -- the kernel -----------------------------------------------------------------------------------------------------------------
 
 constexpr int kMatmulRows = 128;     // of a tile
-constexpr int kMatmulThreads = 192;  // warps 0-3: epilogue, one lane per row; warp 4: copies; warp 5: products
-constexpr int kStagePitch = 36;      // floats per row of an epilogue warp's 32 x 32 staging tile: 16-byte rows, no bank met twice
 
+// Warps 0 .. 7: epilogue, one lane per row, two warps to the same rows; then one for the copies, one for the products.
 template <int PLANES, int COLUMNS>
 struct MatmulConfig {
+    static constexpr int kWarps = 8;
+    static constexpr int kThreadsAll = (kWarps + 2) * 32;
+    static constexpr int kShare = COLUMNS / (kWarps / 4);                      // columns of an epilogue warp
+    static constexpr int kSpan = 16;                                           // of them staged at a time
+    static constexpr int kPitch = kSpan + 4;                                   // floats per row of a staging tile: 16-byte rows on different banks
     static constexpr int kStepBytes = PLANES * (kMatmulRows + COLUMNS) * kChunk * 2;
-    static constexpr int kFit = 196608 / kStepBytes;
+    static constexpr int kStagingBytes = kWarps * 32 * kPitch * 4;
+    static constexpr int kFit = (232448 - 1024 - 256 - kStagingBytes) / kStepBytes;
     static constexpr int kStages = kFit < 6 ? kFit : 6;
-    static constexpr int kSums = PLANES > 1 ? 2 : 1;                           // accumulators of a tile
-    static constexpr int kBuffers = 2 * kSums * COLUMNS <= 512 ? 2 : 1;        // tiles in tensor memory at a time
-    static constexpr int kTensorColumns = kSums * COLUMNS * kBuffers;
-    static constexpr int kSharedBytes = kStages * kStepBytes + 4 * 32 * kStagePitch * 4 + 1024 + 256;
-    static_assert(kStages >= 2 && kSharedBytes <= 232448, "the ring does not fit");
+    static constexpr int kSums = PLANES > 1 && COLUMNS <= 128 ? 2 : 1;         // accumulators: of the large products, of the small ones
+    static constexpr int kTensorColumns = 2 * kSums * COLUMNS;                 // two of each: one is filled while the other is read
+    static constexpr int kSharedBytes = kStages * kStepBytes + kStagingBytes + 1024 + 256;
+    static_assert(kStages >= 2, "the ring does not fit");
     static_assert((kTensorColumns & (kTensorColumns - 1)) == 0 && kTensorColumns >= 32 && kTensorColumns <= 512, "tensor memory");
 };
 
@@ -161,7 +167,7 @@ static __device__ int g_matmul_async_error = 0;   // set when a bounded wait ran
 // tile runs beside the products of the next where tensor memory holds two.  All waits are bounded; when one runs out, the error flag is
 // raised and every role leaves, the copies that are in flight waited for.
 template <int PLANES, int COLUMNS, class Epilogue>
-__global__ void __launch_bounds__(kMatmulThreads, 1)
+__global__ void __launch_bounds__(MatmulConfig<PLANES, COLUMNS>::kThreadsAll, 1)
 matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MatmulShape s, const Epilogue epilogue) {
     using Config = MatmulConfig<PLANES, COLUMNS>;
     constexpr int kStages = Config::kStages;
@@ -169,7 +175,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     extern __shared__ uint8_t s_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
     float *staging = reinterpret_cast<float *>(ring + kStages * Config::kStepBytes);
-    uint64_t *full = reinterpret_cast<uint64_t *>(staging + 4 * 32 * kStagePitch), *empty = full + kStages, *sums_full = empty + kStages,
+    uint64_t *full = reinterpret_cast<uint64_t *>(staging + Config::kStagingBytes / 4), *empty = full + kStages, *sums_full = empty + kStages,
              *sums_empty = sums_full + 2, *drained = sums_empty + 2;
     uint32_t *s_tensor = reinterpret_cast<uint32_t *>(drained + 1);
     volatile uint32_t *s_failed = s_tensor + 1;
@@ -182,14 +188,14 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(sums_full + i, 1);
-            mbar_init(sums_empty + i, 4);
+            mbar_init(sums_empty + i, Config::kWarps);
         }
         mbar_init(drained, 1);
         *s_failed = 0;
         mbar_fence_init();
     }
-    if (warp == 5) tensor_alloc(s_tensor, Config::kTensorColumns);
-    if (warp == 4 && lane == 0) {
+    if (warp == Config::kWarps + 1) tensor_alloc(s_tensor, Config::kTensorColumns);
+    if (warp == Config::kWarps && lane == 0) {
         map_prefetch(&map_a);
         map_prefetch(&map_b);
     }
@@ -200,7 +206,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     grid_dependency_wait();
     grid_dependents_launch();
 
-    if (warp == 4) {
+    if (warp == Config::kWarps) {
         if (lane == 0) {
             int stage = 0, used = 0;   // used: stages with a copy issued
             uint32_t phase = 0;
@@ -246,7 +252,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             // nothing of a CTA's copies is in flight when it ends: the latest copy into each stage
             for (int i = 0; i < used; ++i) mbar_wait(full + i, i < stage ? phase : phase ^ 1);
         }
-    } else if (warp == 5) {
+    } else if (warp == Config::kWarps + 1) {
         if (lane == 0) {
             int stage = 0, buffer = 0;
             uint32_t phase = 0, buffer_phase = 0;
@@ -255,44 +261,45 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             for (int id = blockIdx.x; id < s.tiles && ok; id += gridDim.x) {
                 const Tile t = tile_of<COLUMNS>(id, s);
                 const int first = t.split * s.steps_per_split, last = min(s.k_steps, first + s.steps_per_split);
-                ok = mbar_wait(sums_empty + buffer, buffer_phase ^ 1) && !*s_failed;
-                if (!ok) break;
-                tensor_fence_after();
-                const uint32_t large = tensor + buffer * Config::kSums * COLUMNS, small = large + COLUMNS;
-                for (int step = first; step < last; ++step) {
-                    ok = mbar_wait(full + stage, phase) && !*s_failed;
+                for (int block = first; block < last && ok; block += s.steps_per_sum) {
+                    ok = mbar_wait(sums_empty + buffer, buffer_phase ^ 1) && !*s_failed;
                     if (!ok) break;
                     tensor_fence_after();
-                    const uint32_t at = smem_addr(ring + stage * Config::kStepBytes);
-                    const uint64_t a = operand_descriptor(at), b = operand_descriptor(at + PLANES * kPlaneA);
-                    const auto product = [&](int pa, int pb, uint32_t sum, bool fresh) {
-                        const uint64_t from_a = a + pa * (kPlaneA >> 4), from_b = b + pb * (kPlaneB >> 4);
+                    const uint32_t large = tensor + buffer * Config::kSums * COLUMNS, small = large + (Config::kSums - 1) * COLUMNS;
+                    const int end = min(last, block + s.steps_per_sum);
+                    for (int step = block; step < end; ++step) {
+                        ok = mbar_wait(full + stage, phase) && !*s_failed;
+                        if (!ok) break;
+                        tensor_fence_after();
+                        const uint32_t at = smem_addr(ring + stage * Config::kStepBytes);
+                        const uint64_t a = operand_descriptor(at), b = operand_descriptor(at + PLANES * kPlaneA);
+                        const auto product = [&](int pa, int pb, uint32_t sum, bool fresh) {
+                            const uint64_t from_a = a + pa * (kPlaneA >> 4), from_b = b + pb * (kPlaneB >> 4);
 #pragma unroll
-                        for (int k = 0; k < kChunk / 16; ++k)
-                            tensor_multiply(sum, from_a + k * a_step, from_b + k * b_step, s.instruction, !(fresh && k == 0));
-                    };
-                    const bool fresh = step == first;
-                    product(0, 0, large, fresh);
-                    if (PLANES > 1) {
-                        product(0, 1, small, fresh);
-                        product(1, 0, small, false);
+                            for (int k = 0; k < kChunk / 16; ++k)
+                                tensor_multiply(sum, from_a + k * a_step, from_b + k * b_step, s.instruction, !(fresh && k == 0));
+                        };
+                        const bool fresh = step == block;
+                        product(0, 0, large, fresh);
+                        if (PLANES > 1) {
+                            product(0, 1, small, fresh && Config::kSums == 2);
+                            product(1, 0, small, false);
+                        }
+                        if (PLANES > 2) {
+                            product(1, 1, small, false);
+                            product(0, 2, small, false);
+                            product(2, 0, small, false);
+                        }
+                        tensor_commit(empty + stage);
+                        if (++stage == kStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
                     }
-                    if (PLANES > 2) {
-                        product(1, 1, small, false);
-                        product(0, 2, small, false);
-                        product(2, 0, small, false);
-                    }
-                    tensor_commit(empty + stage);
-                    if (++stage == kStages) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
-                }
-                if (!ok) break;
-                tensor_commit(sums_full + buffer);
-                if (++buffer == Config::kBuffers) {
-                    buffer = 0;
-                    buffer_phase ^= 1;
+                    if (!ok) break;
+                    tensor_commit(sums_full + buffer);
+                    buffer ^= 1;
+                    buffer_phase ^= buffer == 0;
                 }
             }
             if (!ok) {
@@ -303,71 +310,106 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             }
         }
     } else {
-        float *mine = staging + warp * 32 * kStagePitch;
+        constexpr int kSpan = Config::kSpan, kShare = Config::kShare, kPitch = Config::kPitch;
+        constexpr bool kKeep = PLANES > 1;   // sums of several blocks, added up in registers
+        float *mine = staging + warp * 32 * kPitch;
+        const int quarter = warp % 4, from = warp / 4 * kShare;   // a warp reads the lanes of its number modulo 4
         int buffer = 0;
         uint32_t buffer_phase = 0;
-        for (int id = blockIdx.x; id < s.tiles; id += gridDim.x) {
+        bool ok = true;
+        for (int id = blockIdx.x; id < s.tiles && ok; id += gridDim.x) {
             const Tile t = tile_of<COLUMNS>(id, s);
-            if (!mbar_wait(sums_full + buffer, buffer_phase) || *s_failed) {
-                *s_failed = 1;
-                g_matmul_async_error = 1;
-                break;
-            }
-            __syncwarp();
-            tensor_fence_after();
-            const uint32_t sums = tensor + buffer * Config::kSums * COLUMNS + ((uint32_t)warp * 32 << 16);
-            const int row0 = t.row + warp * 32, slice = t.split * s.batch + t.matrix;
-#pragma unroll 1
-            for (int c0 = 0; c0 < COLUMNS && t.col + c0 < s.n; c0 += 32) {
-                uint32_t bits[32];
-                float v[32];
-                tensor_read32(sums + c0, bits);
-                tensor_read_wait();
-#pragma unroll
-                for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(bits[c]);
-                if (Config::kSums == 2) {
-                    tensor_read32(sums + COLUMNS + c0, bits);
-                    tensor_read_wait();
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) v[c] += __uint_as_float(bits[c]);
-                }
-                const int col0 = t.col + c0;
-                if (epilogue.by_column(row0, col0)) {
-                    const int row = row0 + lane;
-#pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (row < s.m && col0 + c < s.n) epilogue.one(slice, row, col0 + c, v[c]);
-                }
+            const int first = t.split * s.steps_per_split, last = min(s.k_steps, first + s.steps_per_split);
+            const int row0 = t.row + quarter * 32, slice = t.split * s.batch + t.matrix;
+            const auto finish = [&](const float (&v)[kSpan], int col0) {
+                if (col0 >= s.n) return;
+                if (epilogue.by_column(row0, col0)) epilogue.template down<kSpan>(slice, row0 + lane, col0, v, s.m, min(kSpan, s.n - col0));
                 if (epilogue.by_row(row0, col0)) {
+                    constexpr int kQuads = kSpan / 4, kStep = 32 / kQuads;
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4)
-                        *reinterpret_cast<float4 *>(mine + lane * kStagePitch + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+                    for (int c = 0; c < kSpan; c += 4)
+                        *reinterpret_cast<float4 *>(mine + lane * kPitch + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
                     __syncwarp();
+                    const int c = lane % kQuads * 4;
+                    float q[kQuads][4];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = i * 4 + lane / 8, c = lane % 8 * 4;
-                        const float4 f = *reinterpret_cast<const float4 *>(mine + r * kStagePitch + c);
-                        const int row = row0 + r, col = col0 + c;
-                        const float four[4] = {f.x, f.y, f.z, f.w};
-                        if (row < s.m && col < s.n) epilogue.four(slice, row, col, four, min(4, s.n - col));
+                    for (int i = 0; i < kQuads; ++i) {
+                        const float4 f = *reinterpret_cast<const float4 *>(mine + (i * kStep + lane / kQuads) * kPitch + c);
+                        q[i][0] = f.x; q[i][1] = f.y; q[i][2] = f.z; q[i][3] = f.w;
                     }
+                    if (col0 + c < s.n) epilogue.template across<kQuads, kStep>(slice, row0 + lane / kQuads, col0 + c, q, s.m, min(4, s.n - col0 - c));
                     __syncwarp();
                 }
+            };
+            float kept[kKeep ? kShare : 1];
+#pragma unroll
+            for (int c = 0; c < (kKeep ? kShare : 1); ++c) kept[c] = 0.f;
+            for (int block = first; block < last; block += s.steps_per_sum) {
+                ok = mbar_wait(sums_full + buffer, buffer_phase) && !*s_failed;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tensor_fence_after();
+                const uint32_t sums = tensor + buffer * Config::kSums * COLUMNS + from + ((uint32_t)quarter * 32 << 16);
+                if constexpr (kKeep) {
+#pragma unroll
+                    for (int c0 = 0; c0 < kShare; c0 += 16) {
+                        uint32_t large[16], small[16];
+                        tensor_read16(sums + c0, large);
+                        if (Config::kSums == 2) tensor_read16(sums + COLUMNS + c0, small);
+                        tensor_read_wait();
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            float v = __uint_as_float(large[c]);
+                            if (Config::kSums == 2) v += __uint_as_float(small[c]);
+                            kept[c0 + c] += v;
+                        }
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c0 = 0; c0 < kShare && t.col + from + c0 < s.n; c0 += kSpan) {
+                        uint32_t bits[kSpan];
+                        float v[kSpan];
+                        tensor_read16(sums + c0, bits);
+                        tensor_read_wait();
+#pragma unroll
+                        for (int c = 0; c < kSpan; ++c) v[c] = __uint_as_float(bits[c]);
+                        finish(v, t.col + from + c0);
+                    }
+                }
+                tensor_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sums_empty + buffer);
+                buffer ^= 1;
+                buffer_phase ^= buffer == 0;
             }
-            tensor_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(sums_empty + buffer);
-            if (++buffer == Config::kBuffers) {
-                buffer = 0;
-                buffer_phase ^= 1;
+            if constexpr (kKeep) {
+                if (ok) {
+#pragma unroll 1
+                    for (int c0 = 0; c0 < kShare; c0 += kSpan) {   // the registers move up: one copy of the epilogue's code
+                        float v[kSpan];
+#pragma unroll
+                        for (int c = 0; c < kSpan; ++c) v[c] = kept[c];
+#pragma unroll
+                        for (int c = 0; c + kSpan < kShare; ++c) kept[c] = kept[c + kSpan];
+                        finish(v, t.col + from + c0);
+                    }
+                }
             }
+        }
+        if (!ok) {
+            *s_failed = 1;
+            g_matmul_async_error = 1;
         }
     }
     __syncwarp();
     tensor_fence_before();
     __syncthreads();
-    if (warp == 5) tensor_free(tensor, Config::kTensorColumns);
+    if (warp == Config::kWarps + 1) tensor_free(tensor, Config::kTensorColumns);
 }
+
+// An epilogue says which way a piece of a tile is handed to it (both, where a symmetric result is stored on both sides):
+//   across: neighbouring lanes have neighbouring columns, a lane four of them in N rows, kStep apart;
+//   down:   neighbouring lanes have neighbouring rows, a lane N columns of one row.
 
 // Sums of a product that was split along k: kept as they are, added up in the order of the splits by matmul_join_kernel.
 struct StorePartial {
@@ -375,9 +417,13 @@ struct StorePartial {
     int64_t n, matrix;   // values of a row, of a matrix
     __device__ __forceinline__ bool by_column(int, int) const { return false; }
     __device__ __forceinline__ bool by_row(int, int) const { return true; }
-    __device__ __forceinline__ void one(int, int, int, float) const {}
-    __device__ __forceinline__ void four(int slice, int row, int col, const float (&v)[4], int valid) const {
-        store4(out, slice * matrix + (int64_t)row * n + col, kFloat32, valid, v);
+    template <int N>
+    __device__ __forceinline__ void down(int, int, int, const float (&)[N], int, int) const {}
+    template <int N, int STEP>
+    __device__ __forceinline__ void across(int slice, int row, int col, const float (&q)[N][4], int m, int valid) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (row + i * STEP < m) store4(out, slice * matrix + (int64_t)(row + i * STEP) * n + col, kFloat32, valid, q[i]);
     }
 };
 
@@ -403,7 +449,8 @@ matmul_join_kernel(const float *__restrict__ partial, int splits, int batch, int
             rest /= m;
         }
         const int z = (int)rest, col = quad * 4, valid = min(4, n - col);
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        float q[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+        float(&v)[4] = q[0];
         const bool mirrored = symmetric && col / kMatmulRows > row / kMatmulRows;   // a multiple of 4 columns: all of a quad alike
         for (int sp = 0; sp < splits; ++sp) {
             const float *p = partial + ((int64_t)sp * batch + z) * matrix;
@@ -417,13 +464,8 @@ matmul_join_kernel(const float *__restrict__ partial, int splits, int batch, int
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] += f[j];
         }
-        if (columns) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < valid) epilogue.one(z, row, col + j, v[j]);
-        } else {
-            epilogue.four(z, row, col, v, valid);
-        }
+        if (columns) epilogue.template down<4>(z, row, col, v, m, valid);
+        else epilogue.template across<1, 1>(z, row, col, q, m, valid);
     }
 }
 #endif  // __CUDACC__

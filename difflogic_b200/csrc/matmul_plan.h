@@ -18,8 +18,9 @@ static inline MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, int64_t ba
     double best_clocks = 0;
     const int64_t steps = ceil_div(k, 64), tiles_m = ceil_div(m, 128);
     const int products = planes == 1 ? 1 : planes == 2 ? 3 : 6;
+    const int only_columns = tuning(DL_TUNE_MATMUL_COLUMNS), only_splits = tuning(DL_TUNE_MATMUL_SPLITS);
     for (int columns = 64; columns <= (planes == 3 ? 128 : 256); columns *= 2) {
-        if (columns > 64 && n <= columns / 2) continue;
+        if (only_columns > 0 ? columns != only_columns && !(planes == 3 && only_columns > 128 && columns == 128) : columns > 64 && n <= columns / 2) continue;
         const int64_t tiles_n = ceil_div(n, columns);
         int64_t per_matrix = tiles_m * tiles_n;
         if (symmetric) {
@@ -34,13 +35,13 @@ static inline MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, int64_t ba
         const double last = 600 + columns * 10.0;   // the epilogue of the last tile
         for (int64_t splits = 1; splits <= 64 && (splits == 1 || steps / splits >= 4); splits += splits < 4 ? 1 : splits / 2) {
             const int64_t per = ceil_div(steps, splits), really = ceil_div(steps, per);
-            if (really != splits) continue;
+            if (really != splits || (only_splits > 0 && splits > only_splits)) continue;
             const int64_t tiles = per_matrix * batch * splits, waves = ceil_div(tiles, sms);
             const int64_t partial = splits > 1 ? splits * batch * m * n * 4 : 0;
             if (partial > (int64_t)64 << 20) continue;
             double clocks = 1500 + waves * (per * step + 150) + last;
             if (splits > 1) clocks += 3000 + (double)partial / 2000;
-            if (best.columns == 0 || clocks < best_clocks) {
+            if (best.columns == 0 || clocks < best_clocks || (only_splits > 0 && splits > best.splits)) {
                 best = {columns, (int)splits, (int)per, partial};
                 best_clocks = clocks;
             }

@@ -75,7 +75,9 @@ enum {
     DL_TUNE_FUSED_CLUSTER = 5,      /* dl_eval_groupbitsum: CTAs per class, 2, 4 or 8                            */
     DL_TUNE_FORWARD_KERNEL = 6,     /* dl_forward_f32: 1 = register kernel, 2 = staged (bulk-copy) kernel        */
     DL_TUNE_WALK_KERNEL = 7,        /* dl_backward_walk_f32: 1 = register kernel, 2 = staged kernel where it can  */
-    DL_TUNE_COUNT = 8
+    DL_TUNE_MATMUL_COLUMNS = 8,     /* matrix products: columns of a tile, 64, 128 or 256 where there is one     */
+    DL_TUNE_MATMUL_SPLITS = 9,      /* matrix products: pieces that the sum is cut into, as far as it goes       */
+    DL_TUNE_COUNT = 10
 };
 DL_API int dl_set_tuning(int key, int value);
 DL_API int dl_get_tuning(int key);
@@ -582,8 +584,8 @@ DL_API int dl_dense_backward(const void *gy, int g_feature_major, const void *sl
 /* X = G / max(|G|_F, eps), then for each step with its (a, b, c) in `coefficients` (steps x 3, on the host)
  *   X <- a X + b (X X^T) X + c (X X^T)^2 X
  * for `batch` contiguous matrices rows x cols; out in G's type.  The iterates are kept to 22 bits (fp16 pairs times 2^12: values up to
- * 16), sums in 32 bits. */
-DL_API int64_t dl_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
+ * 16), sums in 32 bits; bf16 matrices are multiplied with 11 bits, which leaves the result less far off than its rounding does. */
+DL_API int64_t dl_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int type);
 DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, int64_t rows, int64_t cols, int type, int steps,
                             const float *coefficients, double eps, void *workspace, void *stream);
 
