@@ -50,25 +50,35 @@ struct Product {
     int64_t m, n, k, batch;
     int planes, planes_z;   // multiplied; per matrix in memory
     bool bfloat, symmetric;
-    int steps_per_sum;   // 0: a sum stays in tensor memory for the whole product
+    bool exact;   // sums are taken out of tensor memory every so often
 };
-
-// Steps of 64 after which sums are taken out of tensor memory: results of 22 or 24 bits.
-constexpr int kExactSteps = 2;
 
 static bool map_operand(CUtensorMap *map, const Operand &o, const Product &p, int64_t rows) {
     const int64_t inner = o.mn ? rows : p.k, outer = o.mn ? p.k : rows;
     return make_tile_map(map, o.base, p.bfloat, inner, outer, p.planes_z * p.batch, o.pitch * 2, o.plane * 2);
 }
 
-template <int PLANES, int COLUMNS, class Epilogue>
-static int launch_tiles(const Product &p, const MatmulShape &shape, const CUtensorMap &a, const CUtensorMap &b, const Epilogue &epilogue,
-                        int sms, cudaStream_t st, const char *what) {
-    auto kernel = matmul_kernel<PLANES, COLUMNS, Epilogue>;
-    constexpr int kShared = MatmulConfig<PLANES, COLUMNS>::kSharedBytes;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared) != cudaSuccess) return launch_status(what);
-    launch_dependent(true, kernel, dim3((unsigned)(shape.tiles < sms ? shape.tiles : sms)), dim3(MatmulConfig<PLANES, COLUMNS>::kThreadsAll), kShared, st, a, b, shape,
-                     epilogue);
+template <int PLANES, int COLUMNS, bool PAIR, class Epilogue>
+static int launch_tiles(const MatmulShape &shape, const CUtensorMap &a, const CUtensorMap &b, const Epilogue &epilogue, int sms,
+                        cudaStream_t st, const char *what) {
+    using Config = MatmulConfig<PLANES, COLUMNS, PAIR>;
+    auto kernel = matmul_kernel<PLANES, COLUMNS, PAIR, Epilogue>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Config::kSharedBytes) != cudaSuccess) return launch_status(what);
+    const int64_t ctas = PAIR ? 2 * (int64_t)shape.tiles : shape.tiles, most = PAIR ? sms / 2 * 2 : sms;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ctas < most ? ctas : most));
+    cfg.blockDim = dim3(Config::kThreadsAll);
+    cfg.dynamicSmemBytes = Config::kSharedBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = PAIR ? 2 : 1;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = PAIR ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, a, b, shape, epilogue);
     return launch_status(what);
 }
 
@@ -77,36 +87,30 @@ static int launch_columns(const Product &p, const MatmulPlan &plan, const Epilog
     CUtensorMap a, b;
     if (!map_operand(&a, p.a, p, p.m) || !map_operand(&b, p.b, p, p.n))
         return fail(DL_ERR_CUDA, "%s: the driver refuses the map of an operand", what);
+    const int rows = plan.pair ? 2 * kMatmulRows : kMatmulRows;
     MatmulShape s = {};
     s.m = (int32_t)p.m;
     s.n = (int32_t)p.n;
     s.batch = (int32_t)p.batch;
     s.planes_z = p.planes_z;
-    s.tiles_m = (int32_t)ceil_div(p.m, kMatmulRows);
+    s.tiles_m = (int32_t)ceil_div(p.m, rows);
     s.tiles_n = (int32_t)ceil_div(p.n, plan.columns);
     s.splits = plan.splits;
     s.k_steps = (int32_t)ceil_div(p.k, kChunk);
     s.steps_per_split = plan.steps_per_split;
-    s.steps_per_sum = PLANES > 1 && p.steps_per_sum > 0 ? p.steps_per_sum : s.k_steps;   // one plane: nothing adds blocks up
+    // one plane: nothing adds blocks up; wide tiles have one sum for large and small products, three or six of them a step
+    s.steps_per_sum = PLANES > 1 && p.exact ? (plan.columns == 256 ? 4 - PLANES : 2) : s.k_steps;
     s.symmetric = p.symmetric;
-    int64_t per_matrix = (int64_t)s.tiles_m * s.tiles_n;
-    if (p.symmetric) {
-        per_matrix = 0;
-        for (int64_t mi = 0; mi < s.tiles_m; ++mi) {
-            const int64_t across = ceil_div((mi + 1) * kMatmulRows, plan.columns);
-            per_matrix += across < s.tiles_n ? across : s.tiles_n;
-        }
-    }
-    const int64_t tiles = per_matrix * s.splits * p.batch;
+    const int64_t per_matrix = tiles_of(p.m, p.n, rows, plan.columns, p.symmetric), tiles = per_matrix * s.splits * p.batch;
     if (tiles > INT32_MAX / 2) return fail(DL_ERR_TOO_LARGE, "%s: too many tiles", what);
     s.per_matrix = (int32_t)per_matrix;
     s.tiles = (int32_t)tiles;
     s.a_mn = p.a.mn;
     s.b_mn = p.b.mn;
-    s.instruction = instruction_descriptor(p.bfloat, p.a.mn, p.b.mn, plan.columns);
-    if (plan.columns == 64) return launch_tiles<PLANES, 64>(p, s, a, b, epilogue, sms, st, what);
-    if (plan.columns == 128) return launch_tiles<PLANES, 128>(p, s, a, b, epilogue, sms, st, what);
-    if constexpr (PLANES < 3) return launch_tiles<PLANES, 256>(p, s, a, b, epilogue, sms, st, what);
+    s.instruction = instruction_descriptor(p.bfloat, p.a.mn, p.b.mn, rows, plan.columns);
+    if (plan.pair) return launch_tiles<PLANES, 256, true>(s, a, b, epilogue, sms, st, what);
+    if (plan.columns == 64) return launch_tiles<PLANES, 64, false>(s, a, b, epilogue, sms, st, what);
+    if (plan.columns == 128) return launch_tiles<PLANES, 128, false>(s, a, b, epilogue, sms, st, what);
     return fail(DL_ERR_INVALID_ARG, "%s: no such tile", what);
 }
 
@@ -490,7 +494,7 @@ extern "C" DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_fea
     p.batch = 1;
     p.planes = p.planes_z = l.planes;
     p.bfloat = type != kFloat16;
-    p.steps_per_sum = kExactSteps;
+    p.exact = true;
     const DenseEpilogue e = {y, bias, residual, slope, y_feature_major ? batch : outer, rows_are_features ? residual_feature : residual_batch,
                              rows_are_features ? residual_batch : residual_feature, type, act, rows_are_features, y_feature_major != 0};
     return launch_planes(p, plan, e, reinterpret_cast<float *>(workspace), sms, st, what);
@@ -568,7 +572,7 @@ extern "C" DL_API int dl_dense_backward(const void *gy, int g_feature_major, con
     p.batch = 1;
     p.planes = p.planes_z = b.planes;
     p.bfloat = type != kFloat16;
-    p.steps_per_sum = kExactSteps;
+    p.exact = true;
     if (gx) {   // gz [batch][outer] w [outer][inner], summed over the outputs
         p.a = g;
         p.a.mn = g_feature_major != 0;
@@ -815,7 +819,7 @@ static int orthogonalise(const void *g, int type, int64_t batch, int64_t rows, i
     Product p = {};
     p.batch = batch;
     p.planes_z = 2;
-    p.steps_per_sum = light ? 0 : kExactSteps;
+    p.exact = !light;
     const float once = 1.f / kPairScale, twice = once * once;
     for (int i = 0; i < steps; ++i) {
         const float a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];

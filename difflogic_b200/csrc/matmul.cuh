@@ -109,15 +109,18 @@ __device__ __forceinline__ void store4(void *p, int64_t i, int type, int valid, 
 
 constexpr int kMatmulRows = 128;     // of a tile
 
-// Warps 0 .. 7: epilogue, one lane per row, two warps to the same rows; then one for the copies, one for the products.
-template <int PLANES, int COLUMNS>
+// Warps 0 .. 7: epilogue, one lane per row, two warps to the same rows; then one for the copies, one for the products, two idle: the
+// registers that the epilogue does not leave to the others are handed out in groups of four warps.
+template <int PLANES, int COLUMNS, bool PAIR>
 struct MatmulConfig {
     static constexpr int kWarps = 8;
-    static constexpr int kThreadsAll = (kWarps + 2) * 32;
+    static constexpr int kThreadsAll = (kWarps + 4) * 32;   // 384
+    static constexpr int kTileRows = PAIR ? 2 * kMatmulRows : kMatmulRows;
+    static constexpr int kOwnColumns = PAIR ? COLUMNS / 2 : COLUMNS;           // rows of B that a CTA copies
     static constexpr int kShare = COLUMNS / (kWarps / 4);                      // columns of an epilogue warp
     static constexpr int kSpan = 16;                                           // of them staged at a time
     static constexpr int kPitch = kSpan + 4;                                   // floats per row of a staging tile: 16-byte rows on different banks
-    static constexpr int kStepBytes = PLANES * (kMatmulRows + COLUMNS) * kChunk * 2;
+    static constexpr int kStepBytes = PLANES * (kMatmulRows + kOwnColumns) * kChunk * 2;   // of a CTA
     static constexpr int kStagingBytes = kWarps * 32 * kPitch * 4;
     static constexpr int kFit = (232448 - 1024 - 256 - kStagingBytes) / kStepBytes;
     static constexpr int kStages = kFit < 6 ? kFit : 6;
@@ -132,7 +135,7 @@ struct Tile {
     int matrix, split, row, col;  // first row and column
 };
 
-template <int COLUMNS>
+template <int ROWS, int COLUMNS>
 __device__ __forceinline__ Tile tile_of(int id, const MatmulShape &s) {
     Tile t;
     const int all = s.per_matrix * s.splits;
@@ -144,7 +147,7 @@ __device__ __forceinline__ Tile tile_of(int id, const MatmulShape &s) {
     if (s.symmetric) {
         mi = 0;
         for (;;) {
-            const int across = min(s.tiles_n, ((mi + 1) * kMatmulRows + COLUMNS - 1) / COLUMNS);
+            const int across = min(s.tiles_n, ((mi + 1) * ROWS + COLUMNS - 1) / COLUMNS);
             if (id < across) break;
             id -= across;
             ++mi;
@@ -156,7 +159,7 @@ __device__ __forceinline__ Tile tile_of(int id, const MatmulShape &s) {
         mi = first + in_band % high;
         ni = in_band / high;
     }
-    t.row = mi * kMatmulRows;
+    t.row = mi * ROWS;
     t.col = ni * COLUMNS;
     return t;
 }
@@ -166,12 +169,12 @@ static __device__ int g_matmul_async_error = 0;   // set when a bounded wait ran
 // Persistent: every CTA takes tiles blockIdx.x, blockIdx.x + gridDim.x, ...; the copies run ahead across tiles, and the epilogue of a
 // tile runs beside the products of the next where tensor memory holds two.  All waits are bounded; when one runs out, the error flag is
 // raised and every role leaves, the copies that are in flight waited for.
-template <int PLANES, int COLUMNS, class Epilogue>
-__global__ void __launch_bounds__(MatmulConfig<PLANES, COLUMNS>::kThreadsAll, 1)
+template <int PLANES, int COLUMNS, bool PAIR, class Epilogue>
+__global__ void __launch_bounds__(MatmulConfig<PLANES, COLUMNS, PAIR>::kThreadsAll, 1)
 matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MatmulShape s, const Epilogue epilogue) {
-    using Config = MatmulConfig<PLANES, COLUMNS>;
+    using Config = MatmulConfig<PLANES, COLUMNS, PAIR>;
     constexpr int kStages = Config::kStages;
-    constexpr int kPlaneA = kMatmulRows * kChunk * 2, kPlaneB = COLUMNS * kChunk * 2;
+    constexpr int kPlaneA = kMatmulRows * kChunk * 2, kPlaneB = Config::kOwnColumns * kChunk * 2;
     extern __shared__ uint8_t s_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
     float *staging = reinterpret_cast<float *>(ring + kStages * Config::kStepBytes);
@@ -180,6 +183,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     uint32_t *s_tensor = reinterpret_cast<uint32_t *>(drained + 1);
     volatile uint32_t *s_failed = s_tensor + 1;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = PAIR ? cluster_rank() : 0;
+    const int first_tile = PAIR ? blockIdx.x / 2 : blockIdx.x, tile_step = PAIR ? gridDim.x / 2 : gridDim.x;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
@@ -188,36 +193,40 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(sums_full + i, 1);
-            mbar_init(sums_empty + i, Config::kWarps);
+            mbar_init(sums_empty + i, PAIR ? 2 * Config::kWarps : Config::kWarps);
         }
         mbar_init(drained, 1);
         *s_failed = 0;
         mbar_fence_init();
     }
-    if (warp == Config::kWarps + 1) tensor_alloc(s_tensor, Config::kTensorColumns);
+    if (warp == Config::kWarps + 1) tensor_alloc<PAIR>(s_tensor, Config::kTensorColumns);
     if (warp == Config::kWarps && lane == 0) {
         map_prefetch(&map_a);
         map_prefetch(&map_b);
     }
     tensor_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync();   // the other one's barriers are there
     tensor_fence_after();
     const uint32_t tensor = *s_tensor;
     grid_dependency_wait();
     grid_dependents_launch();
 
-    if (warp == Config::kWarps) {
-        if (lane == 0) {
+    // 168 registers a thread at the launch, 384 threads: 216 for the epilogue's 256 and 72 for the other 128 are as many
+    if (warp >= Config::kWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == Config::kWarps && lane == 0) {
             int stage = 0, used = 0;   // used: stages with a copy issued
             uint32_t phase = 0;
             bool ok = true;
-            for (int id = blockIdx.x; id < s.tiles && ok; id += gridDim.x) {
-                const Tile t = tile_of<COLUMNS>(id, s);
+            for (int id = first_tile; id < s.tiles && ok; id += tile_step) {
+                const Tile t = tile_of<Config::kTileRows, COLUMNS>(id, s);
                 const int first = t.split * s.steps_per_split, last = min(s.k_steps, first + s.steps_per_split);
                 for (int step = first; step < last; ++step) {
                     ok = mbar_wait(empty + stage, phase ^ 1) && !*s_failed;
                     if (!ok) break;
-                    mbar_arrive_expect_tx(full + stage, Config::kStepBytes);
+                    if (rank == 0) mbar_arrive_expect_tx(full + stage, PAIR ? 2 * Config::kStepBytes : Config::kStepBytes);
+                    const uint32_t bar = PAIR ? cluster_address(full + stage, 0) : smem_addr(full + stage);
                     uint8_t *at = ring + stage * Config::kStepBytes;
                     const int k = step * kChunk;
 #pragma unroll 1
@@ -225,17 +234,17 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         const int z = t.matrix * s.planes_z + p;
 #pragma unroll
                         for (int c = 0; c < kMatmulRows / kChunk; ++c, at += kChunkBytes) {
-                            const int row = t.row + c * kChunk;
-                            tile_load(at, &map_a, s.a_mn ? row : k, s.a_mn ? k : row, z, full + stage);
+                            const int row = t.row + (int)rank * kMatmulRows + c * kChunk;
+                            tile_load<PAIR>(at, &map_a, s.a_mn ? row : k, s.a_mn ? k : row, z, bar);
                         }
                     }
 #pragma unroll 1
                     for (int p = 0; p < PLANES; ++p) {
                         const int z = t.matrix * s.planes_z + p;
 #pragma unroll
-                        for (int c = 0; c < COLUMNS / kChunk; ++c, at += kChunkBytes) {
-                            const int col = t.col + c * kChunk;
-                            tile_load(at, &map_b, s.b_mn ? col : k, s.b_mn ? k : col, z, full + stage);
+                        for (int c = 0; c < Config::kOwnColumns / kChunk; ++c, at += kChunkBytes) {
+                            const int col = t.col + (int)rank * Config::kOwnColumns + c * kChunk;
+                            tile_load<PAIR>(at, &map_b, s.b_mn ? col : k, s.b_mn ? k : col, z, bar);
                         }
                     }
                     used = max(used, stage + 1);
@@ -249,17 +258,20 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 *s_failed = 1;
                 g_matmul_async_error = 1;
             }
-            // nothing of a CTA's copies is in flight when it ends: the latest copy into each stage
-            for (int i = 0; i < used; ++i) mbar_wait(full + i, i < stage ? phase : phase ^ 1);
+            // nothing of a CTA's copies is in flight when it ends: the latest copy into each stage (in a pair the first CTA's barriers
+            // count both's, and the second CTA does not end before the first)
+            if (rank == 0)
+                for (int i = 0; i < used; ++i) mbar_wait(full + i, i < stage ? phase : phase ^ 1);
+            else if (!ok)   // the first CTA may have given up before it counted these: they land within microseconds
+                for (int i = 0; i < 1000; ++i) __nanosleep(1000);
         }
-    } else if (warp == Config::kWarps + 1) {
-        if (lane == 0) {
+        if (warp == Config::kWarps + 1 && lane == 0 && rank == 0) {
             int stage = 0, buffer = 0;
             uint32_t phase = 0, buffer_phase = 0;
             bool ok = true;
             const uint32_t a_step = s.a_mn ? 2048 >> 4 : 32 >> 4, b_step = s.b_mn ? 2048 >> 4 : 32 >> 4;
-            for (int id = blockIdx.x; id < s.tiles && ok; id += gridDim.x) {
-                const Tile t = tile_of<COLUMNS>(id, s);
+            for (int id = first_tile; id < s.tiles && ok; id += tile_step) {
+                const Tile t = tile_of<Config::kTileRows, COLUMNS>(id, s);
                 const int first = t.split * s.steps_per_split, last = min(s.k_steps, first + s.steps_per_split);
                 for (int block = first; block < last && ok; block += s.steps_per_sum) {
                     ok = mbar_wait(sums_empty + buffer, buffer_phase ^ 1) && !*s_failed;
@@ -277,7 +289,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                             const uint64_t from_a = a + pa * (kPlaneA >> 4), from_b = b + pb * (kPlaneB >> 4);
 #pragma unroll
                             for (int k = 0; k < kChunk / 16; ++k)
-                                tensor_multiply(sum, from_a + k * a_step, from_b + k * b_step, s.instruction, !(fresh && k == 0));
+                                tensor_multiply<PAIR>(sum, from_a + k * a_step, from_b + k * b_step, s.instruction, !(fresh && k == 0));
                         };
                         const bool fresh = step == block;
                         product(0, 0, large, fresh);
@@ -290,14 +302,14 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                             product(0, 2, small, false);
                             product(2, 0, small, false);
                         }
-                        tensor_commit(empty + stage);
+                        tensor_commit<PAIR>(empty + stage);
                         if (++stage == kStages) {
                             stage = 0;
                             phase ^= 1;
                         }
                     }
                     if (!ok) break;
-                    tensor_commit(sums_full + buffer);
+                    tensor_commit<PAIR>(sums_full + buffer);
                     buffer ^= 1;
                     buffer_phase ^= buffer == 0;
                 }
@@ -305,11 +317,12 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             if (!ok) {
                 *s_failed = 1;
                 g_matmul_async_error = 1;
-                tensor_commit(drained);   // tensor memory is given back when nothing writes it any more
+                tensor_commit<PAIR>(drained);   // tensor memory is given back when nothing writes it any more
                 mbar_wait(drained, 0);
             }
         }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         constexpr int kSpan = Config::kSpan, kShare = Config::kShare, kPitch = Config::kPitch;
         constexpr bool kKeep = PLANES > 1;   // sums of several blocks, added up in registers
         float *mine = staging + warp * 32 * kPitch;
@@ -317,10 +330,10 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         int buffer = 0;
         uint32_t buffer_phase = 0;
         bool ok = true;
-        for (int id = blockIdx.x; id < s.tiles && ok; id += gridDim.x) {
-            const Tile t = tile_of<COLUMNS>(id, s);
+        for (int id = first_tile; id < s.tiles && ok; id += tile_step) {
+            const Tile t = tile_of<Config::kTileRows, COLUMNS>(id, s);
             const int first = t.split * s.steps_per_split, last = min(s.k_steps, first + s.steps_per_split);
-            const int row0 = t.row + quarter * 32, slice = t.split * s.batch + t.matrix;
+            const int row0 = t.row + (int)rank * kMatmulRows + quarter * 32, slice = t.split * s.batch + t.matrix;
             const auto finish = [&](const float (&v)[kSpan], int col0) {
                 if (col0 >= s.n) return;
                 if (epilogue.by_column(row0, col0)) epilogue.template down<kSpan>(slice, row0 + lane, col0, v, s.m, min(kSpan, s.n - col0));
@@ -378,7 +391,10 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 }
                 tensor_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(sums_empty + buffer);
+                if (lane == 0) {
+                    if (PAIR) mbar_arrive_in_cluster(cluster_address(sums_empty + buffer, 0));
+                    else mbar_arrive(sums_empty + buffer);
+                }
                 buffer ^= 1;
                 buffer_phase ^= buffer == 0;
             }
@@ -404,7 +420,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     __syncwarp();
     tensor_fence_before();
     __syncthreads();
-    if (warp == Config::kWarps + 1) tensor_free(tensor, Config::kTensorColumns);
+    if (PAIR) cluster_sync();   // neither frees or leaves what the other one still uses
+    if (warp == Config::kWarps + 1) tensor_free<PAIR>(tensor, Config::kTensorColumns);
 }
 
 // An epilogue says which way a piece of a tile is handed to it (both, where a symmetric result is stored on both sides):

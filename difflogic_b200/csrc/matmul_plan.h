@@ -6,43 +6,50 @@
 namespace dl {
 
 struct MatmulPlan {
-    int columns;          // of a tile: 64, 128 or 256
+    int columns;            // of a tile: 64 or 128, or 256 with two CTAs to a tile of 256 rows
+    bool pair;
     int splits, steps_per_split;
     int64_t partial_bytes;  // of the sums of the splits; 0: one split
 };
 
-// Clocks of one SM, fitted to measured times: a step of 64 takes what its products or its copies take, whichever is longer, a tile what
-// it takes to fill and empty the pipe, a join of splits a launch.  The cheapest of the tile widths and splits is taken.
+// Tiles of a matrix; symmetric: those that reach to or below the diagonal.
+static inline int64_t tiles_of(int64_t m, int64_t n, int64_t rows, int64_t columns, bool symmetric) {
+    const int64_t down = ceil_div(m, rows), across = ceil_div(n, columns);
+    if (!symmetric) return down * across;
+    int64_t tiles = 0;
+    for (int64_t i = 0; i < down; ++i) {
+        const int64_t c = ceil_div((i + 1) * rows, columns);
+        tiles += c < across ? c : across;
+    }
+    return tiles;
+}
+
+// Clocks of one SM, fitted to measured times: a step of 64 takes what its products or its copies take (46 bytes a clock when all SMs
+// copy), whichever is longer, a tile what it takes to fill and empty the pipe, a join of splits a launch.  The cheapest of the tile
+// widths and splits is taken.
 static inline MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, int64_t batch, int planes, bool symmetric, int sms) {
     MatmulPlan best = {};
     double best_clocks = 0;
-    const int64_t steps = ceil_div(k, 64), tiles_m = ceil_div(m, 128);
+    const int64_t steps = ceil_div(k, 64);
     const int products = planes == 1 ? 1 : planes == 2 ? 3 : 6;
     const int only_columns = tuning(DL_TUNE_MATMUL_COLUMNS), only_splits = tuning(DL_TUNE_MATMUL_SPLITS);
-    for (int columns = 64; columns <= (planes == 3 ? 128 : 256); columns *= 2) {
-        if (only_columns > 0 ? columns != only_columns && !(planes == 3 && only_columns > 128 && columns == 128) : columns > 64 && n <= columns / 2) continue;
-        const int64_t tiles_n = ceil_div(n, columns);
-        int64_t per_matrix = tiles_m * tiles_n;
-        if (symmetric) {
-            per_matrix = 0;
-            for (int64_t mi = 0; mi < tiles_m; ++mi) {
-                const int64_t across = ceil_div((mi + 1) * 128, columns);
-                per_matrix += across < tiles_n ? across : tiles_n;
-            }
-        }
-        const double multiply = products * 4.0 * (columns < 128 ? 64 : columns / 2), copy = planes * (128 + columns) * 128 / 48.0;
+    for (int columns = 64; columns <= 256; columns *= 2) {
+        const bool pair = columns == 256;
+        if (only_columns > 0 ? columns != only_columns : columns > 64 && n <= columns / 2) continue;
+        const int64_t per_matrix = tiles_of(m, n, pair ? 256 : 128, columns, symmetric);
+        const double multiply = products * 2.0 * (columns < 128 ? 96 : columns), copy = planes * (128 + (pair ? 128 : columns)) * 128 / 46.0;
         const double step = multiply > copy ? multiply : copy;
         const double last = 600 + columns * 10.0;   // the epilogue of the last tile
         for (int64_t splits = 1; splits <= 64 && (splits == 1 || steps / splits >= 4); splits += splits < 4 ? 1 : splits / 2) {
             const int64_t per = ceil_div(steps, splits), really = ceil_div(steps, per);
             if (really != splits || (only_splits > 0 && splits > only_splits)) continue;
-            const int64_t tiles = per_matrix * batch * splits, waves = ceil_div(tiles, sms);
+            const int64_t tiles = per_matrix * batch * splits, waves = ceil_div(tiles, pair ? sms / 2 : sms);
             const int64_t partial = splits > 1 ? splits * batch * m * n * 4 : 0;
             if (partial > (int64_t)64 << 20) continue;
             double clocks = 1500 + waves * (per * step + 150) + last;
             if (splits > 1) clocks += 3000 + (double)partial / 2000;
             if (best.columns == 0 || clocks < best_clocks || (only_splits > 0 && splits > best.splits)) {
-                best = {columns, (int)splits, (int)per, partial};
+                best = {columns, pair, (int)splits, (int)per, partial};
                 best_clocks = clocks;
             }
         }

@@ -17,37 +17,87 @@ constexpr int kChunk = 64;                       // values in a tile's contiguou
 constexpr int kChunkBytes = kChunk * kChunk * 2;  // one copied tile
 
 #ifdef __CUDACC__
-__device__ __forceinline__ void tile_load(void *dst, const CUtensorMap *map, int inner, int row, int plane, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-                     smem_addr(dst)),
-                 "l"(map), "r"(inner), "r"(row), "r"(plane), "r"(smem_addr(bar))
-                 : "memory");
+// PAIR: two CTAs of a cluster work on one tile.  The barrier is then the first one's: `bar` is its address in the cluster.
+template <bool PAIR>
+__device__ __forceinline__ void tile_load(void *dst, const CUtensorMap *map, int inner, int row, int plane, uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                         smem_addr(dst)),
+                     "l"(map), "r"(inner), "r"(row), "r"(plane), "r"(bar)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                         smem_addr(dst)),
+                     "l"(map), "r"(inner), "r"(row), "r"(plane), "r"(bar)
+                     : "memory");
 }
 __device__ __forceinline__ void map_prefetch(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
-// Tensor memory: a whole warp takes `columns` (a power of two, 32 to 512) and gives them back.
-__device__ __forceinline__ void tensor_alloc(uint32_t *where, uint32_t columns) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(where)), "r"(columns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
 }
+// Address in the cluster of what lies at p in the shared memory of its CTA `rank`.
+__device__ __forceinline__ uint32_t cluster_address(const void *p, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void mbar_arrive_in_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Tensor memory: a whole warp (of both CTAs of a pair) takes `columns` (a power of two, 32 to 512) and gives them back.
+template <bool PAIR>
+__device__ __forceinline__ void tensor_alloc(uint32_t *where, uint32_t columns) {
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(where)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(where)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+}
+template <bool PAIR>
 __device__ __forceinline__ void tensor_free(uint32_t address, uint32_t columns) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns) : "memory");
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns) : "memory");
 }
 __device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// D (+)= A B^T over 16 values: 128 rows, the instruction descriptor says how many columns.
+// D (+)= A B^T over 16 values: 128 rows (256 of a pair, 128 in each CTA, which holds those of A and half of B), the instruction
+// descriptor says how many columns.
+template <bool PAIR>
 __device__ __forceinline__ void tensor_multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool add) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.u32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.u32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add)
+            : "memory");
 }
-// Arrives on `bar` once all products issued so far are done (and their reads of shared memory with them).
+// Arrives on `bar` (of both CTAs of a pair) once all products issued so far are done, and their reads of shared memory with them.
+template <bool PAIR>
 __device__ __forceinline__ void tensor_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 // 32 columns of the warp's 32 lanes of tensor memory: lane = row.
 __device__ __forceinline__ void tensor_read32(uint32_t address, uint32_t (&v)[32]) {
@@ -77,10 +127,10 @@ __device__ __forceinline__ uint64_t operand_descriptor(uint32_t address) {
 }
 #endif
 
-// 32-bit accumulation of fp16 (bf16: bfloat) operands, 128 x columns.
-static inline uint32_t instruction_descriptor(bool bfloat, bool a_mn, bool b_mn, int columns) {
+// 32-bit accumulation of fp16 (bf16: bfloat) operands, rows x columns.
+static inline uint32_t instruction_descriptor(bool bfloat, bool a_mn, bool b_mn, int rows, int columns) {
     return 1u << 4 | (uint32_t)bfloat << 7 | (uint32_t)bfloat << 10 | (uint32_t)a_mn << 15 | (uint32_t)b_mn << 16 |
-           (uint32_t)(columns / 8) << 17 | (128u / 16) << 24;
+           (uint32_t)(columns / 8) << 17 | (uint32_t)(rows / 16) << 24;
 }
 
 // Map of `planes` matrices of rows x inner 16-bit values, copied in tiles of 64 x 64; what lies outside reads as zero.  False where the

@@ -75,7 +75,7 @@ enum {
     DL_TUNE_FUSED_CLUSTER = 5,      /* dl_eval_groupbitsum: CTAs per class, 2, 4 or 8                            */
     DL_TUNE_FORWARD_KERNEL = 6,     /* dl_forward_f32: 1 = register kernel, 2 = staged (bulk-copy) kernel        */
     DL_TUNE_WALK_KERNEL = 7,        /* dl_backward_walk_f32: 1 = register kernel, 2 = staged kernel where it can  */
-    DL_TUNE_MATMUL_COLUMNS = 8,     /* matrix products: columns of a tile, 64, 128 or 256 where there is one     */
+    DL_TUNE_MATMUL_COLUMNS = 8,     /* matrix products: columns of a tile, 64, 128 or 256                          */
     DL_TUNE_MATMUL_SPLITS = 9,      /* matrix products: pieces that the sum is cut into, as far as it goes       */
     DL_TUNE_COUNT = 10
 };
