@@ -7,7 +7,7 @@ sm_100a kernels behind a C ABI (include/difflogic_b200.h).
 from .difflogic import LogicLayer, GroupSum
 from .packbitstensor import PackBitsTensor
 from .compiled_model import CompiledLogicNet
-from .dense import DenseLayer, dense
+from .denselayer import DenseLayer, dense
 from . import functional, ops
 
 __all__ = ["LogicLayer", "GroupSum", "PackBitsTensor", "CompiledLogicNet", "DenseLayer", "dense", "functional", "ops"]

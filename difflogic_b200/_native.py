@@ -115,6 +115,8 @@ SIGNATURES = {
     "dl_dense_backward": (_int, [_ptr, _int, _ptr, _ptr, _i64, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _int, _ptr]),
     "dl_orthogonalize_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
     "dl_orthogonalize": (_int, [_ptr, _ptr, _i64, _i64, _i64, _int, _int, _ptr, ctypes.c_double, _ptr, _ptr]),
+    "dl_muon_workspace_bytes": (_i64, [_ptr, _i64]),
+    "dl_muon_step_f32": (_int, [_ptr, _i64, ctypes.c_double, ctypes.c_double, _int, ctypes.c_double, _int, _ptr, ctypes.c_double, _ptr, _ptr]),
     "dl_prefetch_l2": (_int, [_ptr, ctypes.c_size_t, _ptr]),
 }
 

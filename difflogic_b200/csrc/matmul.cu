@@ -1,5 +1,8 @@
 // Dense layers and the orthogonalisation of matrices: the matrix products of matmul.cuh with their epilogues, what lays out their
 // operands, and the entry points.
+#include <math.h>
+
+#include "gram_steps.h"
 #include "matmul.cuh"
 #include "matmul_plan.h"
 
@@ -98,8 +101,8 @@ static int launch_columns(const Product &p, const MatmulPlan &plan, const Epilog
     s.splits = plan.splits;
     s.k_steps = (int32_t)ceil_div(p.k, kChunk);
     s.steps_per_split = plan.steps_per_split;
-    // one plane: nothing adds blocks up; wide tiles have one sum for large and small products, three or six of them a step
-    s.steps_per_sum = PLANES > 1 && p.exact ? (plan.columns == 256 ? 4 - PLANES : 2) : s.k_steps;
+    // one plane: nothing adds blocks up; wide tiles have one sum for large and small products
+    s.steps_per_sum = PLANES > 1 && p.exact ? (plan.columns == 256 ? 1 : 2) : s.k_steps;
     s.symmetric = p.symmetric;
     const int64_t per_matrix = tiles_of(p.m, p.n, rows, plan.columns, p.symmetric), tiles = per_matrix * s.splits * p.batch;
     if (tiles > INT32_MAX / 2) return fail(DL_ERR_TOO_LARGE, "%s: too many tiles", what);
@@ -598,17 +601,43 @@ extern "C" DL_API int dl_dense_backward(const void *gy, int g_feature_major, con
 
 namespace dl {
 
-// Sums of squares of a matrix, one per block, in 64 bits: fp32 values of any size fit.
+// What is orthogonalised: `count` matrices behind each other at entry 0, or one at every entry; with momenta the update of a step,
+// made of gradients and momenta as they are read.
+struct Matrices {
+    static constexpr int kMost = 16;
+    const void *g[kMost];
+    float *momentum[kMost];   // null: g as it is
+    float *weight[kMost];
+    int64_t stride;           // values from one matrix to the next at entry 0
+    int type;
+    float keep, nesterov;     // 1 - momentum; the momentum, or 1: the update is the momentum itself
+};
+
+// Sums of squares of a matrix, one per block, in 64 bits: fp32 values of any size fit.  Momenta are moved on.
 __global__ void __launch_bounds__(kThreads)
-square_sums_kernel(const void *__restrict__ g, int64_t count, int type, double *__restrict__ partial) {
+square_sums_kernel(const Matrices all, int64_t count, double *__restrict__ partial) {
     __shared__ double s_part[kThreads / 32];
     grid_dependency_wait();
     grid_dependents_launch();
-    const int64_t base = (int64_t)blockIdx.y * count, quads = (count + 3) / 4;
+    const int64_t z = blockIdx.y, base = all.stride * z, quads = (count + 3) / 4;
+    const int entry = all.stride ? 0 : (int)z;
+    const void *g = all.g[entry];
+    float *momentum = all.momentum[entry];
     double sum = 0;
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < quads; i += (int64_t)gridDim.x * kThreads) {
+        const int valid = (int)(count - i * 4 < 4 ? count - i * 4 : 4);
         float v[4];
-        load4(g, base + i * 4, type, (int)(count - i * 4 < 4 ? count - i * 4 : 4), v);
+        load4(g, base + i * 4, all.type, valid, v);
+        if (momentum != nullptr) {
+            float m[4];
+            load4(momentum, base + i * 4, kFloat32, valid, m);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                m[j] = new_momentum(m[j], v[j], all.keep);
+                v[j] = update_of(m[j], v[j], all.nesterov);
+            }
+            store4(momentum, base + i * 4, kFloat32, valid, m);
+        }
         sum += ((double)v[0] * v[0] + (double)v[1] * v[1]) + ((double)v[2] * v[2] + (double)v[3] * v[3]);
     }
 #pragma unroll
@@ -617,34 +646,44 @@ square_sums_kernel(const void *__restrict__ g, int64_t count, int type, double *
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int i = 1; i < kThreads / 32; ++i) sum += s_part[i];
-        partial[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = sum;
+        partial[z * gridDim.x + blockIdx.x] = sum;
     }
 }
 
 // X = G / max(|G|, eps) as pairs.
 __global__ void __launch_bounds__(kThreads)
-normalise_kernel(const void *__restrict__ g, int64_t rows, int64_t cols, int type, const double *__restrict__ partial, int parts, double eps,
+normalise_kernel(const Matrices all, int64_t rows, int64_t cols, const double *__restrict__ partial, int parts, double eps,
                  uint16_t *__restrict__ x, int64_t pitch, int64_t plane) {
     __shared__ float s_scale;
     grid_dependency_wait();
     grid_dependents_launch();
-    const int64_t z = blockIdx.y;
+    const int64_t z = blockIdx.y, base = all.stride * z;
+    const int entry = all.stride ? 0 : (int)z;
+    const void *g = all.g[entry];
+    const float *momentum = all.momentum[entry];
     if (threadIdx.x < 32) {
         double sum = 0;
         for (int i = threadIdx.x; i < parts; i += 32) sum += partial[z * parts + i];
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         const double norm = sqrt(sum);
-        // a scale that is not finite (an infinite or undefined entry) makes the whole result undefined
+        // a norm that is not finite (an infinite or undefined entry) makes the whole result undefined
         if (threadIdx.x == 0) s_scale = norm <= 1.7e308 ? (float)((double)kPairScale / (norm > eps ? norm : eps)) : __int_as_float(0x7fc00000);
     }
     __syncthreads();
     const float scale = s_scale;
     const int64_t quads = (cols + 3) / 4, total = rows * quads;
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-        const int64_t row = i / quads, col = (i - row * quads) * 4;
+        const int64_t row = i / quads, col = (i - row * quads) * 4, at = base + row * cols + col;
+        const int valid = (int)(cols - col < 4 ? cols - col : 4);
         float v[4];
-        load4(g, (z * rows + row) * cols + col, type, (int)(cols - col < 4 ? cols - col : 4), v);
+        load4(g, at, all.type, valid, v);
+        if (momentum != nullptr) {
+            float m[4];
+            load4(momentum, at, kFloat32, valid, m);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = update_of(m[j], v[j], all.nesterov);
+        }
         uint16_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) split_pair(v[j] * scale, hi[j], lo[j]);
@@ -722,13 +761,12 @@ struct PairEpilogue {
 // The last product: the result itself, or the weights' update w <- decay w - rate v.
 struct OrthogonalEpilogue {
     static constexpr int kPlanes = 2;
-    void *out;
+    void *out;              // results behind each other; null: the weights of `all` are updated
+    Matrices all;
     int64_t cols, matrix;   // values of a row, of a matrix
     const uint16_t *more;   // added, as in PairEpilogue
     int64_t pitch, plane;
     float scale, factor;
-    int type;
-    bool update;
     float decay, rate;
     __device__ __forceinline__ bool by_column(int, int) const { return false; }
     __device__ __forceinline__ bool by_row(int, int) const { return true; }
@@ -736,11 +774,12 @@ struct OrthogonalEpilogue {
     __device__ __forceinline__ void down(int, int, int, const float (&)[N], int, int) const {}
     template <int N, int STEP>
     __device__ __forceinline__ void across(int z, int row, int col, const float (&sum)[N][4], int m, int valid) const {
+        float *weight = out == nullptr ? all.weight[z] : nullptr;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int r = row + i * STEP;
             if (r >= m) break;
-            const int64_t at = z * matrix + r * cols + col;
+            const int64_t at = r * cols + col;
             float v[4], w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = sum[i][j] * scale;
@@ -752,12 +791,14 @@ struct OrthogonalEpilogue {
                 v[2] += factor * join_pair(hi.z, lo.z);
                 v[3] += factor * join_pair(hi.w, lo.w);
             }
-            if (update) {
-                load4(out, at, kFloat32, valid, w);
+            if (weight != nullptr) {
+                load4(weight, at, kFloat32, valid, w);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] = w[j] * decay - rate * v[j];
+                store4(weight, at, kFloat32, valid, v);
+            } else {
+                store4(out, z * matrix + at, all.type, valid, v);
             }
-            store4(out, at, type, valid, v);
         }
     }
 };
@@ -800,20 +841,20 @@ static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t c
 // 1.7e-3); S^2 from pairs; X M from the first planes, a X added as the pair that it is.  That last form matters: what is rounded away
 // of X in a product with a I + b S + c S^2 grows by a factor of a in every step along directions of small singular values, 4e-2 in the
 // end where X has few large ones; M alone is next to nothing along those.  All together 1.6e-3, half the products.
-static int orthogonalise(const void *g, int type, int64_t batch, int64_t rows, int64_t cols, int steps, const float *coefficients, double eps,
+static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64_t cols, int steps, const float *coefficients, double eps,
                          const OrthogonalEpilogue &last, uint8_t *workspace, int sms, cudaStream_t st, const char *what) {
-    const bool light = type == kBFloat16;
+    const bool light = all.type == kBFloat16;
     const OrthogonalLayout l = orthogonal_layout(batch, rows, cols, light, sms);
     uint16_t *x = reinterpret_cast<uint16_t *>(workspace), *next = reinterpret_cast<uint16_t *>(workspace + l.x_bytes);
     uint16_t *gram = reinterpret_cast<uint16_t *>(workspace + 2 * l.x_bytes), *poly = reinterpret_cast<uint16_t *>(workspace + 2 * l.x_bytes + l.s_bytes);
     double *norms = reinterpret_cast<double *>(workspace + 2 * l.x_bytes + 2 * l.s_bytes);
     float *partial = reinterpret_cast<float *>(workspace + 2 * l.x_bytes + 2 * l.s_bytes + l.norm_bytes);
     int status;
-    launch_dependent(true, square_sums_kernel, dim3((unsigned)l.parts, (unsigned)batch), dim3(kThreads), 0, st, g, rows * cols, type, norms);
+    launch_dependent(true, square_sums_kernel, dim3((unsigned)l.parts, (unsigned)batch), dim3(kThreads), 0, st, all, rows * cols, norms);
     if ((status = launch_status(what)) != DL_OK) return status;
     int64_t blocks = ceil_div(rows * ceil_div(cols, 4), kThreads * 2);
     if (blocks > 16 * sms) blocks = 16 * sms;
-    launch_dependent(true, normalise_kernel, dim3((unsigned)blocks, (unsigned)batch), dim3(kThreads), 0, st, g, rows, cols, type, (const double *)norms,
+    launch_dependent(true, normalise_kernel, dim3((unsigned)blocks, (unsigned)batch), dim3(kThreads), 0, st, all, rows, cols, (const double *)norms,
                      l.parts, eps, x, l.x_pitch, l.x_plane);
     if ((status = launch_status(what)) != DL_OK) return status;
     Product p = {};
@@ -848,6 +889,9 @@ static int orthogonalise(const void *g, int type, int64_t batch, int64_t rows, i
             status = launch_planes(p, l.product, to_next, partial, sms, st, what);
         } else {
             OrthogonalEpilogue e = last;
+            e.all = all;
+            e.cols = cols;
+            e.matrix = rows * cols;
             e.more = more;
             e.pitch = l.x_pitch;
             e.plane = l.x_plane;
@@ -865,9 +909,19 @@ static int orthogonalise(const void *g, int type, int64_t batch, int64_t rows, i
 
 }  // namespace dl
 
+// Matrices of so few columns stay as they are: their Gram matrix is iterated instead (gram_steps.cu).
+static bool few_columns(int64_t cols) { return cols <= kGramColumns; }
+
 extern "C" DL_API int64_t dl_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int type) {
     if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
+    if (few_columns(cols)) return gram_workspace_bytes(batch, batch * rows, current_sms());
     return orthogonal_layout(batch, rows, cols, type == kBFloat16, current_sms()).total();
+}
+
+static int check_steps(int steps, const float *coefficients, double eps, const char *what) {
+    DL_REQUIRE(steps >= 1 && steps <= kMostSteps && coefficients, DL_ERR_INVALID_ARG, "%s: needs 1 to %d steps and their coefficients", what, kMostSteps);
+    DL_REQUIRE(eps > 0, DL_ERR_INVALID_ARG, "%s: eps must be positive", what);
+    return DL_OK;
 }
 
 extern "C" DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, int64_t rows, int64_t cols, int type, int steps,
@@ -876,16 +930,144 @@ extern "C" DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, 
     DL_REQUIRE(batch >= 0 && rows >= 0 && cols >= 0 && rows <= INT32_MAX / 2 && cols <= INT32_MAX / 2, DL_ERR_INVALID_ARG, "%s: bad size", what);
     DL_REQUIRE(batch <= 65535, DL_ERR_TOO_LARGE, "%s: more than 65535 matrices", what);
     DL_REQUIRE(type >= kFloat32 && type <= kFloat16, DL_ERR_INVALID_ARG, "%s: unknown type %d", what, type);
-    DL_REQUIRE(steps >= 1 && steps <= 64 && coefficients, DL_ERR_INVALID_ARG, "%s: needs 1 to 64 steps and their coefficients", what);
-    DL_REQUIRE(eps > 0, DL_ERR_INVALID_ARG, "%s: eps must be positive", what);
+    int status = check_steps(steps, coefficients, eps, what);
+    if (status != DL_OK) return status;
     if (batch == 0 || rows == 0 || cols == 0) return DL_OK;
     DL_REQUIRE(g && out && workspace, DL_ERR_INVALID_ARG, "%s: null pointer", what);
     DL_REQUIRE(aligned_to(workspace, 16), DL_ERR_INVALID_ARG, "%s: the workspace must be 16-byte aligned", what);
+    if (few_columns(cols)) {
+        GramJob job = {};
+        job.count = 1;
+        job.batch = batch;
+        job.matrix[0] = {g, nullptr, out, rows, 0.f};
+        job.cols = (int)cols;
+        job.type = type;
+        return launch_gram_steps(job, steps, coefficients, eps, reinterpret_cast<double *>(workspace), current_sms(), as_stream(stream), what);
+    }
+    Matrices all = {};
+    all.g[0] = g;
+    all.stride = rows * cols;
+    all.type = type;
     OrthogonalEpilogue last = {};
     last.out = out;
-    last.cols = cols;
-    last.matrix = rows * cols;
-    last.type = type;
-    return orthogonalise(g, type, batch, rows, cols, steps, coefficients, eps, last, reinterpret_cast<uint8_t *>(workspace), current_sms(),
+    return orthogonalise(all, batch, rows, cols, steps, coefficients, eps, last, reinterpret_cast<uint8_t *>(workspace), current_sms(),
                          as_stream(stream), what);
+}
+
+// One step: the matrices of few columns together, then those of one shape after the other.
+namespace dl {
+
+template <class Few, class Many>
+static int over_muon_groups(const int64_t *table, int64_t count, const Few &few, const Many &many) {
+    int status = DL_OK;
+    for (int64_t i = 0; i < count && status == DL_OK; ++i) {   // every group at its first matrix
+        const int64_t *at = table + 5 * i;
+        GramJob job = {};
+        if (few_columns(at[4])) {
+            bool taken = false;   // by an earlier group of this number of columns
+            for (int64_t j = 0; j < i; ++j) taken |= table[5 * j + 4] == at[4];
+            if (!taken) {
+                job.cols = (int)at[4];
+                for (int64_t j = i; j < count && status == DL_OK; ++j) {
+                    const int64_t *t = table + 5 * j;
+                    if (t[4] != at[4] || t[3] == 0) continue;
+                    job.matrix[job.count++] = {reinterpret_cast<const void *>(t[1]), reinterpret_cast<float *>(t[2]), reinterpret_cast<void *>(t[0]), t[3], 0.f};
+                    if (job.count == GramJob::kMost) {
+                        status = few(job);
+                        job.count = 0;
+                    }
+                }
+                if (job.count > 0 && status == DL_OK) status = few(job);
+            }
+        } else {
+            bool taken = at[3] == 0;
+            for (int64_t j = 0; j < i; ++j) taken |= table[5 * j + 3] == at[3] && table[5 * j + 4] == at[4];
+            if (!taken) {
+                Matrices all = {};
+                int64_t batch = 0;
+                for (int64_t j = i; j < count && status == DL_OK; ++j) {
+                    const int64_t *t = table + 5 * j;
+                    if (t[3] != at[3] || t[4] != at[4]) continue;
+                    all.weight[batch] = reinterpret_cast<float *>(t[0]);
+                    all.g[batch] = reinterpret_cast<const void *>(t[1]);
+                    all.momentum[batch++] = reinterpret_cast<float *>(t[2]);
+                    if (batch == Matrices::kMost) {
+                        status = many(all, batch, at[3], at[4]);
+                        batch = 0;
+                    }
+                }
+                if (batch > 0 && status == DL_OK) status = many(all, batch, at[3], at[4]);
+            }
+        }
+    }
+    return status;
+}
+
+static int64_t rows_of(const GramJob &job) {
+    int64_t rows = 0;
+    for (int i = 0; i < job.count; ++i) rows += job.matrix[i].rows;
+    return rows * job.batch;
+}
+
+}  // namespace dl
+
+extern "C" DL_API int64_t dl_muon_workspace_bytes(const int64_t *table, int64_t count) {
+    if (table == nullptr) return 0;
+    const int sms = current_sms();
+    int64_t most = 0;
+    over_muon_groups(
+        table, count,
+        [&](GramJob &job) {
+            job.batch = 1;
+            const int64_t bytes = gram_workspace_bytes(job.count, rows_of(job), sms);
+            if (bytes > most) most = bytes;
+            return DL_OK;
+        },
+        [&](Matrices &, int64_t batch, int64_t rows, int64_t cols) {
+            const int64_t bytes = orthogonal_layout(batch, rows, cols, false, sms).total();
+            if (bytes > most) most = bytes;
+            return DL_OK;
+        });
+    return most;
+}
+
+extern "C" DL_API int dl_muon_step_f32(const int64_t *table, int64_t count, double lr, double momentum, int nesterov, double weight_decay, int steps,
+                                       const float *coefficients, double eps, void *workspace, void *stream) {
+    const char *what = "dl_muon_step_f32";
+    DL_REQUIRE(count >= 0 && (table || count == 0), DL_ERR_INVALID_ARG, "%s: null pointer", what);
+    int status = check_steps(steps, coefficients, eps, what);
+    if (status != DL_OK) return status;
+    for (int64_t i = 0; i < count; ++i) {
+        const int64_t *t = table + 5 * i;
+        DL_REQUIRE(t[3] >= 0 && t[4] > 0 && t[3] <= INT32_MAX / 2 && t[4] <= INT32_MAX / 2, DL_ERR_INVALID_ARG, "%s: bad size", what);
+        DL_REQUIRE(t[3] == 0 || (t[0] && t[1] && t[2]), DL_ERR_INVALID_ARG, "%s: null pointer", what);
+        DL_REQUIRE((t[0] | t[1] | t[2]) % 4 == 0, DL_ERR_INVALID_ARG, "%s: misaligned matrix", what);
+    }
+    if (count == 0) return DL_OK;
+    DL_REQUIRE(workspace && aligned_to(workspace, 16), DL_ERR_INVALID_ARG, "%s: the workspace is missing or not 16-byte aligned", what);
+    const int sms = current_sms();
+    cudaStream_t st = as_stream(stream);
+    const auto rate = [&](int64_t rows, int64_t cols) { return (float)(lr * sqrt(rows > cols ? (double)rows / (double)cols : 1.0)); };
+    const float keep = (float)(1.0 - momentum), toward = nesterov ? (float)momentum : 1.f, decay = (float)(1.0 - lr * weight_decay);
+    return over_muon_groups(
+        table, count,
+        [&](GramJob &job) {
+            job.batch = 1;
+            job.type = kFloat32;
+            job.update = true;
+            job.keep = keep;
+            job.nesterov = toward;
+            job.decay = decay;
+            for (int i = 0; i < job.count; ++i) job.matrix[i].rate = rate(job.matrix[i].rows, job.cols);
+            return launch_gram_steps(job, steps, coefficients, eps, reinterpret_cast<double *>(workspace), sms, st, what);
+        },
+        [&](Matrices &all, int64_t batch, int64_t rows, int64_t cols) {
+            all.type = kFloat32;
+            all.keep = keep;
+            all.nesterov = toward;
+            OrthogonalEpilogue last = {};
+            last.decay = decay;
+            last.rate = rate(rows, cols);
+            return orthogonalise(all, batch, rows, cols, steps, coefficients, eps, last, reinterpret_cast<uint8_t *>(workspace), sms, st, what);
+        });
 }

@@ -11,15 +11,10 @@
 // of their own.
 #pragma once
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
+#include "matmul_values.cuh"
 #include "tensor_core.cuh"
 
 namespace dl {
-
-enum MatmulType { kFloat32 = 0, kBFloat16 = 1, kFloat16 = 2 };
-static inline int type_size(int type) { return type == kFloat32 ? 4 : 2; }
 
 struct Operand {       // rows x k, or k x rows where mn: the rows of the result are contiguous
     const void *base;
@@ -64,45 +59,6 @@ __device__ __forceinline__ void split_triple(float x, uint16_t &hi, uint16_t &mi
     h = __float2bfloat16_rn(rest);
     mid = __bfloat16_as_ushort(h);
     lo = __bfloat16_as_ushort(__float2bfloat16_rn(rest - __bfloat162float(h)));
-}
-
-__device__ __forceinline__ float load_as_float(const void *p, int64_t i, int type) {
-    if (type == kFloat32) return reinterpret_cast<const float *>(p)[i];
-    const uint16_t v = reinterpret_cast<const uint16_t *>(p)[i];
-    return type == kBFloat16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
-}
-__device__ __forceinline__ uint16_t to_16bit(float v, int type) {
-    return type == kBFloat16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
-}
-// Up to four neighbouring values, in one access where all are there and the address allows it.
-__device__ __forceinline__ void load4(const void *p, int64_t i, int type, int valid, float (&v)[4]) {
-    const char *at = reinterpret_cast<const char *>(p) + i * (type == kFloat32 ? 4 : 2);
-    if (valid == 4 && type == kFloat32 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
-        const float4 f = *reinterpret_cast<const float4 *>(at);
-        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-    } else if (valid == 4 && type != kFloat32 && (reinterpret_cast<uintptr_t>(at) & 7) == 0) {
-        const ushort4 u = *reinterpret_cast<const ushort4 *>(at);
-        v[0] = load_as_float(&u.x, 0, type); v[1] = load_as_float(&u.y, 0, type);
-        v[2] = load_as_float(&u.z, 0, type); v[3] = load_as_float(&u.w, 0, type);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = j < valid ? load_as_float(p, i + j, type) : 0.f;
-    }
-}
-__device__ __forceinline__ void store4(void *p, int64_t i, int type, int valid, const float (&v)[4]) {
-    char *at = reinterpret_cast<char *>(p) + i * (type == kFloat32 ? 4 : 2);
-    if (valid == 4 && type == kFloat32 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
-        *reinterpret_cast<float4 *>(at) = make_float4(v[0], v[1], v[2], v[3]);
-    } else if (valid == 4 && type != kFloat32 && (reinterpret_cast<uintptr_t>(at) & 7) == 0) {
-        *reinterpret_cast<ushort4 *>(at) = make_ushort4(to_16bit(v[0], type), to_16bit(v[1], type), to_16bit(v[2], type), to_16bit(v[3], type));
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < valid) {
-                if (type == kFloat32) reinterpret_cast<float *>(p)[i + j] = v[j];
-                else reinterpret_cast<uint16_t *>(p)[i + j] = to_16bit(v[j], type);
-            }
-    }
 }
 
 // -- the kernel -----------------------------------------------------------------------------------------------------------------
@@ -292,16 +248,17 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                                 tensor_multiply<PAIR>(sum, from_a + k * a_step, from_b + k * b_step, s.instruction, !(fresh && k == 0));
                         };
                         const bool fresh = step == block;
-                        product(0, 0, large, fresh);
-                        if (PLANES > 1) {
-                            product(0, 1, small, fresh && Config::kSums == 2);
-                            product(1, 0, small, false);
-                        }
+                        // the smallest products first: where they share a sum with the large ones, it cuts off little of them
                         if (PLANES > 2) {
-                            product(1, 1, small, false);
+                            product(1, 1, small, fresh);
                             product(0, 2, small, false);
                             product(2, 0, small, false);
                         }
+                        if (PLANES > 1) {
+                            product(0, 1, small, fresh && PLANES == 2);
+                            product(1, 0, small, false);
+                        }
+                        product(0, 0, large, fresh && (PLANES == 1 || Config::kSums == 2));
                         tensor_commit<PAIR>(empty + stage);
                         if (++stage == kStages) {
                             stage = 0;

@@ -993,3 +993,45 @@ def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
         N.check(lib.dl_orthogonalize(x.data_ptr(), out.data_ptr(), batch, rows, cols, _FLOAT_TYPES[x.dtype], steps, table, eps, work.data_ptr(),
                                      N.stream_of(x)))
     return out
+
+
+def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
+    """One step of the Muon optimizer on matrices, in place: for every weight w with its gradient g and momentum buffer m
+        m += (1 - momentum) (g - m);  u = g + momentum (m - g) (nesterov) or m
+        w = (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) orthogonalize(u)
+    which is torch.optim.Muon's rule, in 32 bits.  weights, grads, momenta: lists of 2-D contiguous float32 tensors on one CUDA device, of
+    which no two weights or momenta share memory."""
+    weights, grads, momenta = list(weights), list(grads), list(momenta)
+    if not len(weights) == len(grads) == len(momenta):
+        raise ValueError("muon_step: %d weights, %d gradients, %d momenta" % (len(weights), len(grads), len(momenta)))
+    table = _newton_schulz(_coefficients(coefficients), steps)
+    if not (0 <= momentum < 1 and lr >= 0 and weight_decay >= 0 and 0 < eps < math.inf):
+        raise ValueError("muon_step: needs 0 <= momentum < 1, lr >= 0, weight_decay >= 0 and eps > 0, got %r, %r, %r, %r" % (momentum, lr, weight_decay, eps))
+    if not weights:
+        return
+    entries, written = [], set()
+    device = weights[0].device
+    for w, g, m in zip(weights, grads, momenta):
+        shape = w.shape
+        for t in (w, g, m):
+            if not (t.is_cuda and t.dtype is torch.float32 and t.dim() == 2 and t.shape == shape and t.is_contiguous() and t.device == device):
+                N.require_cuda(t)
+                raise ValueError("muon_step: needs contiguous 2-D float32 tensors of one shape on one device, got %s %s on %s beside %s on %s"
+                                 % (t.dtype, tuple(t.shape), t.device, tuple(shape), device))
+        if w.numel() == 0:
+            continue
+        pw, pm = w.data_ptr(), m.data_ptr()
+        if pw in written or pm in written or pw == pm:
+            raise ValueError("muon_step: a weight or momentum is in the lists twice")
+        written.add(pw)
+        written.add(pm)
+        entries += (pw, g.data_ptr(), pm, shape[0], shape[1])
+    if not entries:
+        return
+    lib, count = N.lib(), len(entries) // 5
+    entries = (ctypes.c_int64 * len(entries))(*entries)
+    with N.on_device(weights[0]):
+        work = torch.empty(lib.dl_muon_workspace_bytes(entries, count), dtype=torch.uint8, device=device)
+        N.check(lib.dl_muon_step_f32(entries, count, lr, momentum, nesterov, weight_decay, steps, table, eps, work.data_ptr(), N.stream_of(weights[0])))
+    from .optim import count_update
+    count_update(weights)

@@ -10,6 +10,9 @@ LogicLayer's backward writes each layer's weight gradient straight into its slic
 gradient buffer (`grad_view(param)`), so in data-parallel training the buffer can be all-reduced as it
 is and no gradient is copied.  The step counter lives on the device: a step can be captured in a CUDA
 graph and replayed.
+
+`FlatMuon` keeps parameters, gradients and momenta of matrices (logic layers' gate weights, dense layers' weights) in the same
+layout and moves them along the nearest orthogonal matrix to their momentum (ops.muon_step); vectors take Adam's step.
 """
 import torch
 
@@ -496,4 +499,119 @@ class FlatAdam(torch.optim.Optimizer):
                                              float(beta2), float(g['eps']), float(self.grad_scale), self.state_t.data_ptr(),
                                              N.stream_of(self.flat_param)))
         self.mark_updated()
+        return loss
+
+
+class FlatMuon(torch.optim.Optimizer):
+    """Muon for the matrices of a network (ops.muon_step: torch.optim.Muon's rule in 32 bits), Adam for its vectors (biases).
+
+    :param lr, weight_decay, momentum, nesterov, ns_coefficients, eps, ns_steps: of the matrices, as torch.optim.Muon has them; the rate
+                      of a matrix is lr sqrt(max(1, rows / cols))
+    :param adam_lr, betas, adam_eps: of the vectors, which take no weight decay
+
+    The buffers have FlatAdam's layout: LogicLayer's backward writes into `flat_grad`, and TrainStep all-reduces pieces of it.  A parameter
+    without a gradient is left alone.  A step can be captured in a CUDA graph."""
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=None, eps=1e-7, ns_steps=5,
+                 adam_lr=1e-3, betas=(0.9, 0.999), adam_eps=1e-8):
+        from . import ops
+        ns_coefficients = ops.NEWTON_SCHULZ if ns_coefficients is None else ops._coefficients(ns_coefficients)
+        ops._newton_schulz(ns_coefficients, ns_steps)
+        if not (0 <= momentum < 1 and lr >= 0 and weight_decay >= 0 and eps > 0 and adam_lr >= 0 and adam_eps >= 0
+                and 0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError("FlatMuon: a rate, momentum, decay or eps outside its range")
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov, ns_coefficients=ns_coefficients,
+                                      eps=eps, ns_steps=ns_steps, adam_lr=adam_lr, betas=betas, adam_eps=adam_eps))
+        plist = [p for g in self.param_groups for p in g['params']]
+        if len(self.param_groups) != 1:
+            raise ValueError("FlatMuon supports a single parameter group")
+        if not plist:
+            raise ValueError("FlatMuon got an empty parameter list")
+        dev = plist[0].device
+        for p in plist:
+            if not (p.is_cuda and p.dtype == torch.float32 and p.device == dev):
+                raise ValueError("FlatMuon needs float32 CUDA parameters on one device")
+            if p.dim() > 2:
+                raise ValueError("FlatMuon takes matrices and vectors, got a parameter of %d dimensions" % p.dim())
+        self._matrices = [p for p in plist if p.dim() == 2]
+        self._vectors = [p for p in plist if p.dim() < 2]
+        size = lambda p: (p.numel() + 3) // 4 * 4  # noqa: E731  every slice 16-byte aligned
+        total, self._first_vector = sum(map(size, plist)), sum(map(size, self._matrices))
+        self.flat_param, self.flat_grad, self.flat_momentum = (torch.zeros(total, dtype=torch.float32, device=dev) for _ in range(3))
+        self.exp_avg_sq = torch.zeros(total - self._first_vector, dtype=torch.float32, device=dev)   # of the vectors; their momenta are Adam's first moments
+        self.state_t = torch.zeros(2, dtype=torch.int32, device=dev)  # Adam's {steps done, ticket}
+        self._slices = {}
+        off = 0
+        with torch.no_grad():
+            for p in self._matrices + self._vectors:
+                view = self.flat_param[off:off + p.numel()].view_as(p)
+                view.copy_(p)
+                p.data = view
+                self._slices[p] = (off, p.numel())
+                p._dl_grad_out = self.grad_view(p)
+                off += size(p)
+        self._link_state()
+
+    def _link_state(self):
+        """`state` shows the buffers, so that state_dict() has them."""
+        for p, (off, n) in self._slices.items():
+            self.state[p]['momentum_buffer'] = self.flat_momentum[off:off + n].view_as(p)
+            if p.dim() < 2:
+                self.state[p]['exp_avg_sq'] = self.exp_avg_sq[off - self._first_vector:off - self._first_vector + n].view_as(p)
+                self.state[p]['step'] = self.state_t[0]
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        loaded = {p: dict(self.state[p]) for p in self._slices}
+        self.state.clear()
+        self._link_state()
+        with torch.no_grad():
+            for p, kept in loaded.items():
+                for name, value in kept.items():
+                    self.state[p][name].copy_(value)
+
+    def grad_view(self, p):
+        off, n = self._slices[p]
+        return self.flat_grad[off:off + n].view_as(p)
+
+    def zero_grad(self, set_to_none=True):
+        # layers overwrite their gradients; dropping the references is enough
+        for p in self._slices:
+            p.grad = None
+
+    def mark_updated(self):
+        """Tells whoever has derived something from the weights that kernels have updated them (count_update)."""
+        count_update(self._matrices + self._vectors)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        from . import ops
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        g = self.param_groups[0]
+        matrices = [p for p in self._matrices if p.grad is not None]
+        grads = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in matrices]
+        ops.muon_step([p.data for p in matrices], grads, [self.state[p]['momentum_buffer'] for p in matrices], lr=g['lr'], momentum=g['momentum'],
+                      nesterov=g['nesterov'], weight_decay=g['weight_decay'], steps=g['ns_steps'], coefficients=g['ns_coefficients'], eps=g['eps'])
+        count_update(matrices)
+        vectors = [p for p in self._vectors if p.grad is not None]
+        if vectors:
+            # one kernel over the vectors' part of the flat buffers
+            for p in vectors:
+                view = self.grad_view(p)
+                if p.grad.data_ptr() != view.data_ptr():
+                    view.copy_(p.grad)
+            if len(vectors) != len(self._vectors):
+                raise RuntimeError("FlatMuon: some vectors have a gradient and some have none; give those that are not trained requires_grad=False "
+                                   "and leave them out")
+            beta1, beta2 = g['betas']
+            first = self._first_vector
+            with N.on_device(self.flat_param):
+                N.check(N.lib().dl_adam_step_f32(self.flat_param[first:].data_ptr(), self.flat_grad[first:].data_ptr(),
+                                                 self.flat_momentum[first:].data_ptr(), self.exp_avg_sq.data_ptr(), self.exp_avg_sq.numel(),
+                                                 float(g['adam_lr']), float(beta1), float(beta2), float(g['adam_eps']), 1.0, self.state_t.data_ptr(),
+                                                 N.stream_of(self.flat_param)))
+            count_update(vectors)
         return loss

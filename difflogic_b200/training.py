@@ -173,6 +173,10 @@ class TrainStep:
             return
         if param in self._bucket_of:
             bi = self._bucket_of[param]
+            inside = self.optimizer.grad_view(param)
+            if param.grad.data_ptr() != inside.data_ptr():   # a dense layer's: its slice of the flat buffer is what is reduced
+                inside.copy_(param.grad)
+                param.grad = inside
             self._pending[bi] -= 1
             if self._pending[bi] == 0:
                 self._launch_all_reduce(self._bucket_slices[bi])
