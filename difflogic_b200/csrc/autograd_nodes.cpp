@@ -1,4 +1,4 @@
-// Autograd nodes of the training path in native code: one node per LogicLayer and one for GroupSum.
+// Autograd nodes of the training path in native code: one node per LogicLayer, one for GroupSum and one per dense layer.
 //
 // What a training step of a small network costs is the host: a Python autograd function with its views, checks and ctypes calls took
 // 40 us forward and 60 us backward per layer, for kernels of 3 to 10 us.  These nodes do the same -- same kernels, same
@@ -21,6 +21,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/object_ptr.h>
@@ -294,6 +295,171 @@ PyObject *group_sum(PyObject *, PyObject *const *args, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
+// -- dense layers -----------------------------------------------------------------------------------------------------------------
+// What denselayer.py's Python functions do, with its messages left to them.
+
+struct Matrix {   // a 2-D tensor as the kernels read it: its rows apart, or its columns
+    Tensor t;
+    int64_t pitch;
+    bool feature_major;
+};
+Matrix readable(const Tensor &t) {
+    const int64_t rows = t.size(0), cols = t.size(1), s0 = t.stride(0), s1 = t.stride(1);
+    if ((s1 == 1 || cols == 1) && (s0 >= cols || rows == 1)) return {t, rows > 1 ? s0 : cols, false};
+    if ((s0 == 1 || rows == 1) && (s1 >= rows || cols == 1)) return {t, cols > 1 ? s1 : rows, true};
+    return {t.contiguous(), cols, false};
+}
+int kind_of(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : 2; }
+Tensor bytes(int64_t n, const Tensor &like) { return n > 0 ? at::empty({n}, like.options().dtype(at::kByte).requires_grad(false)) : Tensor(); }
+void *pointer(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+struct DenseOut {
+    Tensor y, slope, x_planes, w_planes;
+    Matrix x;
+};
+DenseOut dense_forward(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &residual, int act, bool feature_major, bool want_slope) {
+    const int64_t batch = x.size(0), inner = x.size(1), outer = w.size(0);
+    const int kind = kind_of(x.scalar_type());
+    const auto options = x.options().requires_grad(false);
+    DenseOut o;
+    o.y = feature_major ? at::empty_strided({batch, outer}, {1, batch}, options) : at::empty({batch, outer}, options);
+    if (want_slope && act != DL_ACT_NONE) o.slope = at::empty({batch * outer}, options.dtype(kind == 0 ? at::kFloat : at::kHalf));
+    o.x = readable(x);
+    int64_t sizes[3];
+    dl_dense_forward_sizes(o.x.t.data_ptr(), o.x.pitch, o.x.feature_major, w.data_ptr(), batch, inner, outer, kind, sizes);
+    o.x_planes = bytes(sizes[0], x);
+    o.w_planes = bytes(sizes[1], x);
+    const Tensor work = bytes(sizes[2], x);
+    check(dl_dense_forward(o.x.t.data_ptr(), o.x.pitch, o.x.feature_major, w.data_ptr(), pointer(bias), pointer(residual),
+                           residual.defined() ? residual.stride(0) : 0, residual.defined() ? residual.stride(1) : 0, act, o.y.data_ptr(), feature_major,
+                           pointer(o.slope), pointer(o.x_planes), pointer(o.w_planes), pointer(work), batch, inner, outer, kind, stream_of(x)));
+    return o;
+}
+
+struct DenseNode : torch::autograd::Function<DenseNode> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const std::optional<Tensor> &b, const std::optional<Tensor> &r,
+                          int64_t act, bool feature_major) {
+        const Tensor bias = b.value_or(Tensor()), residual = r.value_or(Tensor());
+        const DenseOut o = dense_forward(x, w, bias, residual, (int)act, feature_major, true);
+        ctx->set_materialize_grads(false);
+        // what was laid out for the product serves the backward pass too, in place of the tensor itself
+        ctx->save_for_backward({o.x_planes.defined() ? Tensor() : o.x.t, o.w_planes.defined() ? Tensor() : w, o.x_planes, o.w_planes, o.slope});
+        ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(0), x.size(1), w.size(0), o.x.pitch, o.x.feature_major, feature_major, b.has_value(), r.has_value()};
+        // their alignment decided what was laid out
+        ctx->saved_data["at"] = std::vector<int64_t>{(int64_t)o.x.t.data_ptr(), (int64_t)w.data_ptr()};
+        return o.y;
+    }
+
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        variable_list out(6);
+        Tensor gy = grads[0];
+        if (!gy.defined()) return out;
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &x_planes = saved[2], &w_planes = saved[3], &slope = saved[4];
+        const auto sizes = ctx->saved_data["sizes"].toIntVector(), at = ctx->saved_data["at"].toIntVector();
+        const int64_t batch = sizes[0], inner = sizes[1], outer = sizes[2], pitch = sizes[3];
+        const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = sizes[6] && ctx->needs_input_grad(2);
+        const c10::cuda::CUDAGuard guard(gy.device());
+        if (want_x || want_w || want_b) {
+            TORCH_CHECK(gy.dim() == 2 && gy.size(0) == batch && gy.size(1) == outer && gy.is_cuda() &&
+                            (!x.defined() || (x.scalar_type() == gy.scalar_type() && x.device() == gy.device() && x.dim() == 2 && x.size(0) == batch &&
+                                              x.size(1) == inner && readable(x).t.is_same(x))) &&
+                            (!w.defined() || matrix_of(w, gy.scalar_type(), outer, inner, gy.device())),
+                        "difflogic_b200: the backward pass of a dense layer got tensors of other types, sizes or layouts than its forward pass");
+            const at::NoGradGuard no_grad;
+            Tensor g = gy;
+            bool feature_major = false;
+            if (!g.is_contiguous()) {
+                feature_major = g.t().is_contiguous();
+                if (!feature_major) g = g.contiguous();
+            }
+            if (slope.defined() && feature_major != (bool)sizes[5] && batch > 1 && outer > 1) {
+                feature_major = sizes[5];
+                g = feature_major ? g.t().contiguous().t() : g.contiguous();
+            }
+            const auto options = gy.options().requires_grad(false);
+            if (want_x) out[0] = at::empty({batch, inner}, options);
+            if (want_w) out[1] = at::empty({outer, inner}, options);
+            if (want_b) out[2] = at::empty({outer}, options);
+            const Matrix read = x.defined() ? readable(x) : Matrix{Tensor(), pitch, (bool)sizes[4]};
+            const void *px = x.defined() ? x.data_ptr() : (const void *)at[0], *pw = w.defined() ? w.data_ptr() : (const void *)at[1];
+            const int kind = kind_of(gy.scalar_type());
+            const Tensor work = bytes(dl_dense_backward_workspace_bytes(g.data_ptr(), feature_major, slope.defined(), px, read.pitch, read.feature_major,
+                                                                        pw, want_w && !x_planes.defined(), want_x && !w_planes.defined(), batch, inner,
+                                                                        outer, kind),
+                                      gy);
+            check(dl_dense_backward(g.data_ptr(), feature_major, pointer(slope), px, read.pitch, read.feature_major, pw, pointer(x_planes),
+                                    pointer(w_planes), pointer(out[0]), pointer(out[1]), pointer(out[2]), pointer(work), batch, inner, outer, kind,
+                                    stream_of(gy)));
+        }
+        if (sizes[7] && ctx->needs_input_grad(sizes[6] ? 3 : 2)) out[3] = gy;   // counted without what was not given
+        if (at::GradMode::is_enabled()) {   // a graph of the gradients is wanted: it would end here without a word
+            variable_list once(out.begin(), out.begin() + 3);
+            for (Tensor &t : once)
+                if (t.defined()) t = t.detach().requires_grad_(true);
+            once = (*std::make_shared<torch::autograd::DelayedError>("difflogic_b200: dense layers are differentiable once", 3))(std::move(once));
+            std::copy(once.begin(), once.end(), out.begin());
+        }
+        return out;
+    }
+};
+
+// dense(x, weight, bias | None, residual | None, activation, feature_major) -> output, or None
+PyObject *dense(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    if (count != 6) {
+        PyErr_SetString(PyExc_TypeError, "dense: six arguments");
+        return nullptr;
+    }
+    if (!ordinary(args[0]) || !ordinary(args[1])) Py_RETURN_NONE;
+    Tensor x = THPVariable_Unpack(args[0]), residual, bias;
+    const Tensor &w = THPVariable_Unpack(args[1]);
+    const c10::Device device = x.device();
+    const at::ScalarType type = x.scalar_type();
+    if (type != at::kFloat && type != at::kBFloat16 && type != at::kHalf) Py_RETURN_NONE;
+    if (!plain(x, type, x.dim(), device) || x.dim() < 1 || x.numel() == 0 || w.dim() != 2 || w.size(0) == 0 ||
+        !matrix_of(w, type, w.size(0), x.size(-1), device))
+        Py_RETURN_NONE;
+    const int64_t outer = w.size(0);
+    if (args[2] != Py_None) {
+        if (!ordinary(args[2])) Py_RETURN_NONE;
+        bias = THPVariable_Unpack(args[2]);
+        if (!vector_of(bias, type, outer, device)) Py_RETURN_NONE;
+    }
+    auto sizes = x.sizes().vec();
+    sizes.back() = outer;
+    if (args[3] != Py_None) {
+        if (!ordinary(args[3])) Py_RETURN_NONE;
+        residual = THPVariable_Unpack(args[3]);
+        if (!plain(residual, type, x.dim(), device) || residual.sizes() != at::IntArrayRef(sizes)) Py_RETURN_NONE;
+    }
+    const long act = PyLong_AsLong(args[4]);
+    if (act == -1 && PyErr_Occurred()) return nullptr;
+    const int feature_major = PyObject_IsTrue(args[5]);
+    if (feature_major < 0) return nullptr;
+    if (act < DL_ACT_NONE || act > DL_ACT_GELU || (feature_major && x.dim() != 2)) Py_RETURN_NONE;
+    if (observed() || x._fw_grad(0).defined() || w._fw_grad(0).defined() || (bias.defined() && bias._fw_grad(0).defined()) ||
+        (residual.defined() && residual._fw_grad(0).defined()))
+        Py_RETURN_NONE;
+    Tensor y;
+    {
+        const WithoutGil nogil;
+        const c10::cuda::CUDAGuard guard(device);
+        if (x.dim() != 2) {
+            x = x.reshape({-1, x.size(-1)});
+            if (residual.defined()) residual = residual.reshape({-1, outer});
+        }
+        const bool graph = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (bias.defined() && bias.requires_grad()) ||
+                                                          (residual.defined() && residual.requires_grad()));
+        const auto given = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+        y = graph ? DenseNode::apply(x, w, given(bias), given(residual), (int64_t)act, (bool)feature_major)
+                  : dense_forward(x, w, bias, residual, (int)act, feature_major, false).y;
+        if (sizes.size() != 2) y = y.reshape(sizes);
+    }
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject *launches(PyObject *, PyObject *) { return PyLong_FromLongLong(g_launches.load()); }
 
 // connect(dict of difflogic.py)
@@ -309,6 +475,7 @@ PyObject *connect(PyObject *, PyObject *dict) {
 
 PyMethodDef kMethods[] = {{"layer", (PyCFunction)(void *)layer, METH_FASTCALL, nullptr},
                           {"group_sum", (PyCFunction)(void *)group_sum, METH_FASTCALL, nullptr},
+                          {"dense", (PyCFunction)(void *)dense, METH_FASTCALL, nullptr},
                           {"launches", launches, METH_NOARGS, nullptr},
                           {"connect", connect, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};

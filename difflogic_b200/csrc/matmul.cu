@@ -2,6 +2,7 @@
 // operands, and the entry points.
 #include <math.h>
 
+#include "dense_epilogue.cuh"
 #include "gram_steps.h"
 #include "matmul.cuh"
 #include "matmul_plan.h"
@@ -144,130 +145,6 @@ static int64_t padded(int64_t n) { return ceil_div(n, 8) * 8; }
 static int64_t padded_bytes(int64_t n) { return ceil_div(n, 256) * 256; }
 
 // ============================================================== dense layers ====================================================
-
-// Derivatives of the activation are kept for the backward pass, in fp32 or -- 16-bit layers -- in fp16 times 2^14: 11 bits, where the
-// layer's own type may have 8, and down to 4e-12, where sigmoids saturate.
-constexpr float kSlopeScale = 16384.f;
-
-// act(z) in place, and its derivatives, four at a time.
-template <int N>
-__device__ __forceinline__ void activate(float (&z)[N], float (&slope)[N], int act) {
-    if (act == DL_ACT_NONE) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) slope[j] = 1.f;
-    } else if (act == DL_ACT_RELU) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            slope[j] = z[j] > 0.f ? 1.f : 0.f;
-            z[j] = z[j] > 0.f || z[j] != z[j] ? z[j] : 0.f;
-        }
-    } else if (act == DL_ACT_GELU) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float phi = 0.5f * (1.f + erff(z[j] * 0.70710678118654752f));
-            // far out the density is zero, and infinity times zero would not be
-            slope[j] = phi + (fabsf(z[j]) > 15.f ? 0.f : z[j] * expf(-0.5f * z[j] * z[j]) * 0.39894228040143268f);
-            z[j] = z[j] == -INFINITY ? 0.f : z[j] * phi;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float s = __fdividef(1.f, 1.f + expf(-z[j]));   // zero below -88, where expf overflows
-            slope[j] = s * (1.f - s);
-            if (act == DL_ACT_SIGMOID) {
-                z[j] = s;
-            } else {
-                slope[j] = s + (slope[j] == 0.f ? 0.f : z[j] * slope[j]);
-                z[j] = z[j] == -INFINITY ? 0.f : z[j] * s;
-            }
-        }
-    }
-}
-
-// y = act(sum + bias) + residual.  rows_are_features: the rows of the product are the layer's outputs, else its columns are; the result
-// lies [batch][feature] or, feature_major, [feature][batch].
-struct DenseEpilogue {
-    static constexpr int kPlanes = 3;
-    void *y;
-    const void *bias, *residual;
-    void *slope;
-    int64_t y_pitch, residual_row, residual_col;   // of the residual: values to the product's next row, to its next column
-    int type, act;
-    bool rows_are_features, feature_major;
-
-    // Neighbouring columns of the product are neighbours in memory, or neighbouring rows are.
-    __device__ __forceinline__ bool by_column(int, int) const { return rows_are_features != feature_major; }
-    __device__ __forceinline__ bool by_row(int, int) const { return rows_are_features == feature_major; }
-
-    template <int N>
-    __device__ __forceinline__ void down(int, int row, int col, const float (&sum)[N], int m, int valid) const {
-        if (row >= m) return;
-        const float row_bias = bias != nullptr && rows_are_features ? load_as_float(bias, row, type) : 0.f;
-        float v[N], d[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            v[j] = sum[j] + row_bias;
-            if (bias != nullptr && !rows_are_features && j < valid) v[j] += load_as_float(bias, col + j, type);
-        }
-        activate(v, d, act);
-        if (residual != nullptr) {
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (j < valid) v[j] += load_as_float(residual, row * residual_row + (col + j) * residual_col, type);
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            if (j >= valid) continue;
-            const int64_t i = (col + j) * y_pitch + row;
-            if (type == kFloat32) reinterpret_cast<float *>(y)[i] = v[j];
-            else reinterpret_cast<uint16_t *>(y)[i] = to_16bit(v[j], type);
-            if (slope != nullptr) {
-                if (type == kFloat32) reinterpret_cast<float *>(slope)[i] = d[j];
-                else reinterpret_cast<uint16_t *>(slope)[i] = to_16bit(d[j] * kSlopeScale, kFloat16);
-            }
-        }
-    }
-    template <int N, int STEP>
-    __device__ __forceinline__ void across(int, int row, int col, const float (&sum)[N][4], int m, int valid) const {
-        float col_bias[4] = {0.f, 0.f, 0.f, 0.f}, more[N][4];
-        if (bias != nullptr && !rows_are_features) load4(bias, col, type, valid, col_bias);
-        if (residual != nullptr) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int r = row + i * STEP;
-                if (residual_col == 1) {
-                    load4(residual, r * residual_row + col, type, r < m ? valid : 0, more[i]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) more[i][j] = r < m && j < valid ? load_as_float(residual, r * residual_row + (col + j) * residual_col, type) : 0.f;
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int r = row + i * STEP;
-            if (r >= m) break;
-            const float row_bias = bias != nullptr && rows_are_features ? load_as_float(bias, r, type) : 0.f;
-            float v[4], d[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = sum[i][j] + (rows_are_features ? row_bias : col_bias[j]);
-            activate(v, d, act);
-            if (residual != nullptr) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] += more[i][j];
-            }
-            const int64_t at = r * y_pitch + col;
-            store4(y, at, type, valid, v);
-            if (slope != nullptr) {
-                if (type != kFloat32) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) d[j] *= kSlopeScale;
-                }
-                store4(slope, at, type == kFloat32 ? kFloat32 : kFloat16, valid, d);
-            }
-        }
-    }
-};
 
 // Gradients: the sums as they are, in the layer's type.
 struct PlainEpilogue {
@@ -454,14 +331,14 @@ static bool dense_sizes(int64_t batch, int64_t inner, int64_t outer, int type, c
 
 using namespace dl;
 
-extern "C" DL_API int64_t dl_dense_planes_bytes(const void *p, int64_t rows, int64_t cols, int64_t pitch, int type) {
-    if (rows <= 0 || cols <= 0 || in_place(p, pitch, type)) return 0;
-    return padded_bytes((type == kFloat32 ? 3 : 1) * rows * padded(cols) * 2);
-}
-
-extern "C" DL_API int64_t dl_dense_forward_workspace_bytes(int64_t batch, int64_t inner, int64_t outer, int type) {
-    if (batch <= 0 || inner <= 0 || outer <= 0) return 0;
-    return plan_forward(batch, inner, outer, type == kFloat32 ? 3 : 1, current_sms()).partial_bytes;
+extern "C" DL_API void dl_dense_forward_sizes(const void *x, int64_t x_pitch, int x_feature_major, const void *w, int64_t batch, int64_t inner,
+                                             int64_t outer, int type, int64_t *sizes) {
+    sizes[0] = sizes[1] = sizes[2] = 0;
+    if (batch <= 0 || inner <= 0 || outer <= 0 || dense_rows_applicable(batch, inner, outer, type)) return;
+    const DenseLayout l = dense_layout(batch, inner, outer, x_pitch, x_feature_major != 0, type, x, w);
+    sizes[0] = l.x_bytes;
+    sizes[1] = l.w_bytes;
+    sizes[2] = plan_forward(batch, inner, outer, l.planes, current_sms()).partial_bytes;
 }
 
 extern "C" DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_feature_major, const void *w, const void *bias, const void *residual,
@@ -477,12 +354,17 @@ extern "C" DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_fea
     DL_REQUIRE(x_pitch >= (x_feature_major ? batch : inner), DL_ERR_INVALID_ARG, "%s: rows of x overlap", what);
     const DenseLayout l = dense_layout(batch, inner, outer, x_pitch, x_feature_major != 0, type, x, w);
     const int sms = current_sms();
+    cudaStream_t st = as_stream(stream);
+    if (dense_rows_applicable(batch, inner, outer, type)) {
+        const DenseEpilogue e = {y, bias, residual, slope, y_feature_major ? batch : outer, residual_feature, residual_batch, type, act, true,
+                                 y_feature_major != 0};
+        return launch_dense_rows(x, x_pitch, x_feature_major != 0, w, e, batch, inner, outer, type, sms, st);
+    }
     const MatmulPlan plan = plan_forward(batch, inner, outer, l.planes, sms);
     DL_REQUIRE((!l.lay_x || x_planes) && (!l.lay_w || w_planes) && (plan.partial_bytes == 0 || workspace), DL_ERR_INVALID_ARG,
                "%s: a workspace is missing", what);
     DL_REQUIRE(aligned_to(x_planes, 16) && aligned_to(w_planes, 16) && aligned_to(workspace, 16), DL_ERR_INVALID_ARG,
                "%s: workspaces must be 16-byte aligned", what);
-    cudaStream_t st = as_stream(stream);
     if (l.lay_x && (status = lay_out(x, l.x_rows, l.x_cols, x_pitch, type, x_planes, l.x_plane_pitch, l.x_plane, sms, st, what)) != DL_OK) return status;
     if (l.lay_w && (status = lay_out(w, outer, inner, inner, type, w_planes, l.w_plane_pitch, l.w_plane, sms, st, what)) != DL_OK) return status;
     const Operand ox = {l.lay_x ? x_planes : x, l.lay_x ? l.x_plane_pitch : x_pitch, l.x_plane, x_feature_major != 0};
@@ -510,10 +392,12 @@ struct DenseBackward {
     bool lay_gz;
     int64_t g_rows, g_cols, g_pitch, g_plane, strips, strip, parts;
     MatmulPlan to_x, to_w;
-    int64_t g_bytes, bias_bytes, x_bytes, w_bytes;   // workspace: gz planes, partial bias sums, splits of the two products
+    int64_t g_bytes, bias_bytes, partial_bytes, x_bytes, w_bytes;   // workspace: gz planes, partial bias sums, splits of a product, x and w laid out
+    int64_t total() const { return g_bytes + bias_bytes + partial_bytes + x_bytes + w_bytes; }
 };
 
-static DenseBackward plan_backward(int64_t batch, int64_t inner, int64_t outer, bool g_feature_major, int type, bool act, const void *gy, int sms) {
+static DenseBackward plan_backward(const DenseLayout &l, int64_t batch, int64_t inner, int64_t outer, bool g_feature_major, int type, bool act,
+                                   const void *gy, bool lay_x, bool lay_w, int sms) {
     DenseBackward b = {};
     b.planes = type == kFloat32 ? 3 : 1;
     b.g_rows = g_feature_major ? outer : batch;
@@ -527,18 +411,20 @@ static DenseBackward plan_backward(int64_t batch, int64_t inner, int64_t outer, 
     b.bias_bytes = padded_bytes(b.parts * outer * 4);
     b.to_x = plan_matmul(batch, inner, outer, 1, b.planes, false, sms);
     b.to_w = plan_matmul(outer, inner, batch, 1, b.planes, false, sms);
-    b.x_bytes = padded_bytes(b.to_x.partial_bytes);
-    b.w_bytes = padded_bytes(b.to_w.partial_bytes);
+    b.partial_bytes = padded_bytes(b.to_x.partial_bytes > b.to_w.partial_bytes ? b.to_x.partial_bytes : b.to_w.partial_bytes);
+    b.x_bytes = lay_x ? l.x_bytes : 0;
+    b.w_bytes = lay_w ? l.w_bytes : 0;
     return b;
 }
 
 }  // namespace dl
 
-extern "C" DL_API int64_t dl_dense_backward_workspace_bytes(int64_t batch, int64_t inner, int64_t outer, int g_feature_major, int type, int has_slope,
-                                                            const void *gy) {
+extern "C" DL_API int64_t dl_dense_backward_workspace_bytes(const void *gy, int g_feature_major, int has_slope, const void *x, int64_t x_pitch,
+                                                            int x_feature_major, const void *w, int lay_x, int lay_w, int64_t batch, int64_t inner,
+                                                            int64_t outer, int type) {
     if (batch <= 0 || inner <= 0 || outer <= 0) return 0;
-    const DenseBackward b = plan_backward(batch, inner, outer, g_feature_major != 0, type, has_slope != 0, gy, current_sms());
-    return b.g_bytes + b.bias_bytes + b.x_bytes + b.w_bytes;
+    const DenseLayout l = dense_layout(batch, inner, outer, x_pitch, x_feature_major != 0, type, x, w);
+    return plan_backward(l, batch, inner, outer, g_feature_major != 0, type, has_slope != 0, gy, lay_x != 0, lay_w != 0, current_sms()).total();
 }
 
 extern "C" DL_API int dl_dense_backward(const void *gy, int g_feature_major, const void *slope, const void *x, int64_t x_pitch, int x_feature_major,
@@ -552,13 +438,23 @@ extern "C" DL_API int dl_dense_backward(const void *gy, int g_feature_major, con
     DL_REQUIRE(workspace && aligned_to(workspace, 16), DL_ERR_INVALID_ARG, "%s: the workspace is missing or not 16-byte aligned", what);
     const int sms = current_sms();
     const DenseLayout l = dense_layout(batch, inner, outer, x_pitch, x_feature_major != 0, type, x, w);
-    const DenseBackward b = plan_backward(batch, inner, outer, g_feature_major != 0, type, slope != nullptr, gy, sms);
-    DL_REQUIRE((!gw || !l.lay_x || x_planes) && (!gx || !l.lay_w || w_planes), DL_ERR_INVALID_ARG, "%s: laid-out operands are missing", what);
+    const bool lay_x = gw && l.lay_x && !x_planes, lay_w = gx && l.lay_w && !w_planes;
+    const DenseBackward b = plan_backward(l, batch, inner, outer, g_feature_major != 0, type, slope != nullptr, gy, lay_x, lay_w, sms);
+    DL_REQUIRE((!lay_x || x) && (!lay_w || w), DL_ERR_INVALID_ARG, "%s: null pointer", what);
     cudaStream_t st = as_stream(stream);
     uint8_t *at = reinterpret_cast<uint8_t *>(workspace);
     uint16_t *gz = reinterpret_cast<uint16_t *>(at);
-    float *sums = reinterpret_cast<float *>(at + b.g_bytes), *part_x = reinterpret_cast<float *>(at + b.g_bytes + b.bias_bytes),
-          *part_w = reinterpret_cast<float *>(at + b.g_bytes + b.bias_bytes + b.x_bytes);
+    float *sums = reinterpret_cast<float *>(at + b.g_bytes), *partial = reinterpret_cast<float *>(at + b.g_bytes + b.bias_bytes);
+    if (lay_x) {
+        void *to = at + b.total() - b.w_bytes - b.x_bytes;
+        if ((status = lay_out(x, l.x_rows, l.x_cols, x_pitch, type, to, l.x_plane_pitch, l.x_plane, sms, st, what)) != DL_OK) return status;
+        x_planes = to;
+    }
+    if (lay_w) {
+        void *to = at + b.total() - b.w_bytes;
+        if ((status = lay_out(w, outer, inner, inner, type, to, l.w_plane_pitch, l.w_plane, sms, st, what)) != DL_OK) return status;
+        w_planes = to;
+    }
     if (b.lay_gz || gb) {
         launch_dependent(true, pre_gradient_kernel, dim3((unsigned)ceil_div(b.g_cols, 128), (unsigned)b.strips), dim3(kThreads), 0, st, gy, slope,
                          b.g_rows, b.g_cols, type, b.lay_gz ? gz : (uint16_t *)nullptr, b.g_pitch, b.g_plane, b.strip, gb ? sums : (float *)nullptr,
@@ -583,7 +479,7 @@ extern "C" DL_API int dl_dense_backward(const void *gy, int g_feature_major, con
         p.m = batch;
         p.n = inner;
         p.k = outer;
-        if ((status = launch_planes(p, b.to_x, PlainEpilogue{gx, inner, type}, part_x, sms, st, what)) != DL_OK) return status;
+        if ((status = launch_planes(p, b.to_x, PlainEpilogue{gx, inner, type}, partial, sms, st, what)) != DL_OK) return status;
     }
     if (gw) {   // gz^T x, summed over the batch
         p.a = g;
@@ -592,7 +488,7 @@ extern "C" DL_API int dl_dense_backward(const void *gy, int g_feature_major, con
         p.m = outer;
         p.n = inner;
         p.k = batch;
-        if ((status = launch_planes(p, b.to_w, PlainEpilogue{gw, inner, type}, part_w, sms, st, what)) != DL_OK) return status;
+        if ((status = launch_planes(p, b.to_w, PlainEpilogue{gw, inner, type}, partial, sms, st, what)) != DL_OK) return status;
     }
     return DL_OK;
 }

@@ -11,6 +11,7 @@ feature-major layout that logic layers read -- or makes the fully connected netw
 
 `implementation='python'` is the pure-torch definition of the same layer and runs anywhere.
 """
+import ctypes
 import math
 
 import torch
@@ -52,9 +53,9 @@ def _forward(x, w, bias, residual, act, feature_major, want_slope):
     lib = N.lib()
     with N.on_device(x):
         px, pw = x.data_ptr(), w.data_ptr()
-        x_planes = _bytes(lib.dl_dense_planes_bytes(px, inner if x_feature else batch, batch if x_feature else inner, pitch, kind), x)
-        w_planes = _bytes(lib.dl_dense_planes_bytes(pw, outer, inner, inner, kind), x)
-        work = _bytes(lib.dl_dense_forward_workspace_bytes(batch, inner, outer, kind), x)
+        sizes = (ctypes.c_int64 * 3)()
+        lib.dl_dense_forward_sizes(px, pitch, x_feature, pw, batch, inner, outer, kind, sizes)
+        x_planes, w_planes, work = (_bytes(n, x) for n in sizes)
         N.check(lib.dl_dense_forward(px, pitch, x_feature, pw, N.ptr(bias), N.ptr(residual), 0 if residual is None else residual.stride(0),
                                      0 if residual is None else residual.stride(1), act, y.data_ptr(), feature_major, N.ptr(slope),
                                      N.ptr(x_planes), N.ptr(w_planes), N.ptr(work), batch, inner, outer, kind, N.stream_of(x)))
@@ -101,9 +102,11 @@ class DenseFunction(torch.autograd.Function):
                     g = gy.t().contiguous().t() if feature else gy.contiguous()
                 lib, kind = N.lib(), TYPES[gy.dtype]
                 with N.on_device(gy):
-                    work = _bytes(lib.dl_dense_backward_workspace_bytes(batch, inner, outer, feature, kind, slope is not None, g.data_ptr()), gy)
-                    N.check(lib.dl_dense_backward(g.data_ptr(), feature, N.ptr(slope), N.ptr(x) if x is not None else ctx.x_ptr, ctx.pitch,
-                                                  ctx.x_feature, N.ptr(w) if w is not None else ctx.w_ptr, N.ptr(x_planes), N.ptr(w_planes),
+                    px, pw = x.data_ptr() if x is not None else ctx.x_ptr, w.data_ptr() if w is not None else ctx.w_ptr
+                    work = _bytes(lib.dl_dense_backward_workspace_bytes(g.data_ptr(), feature, slope is not None, px, ctx.pitch, ctx.x_feature, pw,
+                                                                        want_w and x_planes is None, want_x and w_planes is None, batch, inner,
+                                                                        outer, kind), gy)
+                    N.check(lib.dl_dense_backward(g.data_ptr(), feature, N.ptr(slope), px, ctx.pitch, ctx.x_feature, pw, N.ptr(x_planes), N.ptr(w_planes),
                                                   N.ptr(gx), N.ptr(gw), N.ptr(gb), work.data_ptr(), batch, inner, outer, kind, N.stream_of(gy)))
         return gx, gw, gb, gy if ctx.needs_input_grad[3] else None, None, None
 
@@ -132,6 +135,12 @@ def dense(x, weight, bias=None, residual=None, activation=None, feature_major=Fa
     device; activation: None, 'relu', 'sigmoid', 'silu' or 'gelu' (the exact one).  x may be a transposed view, as logic layers return
     them.  feature_major: a 2-D result lies in memory as `[out, batch]` (same values, other strides), which a LogicLayer reads without a
     copy."""
+    act = ACTIVATIONS.get(activation, -1)
+    if act >= 0 and x.is_cuda:
+        # the native node; None for a call that is not of the ordinary form
+        y = N.nodes().dense(x, weight, bias, residual, act, feature_major)
+        if y is not None:
+            return y
     _check(x, weight, bias, residual, activation)
     N.require_cuda(x)
     if x.dtype not in TYPES:
@@ -144,7 +153,6 @@ def dense(x, weight, bias=None, residual=None, activation=None, feature_major=Fa
         residual = None if residual is None else residual.reshape(-1, outer)
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    act = ACTIVATIONS[activation]
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         y = DenseFunction.apply(x, weight, bias, residual, act, bool(feature_major))
     else:

@@ -560,23 +560,24 @@ DL_API int dl_backward_w_announce_f32(const float *x, const int64_t *a, const in
  *
  * x [batch][inner] with rows x_pitch values apart, or, x_feature_major, [inner][batch]; w [outer][inner] contiguous; bias [outer] and
  * residual may be NULL, residual's strides in values.  y [batch][outer] or, y_feature_major, [outer][batch], contiguous.  slope (NULL:
- * not wanted): act' in y's layout, fp32, or for 16-bit types fp16 times 2^14.  x_planes, w_planes: dl_dense_planes_bytes for x as it
- * lies (rows, cols, pitch) and for w (outer, inner, inner); what is laid out there serves the backward pass.  The workspaces are
- * 16-byte aligned.
+ * not wanted): act' in y's layout, fp32, or for 16-bit types fp16 times 2^14.  x_planes, w_planes, workspace: sizes[0 .. 2] bytes of
+ * dl_dense_forward_sizes, 16-byte aligned; what is laid out in the planes serves the backward pass.
  *
  *   gz = gy * slope;  gx = gz w [batch][inner],  gw = gz^T x [outer][inner],  gb = sum of gz over the batch
  *
- * gy contiguous in y's layout or the other one, slope (NULL: no activation) in gy's; gx, gw, gb NULL: not wanted.
+ * gy contiguous in y's layout or the other one, slope (NULL: no activation) in gy's; gx, gw, gb NULL: not wanted.  x_planes, w_planes:
+ * those of the forward pass, or NULL: then x and w are there, and the workspace has room for them (lay_x, lay_w: asked for with NULL).
  * ---------------------------------------------------------------------------------------- */
 enum { DL_ACT_NONE = 0, DL_ACT_RELU = 1, DL_ACT_SIGMOID = 2, DL_ACT_SILU = 3, DL_ACT_GELU = 4 };
-DL_API int64_t dl_dense_planes_bytes(const void *p, int64_t rows, int64_t cols, int64_t pitch, int type);
-DL_API int64_t dl_dense_forward_workspace_bytes(int64_t batch, int64_t inner, int64_t outer, int type);
+DL_API void dl_dense_forward_sizes(const void *x, int64_t x_pitch, int x_feature_major, const void *w, int64_t batch, int64_t inner,
+                                   int64_t outer, int type, int64_t *sizes);
 DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_feature_major, const void *w, const void *bias, const void *residual,
                             int64_t residual_batch, int64_t residual_feature, int act, void *y, int y_feature_major, void *slope,
                             void *x_planes, void *w_planes, void *workspace, int64_t batch, int64_t inner, int64_t outer, int type,
                             void *stream);
-DL_API int64_t dl_dense_backward_workspace_bytes(int64_t batch, int64_t inner, int64_t outer, int g_feature_major, int type, int has_slope,
-                                                 const void *gy);
+DL_API int64_t dl_dense_backward_workspace_bytes(const void *gy, int g_feature_major, int has_slope, const void *x, int64_t x_pitch,
+                                                 int x_feature_major, const void *w, int lay_x, int lay_w, int64_t batch, int64_t inner,
+                                                 int64_t outer, int type);
 DL_API int dl_dense_backward(const void *gy, int g_feature_major, const void *slope, const void *x, int64_t x_pitch, int x_feature_major,
                              const void *w, const void *x_planes, const void *w_planes, void *gx, void *gw, void *gb, void *workspace,
                              int64_t batch, int64_t inner, int64_t outer, int type, void *stream);
