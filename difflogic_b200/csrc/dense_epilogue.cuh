@@ -146,7 +146,7 @@ struct DenseEpilogue {
 };
 
 // Dense layers of few samples (dense_rows.cu): false where the tensor cores are to be used.
-bool dense_rows_applicable(int64_t batch, int64_t inner, int64_t outer, int type);
+bool dense_rows_applicable(int64_t batch, int type);
 int launch_dense_rows(const void *x, int64_t x_pitch, bool x_feature_major, const void *w, const DenseEpilogue &epilogue, int64_t batch,
                       int64_t inner, int64_t outer, int type, int sms, cudaStream_t st);
 #endif  // __CUDACC__

@@ -1,180 +1,213 @@
 // Dense layers of few samples: y[b][f] = sum_k x[b][k] w[f][k], bound by reading w once.
 //
-// A warp takes R outputs at a time for all samples: its lanes read 16 bytes each of R rows of w (single values where rows are off the
-// 16-byte units), multiply them with the samples, which lie in shared memory as fp32, and add up R x B sums of their own; then the lanes
-// share out the sums, halving them five times.  The ordinary FMA units do: at B samples they have B products for every value of w, 90
-// of 128 a clock for 16 fp32 or 8 bf16 samples at the rate at which memory delivers w.  fp32 values stay as they are here, where the
-// tensor cores would have them laid out in three planes first, four times the bytes of w.
+// A block takes 16 or 32 outputs for all samples; its eight warps take every eighth piece of k each and add their sums up in shared
+// memory.  The products go to the warp-wide matrix instructions (16 outputs x 8 samples), which take their operands from registers, so
+// that w goes from memory straight into them: fp32 values are split there, where the tensor cores' tiles would have them laid out in three planes
+// in memory first, four times the bytes of w; and no tile of 64 columns waits for samples that are not there.
+// The order in which k is summed is free: a lane reads 16 neighbouring bytes of its rows of w and of x, and what the instruction calls
+// columns t and t + 4 (fp32) are neighbours in memory.
 //
-// Samples are a chunk of at most 64 KB at a time, so that two blocks fit an SM.
+// fp32: hi + lo, hi the upper 11 bits of the value (the instruction reads no more), lo the rest, of which it reads 11 bits: lo hi + hi lo,
+// then hi hi, into a sum that is taken out every kAhead pieces, since the instruction cuts off what is below its last bit.
 #include "dense_epilogue.cuh"
 
 namespace dl {
 
 constexpr int kRowsThreads = 256, kRowsWarps = kRowsThreads / 32;
-constexpr int kRowsBytes = 65536;
 
 struct RowsJob {
     const void *x, *w;
     int64_t x_row, x_col;    // values to the next sample, to the next input
     int64_t inner, outer;
     int batch, type;
-    int chunk;               // inputs in shared memory at a time
+    bool x_whole;            // rows of x can be read 16 bytes at a time
 };
 
-template <int WIDTH>
-__device__ __forceinline__ void load_weights(const void *w, int64_t at, int type, float (&v)[WIDTH]) {
-    if constexpr (WIDTH == 4) {
-        const float4 f = __ldcs(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(w) + at));
-        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-    } else if constexpr (WIDTH == 8) {
-        const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(w) + at));
-        const uint32_t p[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (type == kBFloat16) {
-                v[2 * j] = __uint_as_float(p[j] << 16);
-                v[2 * j + 1] = __uint_as_float(p[j] & 0xffff0000u);
-            } else {
-                const __half2 h = *reinterpret_cast<const __half2 *>(&p[j]);
-                v[2 * j] = __low2float(h);
-                v[2 * j + 1] = __high2float(h);
-            }
-        }
-    } else {
-        v[0] = load_as_float(w, at, type);
+__device__ __forceinline__ uint4 load_once(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// 16 bytes' worth of values from input k on, zeros behind the last one.
+template <bool FULL>
+__device__ __forceinline__ uint4 load_piece(const void *row, int64_t step, int64_t k, int64_t inner, bool whole, bool streamed) {
+    constexpr int kValues = FULL ? 4 : 8;
+    if (whole) {
+        if (k >= inner) return make_uint4(0, 0, 0, 0);
+        const void *at = reinterpret_cast<const char *>(row) + k * (FULL ? 4 : 2);
+        return streamed ? load_once(at) : __ldg(reinterpret_cast<const uint4 *>(at));
     }
+    uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < kValues; ++j) {
+        if (k + j >= inner) continue;
+        if (FULL) v[j] = reinterpret_cast<const uint32_t *>(row)[(k + j) * step];
+        else v[j / 2] |= (uint32_t) reinterpret_cast<const uint16_t *>(row)[(k + j) * step] << (j % 2 * 16);
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// Where input k of a chunk lies in shared memory.  Lanes read 8 neighbouring ones as two quads: the first and the second quads of all
-// lanes lie apart, so that 8 lanes meet no bank twice.
-template <int WIDTH>
-__device__ __forceinline__ int place_of(int k, int chunk) {
-    return WIDTH == 8 ? k / 8 * 4 + k % 4 + (k % 8 / 4) * (chunk / 2) : k;
+__device__ __forceinline__ void multiply_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void multiply_16bit(float (&d)[4], bool bfloat, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (bfloat)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+struct Split {
+    uint32_t hi[4], lo[4];
+};
+__device__ __forceinline__ Split split_piece(const uint4 &v) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+    Split s;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        s.hi[j] = u[j] & 0xffffe000u;
+        s.lo[j] = __float_as_uint(__uint_as_float(u[j]) - __uint_as_float(s.hi[j]));
+    }
+    return s;
 }
 
-template <int B, int R, int WIDTH>
-__global__ void __launch_bounds__(kRowsThreads)
+// MT groups of 16 outputs, NT of 8 samples; FULL: fp32; WHOLE: rows of w can be read 16 bytes at a time.
+template <int MT, int NT, bool FULL, bool WHOLE>
+__global__ void __launch_bounds__(kRowsThreads, MT * NT == 1 ? 3 : 2)
 dense_rows_kernel(const RowsJob j, const DenseEpilogue epilogue) {
-    extern __shared__ float s_x[];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    constexpr int kAll = R * B;
+    constexpr int kPiece = FULL ? 16 : 32;   // values of k that a warp's four lanes of a row read at a time
+    constexpr int kAhead = NT == 1 ? 4 : 2;
+    constexpr int kOutputs = 16 * MT, kSamples = 8 * NT;
+    __shared__ float s_sum[kRowsWarps][kOutputs][kSamples + 1];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
+    const int64_t base = (int64_t)blockIdx.x * kOutputs;
+    const char *rows[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t f = base + m * 16 + h * 8 + g;   // outputs behind the last one: its row once more
+            rows[m][h] = reinterpret_cast<const char *>(j.w) + (f < j.outer ? f : j.outer - 1) * j.inner * (FULL ? 4 : 2);
+        }
+    float sum[MT][NT][4] = {};
     grid_dependency_wait();
     grid_dependents_launch();
-    for (int64_t group = (int64_t)blockIdx.x * kRowsWarps * R; group < j.outer; group += (int64_t)gridDim.x * kRowsWarps * R) {
-        const int64_t feature = group + warp * R;
-        float sum[kAll];
+    for (int64_t first = (int64_t)warp * kPiece; first < j.inner; first += (int64_t)kAhead * kRowsWarps * kPiece) {
+        uint4 w[kAhead][MT][2], x[kAhead][NT];
 #pragma unroll
-        for (int i = 0; i < kAll; ++i) sum[i] = 0.f;
-        for (int64_t from = 0; from < j.inner; from += j.chunk) {
-            const int count = (int)(j.inner - from < j.chunk ? j.inner - from : j.chunk);
-            if (j.inner > j.chunk || group == (int64_t)blockIdx.x * kRowsWarps * R) {
-                __syncthreads();
-                for (int i = threadIdx.x; i < B * j.chunk; i += kRowsThreads) {   // zeros behind the last sample and input
-                    const int b = i / j.chunk, k = i - b * j.chunk;
-                    s_x[b * j.chunk + place_of<WIDTH>(k, j.chunk)] =
-                        b < j.batch && k < count ? load_as_float(j.x, b * j.x_row + (from + k) * j.x_col, j.type) : 0.f;
-                }
-                __syncthreads();
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t k = first + (int64_t)i * kRowsWarps * kPiece + t * (kPiece / 4);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) w[i][m][h] = load_piece<FULL>(rows[m][h], 1, k, j.inner, WHOLE, true);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int b = n * 8 + g;
+                x[i][n] = make_uint4(0, 0, 0, 0);
+                if (b < j.batch)
+                    x[i][n] = load_piece<FULL>(reinterpret_cast<const char *>(j.x) + b * j.x_row * (FULL ? 4 : 2), j.x_col, k, j.inner, j.x_whole, false);
             }
-            if (feature >= j.outer) continue;
-            // WIDTH divides j.inner where it is not 1: whole vectors only
-#pragma unroll 4
-            for (int k = lane * WIDTH; k < count; k += 32 * WIDTH) {
-                float w[R][WIDTH];
+        }
+        float part[MT][NT][4] = {};
+        if constexpr (FULL) {
+            // the small products of all pieces, then the large ones
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const int64_t f = feature + r < j.outer ? feature + r : j.outer - 1;
-                    load_weights<WIDTH>(j.w, f * j.inner + from + k, j.type, w[r]);
-                }
+            for (int large = 0; large < 2; ++large)
 #pragma unroll
-                for (int b = 0; b < B; ++b) {
-                    float x[WIDTH];
-                    if constexpr (WIDTH == 1) {
-                        x[0] = s_x[b * j.chunk + k];
-                    } else {
+                for (int i = 0; i < kAhead; ++i) {
+                    Split b[NT];
 #pragma unroll
-                        for (int q = 0; q < WIDTH / 4; ++q) {
-                            const float4 f = *reinterpret_cast<const float4 *>(s_x + b * j.chunk + place_of<WIDTH>(k + 4 * q, j.chunk));
-                            x[4 * q] = f.x; x[4 * q + 1] = f.y; x[4 * q + 2] = f.z; x[4 * q + 3] = f.w;
-                        }
+                    for (int n = 0; n < NT; ++n) b[n] = split_piece(x[i][n]);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        const Split up = split_piece(w[i][m][0]), down = split_piece(w[i][m][1]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int q = 0; q < 4; q += 2) {
+                                if (large) {
+                                    multiply_tf32(part[m][n], up.hi[q], down.hi[q], up.hi[q + 1], down.hi[q + 1], b[n].hi[q], b[n].hi[q + 1]);
+                                } else {
+                                    multiply_tf32(part[m][n], up.lo[q], down.lo[q], up.lo[q + 1], down.lo[q + 1], b[n].hi[q], b[n].hi[q + 1]);
+                                    multiply_tf32(part[m][n], up.hi[q], down.hi[q], up.hi[q + 1], down.hi[q + 1], b[n].lo[q], b[n].lo[q + 1]);
+                                }
+                            }
                     }
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-#pragma unroll
-                        for (int i = 0; i < WIDTH; ++i) sum[r * B + b] = fmaf(w[r][i], x[i], sum[r * B + b]);
                 }
-            }
-        }
-        if (feature >= j.outer) continue;
-        // halve the sums as long as there are two: a lane with the bit set keeps the upper half
-        int index = 0;
+        } else {
+            const bool bfloat = j.type == kBFloat16;
 #pragma unroll
-        for (int off = 16, left = kAll; off > 0; off >>= 1) {
-            if (left > 1) {
-                left /= 2;
-                const bool upper = lane & off;
+            for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-                for (int i = 0; i < kAll / 2; ++i) {
-                    if (i >= left) break;
-                    const float give = upper ? sum[i] : sum[i + left], keep = upper ? sum[i + left] : sum[i];
-                    sum[i] = keep + __shfl_xor_sync(0xffffffffu, give, off);
-                }
-                index += upper ? left : 0;
-            } else {
-                sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], off);
-            }
-        }
-        constexpr int kLeft = kAll > 32 ? kAll / 32 : 1, kShared = kAll < 32 ? 32 / kAll : 1;   // sums of a lane; lanes with the same one
-        if (lane % kShared != 0) continue;
+                for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < kLeft; ++i) {
-            const int at = index + i, r = at / B, b = at % B;
-            if (feature + r < j.outer && b < j.batch) epilogue.one((int)(feature + r), b, sum[i]);
+                    for (int n = 0; n < NT; ++n) {
+                        const uint4 &a = w[i][m][0], &c = w[i][m][1], &b = x[i][n];
+                        multiply_16bit(part[m][n], bfloat, a.x, c.x, a.y, c.y, b.x, b.y);
+                        multiply_16bit(part[m][n], bfloat, a.z, c.z, a.w, c.w, b.z, b.w);
+                    }
         }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[m][n][i] += part[m][n][i];
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_sum[warp][m * 16 + i / 2 * 8 + g][n * 8 + t * 2 + i % 2] = sum[m][n][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < kOutputs * j.batch; i += kRowsThreads) {
+        const int f = epilogue.feature_major ? i / j.batch : i % kOutputs, b = epilogue.feature_major ? i % j.batch : i / kOutputs;
+        if (base + f >= j.outer) continue;
+        float r = 0.f;
+#pragma unroll
+        for (int v = 0; v < kRowsWarps; ++v) r += s_sum[v][f][b];
+        epilogue.one((int)(base + f), b, r);
     }
 }
 
-// fp32: the tensor cores' way reads w, writes it in planes and reads those.  16-bit types: a tile of 64 columns is empty but for the
-// samples there, but costs no more than the FMA units from here on.
-bool dense_rows_applicable(int64_t batch, int64_t inner, int64_t outer, int type) {
-    (void)inner;
-    (void)outer;
-    return batch <= (type == kFloat32 ? 16 : 4);
+// This way / the tensor cores' way, us: fp32 784 -> 16000, 16 samples: 18 / 54, 32: 37 / 54; 2048 -> 2048: 12 / 26, 15 / 26; bf16 784 -> 16000,
+// 8: 9.6 / 11.2, 16: 12.7 / 11.2, 32: 29 / 12.4; 2048 -> 2048, 16: 7.0 / 9.0; rows off the 16-byte units, 783 -> 2001, 16: 7.0 / 13.3.
+bool dense_rows_applicable(int64_t batch, int type) { return batch <= (type == kFloat32 ? 32 : 16); }
+
+template <int NT, bool FULL, bool WHOLE>
+static void launch_outputs(const RowsJob &j, const DenseEpilogue &e, int sms, cudaStream_t st) {
+    // 32 outputs to a block read x half as often as 16, where there are blocks for all SMs all the same (and registers: NT < 4)
+    if constexpr (NT < 4)
+        if (j.outer >= 32 * 2 * sms) {
+            launch_dependent(true, dense_rows_kernel<2, NT, FULL, WHOLE>, dim3((unsigned)ceil_div(j.outer, 32)), dim3(kRowsThreads), 0, st, j, e);
+            return;
+        }
+    launch_dependent(true, dense_rows_kernel<1, NT, FULL, WHOLE>, dim3((unsigned)ceil_div(j.outer, 16)), dim3(kRowsThreads), 0, st, j, e);
 }
 
-template <int B, int R, int WIDTH>
-static void launch_rows(const RowsJob &job, const DenseEpilogue &epilogue, int sms, cudaStream_t st) {
-    RowsJob j = job;
-    int64_t chunk = kRowsBytes / (4 * B);
-    if (chunk > ceil_div(j.inner, 8) * 8) chunk = ceil_div(j.inner, 8) * 8;   // a multiple of 8
-    j.chunk = (int)chunk;
-    const size_t shared = (size_t)B * chunk * 4;
-    int64_t blocks = ceil_div(j.outer, kRowsWarps * R);
-    const int64_t most = (int64_t)sms * (shared > 32768 ? 2 : 4);
-    if (blocks > most) blocks = most;
-    cudaFuncSetAttribute(dense_rows_kernel<B, R, WIDTH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsBytes);
-    launch_dependent(true, dense_rows_kernel<B, R, WIDTH>, dim3((unsigned)blocks), dim3(kRowsThreads), shared, st, j, epilogue);
-}
-
-template <int B>
-static void launch_batch(const RowsJob &j, const DenseEpilogue &e, bool whole, int sms, cudaStream_t st) {
-    // one output to a warp where four would leave warps without any
-    const bool four = j.outer >= (int64_t)4 * kRowsWarps * 2 * sms || B > 4;
-    if (!whole) four ? launch_rows<B, 4, 1>(j, e, sms, st) : launch_rows<B, 1, 1>(j, e, sms, st);
-    else if (j.type == kFloat32) four ? launch_rows<B, 4, 4>(j, e, sms, st) : launch_rows<B, 1, 4>(j, e, sms, st);
-    else four ? launch_rows<B, 4, 8>(j, e, sms, st) : launch_rows<B, 1, 8>(j, e, sms, st);
+template <int NT>
+static void launch_samples(const RowsJob &j, const DenseEpilogue &e, bool whole, int sms, cudaStream_t st) {
+    if (j.type == kFloat32) whole ? launch_outputs<NT, true, true>(j, e, sms, st) : launch_outputs<NT, true, false>(j, e, sms, st);
+    else whole ? launch_outputs<NT, false, true>(j, e, sms, st) : launch_outputs<NT, false, false>(j, e, sms, st);
 }
 
 int launch_dense_rows(const void *x, int64_t x_pitch, bool x_feature_major, const void *w, const DenseEpilogue &epilogue, int64_t batch,
                       int64_t inner, int64_t outer, int type, int sms, cudaStream_t st) {
-    const RowsJob j = {x, w, x_feature_major ? 1 : x_pitch, x_feature_major ? x_pitch : 1, inner, outer, (int)batch, type, 0};
-    const bool whole = aligned_to(w, 16) && inner % (type == kFloat32 ? 4 : 8) == 0;
-    if (batch <= 1) launch_batch<1>(j, epilogue, whole, sms, st);
-    else if (batch <= 2) launch_batch<2>(j, epilogue, whole, sms, st);
-    else if (batch <= 4) launch_batch<4>(j, epilogue, whole, sms, st);
-    else if (batch <= 8) launch_batch<8>(j, epilogue, whole, sms, st);
-    else launch_batch<16>(j, epilogue, whole, sms, st);
+    const int values = type == kFloat32 ? 4 : 8;
+    const bool x_whole = !x_feature_major && aligned_to(x, 16) && inner % values == 0 && (batch == 1 || x_pitch % values == 0);
+    const RowsJob j = {x, w, x_feature_major ? 1 : x_pitch, x_feature_major ? x_pitch : 1, inner, outer, (int)batch, type, x_whole};
+    const bool whole = aligned_to(w, 16) && inner % values == 0;
+    if (batch <= 8) launch_samples<1>(j, epilogue, whole, sms, st);
+    else if (batch <= 16) launch_samples<2>(j, epilogue, whole, sms, st);
+    else launch_samples<4>(j, epilogue, whole, sms, st);
     return launch_status("dl_dense_forward");
 }
 

@@ -334,7 +334,7 @@ using namespace dl;
 extern "C" DL_API void dl_dense_forward_sizes(const void *x, int64_t x_pitch, int x_feature_major, const void *w, int64_t batch, int64_t inner,
                                              int64_t outer, int type, int64_t *sizes) {
     sizes[0] = sizes[1] = sizes[2] = 0;
-    if (batch <= 0 || inner <= 0 || outer <= 0 || dense_rows_applicable(batch, inner, outer, type)) return;
+    if (batch <= 0 || inner <= 0 || outer <= 0 || dense_rows_applicable(batch, type)) return;
     const DenseLayout l = dense_layout(batch, inner, outer, x_pitch, x_feature_major != 0, type, x, w);
     sizes[0] = l.x_bytes;
     sizes[1] = l.w_bytes;
@@ -355,7 +355,7 @@ extern "C" DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_fea
     const DenseLayout l = dense_layout(batch, inner, outer, x_pitch, x_feature_major != 0, type, x, w);
     const int sms = current_sms();
     cudaStream_t st = as_stream(stream);
-    if (dense_rows_applicable(batch, inner, outer, type)) {
+    if (dense_rows_applicable(batch, type)) {
         const DenseEpilogue e = {y, bias, residual, slope, y_feature_major ? batch : outer, residual_feature, residual_batch, type, act, true,
                                  y_feature_major != 0};
         return launch_dense_rows(x, x_pitch, x_feature_major != 0, w, e, batch, inner, outer, type, sms, st);
