@@ -326,7 +326,7 @@ DenseOut dense_forward(const Tensor &x, const Tensor &w, const Tensor &bias, con
     if (want_slope && act != DL_ACT_NONE) o.slope = at::empty({batch * outer}, options.dtype(kind == 0 ? at::kFloat : at::kHalf));
     o.x = readable(x);
     int64_t sizes[3];
-    dl_dense_forward_sizes(o.x.t.data_ptr(), o.x.pitch, o.x.feature_major, w.data_ptr(), batch, inner, outer, kind, sizes);
+    dl_dense_forward_sizes(o.x.t.data_ptr(), o.x.pitch, o.x.feature_major, w.data_ptr(), batch, inner, outer, feature_major, kind, sizes);
     o.x_planes = bytes(sizes[0], x);
     o.w_planes = bytes(sizes[1], x);
     const Tensor work = bytes(sizes[2], x);

@@ -80,7 +80,7 @@ __device__ __forceinline__ Split split_piece(const uint4 &v) {
 // MT groups of 16 outputs, NT of 8 samples; FULL: fp32; WHOLE: rows of w can be read 16 bytes at a time.
 template <int MT, int NT, bool FULL, bool WHOLE>
 __global__ void __launch_bounds__(kRowsThreads, MT * NT == 1 ? 3 : 2)
-dense_rows_kernel(const RowsJob j, const DenseEpilogue epilogue) {
+dense_rows_kernel(const RowsJob j, const DenseOutput output) {
     constexpr int kPiece = FULL ? 16 : 32;   // values of k that a warp's four lanes of a row read at a time
     constexpr int kAhead = NT == 1 ? 4 : 2;
     constexpr int kOutputs = 16 * MT, kSamples = 8 * NT;
@@ -169,12 +169,12 @@ dense_rows_kernel(const RowsJob j, const DenseEpilogue epilogue) {
             for (int i = 0; i < 4; ++i) s_sum[warp][m * 16 + i / 2 * 8 + g][n * 8 + t * 2 + i % 2] = sum[m][n][i];
     __syncthreads();
     for (int i = threadIdx.x; i < kOutputs * j.batch; i += kRowsThreads) {
-        const int f = epilogue.feature_major ? i / j.batch : i % kOutputs, b = epilogue.feature_major ? i % j.batch : i / kOutputs;
+        const int f = output.feature_major ? i / j.batch : i % kOutputs, b = output.feature_major ? i % j.batch : i / kOutputs;
         if (base + f >= j.outer) continue;
         float r = 0.f;
 #pragma unroll
         for (int v = 0; v < kRowsWarps; ++v) r += s_sum[v][f][b];
-        epilogue.one((int)(base + f), b, r);
+        output.one((int)(base + f), b, r);
     }
 }
 
@@ -183,7 +183,7 @@ dense_rows_kernel(const RowsJob j, const DenseEpilogue epilogue) {
 bool dense_rows_applicable(int64_t batch, int type) { return batch <= (type == kFloat32 ? 32 : 16); }
 
 template <int NT, bool FULL, bool WHOLE>
-static void launch_outputs(const RowsJob &j, const DenseEpilogue &e, int sms, cudaStream_t st) {
+static void launch_outputs(const RowsJob &j, const DenseOutput &e, int sms, cudaStream_t st) {
     // 32 outputs to a block read x half as often as 16, where there are blocks for all SMs all the same (and registers: NT < 4)
     if constexpr (NT < 4)
         if (j.outer >= 32 * 2 * sms) {
@@ -194,20 +194,20 @@ static void launch_outputs(const RowsJob &j, const DenseEpilogue &e, int sms, cu
 }
 
 template <int NT>
-static void launch_samples(const RowsJob &j, const DenseEpilogue &e, bool whole, int sms, cudaStream_t st) {
+static void launch_samples(const RowsJob &j, const DenseOutput &e, bool whole, int sms, cudaStream_t st) {
     if (j.type == kFloat32) whole ? launch_outputs<NT, true, true>(j, e, sms, st) : launch_outputs<NT, true, false>(j, e, sms, st);
     else whole ? launch_outputs<NT, false, true>(j, e, sms, st) : launch_outputs<NT, false, false>(j, e, sms, st);
 }
 
-int launch_dense_rows(const void *x, int64_t x_pitch, bool x_feature_major, const void *w, const DenseEpilogue &epilogue, int64_t batch,
+int launch_dense_rows(const void *x, int64_t x_pitch, bool x_feature_major, const void *w, const DenseOutput &output, int64_t batch,
                       int64_t inner, int64_t outer, int type, int sms, cudaStream_t st) {
     const int values = type == kFloat32 ? 4 : 8;
     const bool x_whole = !x_feature_major && aligned_to(x, 16) && inner % values == 0 && (batch == 1 || x_pitch % values == 0);
     const RowsJob j = {x, w, x_feature_major ? 1 : x_pitch, x_feature_major ? x_pitch : 1, inner, outer, (int)batch, type, x_whole};
     const bool whole = aligned_to(w, 16) && inner % values == 0;
-    if (batch <= 8) launch_samples<1>(j, epilogue, whole, sms, st);
-    else if (batch <= 16) launch_samples<2>(j, epilogue, whole, sms, st);
-    else launch_samples<4>(j, epilogue, whole, sms, st);
+    if (batch <= 8) launch_samples<1>(j, output, whole, sms, st);
+    else if (batch <= 16) launch_samples<2>(j, output, whole, sms, st);
+    else launch_samples<4>(j, output, whole, sms, st);
     return launch_status("dl_dense_forward");
 }
 

@@ -174,7 +174,8 @@ eval_tma_kernel(const SplitRows x, const int64_t *__restrict__ a, const int64_t 
 int groupbitsum_async_error();       // groupbitsum_tma.cu
 int eval_groupbitsum_async_error();  // eval_groupbitsum.cu
 int forward_tma_async_error();       // forward_tma.cu
-int matmul_async_error();            // matmul.cu
+int dense_async_error();             // dense.cu
+int orthogonalize_async_error();     // orthogonalize.cu
 
 static int sm_count() {
     static int cached[64] = {0};
@@ -277,7 +278,9 @@ extern "C" DL_API int dl_async_error(void) {
     if (fused < 0) return fused;
     const int fwd = dl::forward_tma_async_error();
     if (fwd < 0) return fwd;
-    const int products = dl::matmul_async_error();
-    if (products < 0) return products;
-    return flag | other | fused | fwd | products;
+    const int dense = dl::dense_async_error();
+    if (dense < 0) return dense;
+    const int steps = dl::orthogonalize_async_error();
+    if (steps < 0) return steps;
+    return flag | other | fused | fwd | dense | steps;
 }

@@ -64,6 +64,36 @@ __device__ __forceinline__ void split_triple(float x, uint16_t &hi, uint16_t &mi
 // -- the kernel -----------------------------------------------------------------------------------------------------------------
 
 constexpr int kMatmulRows = 128;     // of a tile
+constexpr int kPieceColumns = 16;    // a piece: 32 rows of 16 columns, lane = row
+constexpr int kPiecePitch = kPieceColumns + 4;   // floats per row of a piece in shared memory: 16-byte rows, 8 lanes on 8 banks
+
+// An epilogue takes pieces: `begin` says where the first piece of a warp's share of a tile lies (row, col: of its first value), `piece`
+// takes the one `across` columns further, from registers.  The functions below turn a piece by way of shared memory: into quads, lane l
+// having rows l / 4 + 8 i and columns 4 (l % 4) .. + 3, or into columns, lane l having rows 4 (l % 8) .. + 3 of columns l / 8 + 4 i.
+__device__ __forceinline__ void piece_store(float *stage, int lane, const float (&v)[kPieceColumns]) {
+#pragma unroll
+    for (int c = 0; c < kPieceColumns; c += 4)
+        *reinterpret_cast<float4 *>(stage + lane * kPiecePitch + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+    __syncwarp();
+}
+__device__ __forceinline__ void piece_quads(const float *stage, int lane, float (&q)[4][4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float4 f = *reinterpret_cast<const float4 *>(stage + (lane / 4 + 8 * i) * kPiecePitch + lane % 4 * 4);
+        q[i][0] = f.x; q[i][1] = f.y; q[i][2] = f.z; q[i][3] = f.w;
+    }
+}
+__device__ __forceinline__ void piece_put_quads(float *stage, int lane, const float (&q)[4][4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4 *>(stage + (lane / 4 + 8 * i) * kPiecePitch + lane % 4 * 4) = make_float4(q[i][0], q[i][1], q[i][2], q[i][3]);
+}
+__device__ __forceinline__ void piece_columns(const float *stage, int lane, float (&q)[4][4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[i][j] = stage[(lane % 8 * 4 + j) * kPiecePitch + lane / 8 + 4 * i];
+}
 
 // Warps 0 .. 7: epilogue, one lane per row, two warps to the same rows; then one for the copies, one for the products, two idle: the
 // registers that the epilogue does not leave to the others are handed out in groups of four warps.
@@ -74,8 +104,8 @@ struct MatmulConfig {
     static constexpr int kTileRows = PAIR ? 2 * kMatmulRows : kMatmulRows;
     static constexpr int kOwnColumns = PAIR ? COLUMNS / 2 : COLUMNS;           // rows of B that a CTA copies
     static constexpr int kShare = COLUMNS / (kWarps / 4);                      // columns of an epilogue warp
-    static constexpr int kSpan = 16;                                           // of them staged at a time
-    static constexpr int kPitch = kSpan + 4;                                   // floats per row of a staging tile: 16-byte rows on different banks
+    static constexpr int kSpan = kPieceColumns;                                // of them handed to the epilogue at a time
+    static constexpr int kPitch = kPiecePitch;
     static constexpr int kStepBytes = PLANES * (kMatmulRows + kOwnColumns) * kChunk * 2;   // of a CTA
     static constexpr int kStagingBytes = kWarps * 32 * kPitch * 4;
     static constexpr int kFit = (232448 - 1024 - 256 - kStagingBytes) / kStepBytes;
@@ -88,7 +118,8 @@ struct MatmulConfig {
 };
 
 struct Tile {
-    int matrix, split, row, col;  // first row and column
+    int matrix, split, index;     // of the matrix' tiles
+    int row, col;                 // first ones
 };
 
 template <int ROWS, int COLUMNS>
@@ -99,6 +130,7 @@ __device__ __forceinline__ Tile tile_of(int id, const MatmulShape &s) {
     id -= t.matrix * all;
     t.split = id / s.per_matrix;
     id -= t.split * s.per_matrix;
+    t.index = id;
     int mi, ni;
     if (s.symmetric) {
         mi = 0;
@@ -290,26 +322,10 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         for (int id = first_tile; id < s.tiles && ok; id += tile_step) {
             const Tile t = tile_of<Config::kTileRows, COLUMNS>(id, s);
             const int first = t.split * s.steps_per_split, last = min(s.k_steps, first + s.steps_per_split);
-            const int row0 = t.row + (int)rank * kMatmulRows + quarter * 32, slice = t.split * s.batch + t.matrix;
-            const auto finish = [&](const float (&v)[kSpan], int col0) {
-                if (col0 >= s.n) return;
-                if (epilogue.by_column(row0, col0)) epilogue.template down<kSpan>(slice, row0 + lane, col0, v, s.m, min(kSpan, s.n - col0));
-                if (epilogue.by_row(row0, col0)) {
-                    constexpr int kQuads = kSpan / 4, kStep = 32 / kQuads;
-#pragma unroll
-                    for (int c = 0; c < kSpan; c += 4)
-                        *reinterpret_cast<float4 *>(mine + lane * kPitch + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
-                    __syncwarp();
-                    const int c = lane % kQuads * 4;
-                    float q[kQuads][4];
-#pragma unroll
-                    for (int i = 0; i < kQuads; ++i) {
-                        const float4 f = *reinterpret_cast<const float4 *>(mine + (i * kStep + lane / kQuads) * kPitch + c);
-                        q[i][0] = f.x; q[i][1] = f.y; q[i][2] = f.z; q[i][3] = f.w;
-                    }
-                    if (col0 + c < s.n) epilogue.template across<kQuads, kStep>(slice, row0 + lane / kQuads, col0 + c, q, s.m, min(4, s.n - col0 - c));
-                    __syncwarp();
-                }
+            const int row0 = t.row + (int)rank * kMatmulRows + quarter * 32;
+            const auto place = epilogue.begin(t, s, row0, t.col + from, lane);
+            const auto finish = [&](const float (&v)[kSpan], int across) {
+                if (t.col + from + across < s.n || Epilogue::kWholeTiles) epilogue.piece(place, across, v, mine, lane);
             };
             float kept[kKeep ? kShare : 1];
 #pragma unroll
@@ -321,29 +337,38 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 tensor_fence_after();
                 const uint32_t sums = tensor + buffer * Config::kSums * COLUMNS + from + ((uint32_t)quarter * 32 << 16);
                 if constexpr (kKeep) {
+                    // 64 values on their way at a time
+                    constexpr int kTake = Config::kSums == 2 ? 32 : kShare < 64 ? kShare : 64;
 #pragma unroll
-                    for (int c0 = 0; c0 < kShare; c0 += 16) {
-                        uint32_t large[16], small[16];
-                        tensor_read16(sums + c0, large);
-                        if (Config::kSums == 2) tensor_read16(sums + COLUMNS + c0, small);
+                    for (int c0 = 0; c0 < kShare; c0 += kTake) {
+                        uint32_t one[32], other[32];
+                        tensor_read32(sums + c0, one);
+                        if (Config::kSums == 2) tensor_read32(sums + COLUMNS + c0, other);
+                        else if (kTake == 64) tensor_read32(sums + c0 + 32, other);
                         tensor_read_wait();
 #pragma unroll
-                        for (int c = 0; c < 16; ++c) {
-                            float v = __uint_as_float(large[c]);
-                            if (Config::kSums == 2) v += __uint_as_float(small[c]);
-                            kept[c0 + c] += v;
+                        for (int c = 0; c < 32; ++c) {
+                            if (Config::kSums == 2) {
+                                kept[c0 + c] += __uint_as_float(one[c]) + __uint_as_float(other[c]);
+                            } else {
+                                kept[c0 + c] += __uint_as_float(one[c]);
+                                if (kTake == 64) kept[c0 + 32 + c] += __uint_as_float(other[c]);
+                            }
                         }
                     }
                 } else {
 #pragma unroll 1
-                    for (int c0 = 0; c0 < kShare && t.col + from + c0 < s.n; c0 += kSpan) {
-                        uint32_t bits[kSpan];
-                        float v[kSpan];
-                        tensor_read16(sums + c0, bits);
+                    for (int c0 = 0; c0 < kShare && (t.col + from + c0 < s.n || Epilogue::kWholeTiles); c0 += 32) {
+                        uint32_t bits[32];
+                        tensor_read32(sums + c0, bits);
                         tensor_read_wait();
 #pragma unroll
-                        for (int c = 0; c < kSpan; ++c) v[c] = __uint_as_float(bits[c]);
-                        finish(v, t.col + from + c0);
+                        for (int h = 0; h < 2; ++h) {
+                            float v[kSpan];
+#pragma unroll
+                            for (int c = 0; c < kSpan; ++c) v[c] = __uint_as_float(bits[h * kSpan + c]);
+                            finish(v, c0 + h * kSpan);
+                        }
                     }
                 }
                 tensor_fence_before();
@@ -364,7 +389,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         for (int c = 0; c < kSpan; ++c) v[c] = kept[c];
 #pragma unroll
                         for (int c = 0; c + kSpan < kShare; ++c) kept[c] = kept[c + kSpan];
-                        finish(v, t.col + from + c0);
+                        finish(v, c0);
                     }
                 }
             }
@@ -381,65 +406,54 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     if (warp == Config::kWarps + 1) tensor_free<PAIR>(tensor, Config::kTensorColumns);
 }
 
-// An epilogue says which way a piece of a tile is handed to it (both, where a symmetric result is stored on both sides):
-//   across: neighbouring lanes have neighbouring columns, a lane four of them in N rows, kStep apart;
-//   down:   neighbouring lanes have neighbouring rows, a lane N columns of one row.
-
-// Sums of a product that was split along k: kept as they are, added up in the order of the splits by matmul_join_kernel.
+// Sums of a product that was split along k, whole tiles of them, each piece as its lanes have it; matmul_join_kernel adds them up in the
+// order of the splits.
 struct StorePartial {
+    static constexpr bool kWholeTiles = true;
     float *out;
-    int64_t n, matrix;   // values of a row, of a matrix
-    __device__ __forceinline__ bool by_column(int, int) const { return false; }
-    __device__ __forceinline__ bool by_row(int, int) const { return true; }
-    template <int N>
-    __device__ __forceinline__ void down(int, int, int, const float (&)[N], int, int) const {}
-    template <int N, int STEP>
-    __device__ __forceinline__ void across(int slice, int row, int col, const float (&q)[N][4], int m, int valid) const {
+    int tile_rows, columns;
+    struct Place {
+        float4 *to;
+    };
+    // pieces of a tile, down and then across
+    __device__ __forceinline__ Place begin(const Tile &t, const MatmulShape &s, int row, int col, int lane) const {
+        const int64_t tile = (int64_t)(t.split * s.batch + t.matrix) * s.per_matrix + t.index;
+        const int piece = (row - t.row) / 32 + (col - t.col) / kPieceColumns * (tile_rows / 32);
+        return {reinterpret_cast<float4 *>(out + tile * tile_rows * columns) + piece * (8 * kPieceColumns) + lane};
+    }
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kPieceColumns], float *, int) const {
+        float4 *to = p.to + across / kPieceColumns * (tile_rows / 32) * (8 * kPieceColumns);
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (row + i * STEP < m) store4(out, slice * matrix + (int64_t)(row + i * STEP) * n + col, kFloat32, valid, q[i]);
+        for (int c = 0; c < kPieceColumns; c += 4) to[c * 8] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
     }
 };
 
-template <class Epilogue>
+template <int ROWS, int COLUMNS, class Epilogue>
 __global__ void __launch_bounds__(kThreads)
-matmul_join_kernel(const float *__restrict__ partial, int splits, int batch, int m, int n, int symmetric, const Epilogue epilogue) {
+matmul_join_kernel(const float *__restrict__ partial, const MatmulShape s, const Epilogue epilogue) {
+    __shared__ __align__(16) float s_stage[kThreads / 32][32 * kPiecePitch];
     grid_dependency_wait();
     grid_dependents_launch();
-    const int64_t quads = (n + 3) / 4, matrix = (int64_t)m * n, total = quads * m * batch;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-        const bool columns = epilogue.by_column(0, 0) && !symmetric;
-        int64_t rest = i;
-        int row, quad;
-        if (columns) {   // neighbouring threads write neighbouring rows
-            row = (int)(rest % m);
-            rest /= m;
-            quad = (int)(rest % quads);
-            rest /= quads;
-        } else {
-            quad = (int)(rest % quads);
-            rest /= quads;
-            row = (int)(rest % m);
-            rest /= m;
-        }
-        const int z = (int)rest, col = quad * 4, valid = min(4, n - col);
-        float q[1][4] = {{0.f, 0.f, 0.f, 0.f}};
-        float(&v)[4] = q[0];
-        const bool mirrored = symmetric && col / kMatmulRows > row / kMatmulRows;   // a multiple of 4 columns: all of a quad alike
-        for (int sp = 0; sp < splits; ++sp) {
-            const float *p = partial + ((int64_t)sp * batch + z) * matrix;
-            float f[4];
-            if (mirrored) {
+    constexpr int kDown = ROWS / 32, kPieces = kDown * COLUMNS / kPieceColumns;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int64_t tiles = (int64_t)s.per_matrix * s.batch;
+    for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + warp; i < tiles * kPieces; i += (int64_t)gridDim.x * (kThreads / 32)) {
+        const int64_t tile = i / kPieces;
+        const int piece = (int)(i - tile * kPieces), matrix = (int)(tile / s.per_matrix);
+        const Tile t = tile_of<ROWS, COLUMNS>((int)(tile - (int64_t)matrix * s.per_matrix) + matrix * s.per_matrix * s.splits, s);
+        const int row = t.row + piece % kDown * 32, col = t.col + piece / kDown * kPieceColumns;
+        if (row >= s.m || col >= s.n) continue;
+        const float4 *from = reinterpret_cast<const float4 *>(partial + tile * ROWS * COLUMNS) + piece * (8 * kPieceColumns) + lane;
+        const int64_t split = tiles * ROWS * COLUMNS / 4;
+        float v[kPieceColumns] = {};
+        for (int sp = 0; sp < s.splits; ++sp, from += split) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) f[j] = j < valid ? p[(int64_t)(col + j) * n + row] : 0.f;
-            } else {
-                load4(p, (int64_t)row * n + col, kFloat32, valid, f);
+            for (int c = 0; c < kPieceColumns; c += 4) {
+                const float4 f = from[c * 8];
+                v[c] += f.x; v[c + 1] += f.y; v[c + 2] += f.z; v[c + 3] += f.w;
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] += f[j];
         }
-        if (columns) epilogue.template down<4>(z, row, col, v, m, valid);
-        else epilogue.template across<1, 1>(z, row, col, q, m, valid);
+        epilogue.piece(epilogue.begin(t, s, row, col, lane), 0, v, s_stage[warp], lane);
     }
 }
 #endif  // __CUDACC__

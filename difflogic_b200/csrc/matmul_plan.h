@@ -44,7 +44,7 @@ static inline MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, int64_t ba
             const int64_t per = ceil_div(steps, splits), really = ceil_div(steps, per);
             if (really != splits || (only_splits > 0 && splits > only_splits)) continue;
             const int64_t tiles = per_matrix * batch * splits, waves = ceil_div(tiles, pair ? sms / 2 : sms);
-            const int64_t partial = splits > 1 ? splits * batch * m * n * 4 : 0;
+            const int64_t partial = splits > 1 ? tiles * (pair ? 256 : 128) * columns * 4 : 0;
             if (partial > (int64_t)64 << 20) continue;
             double clocks = 1500 + waves * (per * step + 150) + last;
             if (splits > 1) clocks += 3000 + (double)partial / 2000;

@@ -1,0 +1,517 @@
+// Newton-Schulz steps on matrices by the matrix products of matmul.cuh, the Muon step made of them, and their entry points.
+#include <math.h>
+
+#include "gram_steps.h"
+#include "matmul_launch.cuh"
+
+namespace dl {
+
+int orthogonalize_async_error() { return matmul_error_flag(); }
+
+// What is orthogonalised: `count` matrices behind each other at entry 0, or one at every entry; with momenta the update of a step,
+// made of gradients and momenta as they are read.
+struct Matrices {
+    static constexpr int kMost = 16;
+    const void *g[kMost];
+    float *momentum[kMost];   // null: g as it is
+    float *weight[kMost];
+    int64_t stride;           // values from one matrix to the next at entry 0
+    int type;
+    float keep, nesterov;     // 1 - momentum; the momentum, or 1: the update is the momentum itself
+};
+
+// Sums of squares of a matrix, one per block, in 64 bits: fp32 values of any size fit.  Momenta are moved on.
+__global__ void __launch_bounds__(kThreads)
+square_sums_kernel(const Matrices all, int64_t count, double *__restrict__ partial) {
+    __shared__ double s_part[kThreads / 32];
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const int64_t z = blockIdx.y, base = all.stride * z, quads = (count + 3) / 4;
+    const int entry = all.stride ? 0 : (int)z;
+    const void *g = all.g[entry];
+    float *momentum = all.momentum[entry];
+    double sum = 0;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < quads; i += (int64_t)gridDim.x * kThreads) {
+        const int valid = (int)(count - i * 4 < 4 ? count - i * 4 : 4);
+        float v[4];
+        load4(g, base + i * 4, all.type, valid, v);
+        if (momentum != nullptr) {
+            float m[4];
+            load4(momentum, base + i * 4, kFloat32, valid, m);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                m[j] = new_momentum(m[j], v[j], all.keep);
+                v[j] = update_of(m[j], v[j], all.nesterov);
+            }
+            store4(momentum, base + i * 4, kFloat32, valid, m);
+        }
+        sum += ((double)v[0] * v[0] + (double)v[1] * v[1]) + ((double)v[2] * v[2] + (double)v[3] * v[3]);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (threadIdx.x % 32 == 0) s_part[threadIdx.x / 32] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kThreads / 32; ++i) sum += s_part[i];
+        partial[z * gridDim.x + blockIdx.x] = sum;
+    }
+}
+
+// X = G / max(|G|, eps) as pairs.
+__global__ void __launch_bounds__(kThreads)
+normalise_kernel(const Matrices all, int64_t rows, int64_t cols, const double *__restrict__ partial, int parts, double eps,
+                 uint16_t *__restrict__ x, int64_t pitch, int64_t plane) {
+    __shared__ float s_scale;
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const int64_t z = blockIdx.y, base = all.stride * z;
+    const int entry = all.stride ? 0 : (int)z;
+    const void *g = all.g[entry];
+    const float *momentum = all.momentum[entry];
+    if (threadIdx.x < 32) {
+        double sum = 0;
+        for (int i = threadIdx.x; i < parts; i += 32) sum += partial[z * parts + i];
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        const double norm = sqrt(sum);
+        // a norm that is not finite (an infinite or undefined entry) makes the whole result undefined
+        if (threadIdx.x == 0) s_scale = norm <= 1.7e308 ? (float)((double)kPairScale / (norm > eps ? norm : eps)) : __int_as_float(0x7fc00000);
+    }
+    __syncthreads();
+    const float scale = s_scale;
+    const int64_t quads = (cols + 3) / 4, total = rows * quads;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t row = i / quads, col = (i - row * quads) * 4, at = base + row * cols + col;
+        const int valid = (int)(cols - col < 4 ? cols - col : 4);
+        float v[4];
+        load4(g, at, all.type, valid, v);
+        if (momentum != nullptr) {
+            float m[4];
+            load4(momentum, at, kFloat32, valid, m);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = update_of(m[j], v[j], all.nesterov);
+        }
+        uint16_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_pair(v[j] * scale, hi[j], lo[j]);
+        uint16_t *to = x + 2 * z * plane + row * pitch + col;
+        *reinterpret_cast<ushort4 *>(to) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<ushort4 *>(to + plane) = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+    }
+}
+
+// Results of the iteration as pairs: v = scale * sum (+ factor * the pair in `more`) (+ diagonal on the diagonal).  Of a symmetric result
+// the blocks of 128 x 128 below the diagonal are stored on both sides, those above it not looked at.  Rows are padded to whole units: the values behind the
+// last one are written too, and read by nothing.
+struct PairEpilogue {
+    static constexpr bool kWholeTiles = false;
+    uint16_t *out;
+    const uint16_t *more;   // laid out as `out`; null: none
+    int64_t pitch, plane;
+    float scale, factor, diagonal;
+    bool symmetric;
+    struct Place {
+        int row, col, m, n;          // of the warp's first value
+        int64_t matrix;
+    };
+    __device__ __forceinline__ Place begin(const Tile &t, const MatmulShape &s, int row, int col, int) const {
+        return {row, col, s.m, s.n, 2 * t.matrix * plane};
+    }
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kPieceColumns], float *stage, int lane) const {
+        const int first = p.col + across, below = p.row / kMatmulRows - first / kMatmulRows;
+        if (symmetric && below < 0) return;
+        piece_store(stage, lane, v);
+        float q[4][4];
+        piece_quads(stage, lane, q);
+        __syncwarp();
+        const int row = p.row + lane / 4, col = first + lane % 4 * 4;
+        const int64_t at = p.matrix + row * pitch + col;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[i][j] *= scale;
+        if (diagonal != 0.f && below == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (row + 8 * i == col + j) q[i][j] += diagonal;
+        }
+        if (more != nullptr && col < p.n) {
+            ushort4 hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                hi[i] = lo[i] = make_ushort4(0, 0, 0, 0);
+                if (row + 8 * i >= p.m) continue;
+                hi[i] = *reinterpret_cast<const ushort4 *>(more + at + 8 * i * pitch);
+                lo[i] = *reinterpret_cast<const ushort4 *>(more + at + 8 * i * pitch + plane);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                q[i][0] += factor * join_pair(hi[i].x, lo[i].x);
+                q[i][1] += factor * join_pair(hi[i].y, lo[i].y);
+                q[i][2] += factor * join_pair(hi[i].z, lo[i].z);
+                q[i][3] += factor * join_pair(hi[i].w, lo[i].w);
+            }
+        }
+        if (symmetric && below > 0) {   // from here the mirrored values are taken
+            piece_put_quads(stage, lane, q);
+            __syncwarp();
+        }
+        if (col < p.n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (row + 8 * i < p.m) store_pairs(out + at + 8 * i * pitch, q[i]);
+        }
+        if (symmetric && below > 0) {
+            piece_columns(stage, lane, q);
+            __syncwarp();
+            const int from = p.row + lane % 8 * 4, to = first + lane / 8;   // columns of the result: rows of the piece
+            if (from < p.m) {
+                uint16_t *mirrored = out + p.matrix + to * pitch + from;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (to + 4 * i < p.n) store_pairs(mirrored + 4 * i * pitch, q[i]);
+            }
+        }
+    }
+    __device__ __forceinline__ void store_pairs(uint16_t *to, const float (&v)[4]) const {
+        uint16_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_pair(v[j], hi[j], lo[j]);
+        *reinterpret_cast<ushort4 *>(to) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<ushort4 *>(to + plane) = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+    }
+};
+
+// The last product: the result itself, or the weights' update w <- decay w - rate v.
+struct OrthogonalEpilogue {
+    static constexpr bool kWholeTiles = false;
+    void *out;              // results behind each other; null: the weights of `all` are updated
+    Matrices all;
+    int64_t cols;           // values of a row
+    const uint16_t *more;   // added, as in PairEpilogue
+    int64_t pitch, plane;
+    float scale, factor;
+    float decay, rate;
+    struct Place {
+        int row, col, m, n;   // of the lane's first value
+        int64_t at, matrix;
+        float *weight;
+    };
+    __device__ __forceinline__ Place begin(const Tile &t, const MatmulShape &s, int row, int col, int lane) const {
+        const int r = row + lane / 4, c = col + lane % 4 * 4;
+        const int64_t at = r * cols + c;
+        return {r, c, s.m, s.n, out == nullptr ? at : at + t.matrix * s.m * cols, 2 * t.matrix * plane, out == nullptr ? all.weight[t.matrix] : nullptr};
+    }
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kPieceColumns], float *stage, int lane) const {
+        piece_store(stage, lane, v);
+        float q[4][4], w[4][4];
+        piece_quads(stage, lane, q);
+        __syncwarp();
+        const int left = p.n - p.col - across;
+        if (left <= 0) return;
+        if (p.weight != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (p.row + 8 * i < p.m) load4(p.weight, p.at + across + 8 * i * cols, kFloat32, left < 4 ? left : 4, w[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (p.row + 8 * i >= p.m) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[i][j] *= scale;
+            if (more != nullptr) {
+                const uint16_t *from = more + p.matrix + (p.row + 8 * i) * pitch + p.col + across;
+                const ushort4 hi = *reinterpret_cast<const ushort4 *>(from), lo = *reinterpret_cast<const ushort4 *>(from + plane);
+                q[i][0] += factor * join_pair(hi.x, lo.x);
+                q[i][1] += factor * join_pair(hi.y, lo.y);
+                q[i][2] += factor * join_pair(hi.z, lo.z);
+                q[i][3] += factor * join_pair(hi.w, lo.w);
+            }
+            if (p.weight != nullptr) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q[i][j] = w[i][j] * decay - rate * q[i][j];
+                store4(p.weight, p.at + across + 8 * i * cols, kFloat32, left < 4 ? left : 4, q[i]);
+            } else {
+                store4(out, p.at + across + 8 * i * cols, all.type, left < 4 ? left : 4, q[i]);
+            }
+        }
+    }
+};
+
+// The iterations multiply one plane or two.
+template <class Epilogue>
+static int launch_planes(const Product &p, const MatmulPlan &plan, const Epilogue &e, float *partial, int sms, cudaStream_t st, const char *what) {
+    return p.planes == 1 ? launch_product<1>(p, plan, e, partial, sms, st, what) : launch_product<2>(p, plan, e, partial, sms, st, what);
+}
+
+struct OrthogonalLayout {
+    int64_t side, x_pitch, x_plane, s_pitch, s_plane;   // side: the smaller one
+    bool tall;
+    int parts;
+    MatmulPlan gram, square, product;
+    int64_t x_bytes, s_bytes, norm_bytes, partial_bytes;
+    int64_t total() const { return 2 * x_bytes + 2 * s_bytes + norm_bytes + partial_bytes; }
+};
+
+static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t cols, bool light, int sms) {
+    OrthogonalLayout l = {};
+    l.tall = rows >= cols;
+    l.side = l.tall ? cols : rows;
+    l.x_pitch = padded(cols);
+    l.x_plane = rows * l.x_pitch;
+    l.s_pitch = padded(l.side);
+    l.s_plane = l.side * l.s_pitch;
+    l.parts = (int)(ceil_div(rows * cols, 4 * kThreads * 4) < 2 * sms ? ceil_div(rows * cols, 4 * kThreads * 4) : 2 * sms);
+    l.gram = plan_matmul(l.side, l.side, l.tall ? rows : cols, batch, light ? 1 : 2, true, sms);
+    l.square = plan_matmul(l.side, l.side, l.side, batch, 2, true, sms);
+    l.product = plan_matmul(rows, cols, l.side, batch, light ? 1 : 2, false, sms);
+    l.x_bytes = padded_bytes(batch * 2 * l.x_plane * 2);
+    l.s_bytes = padded_bytes(batch * 2 * l.s_plane * 2);
+    l.norm_bytes = padded_bytes(batch * l.parts * 8);
+    l.partial_bytes = l.gram.partial_bytes;
+    if (l.square.partial_bytes > l.partial_bytes) l.partial_bytes = l.square.partial_bytes;
+    if (l.product.partial_bytes > l.partial_bytes) l.partial_bytes = l.product.partial_bytes;
+    return l;
+}
+
+// steps times: S = X^T X (X X^T where X is wide), M = b S + c S^2, X = a X + X M (M X).  `last` takes the last product.
+//
+// Results of 22 bits (fp32, fp16): every product is one of pairs, and a X comes out of the product too, as the diagonal of M, since
+// the pair of a X would have to be read again.  bf16 results have 8 bits, and the steps need no more than this: S from the first planes
+// alone, which leaves the result 6e-4 off (relative, over random, low-rank and steeply falling spectra; rounding it to bf16 is
+// 1.7e-3); S^2 from pairs; X M from the first planes, a X added as the pair that it is.  That last form matters: what is rounded away
+// of X in a product with a I + b S + c S^2 grows by a factor of a in every step along directions of small singular values, 4e-2 in the
+// end where X has few large ones; M alone is next to nothing along those.  All together 1.6e-3, half the products.
+static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64_t cols, int steps, const float *coefficients, double eps,
+                         const OrthogonalEpilogue &last, uint8_t *workspace, int sms, cudaStream_t st, const char *what) {
+    const bool light = all.type == kBFloat16;
+    const OrthogonalLayout l = orthogonal_layout(batch, rows, cols, light, sms);
+    uint16_t *x = reinterpret_cast<uint16_t *>(workspace), *next = reinterpret_cast<uint16_t *>(workspace + l.x_bytes);
+    uint16_t *gram = reinterpret_cast<uint16_t *>(workspace + 2 * l.x_bytes), *poly = reinterpret_cast<uint16_t *>(workspace + 2 * l.x_bytes + l.s_bytes);
+    double *norms = reinterpret_cast<double *>(workspace + 2 * l.x_bytes + 2 * l.s_bytes);
+    float *partial = reinterpret_cast<float *>(workspace + 2 * l.x_bytes + 2 * l.s_bytes + l.norm_bytes);
+    int status;
+    launch_dependent(true, square_sums_kernel, dim3((unsigned)l.parts, (unsigned)batch), dim3(kThreads), 0, st, all, rows * cols, norms);
+    if ((status = launch_status(what)) != DL_OK) return status;
+    int64_t blocks = ceil_div(rows * ceil_div(cols, 4), kThreads * 2);
+    if (blocks > 16 * sms) blocks = 16 * sms;
+    launch_dependent(true, normalise_kernel, dim3((unsigned)blocks, (unsigned)batch), dim3(kThreads), 0, st, all, rows, cols, (const double *)norms,
+                     l.parts, eps, x, l.x_pitch, l.x_plane);
+    if ((status = launch_status(what)) != DL_OK) return status;
+    Product p = {};
+    p.batch = batch;
+    p.planes_z = 2;
+    p.exact = !light;
+    const float once = 1.f / kPairScale, twice = once * once;
+    for (int i = 0; i < steps; ++i) {
+        const float a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
+        p.a = p.b = {x, l.x_pitch, l.x_plane, l.tall};
+        p.m = p.n = l.side;
+        p.k = l.tall ? rows : cols;
+        p.symmetric = true;
+        p.planes = light ? 1 : 2;
+        const PairEpilogue to_gram = {gram, nullptr, l.s_pitch, l.s_plane, once, 0.f, 0.f, true};
+        if ((status = launch_planes(p, l.gram, to_gram, partial, sms, st, what)) != DL_OK) return status;
+        p.a = p.b = {gram, l.s_pitch, l.s_plane, false};
+        p.k = l.side;
+        p.planes = 2;
+        const PairEpilogue to_poly = {poly, gram, l.s_pitch, l.s_plane, c * once, b, light ? 0.f : a * kPairScale, true};
+        if ((status = launch_planes(p, l.square, to_poly, partial, sms, st, what)) != DL_OK) return status;
+        const Operand m = {poly, l.s_pitch, l.s_plane, false};
+        p.a = l.tall ? Operand{x, l.x_pitch, l.x_plane, false} : m;
+        p.b = l.tall ? m : Operand{x, l.x_pitch, l.x_plane, true};
+        p.m = rows;
+        p.n = cols;
+        p.symmetric = false;
+        p.planes = light ? 1 : 2;
+        const uint16_t *more = light ? x : nullptr;
+        if (i + 1 < steps) {
+            const PairEpilogue to_next = {next, more, l.x_pitch, l.x_plane, once, a, 0.f, false};
+            status = launch_planes(p, l.product, to_next, partial, sms, st, what);
+        } else {
+            OrthogonalEpilogue e = last;
+            e.all = all;
+            e.cols = cols;
+            e.more = more;
+            e.pitch = l.x_pitch;
+            e.plane = l.x_plane;
+            e.scale = twice;
+            e.factor = a * once;
+            status = launch_planes(p, l.product, e, partial, sms, st, what);
+        }
+        if (status != DL_OK) return status;
+        uint16_t *done = x;
+        x = next;
+        next = done;
+    }
+    return DL_OK;
+}
+
+}  // namespace dl
+
+using namespace dl;
+
+// Matrices of so few columns stay as they are: their Gram matrix is iterated instead (gram_steps.cu).
+static bool few_columns(int64_t cols) { return cols <= kGramColumns; }
+
+extern "C" DL_API int64_t dl_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int type) {
+    if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
+    if (few_columns(cols)) return gram_workspace_bytes(batch, batch * rows, current_sms());
+    return orthogonal_layout(batch, rows, cols, type == kBFloat16, current_sms()).total();
+}
+
+static int check_steps(int steps, const float *coefficients, double eps, const char *what) {
+    DL_REQUIRE(steps >= 1 && steps <= kMostSteps && coefficients, DL_ERR_INVALID_ARG, "%s: needs 1 to %d steps and their coefficients", what, kMostSteps);
+    DL_REQUIRE(eps > 0, DL_ERR_INVALID_ARG, "%s: eps must be positive", what);
+    return DL_OK;
+}
+
+extern "C" DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, int64_t rows, int64_t cols, int type, int steps,
+                                       const float *coefficients, double eps, void *workspace, void *stream) {
+    const char *what = "dl_orthogonalize";
+    DL_REQUIRE(batch >= 0 && rows >= 0 && cols >= 0 && rows <= INT32_MAX / 2 && cols <= INT32_MAX / 2, DL_ERR_INVALID_ARG, "%s: bad size", what);
+    DL_REQUIRE(batch <= 65535, DL_ERR_TOO_LARGE, "%s: more than 65535 matrices", what);
+    DL_REQUIRE(type >= kFloat32 && type <= kFloat16, DL_ERR_INVALID_ARG, "%s: unknown type %d", what, type);
+    int status = check_steps(steps, coefficients, eps, what);
+    if (status != DL_OK) return status;
+    if (batch == 0 || rows == 0 || cols == 0) return DL_OK;
+    DL_REQUIRE(g && out && workspace, DL_ERR_INVALID_ARG, "%s: null pointer", what);
+    DL_REQUIRE(aligned_to(workspace, 16), DL_ERR_INVALID_ARG, "%s: the workspace must be 16-byte aligned", what);
+    if (few_columns(cols)) {
+        GramJob job = {};
+        job.count = 1;
+        job.batch = batch;
+        job.matrix[0] = {g, nullptr, out, rows, 0.f};
+        job.cols = (int)cols;
+        job.type = type;
+        return launch_gram_steps(job, steps, coefficients, eps, reinterpret_cast<double *>(workspace), current_sms(), as_stream(stream), what);
+    }
+    Matrices all = {};
+    all.g[0] = g;
+    all.stride = rows * cols;
+    all.type = type;
+    OrthogonalEpilogue last = {};
+    last.out = out;
+    return orthogonalise(all, batch, rows, cols, steps, coefficients, eps, last, reinterpret_cast<uint8_t *>(workspace), current_sms(),
+                         as_stream(stream), what);
+}
+
+// One step: the matrices of few columns together, then those of one shape after the other.
+namespace dl {
+
+template <class Few, class Many>
+static int over_muon_groups(const int64_t *table, int64_t count, const Few &few, const Many &many) {
+    int status = DL_OK;
+    for (int64_t i = 0; i < count && status == DL_OK; ++i) {   // every group at its first matrix
+        const int64_t *at = table + 5 * i;
+        GramJob job = {};
+        if (few_columns(at[4])) {
+            bool taken = false;   // by an earlier group of this number of columns
+            for (int64_t j = 0; j < i; ++j) taken |= table[5 * j + 4] == at[4];
+            if (!taken) {
+                job.cols = (int)at[4];
+                for (int64_t j = i; j < count && status == DL_OK; ++j) {
+                    const int64_t *t = table + 5 * j;
+                    if (t[4] != at[4] || t[3] == 0) continue;
+                    job.matrix[job.count++] = {reinterpret_cast<const void *>(t[1]), reinterpret_cast<float *>(t[2]), reinterpret_cast<void *>(t[0]), t[3], 0.f};
+                    if (job.count == GramJob::kMost) {
+                        status = few(job);
+                        job.count = 0;
+                    }
+                }
+                if (job.count > 0 && status == DL_OK) status = few(job);
+            }
+        } else {
+            bool taken = at[3] == 0;
+            for (int64_t j = 0; j < i; ++j) taken |= table[5 * j + 3] == at[3] && table[5 * j + 4] == at[4];
+            if (!taken) {
+                Matrices all = {};
+                int64_t batch = 0;
+                for (int64_t j = i; j < count && status == DL_OK; ++j) {
+                    const int64_t *t = table + 5 * j;
+                    if (t[3] != at[3] || t[4] != at[4]) continue;
+                    all.weight[batch] = reinterpret_cast<float *>(t[0]);
+                    all.g[batch] = reinterpret_cast<const void *>(t[1]);
+                    all.momentum[batch++] = reinterpret_cast<float *>(t[2]);
+                    if (batch == Matrices::kMost) {
+                        status = many(all, batch, at[3], at[4]);
+                        batch = 0;
+                    }
+                }
+                if (batch > 0 && status == DL_OK) status = many(all, batch, at[3], at[4]);
+            }
+        }
+    }
+    return status;
+}
+
+static int64_t rows_of(const GramJob &job) {
+    int64_t rows = 0;
+    for (int i = 0; i < job.count; ++i) rows += job.matrix[i].rows;
+    return rows * job.batch;
+}
+
+}  // namespace dl
+
+extern "C" DL_API int64_t dl_muon_workspace_bytes(const int64_t *table, int64_t count) {
+    if (table == nullptr) return 0;
+    const int sms = current_sms();
+    int64_t most = 0;
+    over_muon_groups(
+        table, count,
+        [&](GramJob &job) {
+            job.batch = 1;
+            const int64_t bytes = gram_workspace_bytes(job.count, rows_of(job), sms);
+            if (bytes > most) most = bytes;
+            return DL_OK;
+        },
+        [&](Matrices &, int64_t batch, int64_t rows, int64_t cols) {
+            const int64_t bytes = orthogonal_layout(batch, rows, cols, false, sms).total();
+            if (bytes > most) most = bytes;
+            return DL_OK;
+        });
+    return most;
+}
+
+extern "C" DL_API int dl_muon_step_f32(const int64_t *table, int64_t count, double lr, double momentum, int nesterov, double weight_decay, int steps,
+                                       const float *coefficients, double eps, void *workspace, void *stream) {
+    const char *what = "dl_muon_step_f32";
+    DL_REQUIRE(count >= 0 && (table || count == 0), DL_ERR_INVALID_ARG, "%s: null pointer", what);
+    int status = check_steps(steps, coefficients, eps, what);
+    if (status != DL_OK) return status;
+    for (int64_t i = 0; i < count; ++i) {
+        const int64_t *t = table + 5 * i;
+        DL_REQUIRE(t[3] >= 0 && t[4] > 0 && t[3] <= INT32_MAX / 2 && t[4] <= INT32_MAX / 2, DL_ERR_INVALID_ARG, "%s: bad size", what);
+        DL_REQUIRE(t[3] == 0 || (t[0] && t[1] && t[2]), DL_ERR_INVALID_ARG, "%s: null pointer", what);
+        DL_REQUIRE((t[0] | t[1] | t[2]) % 4 == 0, DL_ERR_INVALID_ARG, "%s: misaligned matrix", what);
+    }
+    if (count == 0) return DL_OK;
+    DL_REQUIRE(workspace && aligned_to(workspace, 16), DL_ERR_INVALID_ARG, "%s: the workspace is missing or not 16-byte aligned", what);
+    const int sms = current_sms();
+    cudaStream_t st = as_stream(stream);
+    const auto rate = [&](int64_t rows, int64_t cols) { return (float)(lr * sqrt(rows > cols ? (double)rows / (double)cols : 1.0)); };
+    const float keep = (float)(1.0 - momentum), toward = nesterov ? (float)momentum : 1.f, decay = (float)(1.0 - lr * weight_decay);
+    return over_muon_groups(
+        table, count,
+        [&](GramJob &job) {
+            job.batch = 1;
+            job.type = kFloat32;
+            job.update = true;
+            job.keep = keep;
+            job.nesterov = toward;
+            job.decay = decay;
+            for (int i = 0; i < job.count; ++i) job.matrix[i].rate = rate(job.matrix[i].rows, job.cols);
+            return launch_gram_steps(job, steps, coefficients, eps, reinterpret_cast<double *>(workspace), sms, st, what);
+        },
+        [&](Matrices &all, int64_t batch, int64_t rows, int64_t cols) {
+            all.type = kFloat32;
+            all.keep = keep;
+            all.nesterov = toward;
+            OrthogonalEpilogue last = {};
+            last.decay = decay;
+            last.rate = rate(rows, cols);
+            return orthogonalise(all, batch, rows, cols, steps, coefficients, eps, last, reinterpret_cast<uint8_t *>(workspace), sms, st, what);
+        });
+}

@@ -2,7 +2,7 @@
 
 A logic network reads values between 0 and 1.  `DenseLayer` learns them -- an encoder whose sigmoid feeds the first LogicLayer, in the
 feature-major layout that logic layers read -- or makes the fully connected networks that the reference compares with
-(experiments/main_baseline.py).  With `implementation='cuda'` it runs on csrc/matmul.cu:
+(experiments/main_baseline.py).  With `implementation='cuda'` it runs on csrc/dense.cu:
 
 * bf16 and fp16 layers multiply their values as they are, fp32 layers three bf16 planes of each value, which is as exact as 32-bit
   arithmetic; all sums are 32-bit, results are rounded once;
@@ -54,7 +54,7 @@ def _forward(x, w, bias, residual, act, feature_major, want_slope):
     with N.on_device(x):
         px, pw = x.data_ptr(), w.data_ptr()
         sizes = (ctypes.c_int64 * 3)()
-        lib.dl_dense_forward_sizes(px, pitch, x_feature, pw, batch, inner, outer, kind, sizes)
+        lib.dl_dense_forward_sizes(px, pitch, x_feature, pw, batch, inner, outer, feature_major, kind, sizes)
         x_planes, w_planes, work = (_bytes(n, x) for n in sizes)
         N.check(lib.dl_dense_forward(px, pitch, x_feature, pw, N.ptr(bias), N.ptr(residual), 0 if residual is None else residual.stride(0),
                                      0 if residual is None else residual.stride(1), act, y.data_ptr(), feature_major, N.ptr(slope),

@@ -570,7 +570,7 @@ DL_API int dl_backward_w_announce_f32(const float *x, const int64_t *a, const in
  * ---------------------------------------------------------------------------------------- */
 enum { DL_ACT_NONE = 0, DL_ACT_RELU = 1, DL_ACT_SIGMOID = 2, DL_ACT_SILU = 3, DL_ACT_GELU = 4 };
 DL_API void dl_dense_forward_sizes(const void *x, int64_t x_pitch, int x_feature_major, const void *w, int64_t batch, int64_t inner,
-                                   int64_t outer, int type, int64_t *sizes);
+                                   int64_t outer, int y_feature_major, int type, int64_t *sizes);
 DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_feature_major, const void *w, const void *bias, const void *residual,
                             int64_t residual_batch, int64_t residual_feature, int act, void *y, int y_feature_major, void *slope,
                             void *x_planes, void *w_planes, void *workspace, int64_t batch, int64_t inner, int64_t outer, int type,

@@ -121,7 +121,7 @@ def test_entry_points_check_their_arguments():
     assert lib.dl_dense_backward(None, 0, None, None, 4, 0, None, None, None, None, None, None, None, 2, 4, 4, 0, None) == bad
     sizes = (ctypes.c_int64 * 3)()
     for pitch, kind, least in [(8, 1, 0), (7, 1, 100 * 8 * 2), (8, 0, 3 * 100 * 8 * 2)]:     # rows on 16-byte units are read in place
-        lib.dl_dense_forward_sizes(16, pitch, 0, 16, 100, 7 if pitch == 7 else 8, 8, kind, sizes)
+        lib.dl_dense_forward_sizes(16, pitch, 0, 16, 100, 7 if pitch == 7 else 8, 8, 0, kind, sizes)
         assert (sizes[0] == 0) == (least == 0) and sizes[0] >= least
     assert "dl_dense" in N.last_error()
 
@@ -132,7 +132,7 @@ def test_workspaces_follow_the_sizes(rows, cols, k, batch, kind):
     for value in (64, 128, 256, 0):
         with N.tuning(N.TUNE_MATMUL_COLUMNS, value):
             sizes = (ctypes.c_int64 * 3)()
-            lib.dl_dense_forward_sizes(16, k, 0, 16, rows, k, cols, kind, sizes)
+            lib.dl_dense_forward_sizes(16, k, 0, 16, rows, k, cols, value == 64, kind, sizes)
             assert 0 <= sizes[2] <= 64 << 20
             assert lib.dl_orthogonalize_workspace_bytes(batch, rows, cols, kind) > 0
             assert lib.dl_dense_backward_workspace_bytes(16, 0, 1, 16, k, 0, 16, 1, 1, rows, k, cols, kind) > 0
