@@ -62,6 +62,7 @@ struct DenseEpilogue {
 
     struct Place {
         int row, col, m, n;   // of the lane's first value; lane = row, where neighbouring rows are neighbours in memory
+        int whole;            // columns that the warp's pieces may reach over and be whole, on addresses that allow wide accesses
         int64_t at;
         bool wide, bias_wide, residual_wide;
     };
@@ -85,7 +86,56 @@ struct DenseEpilogue {
         p.wide = quads_at(y, o.y_pitch);
         p.bias_wide = quads_at(reinterpret_cast<const T *>(o.bias), 0);
         p.residual_wide = o.residual_col == 1 && quads_at(r, o.residual_row);
+        const bool fast = by_rows() && p.wide && row + 32 <= s.m && (o.bias == nullptr || o.rows_are_features || p.bias_wide) &&
+                          (o.residual == nullptr || p.residual_wide);
+        p.whole = fast ? s.n - col : 0;
         return p;
+    }
+
+    template <bool SLOPE>
+    __device__ __forceinline__ void whole_piece(const Place &p, int across, float (&q)[4][4]) const {
+        const T *bias = reinterpret_cast<const T *>(o.bias), *residual = reinterpret_cast<const T *>(o.residual);
+        float z[16], d[16];
+        Quad<T> more[4];
+        if (residual != nullptr) {
+            const T *from = residual + p.row * o.residual_row + p.col + across;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) more[i] = *reinterpret_cast<const Quad<T> *>(from + 8 * i * o.residual_row);
+        }
+        float b[4][4] = {};
+        if (bias != nullptr) {
+            if (o.rows_are_features) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b[i][0] = b[i][1] = b[i][2] = b[i][3] = to_float(bias[p.row + 8 * i]);
+            } else {
+                const Quad<T> c = *reinterpret_cast<const Quad<T> *>(bias + p.col + across);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) b[i / 4][i % 4] = to_float(c.v[i % 4]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z[i] = q[i / 4][i % 4] + b[i / 4][i % 4];
+        activate<SLOPE>(z, d, o.act);
+        if (residual != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) z[i] += to_float(more[i / 4].v[i % 4]);
+        }
+        const int64_t step = 8 * o.y_pitch;
+        T *y = reinterpret_cast<T *>(o.y) + p.at + across;
+        Slope *slope = reinterpret_cast<Slope *>(o.slope) + p.at + across;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            Quad<T> v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v.v[j] = from_float<T>(z[4 * i + j]);
+            *reinterpret_cast<Quad<T> *>(y + i * step) = v;
+            if (SLOPE) {
+                Quad<Slope> u;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) u.v[j] = from_float<Slope>(d[4 * i + j] * (sizeof(T) == 4 ? 1.f : kSlopeScale));
+                *reinterpret_cast<Quad<Slope> *>(slope + i * step) = u;
+            }
+        }
     }
 
     __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kPieceColumns], float *stage, int lane) const {
@@ -97,22 +147,24 @@ struct DenseEpilogue {
         if (!by_rows()) {
             if (p.row >= p.m) return;
             const float row_bias = bias != nullptr && o.rows_are_features ? to_float(bias[p.row]) : 0.f;
+            const int left = p.n - col;
+            float z[kPieceColumns], d[kPieceColumns];
 #pragma unroll
-            for (int c = 0; c < kPieceColumns; c += 4) {
-                const int left = p.n - col - c;
-                float z[4], d[4];
+            for (int j = 0; j < kPieceColumns; ++j)
+                z[j] = v[j] + (bias != nullptr && !o.rows_are_features && j < left ? to_float(bias[col + j]) : row_bias);
+            activate<true>(z, d, o.act);
+            if (residual != nullptr) {
+                const T *from = residual + p.row * o.residual_row + col * o.residual_col;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    z[j] = v[c + j] + (bias != nullptr && !o.rows_are_features && j < left ? to_float(bias[col + c + j]) : row_bias);
-                activate(z, d, o.act);
-                const int64_t at = p.at + (across + c) * o.y_pitch;
+                for (int j = 0; j < kPieceColumns; ++j)
+                    if (j < left) z[j] += to_float(from[j * o.residual_col]);
+            }
+            const int64_t at = p.at + across * o.y_pitch;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j >= left) continue;
-                    if (residual != nullptr) z[j] += to_float(residual[p.row * o.residual_row + (col + c + j) * o.residual_col]);
-                    y[at + j * o.y_pitch] = from_float<T>(z[j]);
-                    if (slope != nullptr) slope[at + j * o.y_pitch] = from_float<Slope>(d[j] * kScale);
-                }
+            for (int j = 0; j < kPieceColumns; ++j) {
+                if (j >= left) continue;
+                y[at + j * o.y_pitch] = from_float<T>(z[j]);
+                if (slope != nullptr) slope[at + j * o.y_pitch] = from_float<Slope>(d[j] * kScale);
             }
             return;
         }
@@ -120,58 +172,38 @@ struct DenseEpilogue {
         float q[4][4];
         piece_quads(stage, lane, q);
         __syncwarp();
+        if (across + kPieceColumns <= p.whole) {
+            if (slope != nullptr) whole_piece<true>(p, across, q);
+            else whole_piece<false>(p, across, q);
+            return;
+        }
         const int left = p.n - col;
         if (left <= 0) return;
-        if (bias != nullptr) {
-            if (o.rows_are_features) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float b = p.row + 8 * i < p.m ? to_float(bias[p.row + 8 * i]) : 0.f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) q[i][j] += b;
-                }
-            } else {
-                float b[4];
-                read_quad(bias + col, p.bias_wide, left, b);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) q[i][j] += b[j];
-            }
-        }
-        float more[4][4];
-        if (residual != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = p.row + 8 * i;
-                const T *from = residual + r * o.residual_row + col * o.residual_col;
-                if (r >= p.m) continue;
-                if (o.residual_col == 1) {
-                    read_quad(from, p.residual_wide, left, more[i]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) more[i][j] = j < left ? to_float(from[j * o.residual_col]) : 0.f;
-                }
-            }
-        }
-        float d[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) activate(q[i], d[i], o.act);
+        // a piece over the edge, or on addresses that allow single values only
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (p.row + 8 * i >= p.m) continue;
-            const int64_t at = p.at + across + 8 * i * o.y_pitch;
-            if (residual != nullptr) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) q[i][j] += more[i][j];
+            const int row = p.row + 8 * i;
+            if (row >= p.m) continue;
+            float d[4], b[4] = {0.f, 0.f, 0.f, 0.f};
+            if (bias != nullptr) {
+                if (o.rows_are_features) b[0] = b[1] = b[2] = b[3] = to_float(bias[row]);
+                else read_quad(bias + col, p.bias_wide, left, b);
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[i][j] += b[j];
+            activate<true>(q[i], d, o.act);
+            if (residual != nullptr) {
+                const T *from = residual + row * o.residual_row + col * o.residual_col;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < left) q[i][j] += to_float(from[j * o.residual_col]);
+            }
+            const int64_t at = p.at + across + 8 * i * o.y_pitch;
             write_quad(y + at, p.wide, left, q[i]);
             if (slope != nullptr) {
-                if (kScale != 1.f) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) d[i][j] *= kScale;
-                }
-                write_quad(slope + at, p.wide, left, d[i]);
+                for (int j = 0; j < 4; ++j) d[j] *= kScale;
+                write_quad(slope + at, p.wide, left, d);
             }
         }
     }
@@ -184,24 +216,37 @@ struct PlainEpilogue {
     T *out;
     int64_t pitch;
     struct Place {
-        int row, col, m, n;
+        int row, col, m, n, whole;   // as DenseEpilogue's
         T *at;
         bool wide;
     };
     __device__ __forceinline__ Place begin(const Tile &, const MatmulShape &s, int row, int col, int lane) const {
         const int r = row + lane / 4, c = col + lane % 4 * 4;
-        return {r, c, s.m, s.n, out + r * pitch + c, quads_at(out, pitch)};
+        const bool wide = quads_at(out, pitch);
+        return {r, c, s.m, s.n, wide && row + 32 <= s.m ? s.n - col : 0, out + r * pitch + c, wide};
     }
     __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kPieceColumns], float *stage, int lane) const {
         piece_store(stage, lane, v);
         float q[4][4];
         piece_quads(stage, lane, q);
         __syncwarp();
+        T *to = p.at + across;
+        const int64_t step = 8 * pitch;
+        if (across + kPieceColumns <= p.whole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                Quad<T> u;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) u.v[j] = from_float<T>(q[i][j]);
+                *reinterpret_cast<Quad<T> *>(to + i * step) = u;
+            }
+            return;
+        }
         const int left = p.n - p.col - across;
         if (left <= 0) return;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (p.row + 8 * i < p.m) write_quad(p.at + across + 8 * i * pitch, p.wide, left, q[i]);
+            if (p.row + 8 * i < p.m) write_quad(to + i * step, p.wide, left, q[i]);
     }
 };
 

@@ -10,16 +10,18 @@ namespace dl {
 // layer's own type may have 8, and down to 4e-12, where sigmoids saturate.
 constexpr float kSlopeScale = 16384.f;
 
-// act(z) in place, and its derivatives, four at a time.
-template <int N>
+// act(z) in place, and its derivatives where they are wanted.
+template <bool SLOPE, int N>
 __device__ __forceinline__ void activate(float (&z)[N], float (&slope)[N], int act) {
     if (act == DL_ACT_NONE) {
+        if (SLOPE) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) slope[j] = 1.f;
+            for (int j = 0; j < N; ++j) slope[j] = 1.f;
+        }
     } else if (act == DL_ACT_RELU) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            slope[j] = z[j] > 0.f ? 1.f : 0.f;
+            if (SLOPE) slope[j] = z[j] > 0.f ? 1.f : 0.f;
             z[j] = z[j] > 0.f || z[j] != z[j] ? z[j] : 0.f;
         }
     } else if (act == DL_ACT_GELU) {
@@ -27,20 +29,24 @@ __device__ __forceinline__ void activate(float (&z)[N], float (&slope)[N], int a
         for (int j = 0; j < N; ++j) {
             const float phi = 0.5f * (1.f + erff(z[j] * 0.70710678118654752f));
             // far out the density is zero, and infinity times zero would not be
-            slope[j] = phi + (fabsf(z[j]) > 15.f ? 0.f : z[j] * expf(-0.5f * z[j] * z[j]) * 0.39894228040143268f);
+            if (SLOPE) slope[j] = phi + (fabsf(z[j]) > 15.f ? 0.f : z[j] * expf(-0.5f * z[j] * z[j]) * 0.39894228040143268f);
             z[j] = z[j] == -INFINITY ? 0.f : z[j] * phi;
+        }
+    } else if (act == DL_ACT_SIGMOID) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            z[j] = __fdividef(1.f, 1.f + expf(-z[j]));   // zero below -88, where expf overflows
+            if (SLOPE) slope[j] = z[j] * (1.f - z[j]);
         }
     } else {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const float s = __fdividef(1.f, 1.f + expf(-z[j]));   // zero below -88, where expf overflows
-            slope[j] = s * (1.f - s);
-            if (act == DL_ACT_SIGMOID) {
-                z[j] = s;
-            } else {
-                slope[j] = s + (slope[j] == 0.f ? 0.f : z[j] * slope[j]);
-                z[j] = z[j] == -INFINITY ? 0.f : z[j] * s;
+            const float s = __fdividef(1.f, 1.f + expf(-z[j]));
+            if (SLOPE) {
+                const float d = s * (1.f - s);
+                slope[j] = s + (d == 0.f ? 0.f : z[j] * d);
             }
+            z[j] = z[j] == -INFINITY ? 0.f : z[j] * s;
         }
     }
 }
@@ -58,7 +64,7 @@ struct DenseOutput {
     // One output of one sample, where the rows are the features.
     __device__ __forceinline__ void one(int feature, int sample, float sum) const {
         float v[1] = {bias != nullptr ? sum + load_as_float(bias, feature, type) : sum}, d[1];
-        activate(v, d, act);
+        activate<true>(v, d, act);
         if (residual != nullptr) v[0] += load_as_float(residual, feature * residual_row + sample * residual_col, type);
         const int64_t i = feature_major ? feature * y_pitch + sample : sample * y_pitch + feature;
         if (type == kFloat32) reinterpret_cast<float *>(y)[i] = v[0];

@@ -220,20 +220,26 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 #pragma unroll 1
                     for (int p = 0; p < PLANES; ++p) {
                         const int z = t.matrix * s.planes_z + p;
+const int row = t.row + (int)rank * kMatmulRows;
+                        if (!s.a_mn) {
+                            tile_load<PAIR>(at, &map_a, k, row, z, bar);
+                        } else {
 #pragma unroll
-                        for (int c = 0; c < kMatmulRows / kChunk; ++c, at += kChunkBytes) {
-                            const int row = t.row + (int)rank * kMatmulRows + c * kChunk;
-                            tile_load<PAIR>(at, &map_a, s.a_mn ? row : k, s.a_mn ? k : row, z, bar);
+                            for (int c = 0; c < kMatmulRows / kChunk; ++c) tile_load<PAIR>(at + c * kChunkBytes, &map_a, row + c * kChunk, k, z, bar);
                         }
+                        at += kPlaneA;
                     }
 #pragma unroll 1
                     for (int p = 0; p < PLANES; ++p) {
                         const int z = t.matrix * s.planes_z + p;
+const int col = t.col + (int)rank * Config::kOwnColumns;
+                        if (!s.b_mn) {
+                            tile_load<PAIR>(at, &map_b, k, col, z, bar);
+                        } else {
 #pragma unroll
-                        for (int c = 0; c < Config::kOwnColumns / kChunk; ++c, at += kChunkBytes) {
-                            const int col = t.col + (int)rank * Config::kOwnColumns + c * kChunk;
-                            tile_load<PAIR>(at, &map_b, s.b_mn ? col : k, s.b_mn ? k : col, z, bar);
+                            for (int c = 0; c < Config::kOwnColumns / kChunk; ++c) tile_load<PAIR>(at + c * kChunkBytes, &map_b, col + c * kChunk, k, z, bar);
                         }
+                        at += kPlaneB;
                     }
                     used = max(used, stage + 1);
                     if (++stage == kStages) {
@@ -357,18 +363,19 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         }
                     }
                 } else {
+// the next 32 columns are on their way while these are worked on
+                    uint32_t bits[32];
+                    tensor_read32(sums, bits);
+                    tensor_read_wait();
 #pragma unroll 1
                     for (int c0 = 0; c0 < kShare && (t.col + from + c0 < s.n || Epilogue::kWholeTiles); c0 += 32) {
-                        uint32_t bits[32];
-                        tensor_read32(sums + c0, bits);
+                        float v[2][kSpan];
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) v[c / kSpan][c % kSpan] = __uint_as_float(bits[c]);
+                        if (c0 + 32 < kShare) tensor_read32(sums + c0 + 32, bits);
+                        finish(v[0], c0);
+                        finish(v[1], c0 + kSpan);
                         tensor_read_wait();
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float v[kSpan];
-#pragma unroll
-                            for (int c = 0; c < kSpan; ++c) v[c] = __uint_as_float(bits[h * kSpan + c]);
-                            finish(v, c0 + h * kSpan);
-                        }
                     }
                 }
                 tensor_fence_before();

@@ -23,9 +23,10 @@ struct Product {
     bool exact;   // sums are taken out of tensor memory every so often
 };
 
-static bool map_operand(CUtensorMap *map, const Operand &o, const Product &p, int64_t rows) {
+// `own`: rows of it that a CTA copies for a tile, at once where they are K-major.
+static bool map_operand(CUtensorMap *map, const Operand &o, const Product &p, int64_t rows, int own) {
     const int64_t inner = o.mn ? rows : p.k, outer = o.mn ? p.k : rows;
-    return make_tile_map(map, o.base, p.bfloat, inner, outer, p.planes_z * p.batch, o.pitch * 2, o.plane * 2);
+    return make_tile_map(map, o.base, p.bfloat, inner, outer, p.planes_z * p.batch, o.pitch * 2, o.plane * 2, o.mn ? kChunk : own);
 }
 
 template <int PLANES, int COLUMNS, bool PAIR, class Epilogue>
@@ -71,7 +72,7 @@ template <int PLANES, class Epilogue>
 static int launch_product(const Product &p, const MatmulPlan &plan, const Epilogue &epilogue, float *partial, int sms, cudaStream_t st,
                           const char *what) {
     CUtensorMap a, b;
-    if (!map_operand(&a, p.a, p, p.m) || !map_operand(&b, p.b, p, p.n))
+    if (!map_operand(&a, p.a, p, p.m, kMatmulRows) || !map_operand(&b, p.b, p, p.n, plan.pair ? plan.columns / 2 : plan.columns))
         return fail(DL_ERR_CUDA, "%s: the driver refuses the map of an operand", what);
     const int rows = plan.pair ? 2 * kMatmulRows : kMatmulRows;
     MatmulShape s = {};

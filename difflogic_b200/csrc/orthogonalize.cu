@@ -112,20 +112,24 @@ struct PairEpilogue {
     bool symmetric;
     struct Place {
         int row, col, m, n;          // of the warp's first value
-        int64_t matrix;
+        bool whole;                  // its 32 rows are all there
+        int64_t at, mirrored;        // of the lane's first value: of its own, of the mirrored ones
     };
-    __device__ __forceinline__ Place begin(const Tile &t, const MatmulShape &s, int row, int col, int) const {
-        return {row, col, s.m, s.n, 2 * t.matrix * plane};
+    __device__ __forceinline__ Place begin(const Tile &t, const MatmulShape &s, int row, int col, int lane) const {
+        const int64_t matrix = 2 * t.matrix * plane;
+        return {row, col, s.m, s.n, row + 32 <= s.m, matrix + (row + lane / 4) * pitch + col + lane % 4 * 4,
+                matrix + (col + lane / 8) * pitch + row + lane % 8 * 4};
     }
     __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kPieceColumns], float *stage, int lane) const {
         const int first = p.col + across, below = p.row / kMatmulRows - first / kMatmulRows;
         if (symmetric && below < 0) return;
+        const bool whole = p.whole && first + kPieceColumns <= p.n;
         piece_store(stage, lane, v);
         float q[4][4];
         piece_quads(stage, lane, q);
         __syncwarp();
         const int row = p.row + lane / 4, col = first + lane % 4 * 4;
-        const int64_t at = p.matrix + row * pitch + col;
+        const int64_t at = p.at + across, step = 8 * pitch;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -137,14 +141,16 @@ struct PairEpilogue {
                 for (int j = 0; j < 4; ++j)
                     if (row + 8 * i == col + j) q[i][j] += diagonal;
         }
-        if (more != nullptr && col < p.n) {
+        if (more != nullptr) {
             ushort4 hi[4], lo[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                hi[i] = lo[i] = make_ushort4(0, 0, 0, 0);
-                if (row + 8 * i >= p.m) continue;
-                hi[i] = *reinterpret_cast<const ushort4 *>(more + at + 8 * i * pitch);
-                lo[i] = *reinterpret_cast<const ushort4 *>(more + at + 8 * i * pitch + plane);
+                if (whole || (row + 8 * i < p.m && col < p.n)) {
+                    hi[i] = *reinterpret_cast<const ushort4 *>(more + at + i * step);
+                    lo[i] = *reinterpret_cast<const ushort4 *>(more + at + i * step + plane);
+                } else {
+                    hi[i] = lo[i] = make_ushort4(0, 0, 0, 0);
+                }
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -154,25 +160,22 @@ struct PairEpilogue {
                 q[i][3] += factor * join_pair(hi[i].w, lo[i].w);
             }
         }
-        if (symmetric && below > 0) {   // from here the mirrored values are taken
+        const bool mirror = symmetric && below > 0;
+        if (mirror) {   // from here the mirrored values are taken
             piece_put_quads(stage, lane, q);
             __syncwarp();
         }
-        if (col < p.n) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (row + 8 * i < p.m) store_pairs(out + at + 8 * i * pitch, q[i]);
-        }
-        if (symmetric && below > 0) {
+        for (int i = 0; i < 4; ++i)
+            if (whole || (row + 8 * i < p.m && col < p.n)) store_pairs(out + at + i * step, q[i]);
+        if (mirror) {
             piece_columns(stage, lane, q);
             __syncwarp();
-            const int from = p.row + lane % 8 * 4, to = first + lane / 8;   // columns of the result: rows of the piece
-            if (from < p.m) {
-                uint16_t *mirrored = out + p.matrix + to * pitch + from;
+            // columns of the result: rows of the piece
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (to + 4 * i < p.n) store_pairs(mirrored + 4 * i * pitch, q[i]);
-            }
+            for (int i = 0; i < 4; ++i)
+                if (whole || (p.row + lane % 8 * 4 < p.m && first + lane / 8 + 4 * i < p.n))
+                    store_pairs(out + p.mirrored + (across + 4 * i) * pitch, q[i]);
         }
     }
     __device__ __forceinline__ void store_pairs(uint16_t *to, const float (&v)[4]) const {

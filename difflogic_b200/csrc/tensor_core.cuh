@@ -133,9 +133,9 @@ static inline uint32_t instruction_descriptor(bool bfloat, bool a_mn, bool b_mn,
            (uint32_t)(columns / 8) << 17 | (uint32_t)(rows / 16) << 24;
 }
 
-// Map of `planes` matrices of rows x inner 16-bit values, copied in tiles of 64 x 64; what lies outside reads as zero.  False where the
+// Map of `planes` matrices of rows x inner 16-bit values, copied in tiles of tile_rows x 64; what lies outside reads as zero.  False where the
 // driver does not take it (base and pitches must be multiples of 16 bytes).
 bool make_tile_map(CUtensorMap *map, const void *base, bool bfloat, int64_t inner, int64_t rows, int64_t planes, int64_t row_bytes,
-                   int64_t plane_bytes);
+                   int64_t plane_bytes, int tile_rows);
 
 }  // namespace dl
