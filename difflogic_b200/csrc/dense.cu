@@ -20,190 +20,176 @@ __device__ __forceinline__ T from_float(float v) {
     else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
     else return __float2bfloat16_rn(v);
 }
-template <class T>
-struct __align__(4 * sizeof(T)) Quad {
-    T v[4];
+// 64 bytes of neighbouring values, and value j of them.
+struct Units {
+    uint4 u[4];
 };
-// Four neighbouring values of which `left` are there; wide: their address is a multiple of their size.
 template <class T>
-__device__ __forceinline__ void read_quad(const T *p, bool wide, int left, float (&v)[4]) {
-    if (wide && left >= 4) {
-        const Quad<T> q = *reinterpret_cast<const Quad<T> *>(p);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = to_float(q.v[j]);
+__device__ __forceinline__ float value_of(const Units &from, int j) {
+    constexpr int kUnit = 16 / sizeof(T);
+    const uint4 &u = from.u[j / kUnit];
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(w[j % 4]);
     } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = j < left ? to_float(p[j]) : 0.f;
+        const uint16_t half = (uint16_t)(w[j % 8 / 2] >> (j % 2 * 16));
+        return to_float(*reinterpret_cast<const T *>(&half));
     }
 }
+
+// 32 rows of values, a row in each lane, to where they lie in memory: rows `pitch` values apart, those from m on and columns from n on
+// left out.
 template <class T>
-__device__ __forceinline__ void write_quad(T *p, bool wide, int left, const float (&v)[4]) {
-    if (wide && left >= 4) {
-        Quad<T> q;
+__device__ __forceinline__ void store_rows(uint8_t *slot, int lane, const float (&v)[64 / sizeof(T)], T *to, int64_t pitch, int row, int col, int m, int n) {
+    uint32_t w[16];
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q.v[j] = from_float<T>(v[j]);
-        *reinterpret_cast<Quad<T> *>(p) = q;
+        for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[j]);
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < left) p[j] = from_float<T>(v[j]);
+        for (int j = 0; j < 16; ++j) {
+            const T lo = from_float<T>(v[2 * j]), hi = from_float<T>(v[2 * j + 1]);
+            w[j] = (uint32_t)*reinterpret_cast<const uint16_t *>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t *>(&hi) << 16;
+        }
     }
-}
-template <class T>
-__device__ __forceinline__ bool quads_at(const T *p, int64_t pitch) {
-    return (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0 && pitch % 4 == 0;
+    slot_row(slot, lane, w);
+    __syncwarp();
+    const int r = row + lane / 4, c = col + lane % 4 * (16 / (int)sizeof(T));
+    T *at = to + r * pitch + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (r + 8 * i < m && c < n) *reinterpret_cast<uint4 *>(at + 8 * i * pitch) = *slot_unit(slot, lane, i);
 }
 
 template <class T>
 struct DenseEpilogue {
     static constexpr bool kWholeTiles = false;
+    static constexpr int kColumns = 64 / sizeof(T);   // 64 bytes
     using Slope = typename std::conditional<sizeof(T) == 4, float, __half>::type;
     DenseOutput o;
+    bool whole;    // rows of y and slope lie and end on 16-byte units, and those of the residual
+    bool bias_wide;
 
     struct Place {
-        int row, col, m, n;   // of the lane's first value; lane = row, where neighbouring rows are neighbours in memory
-        int whole;            // columns that the warp's pieces may reach over and be whole, on addresses that allow wide accesses
-        int64_t at;
-        bool wide, bias_wide, residual_wide;
+        int row, col, m, n;   // of the warp's first value
     };
-    // Neighbouring columns of the product are neighbours in memory, or neighbouring rows are.
-    __device__ __forceinline__ bool by_rows() const { return o.rows_are_features == o.feature_major; }
-
-    __device__ __forceinline__ Place begin(const Tile &, const MatmulShape &s, int row, int col, int lane) const {
-        Place p;
-        p.m = s.m;
-        p.n = s.n;
-        if (by_rows()) {
-            p.row = row + lane / 4;
-            p.col = col + lane % 4 * 4;
-            p.at = (int64_t)p.row * o.y_pitch + p.col;
-        } else {
-            p.row = row + lane;
-            p.col = col;
-            p.at = (int64_t)p.col * o.y_pitch + p.row;
-        }
-        const T *y = reinterpret_cast<const T *>(o.y), *r = reinterpret_cast<const T *>(o.residual);
-        p.wide = quads_at(y, o.y_pitch);
-        p.bias_wide = quads_at(reinterpret_cast<const T *>(o.bias), 0);
-        p.residual_wide = o.residual_col == 1 && quads_at(r, o.residual_row);
-        const bool fast = by_rows() && p.wide && row + 32 <= s.m && (o.bias == nullptr || o.rows_are_features || p.bias_wide) &&
-                          (o.residual == nullptr || p.residual_wide);
-        p.whole = fast ? s.n - col : 0;
-        return p;
-    }
+    __device__ __forceinline__ Place begin(const Tile &, const MatmulShape &s, int row, int col, int) const { return {row, col, s.m, s.n}; }
 
     template <bool SLOPE>
-    __device__ __forceinline__ void whole_piece(const Place &p, int across, float (&q)[4][4]) const {
+    __device__ __forceinline__ void tile_piece(const Place &p, int across, const float (&v)[kColumns], uint8_t *stage, int lane) const {
         const T *bias = reinterpret_cast<const T *>(o.bias), *residual = reinterpret_cast<const T *>(o.residual);
-        float z[16], d[16];
-        Quad<T> more[4];
+        const int row = p.row + lane, col = p.col + across;
+        const bool there = row < p.m;
+        constexpr int kUnit = 16 / sizeof(T);   // values of 16 bytes
+        Units more;
         if (residual != nullptr) {
-            const T *from = residual + p.row * o.residual_row + p.col + across;
+            const T *from = residual + row * o.residual_row + col;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) more[i] = *reinterpret_cast<const Quad<T> *>(from + 8 * i * o.residual_row);
+            for (int j = 0; j < 4; ++j)
+                more.u[j] = there && col + (j + 1) * kUnit <= p.n ? *reinterpret_cast<const uint4 *>(from + j * kUnit) : make_uint4(0, 0, 0, 0);
         }
-        float b[4][4] = {};
-        if (bias != nullptr) {
-            if (o.rows_are_features) {
+        float z[kColumns], d[kColumns];
+        if (bias == nullptr || o.rows_are_features) {
+            const float b = bias != nullptr && there ? to_float(bias[row]) : 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) b[i][0] = b[i][1] = b[i][2] = b[i][3] = to_float(bias[p.row + 8 * i]);
-            } else {
-                const Quad<T> c = *reinterpret_cast<const Quad<T> *>(bias + p.col + across);
+            for (int j = 0; j < kColumns; ++j) z[j] = v[j] + b;
+        } else if (bias_wide && col + kColumns <= p.n) {   // the same for all lanes
+            Units b;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) b[i / 4][i % 4] = to_float(c.v[i % 4]);
-            }
+            for (int j = 0; j < 4; ++j) b.u[j] = *reinterpret_cast<const uint4 *>(bias + col + j * kUnit);
+#pragma unroll
+            for (int j = 0; j < kColumns; ++j) z[j] = v[j] + value_of<T>(b, j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kColumns; ++j) z[j] = v[j] + (col + j < p.n ? to_float(bias[col + j]) : 0.f);
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) z[i] = q[i / 4][i % 4] + b[i / 4][i % 4];
         activate<SLOPE>(z, d, o.act);
         if (residual != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) z[i] += to_float(more[i / 4].v[i % 4]);
+            for (int j = 0; j < kColumns; ++j) z[j] += value_of<T>(more, j);
         }
-        const int64_t step = 8 * o.y_pitch;
-        T *y = reinterpret_cast<T *>(o.y) + p.at + across;
-        Slope *slope = reinterpret_cast<Slope *>(o.slope) + p.at + across;
+        // The slots take turns: who writes one has met all others behind their reading of it.
+        T *y = reinterpret_cast<T *>(o.y);
+        if (SLOPE) {
+            store_rows(stage, lane, z, y, o.y_pitch, p.row, col, p.m, p.n);
+            if (sizeof(T) != 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            Quad<T> v;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v.v[j] = from_float<T>(z[4 * i + j]);
-            *reinterpret_cast<Quad<T> *>(y + i * step) = v;
-            if (SLOPE) {
-                Quad<Slope> u;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) u.v[j] = from_float<Slope>(d[4 * i + j] * (sizeof(T) == 4 ? 1.f : kSlopeScale));
-                *reinterpret_cast<Quad<Slope> *>(slope + i * step) = u;
+                for (int j = 0; j < kColumns; ++j) d[j] *= kSlopeScale;
             }
+            store_rows(stage + kSlotBytes, lane, d, reinterpret_cast<Slope *>(o.slope), o.y_pitch, p.row, col, p.m, p.n);
+        } else {
+            if (across == 0) __syncwarp();   // the last share may have ended on this slot
+            store_rows(stage + across / kColumns % 2 * kSlotBytes, lane, z, y, o.y_pitch, p.row, col, p.m, p.n);
         }
     }
 
-    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kPieceColumns], float *stage, int lane) const {
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], uint8_t *stage, int lane) const {
+        if (p.row >= p.m) return;
+        if (whole) {
+            if (o.slope != nullptr) tile_piece<true>(p, across, v, stage, lane);
+            else tile_piece<false>(p, across, v, stage, lane);
+            return;
+        }
+        // results whose rows are off the 16-byte units, or that lie the other way: neighbouring lanes have neighbouring rows
         const T *bias = reinterpret_cast<const T *>(o.bias), *residual = reinterpret_cast<const T *>(o.residual);
         T *y = reinterpret_cast<T *>(o.y);
         Slope *slope = reinterpret_cast<Slope *>(o.slope);
         constexpr float kScale = sizeof(T) == 4 ? 1.f : kSlopeScale;
-        const int col = p.col + across;
-        if (!by_rows()) {
-            if (p.row >= p.m) return;
-            const float row_bias = bias != nullptr && o.rows_are_features ? to_float(bias[p.row]) : 0.f;
-            const int left = p.n - col;
-            float z[kPieceColumns], d[kPieceColumns];
+        const bool by_rows = o.rows_are_features == o.feature_major;
+#pragma unroll 1
+        for (int part = 0; part < kColumns; part += kPieceColumns) {
+            float t[kPieceColumns], d[kPieceColumns];
 #pragma unroll
-            for (int j = 0; j < kPieceColumns; ++j)
-                z[j] = v[j] + (bias != nullptr && !o.rows_are_features && j < left ? to_float(bias[col + j]) : row_bias);
-            activate<true>(z, d, o.act);
-            if (residual != nullptr) {
-                const T *from = residual + p.row * o.residual_row + col * o.residual_col;
+            for (int j = 0; j < kPieceColumns; ++j) t[j] = kColumns == kPieceColumns || part == 0 ? v[j] : v[kColumns - kPieceColumns + j];
+            if (!by_rows) {
+                const int row = p.row + lane, col = p.col + across + part, left = p.n - col;
+                if (row >= p.m) continue;
+                const float row_bias = bias != nullptr && o.rows_are_features ? to_float(bias[row]) : 0.f;
 #pragma unroll
                 for (int j = 0; j < kPieceColumns; ++j)
-                    if (j < left) z[j] += to_float(from[j * o.residual_col]);
-            }
-            const int64_t at = p.at + across * o.y_pitch;
+                    t[j] += bias != nullptr && !o.rows_are_features && j < left ? to_float(bias[col + j]) : row_bias;
+                activate<true>(t, d, o.act);
+                if (residual != nullptr) {
+                    const T *from = residual + row * o.residual_row + col * o.residual_col;
 #pragma unroll
-            for (int j = 0; j < kPieceColumns; ++j) {
-                if (j >= left) continue;
-                y[at + j * o.y_pitch] = from_float<T>(z[j]);
-                if (slope != nullptr) slope[at + j * o.y_pitch] = from_float<Slope>(d[j] * kScale);
-            }
-            return;
-        }
-        piece_store(stage, lane, v);
-        float q[4][4];
-        piece_quads(stage, lane, q);
-        __syncwarp();
-        if (across + kPieceColumns <= p.whole) {
-            if (slope != nullptr) whole_piece<true>(p, across, q);
-            else whole_piece<false>(p, across, q);
-            return;
-        }
-        const int left = p.n - col;
-        if (left <= 0) return;
-        // a piece over the edge, or on addresses that allow single values only
+                    for (int j = 0; j < kPieceColumns; ++j)
+                        if (j < left) t[j] += to_float(from[j * o.residual_col]);
+                }
+                const int64_t at = col * o.y_pitch + row;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = p.row + 8 * i;
-            if (row >= p.m) continue;
-            float d[4], b[4] = {0.f, 0.f, 0.f, 0.f};
-            if (bias != nullptr) {
-                if (o.rows_are_features) b[0] = b[1] = b[2] = b[3] = to_float(bias[row]);
-                else read_quad(bias + col, p.bias_wide, left, b);
+                for (int j = 0; j < kPieceColumns; ++j) {
+                    if (j >= left) continue;
+                    y[at + j * o.y_pitch] = from_float<T>(t[j]);
+                    if (slope != nullptr) slope[at + j * o.y_pitch] = from_float<Slope>(d[j] * kScale);
+                }
+                continue;
             }
+            float q[4][4];
+            piece_quads(stage, lane, t, q);
+            const int col = p.col + across + part + lane % 4 * 4, left = p.n - col;
+            if (left <= 0) continue;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) q[i][j] += b[j];
-            activate<true>(q[i], d, o.act);
-            if (residual != nullptr) {
-                const T *from = residual + row * o.residual_row + col * o.residual_col;
+            for (int i = 0; i < 4; ++i) {
+                const int row = p.row + lane / 4 + 8 * i;
+                if (row >= p.m) continue;
+                float e[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (j < left) q[i][j] += to_float(from[j * o.residual_col]);
-            }
-            const int64_t at = p.at + across + 8 * i * o.y_pitch;
-            write_quad(y + at, p.wide, left, q[i]);
-            if (slope != nullptr) {
+                    if (bias != nullptr && j < left) q[i][j] += to_float(bias[o.rows_are_features ? row : col + j]);
+                activate<true>(q[i], e, o.act);
+                if (residual != nullptr) {
+                    const T *from = residual + row * o.residual_row + col * o.residual_col;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) d[j] *= kScale;
-                write_quad(slope + at, p.wide, left, d);
+                    for (int j = 0; j < 4; ++j)
+                        if (j < left) q[i][j] += to_float(from[j * o.residual_col]);
+                }
+                const int64_t at = row * o.y_pitch + col;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (j >= left) continue;
+                    y[at + j] = from_float<T>(q[i][j]);
+                    if (slope != nullptr) slope[at + j] = from_float<Slope>(e[j] * kScale);
+                }
             }
         }
     }
@@ -213,40 +199,36 @@ struct DenseEpilogue {
 template <class T>
 struct PlainEpilogue {
     static constexpr bool kWholeTiles = false;
+    static constexpr int kColumns = 64 / sizeof(T);
     T *out;
     int64_t pitch;
+    bool whole;    // rows lie and end on 16-byte units
     struct Place {
-        int row, col, m, n, whole;   // as DenseEpilogue's
-        T *at;
-        bool wide;
+        int row, col, m, n;   // of the warp's first value
     };
-    __device__ __forceinline__ Place begin(const Tile &, const MatmulShape &s, int row, int col, int lane) const {
-        const int r = row + lane / 4, c = col + lane % 4 * 4;
-        const bool wide = quads_at(out, pitch);
-        return {r, c, s.m, s.n, wide && row + 32 <= s.m ? s.n - col : 0, out + r * pitch + c, wide};
-    }
-    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kPieceColumns], float *stage, int lane) const {
-        piece_store(stage, lane, v);
-        float q[4][4];
-        piece_quads(stage, lane, q);
-        __syncwarp();
-        T *to = p.at + across;
-        const int64_t step = 8 * pitch;
-        if (across + kPieceColumns <= p.whole) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                Quad<T> u;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) u.v[j] = from_float<T>(q[i][j]);
-                *reinterpret_cast<Quad<T> *>(to + i * step) = u;
-            }
+    __device__ __forceinline__ Place begin(const Tile &, const MatmulShape &s, int row, int col, int) const { return {row, col, s.m, s.n}; }
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], uint8_t *stage, int lane) const {
+        if (p.row >= p.m) return;
+        if (whole) {
+            if (across == 0) __syncwarp();   // as DenseEpilogue's
+            store_rows(stage + across / kColumns % 2 * kSlotBytes, lane, v, out, pitch, p.row, p.col + across, p.m, p.n);
             return;
         }
-        const int left = p.n - p.col - across;
-        if (left <= 0) return;
+#pragma unroll 1
+        for (int part = 0; part < kColumns; part += kPieceColumns) {
+            float t[kPieceColumns], q[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (p.row + 8 * i < p.m) write_quad(to + i * step, p.wide, left, q[i]);
+            for (int j = 0; j < kPieceColumns; ++j) t[j] = kColumns == kPieceColumns || part == 0 ? v[j] : v[kColumns - kPieceColumns + j];
+            piece_quads(stage, lane, t, q);
+            const int col = p.col + across + part + lane % 4 * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = p.row + lane / 4 + 8 * i;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (row < p.m && col + j < p.n) out[row * pitch + col + j] = from_float<T>(q[i][j]);
+            }
+        }
     }
 };
 
@@ -388,6 +370,22 @@ static int lay_out(const void *src, int64_t rows, int64_t cols, int64_t pitch, i
     return launch_status(what);
 }
 
+template <class T>
+static bool whole_units(const void *p, int64_t values) {
+    return aligned_to(p, 16) && values * sizeof(T) % 16 == 0;
+}
+
+template <int PLANES, class T>
+static int launch_layer(const Product &p, const MatmulPlan &plan, const DenseOutput &o, float *partial, int sms, cudaStream_t st, const char *what) {
+    DenseEpilogue<T> e = {};
+    e.o = o;
+    e.bias_wide = aligned_to(o.bias, 16);
+    e.whole = o.rows_are_features == o.feature_major && whole_units<T>(o.y, p.n) && whole_units<T>(o.y, o.y_pitch) &&
+              (o.slope == nullptr || aligned_to(o.slope, 16)) &&
+              (o.residual == nullptr || (o.residual_col == 1 && whole_units<T>(o.residual, o.residual_row)));
+    return launch_product<PLANES>(p, plan, e, partial, sms, st, what);
+}
+
 // Whether the layer's outputs are the rows of the product: as they lie in the result, so that neighbouring columns are stored by
 // neighbouring lanes; but few samples fill half of a tile's 64 columns rather than half of its 128 rows.
 static bool features_as_rows(int64_t batch, bool feature_major) { return feature_major || batch <= 64; }
@@ -471,19 +469,27 @@ extern "C" DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_fea
     const DenseOutput o = {y, bias, residual, slope, y_feature_major ? batch : outer, rows_are_features ? residual_feature : residual_batch,
                            rows_are_features ? residual_batch : residual_feature, type, act, rows_are_features, y_feature_major != 0};
     float *partial = reinterpret_cast<float *>(workspace);
-    if (type == kFloat32) return launch_product<3>(p, plan, DenseEpilogue<float>{o}, partial, sms, st, what);
-    if (type == kBFloat16) return launch_product<1>(p, plan, DenseEpilogue<__nv_bfloat16>{o}, partial, sms, st, what);
-    return launch_product<1>(p, plan, DenseEpilogue<__half>{o}, partial, sms, st, what);
+    if (type == kFloat32) return launch_layer<3, float>(p, plan, o, partial, sms, st, what);
+    if (type == kBFloat16) return launch_layer<1, __nv_bfloat16>(p, plan, o, partial, sms, st, what);
+    return launch_layer<1, __half>(p, plan, o, partial, sms, st, what);
 }
 
 namespace dl {
 
+template <int PLANES, class T>
+static int launch_gradient(const Product &p, const MatmulPlan &plan, void *out, int64_t pitch, float *partial, int sms, cudaStream_t st,
+                           const char *what) {
+    PlainEpilogue<T> e = {};
+    e.out = reinterpret_cast<T *>(out);
+    e.pitch = pitch;
+    e.whole = whole_units<T>(out, p.n) && whole_units<T>(out, pitch);
+    return launch_product<PLANES>(p, plan, e, partial, sms, st, what);
+}
 static int launch_gradient(const Product &p, const MatmulPlan &plan, void *out, int64_t pitch, int type, float *partial, int sms, cudaStream_t st,
                            const char *what) {
-    if (type == kFloat32) return launch_product<3>(p, plan, PlainEpilogue<float>{reinterpret_cast<float *>(out), pitch}, partial, sms, st, what);
-    if (type == kBFloat16)
-        return launch_product<1>(p, plan, PlainEpilogue<__nv_bfloat16>{reinterpret_cast<__nv_bfloat16 *>(out), pitch}, partial, sms, st, what);
-    return launch_product<1>(p, plan, PlainEpilogue<__half>{reinterpret_cast<__half *>(out), pitch}, partial, sms, st, what);
+    if (type == kFloat32) return launch_gradient<3, float>(p, plan, out, pitch, partial, sms, st, what);
+    if (type == kBFloat16) return launch_gradient<1, __nv_bfloat16>(p, plan, out, pitch, partial, sms, st, what);
+    return launch_gradient<1, __half>(p, plan, out, pitch, partial, sms, st, what);
 }
 
 struct DenseBackward {

@@ -64,35 +64,51 @@ __device__ __forceinline__ void split_triple(float x, uint16_t &hi, uint16_t &mi
 // -- the kernel -----------------------------------------------------------------------------------------------------------------
 
 constexpr int kMatmulRows = 128;     // of a tile
-constexpr int kPieceColumns = 16;    // a piece: 32 rows of 16 columns, lane = row
-constexpr int kPiecePitch = kPieceColumns + 4;   // floats per row of a piece in shared memory: 16-byte rows, 8 lanes on 8 banks
+constexpr int kPieceColumns = 16;    // columns of which sums are kept together where a product is split
+constexpr int kSlotBytes = 2048;     // 32 rows of 64 bytes
+constexpr int kStageBytes = 2 * kSlotBytes;   // shared memory of an epilogue warp
 
-// An epilogue takes pieces: `begin` says where the first piece of a warp's share of a tile lies (row, col: of its first value), `piece`
-// takes the one `across` columns further, from registers.  The functions below turn a piece by way of shared memory: into quads, lane l
-// having rows l / 4 + 8 i and columns 4 (l % 4) .. + 3, or into columns, lane l having rows 4 (l % 8) .. + 3 of columns l / 8 + 4 i.
-__device__ __forceinline__ void piece_store(float *stage, int lane, const float (&v)[kPieceColumns]) {
+// An epilogue takes pieces of 32 rows (lane = row) and kColumns columns from registers: `begin` says where the first piece of a warp's
+// share of a tile lies (row, col: of its first value), `piece` takes the one `across` columns further.
+//
+// Results leave by way of shared memory in tiles of 32 rows of 64 bytes, a slot each: written as the lanes have them, rows or columns as
+// rows, and read back with 8 rows of four lanes at a time, so that a warp's store is of eight whole 64-byte rows.  The swizzle puts the
+// 16-byte unit j of row r at j ^ (r / 2 % 4): 8 lanes meet no bank twice either way.  (Tiled copies out of the slots instead made the
+// 4096 x 4096 iteration 5.8 ms for 4.0: the unit that does them has the operands' copies to do, 60 bytes a clock of them.)
+__device__ __forceinline__ void slot_row(uint8_t *slot, int lane, const uint32_t (&v)[16]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<uint4 *>(slot + lane * 64 + ((j ^ (lane / 2 % 4)) << 4)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+}
+__device__ __forceinline__ void slot_read_row(const uint8_t *slot, int lane, uint4 (&u)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = *reinterpret_cast<const uint4 *>(slot + lane * 64 + ((j ^ (lane / 2 % 4)) << 4));
+}
+__device__ __forceinline__ void slot_column(uint8_t *slot, int lane, int column, uint16_t v) {
+    *reinterpret_cast<uint16_t *>(slot + column * 64 + ((lane / 8 ^ (column / 2 % 4)) << 4) + lane % 8 * 2) = v;
+}
+// Unit lane % 4 of row lane / 4 + 8 i.
+__device__ __forceinline__ uint4 *slot_unit(uint8_t *slot, int lane, int i) {
+    const int row = lane / 4 + 8 * i;
+    return reinterpret_cast<uint4 *>(slot + row * 64 + ((lane % 4 ^ (row / 2 % 4)) << 4));
+}
+
+// Where a result cannot be stored that way: 32 rows of 16 columns turned into quads, lane l having rows l / 4 + 8 i and columns
+// 4 (l % 4) .. + 3.
+constexpr int kPiecePitch = kPieceColumns + 4;   // floats: 16-byte rows, 8 lanes on 8 banks
+static_assert(32 * kPiecePitch * 4 <= kStageBytes, "a piece fits");
+__device__ __forceinline__ void piece_quads(uint8_t *shared, int lane, const float (&v)[kPieceColumns], float (&q)[4][4]) {
+    float *stage = reinterpret_cast<float *>(shared);
 #pragma unroll
     for (int c = 0; c < kPieceColumns; c += 4)
         *reinterpret_cast<float4 *>(stage + lane * kPiecePitch + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
     __syncwarp();
-}
-__device__ __forceinline__ void piece_quads(const float *stage, int lane, float (&q)[4][4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float4 f = *reinterpret_cast<const float4 *>(stage + (lane / 4 + 8 * i) * kPiecePitch + lane % 4 * 4);
         q[i][0] = f.x; q[i][1] = f.y; q[i][2] = f.z; q[i][3] = f.w;
     }
-}
-__device__ __forceinline__ void piece_put_quads(float *stage, int lane, const float (&q)[4][4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<float4 *>(stage + (lane / 4 + 8 * i) * kPiecePitch + lane % 4 * 4) = make_float4(q[i][0], q[i][1], q[i][2], q[i][3]);
-}
-__device__ __forceinline__ void piece_columns(const float *stage, int lane, float (&q)[4][4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) q[i][j] = stage[(lane % 8 * 4 + j) * kPiecePitch + lane / 8 + 4 * i];
+    __syncwarp();
 }
 
 // Warps 0 .. 7: epilogue, one lane per row, two warps to the same rows; then one for the copies, one for the products, two idle: the
@@ -104,10 +120,8 @@ struct MatmulConfig {
     static constexpr int kTileRows = PAIR ? 2 * kMatmulRows : kMatmulRows;
     static constexpr int kOwnColumns = PAIR ? COLUMNS / 2 : COLUMNS;           // rows of B that a CTA copies
     static constexpr int kShare = COLUMNS / (kWarps / 4);                      // columns of an epilogue warp
-    static constexpr int kSpan = kPieceColumns;                                // of them handed to the epilogue at a time
-    static constexpr int kPitch = kPiecePitch;
     static constexpr int kStepBytes = PLANES * (kMatmulRows + kOwnColumns) * kChunk * 2;   // of a CTA
-    static constexpr int kStagingBytes = kWarps * 32 * kPitch * 4;
+    static constexpr int kStagingBytes = kWarps * kStageBytes;
     static constexpr int kFit = (232448 - 1024 - 256 - kStagingBytes) / kStepBytes;
     static constexpr int kStages = kFit < 6 ? kFit : 6;
     static constexpr int kSums = PLANES > 1 && COLUMNS <= 128 ? 2 : 1;         // accumulators: of the large products, of the small ones
@@ -159,14 +173,14 @@ static __device__ int g_matmul_async_error = 0;   // set when a bounded wait ran
 // raised and every role leaves, the copies that are in flight waited for.
 template <int PLANES, int COLUMNS, bool PAIR, class Epilogue>
 __global__ void __launch_bounds__(MatmulConfig<PLANES, COLUMNS, PAIR>::kThreadsAll, 1)
-matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MatmulShape s, const Epilogue epilogue) {
+matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MatmulShape s, const __grid_constant__ Epilogue epilogue) {
     using Config = MatmulConfig<PLANES, COLUMNS, PAIR>;
     constexpr int kStages = Config::kStages;
     constexpr int kPlaneA = kMatmulRows * kChunk * 2, kPlaneB = Config::kOwnColumns * kChunk * 2;
     extern __shared__ uint8_t s_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
-    float *staging = reinterpret_cast<float *>(ring + kStages * Config::kStepBytes);
-    uint64_t *full = reinterpret_cast<uint64_t *>(staging + Config::kStagingBytes / 4), *empty = full + kStages, *sums_full = empty + kStages,
+    uint8_t *staging = ring + kStages * Config::kStepBytes;
+    uint64_t *full = reinterpret_cast<uint64_t *>(staging + Config::kStagingBytes), *empty = full + kStages, *sums_full = empty + kStages,
              *sums_empty = sums_full + 2, *drained = sums_empty + 2;
     uint32_t *s_tensor = reinterpret_cast<uint32_t *>(drained + 1);
     volatile uint32_t *s_failed = s_tensor + 1;
@@ -318,9 +332,9 @@ const int col = t.col + (int)rank * Config::kOwnColumns;
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        constexpr int kSpan = Config::kSpan, kShare = Config::kShare, kPitch = Config::kPitch;
+        constexpr int kSpan = Epilogue::kColumns, kShare = Config::kShare;
         constexpr bool kKeep = PLANES > 1;   // sums of several blocks, added up in registers
-        float *mine = staging + warp * 32 * kPitch;
+        uint8_t *mine = staging + warp * kStageBytes;
         const int quarter = warp % 4, from = warp / 4 * kShare;   // a warp reads the lanes of its number modulo 4
         int buffer = 0;
         uint32_t buffer_phase = 0;
@@ -369,12 +383,12 @@ const int col = t.col + (int)rank * Config::kOwnColumns;
                     tensor_read_wait();
 #pragma unroll 1
                     for (int c0 = 0; c0 < kShare && (t.col + from + c0 < s.n || Epilogue::kWholeTiles); c0 += 32) {
-                        float v[2][kSpan];
+                        float v[32 / kSpan][kSpan];
 #pragma unroll
                         for (int c = 0; c < 32; ++c) v[c / kSpan][c % kSpan] = __uint_as_float(bits[c]);
                         if (c0 + 32 < kShare) tensor_read32(sums + c0 + 32, bits);
-                        finish(v[0], c0);
-                        finish(v[1], c0 + kSpan);
+#pragma unroll
+                        for (int h = 0; h < 32 / kSpan; ++h) finish(v[h], c0 + h * kSpan);
                         tensor_read_wait();
                     }
                 }
@@ -389,13 +403,15 @@ const int col = t.col + (int)rank * Config::kOwnColumns;
             }
             if constexpr (kKeep) {
                 if (ok) {
-#pragma unroll 1
-                    for (int c0 = 0; c0 < kShare; c0 += kSpan) {   // the registers move up: one copy of the epilogue's code
+#pragma unroll(kSpan == 32 ? 4 : 1)
+                    for (int c0 = 0; c0 < kShare; c0 += kSpan) {
                         float v[kSpan];
 #pragma unroll
-                        for (int c = 0; c < kSpan; ++c) v[c] = kept[c];
+                        for (int c = 0; c < kSpan; ++c) v[c] = kept[kSpan == 32 ? c0 + c : c];
+                        if (kSpan != 32) {   // the registers move up: one copy of the epilogue's code
 #pragma unroll
-                        for (int c = 0; c + kSpan < kShare; ++c) kept[c] = kept[c + kSpan];
+                            for (int c = 0; c + kSpan < kShare; ++c) kept[c] = kept[c + kSpan];
+                        }
                         finish(v, c0);
                     }
                 }
@@ -417,6 +433,7 @@ const int col = t.col + (int)rank * Config::kOwnColumns;
 // order of the splits.
 struct StorePartial {
     static constexpr bool kWholeTiles = true;
+    static constexpr int kColumns = kPieceColumns;
     float *out;
     int tile_rows, columns;
     struct Place {
@@ -428,7 +445,7 @@ struct StorePartial {
         const int piece = (row - t.row) / 32 + (col - t.col) / kPieceColumns * (tile_rows / 32);
         return {reinterpret_cast<float4 *>(out + tile * tile_rows * columns) + piece * (8 * kPieceColumns) + lane};
     }
-    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kPieceColumns], float *, int) const {
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], uint8_t *, int) const {
         float4 *to = p.to + across / kPieceColumns * (tile_rows / 32) * (8 * kPieceColumns);
 #pragma unroll
         for (int c = 0; c < kPieceColumns; c += 4) to[c * 8] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
@@ -437,26 +454,27 @@ struct StorePartial {
 
 template <int ROWS, int COLUMNS, class Epilogue>
 __global__ void __launch_bounds__(kThreads)
-matmul_join_kernel(const float *__restrict__ partial, const MatmulShape s, const Epilogue epilogue) {
-    __shared__ __align__(16) float s_stage[kThreads / 32][32 * kPiecePitch];
+matmul_join_kernel(const float *__restrict__ partial, const MatmulShape s, const __grid_constant__ Epilogue epilogue) {
+    __shared__ __align__(1024) uint8_t s_stage[kThreads / 32][kStageBytes];
     grid_dependency_wait();
     grid_dependents_launch();
-    constexpr int kDown = ROWS / 32, kPieces = kDown * COLUMNS / kPieceColumns;
+    constexpr int kDown = ROWS / 32, kTake = Epilogue::kColumns, kPieces = kDown * COLUMNS / kTake;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int64_t tiles = (int64_t)s.per_matrix * s.batch;
     for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + warp; i < tiles * kPieces; i += (int64_t)gridDim.x * (kThreads / 32)) {
         const int64_t tile = i / kPieces;
         const int piece = (int)(i - tile * kPieces), matrix = (int)(tile / s.per_matrix);
         const Tile t = tile_of<ROWS, COLUMNS>((int)(tile - (int64_t)matrix * s.per_matrix) + matrix * s.per_matrix * s.splits, s);
-        const int row = t.row + piece % kDown * 32, col = t.col + piece / kDown * kPieceColumns;
+        const int row = t.row + piece % kDown * 32, col = t.col + piece / kDown * kTake;
         if (row >= s.m || col >= s.n) continue;
-        const float4 *from = reinterpret_cast<const float4 *>(partial + tile * ROWS * COLUMNS) + piece * (8 * kPieceColumns) + lane;
+        const float4 *from = reinterpret_cast<const float4 *>(partial + tile * ROWS * COLUMNS) +
+                             (piece % kDown + piece / kDown * (kTake / kPieceColumns) * kDown) * (8 * kPieceColumns) + lane;
         const int64_t split = tiles * ROWS * COLUMNS / 4;
-        float v[kPieceColumns] = {};
+        float v[kTake] = {};
         for (int sp = 0; sp < s.splits; ++sp, from += split) {
 #pragma unroll
-            for (int c = 0; c < kPieceColumns; c += 4) {
-                const float4 f = from[c * 8];
+            for (int c = 0; c < kTake; c += 4) {
+                const float4 f = from[(c % kPieceColumns) * 8 + c / kPieceColumns * (kDown * 8 * kPieceColumns)];
                 v[c] += f.x; v[c + 1] += f.y; v[c + 2] += f.z; v[c + 3] += f.w;
             }
         }

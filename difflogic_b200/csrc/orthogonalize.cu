@@ -101,95 +101,115 @@ normalise_kernel(const Matrices all, int64_t rows, int64_t cols, const double *_
 }
 
 // Results of the iteration as pairs: v = scale * sum (+ factor * the pair in `more`) (+ diagonal on the diagonal).  Of a symmetric result
-// the blocks of 128 x 128 below the diagonal are stored on both sides, those above it not looked at.  Rows are padded to whole units: the values behind the
-// last one are written too, and read by nothing.
+// the blocks of 128 x 128 below the diagonal are stored on both sides, those above it not looked at.  `shifted`: a second result,
+// v + shift on the diagonal and v elsewhere.
 struct PairEpilogue {
     static constexpr bool kWholeTiles = false;
-    uint16_t *out;
-    const uint16_t *more;   // laid out as `out`; null: none
-    int64_t pitch, plane;
-    float scale, factor, diagonal;
+    static constexpr int kColumns = 32;
+    uint16_t *out, *shifted;   // null: no second result
+    const uint16_t *more;      // null: none
+    int64_t pitch, plane;      // of all three; rows are padded to whole units, whose last values are written too and read by nothing
+    float scale, factor, diagonal, shift;
     bool symmetric;
     struct Place {
-        int row, col, m, n;          // of the warp's first value
-        bool whole;                  // its 32 rows are all there
-        int64_t at, mirrored;        // of the lane's first value: of its own, of the mirrored ones
+        int row, col, m, n;    // of the warp's first value
+        int64_t matrix;
     };
-    __device__ __forceinline__ Place begin(const Tile &t, const MatmulShape &s, int row, int col, int lane) const {
-        const int64_t matrix = 2 * t.matrix * plane;
-        return {row, col, s.m, s.n, row + 32 <= s.m, matrix + (row + lane / 4) * pitch + col + lane % 4 * 4,
-                matrix + (col + lane / 8) * pitch + row + lane % 8 * 4};
+    __device__ __forceinline__ Place begin(const Tile &t, const MatmulShape &s, int row, int col, int) const {
+        return {row, col, s.m, s.n, 2 * t.matrix * plane};
     }
-    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kPieceColumns], float *stage, int lane) const {
-        const int first = p.col + across, below = p.row / kMatmulRows - first / kMatmulRows;
-        if (symmetric && below < 0) return;
-        const bool whole = p.whole && first + kPieceColumns <= p.n;
-        piece_store(stage, lane, v);
-        float q[4][4];
-        piece_quads(stage, lane, q);
+    // The slots' rows -- high and low halves -- to rows row .. of the result(s), columns col .., of which those below `rows`, `cols` are there.
+    __device__ __forceinline__ void store(uint8_t *stage, int lane, const Place &p, uint16_t *to, uint16_t *as_well, int row, int col, int rows,
+                                          int cols) const {
+        const int r = row + lane / 4, c = col + lane % 4 * 8;
+        const int64_t at = p.matrix + r * pitch + c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (r + 8 * i >= rows || c >= cols) continue;
+            const uint4 hi = *slot_unit(stage, lane, i), lo = *slot_unit(stage + kSlotBytes, lane, i);
+            *reinterpret_cast<uint4 *>(to + at + 8 * i * pitch) = hi;
+            *reinterpret_cast<uint4 *>(to + at + 8 * i * pitch + plane) = lo;
+            if (as_well != nullptr) {
+                *reinterpret_cast<uint4 *>(as_well + at + 8 * i * pitch) = hi;
+                *reinterpret_cast<uint4 *>(as_well + at + 8 * i * pitch + plane) = lo;
+            }
+        }
         __syncwarp();
-        const int row = p.row + lane / 4, col = first + lane % 4 * 4;
-        const int64_t at = p.at + across, step = 8 * pitch;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) q[i][j] *= scale;
-        if (diagonal != 0.f && below == 0) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (row + 8 * i == col + j) q[i][j] += diagonal;
-        }
+    }
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], uint8_t *stage, int lane) const {
+        const int col = p.col + across, below = p.row / kMatmulRows - col / kMatmulRows, row = p.row + lane;
+        if (p.row >= p.m || (symmetric && below < 0)) return;
+        const bool on_diagonal = p.row < col + kColumns && col < p.row + 32;
+        uint32_t hi[16], lo[16];
         if (more != nullptr) {
-            ushort4 hi[4], lo[4];
+            const int r = p.row + lane / 4, c = col + lane % 4 * 8;
+            const int64_t at = p.matrix + r * pitch + c;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (whole || (row + 8 * i < p.m && col < p.n)) {
-                    hi[i] = *reinterpret_cast<const ushort4 *>(more + at + i * step);
-                    lo[i] = *reinterpret_cast<const ushort4 *>(more + at + i * step + plane);
-                } else {
-                    hi[i] = lo[i] = make_ushort4(0, 0, 0, 0);
-                }
+                const bool there = r + 8 * i < p.m && c < p.n;
+                *slot_unit(stage, lane, i) = there ? *reinterpret_cast<const uint4 *>(more + at + 8 * i * pitch) : make_uint4(0, 0, 0, 0);
+                *slot_unit(stage + kSlotBytes, lane, i) = there ? *reinterpret_cast<const uint4 *>(more + at + 8 * i * pitch + plane) : make_uint4(0, 0, 0, 0);
+            }
+            __syncwarp();
+            uint4 h[4], l[4];
+            slot_read_row(stage, lane, h);
+            slot_read_row(stage + kSlotBytes, lane, l);
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                hi[4 * j] = h[j].x; hi[4 * j + 1] = h[j].y; hi[4 * j + 2] = h[j].z; hi[4 * j + 3] = h[j].w;
+                lo[4 * j] = l[j].x; lo[4 * j + 1] = l[j].y; lo[4 * j + 2] = l[j].z; lo[4 * j + 3] = l[j].w;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                q[i][0] += factor * join_pair(hi[i].x, lo[i].x);
-                q[i][1] += factor * join_pair(hi[i].y, lo[i].y);
-                q[i][2] += factor * join_pair(hi[i].z, lo[i].z);
-                q[i][3] += factor * join_pair(hi[i].w, lo[i].w);
+            for (int j = 0; j < 16; ++j)
+                split_two(v[2 * j] * scale + factor * join_pair((uint16_t)hi[j], (uint16_t)lo[j]) + (diagonal != 0.f && row == col + 2 * j ? diagonal : 0.f),
+                          v[2 * j + 1] * scale + factor * join_pair((uint16_t)(hi[j] >> 16), (uint16_t)(lo[j] >> 16)) +
+                              (diagonal != 0.f && row == col + 2 * j + 1 ? diagonal : 0.f),
+                          hi[j], lo[j]);
+        } else if (diagonal != 0.f && on_diagonal) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                split_two(v[2 * j] * scale + (row == col + 2 * j ? diagonal : 0.f), v[2 * j + 1] * scale + (row == col + 2 * j + 1 ? diagonal : 0.f), hi[j],
+                          lo[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) split_two(v[2 * j] * scale, v[2 * j + 1] * scale, hi[j], lo[j]);
+        }
+        slot_row(stage, lane, hi);
+        slot_row(stage + kSlotBytes, lane, lo);
+        __syncwarp();
+        store(stage, lane, p, out, on_diagonal ? nullptr : shifted, p.row, col, p.m, p.n);
+        if (symmetric && below > 0) {   // columns as rows
+#pragma unroll
+            for (int j = 0; j < kColumns; ++j) {
+                slot_column(stage, lane, j, (uint16_t)(hi[j / 2] >> (j % 2 * 16)));
+                slot_column(stage + kSlotBytes, lane, j, (uint16_t)(lo[j / 2] >> (j % 2 * 16)));
             }
-        }
-        const bool mirror = symmetric && below > 0;
-        if (mirror) {   // from here the mirrored values are taken
-            piece_put_quads(stage, lane, q);
             __syncwarp();
-        }
+            store(stage, lane, p, out, shifted, col, p.row, p.n, p.m);
+        } else if (shifted != nullptr && on_diagonal) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (whole || (row + 8 * i < p.m && col < p.n)) store_pairs(out + at + i * step, q[i]);
-        if (mirror) {
-            piece_columns(stage, lane, q);
+            for (int j = 0; j < 16; ++j)
+                split_two(v[2 * j] * scale + (row == col + 2 * j ? shift : 0.f), v[2 * j + 1] * scale + (row == col + 2 * j + 1 ? shift : 0.f), hi[j], lo[j]);
+            slot_row(stage, lane, hi);
+            slot_row(stage + kSlotBytes, lane, lo);
             __syncwarp();
-            // columns of the result: rows of the piece
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (whole || (p.row + lane % 8 * 4 < p.m && first + lane / 8 + 4 * i < p.n))
-                    store_pairs(out + p.mirrored + (across + 4 * i) * pitch, q[i]);
+            store(stage, lane, p, shifted, nullptr, p.row, col, p.m, p.n);
         }
     }
-    __device__ __forceinline__ void store_pairs(uint16_t *to, const float (&v)[4]) const {
-        uint16_t hi[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) split_pair(v[j], hi[j], lo[j]);
-        *reinterpret_cast<ushort4 *>(to) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<ushort4 *>(to + plane) = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+    static __device__ __forceinline__ void split_two(float a, float b, uint32_t &hi, uint32_t &lo) {
+        uint16_t h[2], l[2];
+        split_pair(a, h[0], l[0]);
+        split_pair(b, h[1], l[1]);
+        hi = (uint32_t)h[0] | (uint32_t)h[1] << 16;
+        lo = (uint32_t)l[0] | (uint32_t)l[1] << 16;
     }
 };
 
 // The last product: the result itself, or the weights' update w <- decay w - rate v.
 struct OrthogonalEpilogue {
     static constexpr bool kWholeTiles = false;
+    static constexpr int kColumns = kPieceColumns;
     void *out;              // results behind each other; null: the weights of `all` are updated
     Matrices all;
     int64_t cols;           // values of a row
@@ -207,11 +227,9 @@ struct OrthogonalEpilogue {
         const int64_t at = r * cols + c;
         return {r, c, s.m, s.n, out == nullptr ? at : at + t.matrix * s.m * cols, 2 * t.matrix * plane, out == nullptr ? all.weight[t.matrix] : nullptr};
     }
-    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kPieceColumns], float *stage, int lane) const {
-        piece_store(stage, lane, v);
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], uint8_t *stage, int lane) const {
         float q[4][4], w[4][4];
-        piece_quads(stage, lane, q);
-        __syncwarp();
+        piece_quads(stage, lane, v, q);
         const int left = p.n - p.col - across;
         if (left <= 0) return;
         if (p.weight != nullptr) {
@@ -255,7 +273,7 @@ struct OrthogonalLayout {
     int parts;
     MatmulPlan gram, square, product;
     int64_t x_bytes, s_bytes, norm_bytes, partial_bytes;
-    int64_t total() const { return 2 * x_bytes + 2 * s_bytes + norm_bytes + partial_bytes; }
+    int64_t total() const { return 2 * x_bytes + 3 * s_bytes + norm_bytes + partial_bytes; }
 };
 
 static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t cols, bool light, int sms) {
@@ -280,6 +298,7 @@ static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t c
 }
 
 // steps times: S = X^T X (X X^T where X is wide), M = b S + c S^2, X = a X + X M (M X).  `last` takes the last product.
+// b S + c S^2 is one product, of S with S + b / c I, which the first product stores beside S.
 //
 // Results of 22 bits (fp32, fp16): every product is one of pairs, and a X comes out of the product too, as the diagonal of M, since
 // the pair of a X would have to be read again.  bf16 results have 8 bits, and the steps need no more than this: S from the first planes
@@ -291,10 +310,17 @@ static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64
                          const OrthogonalEpilogue &last, uint8_t *workspace, int sms, cudaStream_t st, const char *what) {
     const bool light = all.type == kBFloat16;
     const OrthogonalLayout l = orthogonal_layout(batch, rows, cols, light, sms);
-    uint16_t *x = reinterpret_cast<uint16_t *>(workspace), *next = reinterpret_cast<uint16_t *>(workspace + l.x_bytes);
-    uint16_t *gram = reinterpret_cast<uint16_t *>(workspace + 2 * l.x_bytes), *poly = reinterpret_cast<uint16_t *>(workspace + 2 * l.x_bytes + l.s_bytes);
-    double *norms = reinterpret_cast<double *>(workspace + 2 * l.x_bytes + 2 * l.s_bytes);
-    float *partial = reinterpret_cast<float *>(workspace + 2 * l.x_bytes + 2 * l.s_bytes + l.norm_bytes);
+    uint8_t *at = workspace;
+    const auto take = [&](int64_t bytes) {
+        uint8_t *p = at;
+        at += bytes;
+        return p;
+    };
+    uint16_t *x = reinterpret_cast<uint16_t *>(take(l.x_bytes)), *next = reinterpret_cast<uint16_t *>(take(l.x_bytes));
+    uint16_t *gram = reinterpret_cast<uint16_t *>(take(l.s_bytes)), *shifted = reinterpret_cast<uint16_t *>(take(l.s_bytes)),
+             *poly = reinterpret_cast<uint16_t *>(take(l.s_bytes));
+    double *norms = reinterpret_cast<double *>(take(l.norm_bytes));
+    float *partial = reinterpret_cast<float *>(at);
     int status;
     launch_dependent(true, square_sums_kernel, dim3((unsigned)l.parts, (unsigned)batch), dim3(kThreads), 0, st, all, rows * cols, norms);
     if ((status = launch_status(what)) != DL_OK) return status;
@@ -315,14 +341,36 @@ static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64
         p.k = l.tall ? rows : cols;
         p.symmetric = true;
         p.planes = light ? 1 : 2;
-        const PairEpilogue to_gram = {gram, nullptr, l.s_pitch, l.s_plane, once, 0.f, 0.f, true};
-        if ((status = launch_planes(p, l.gram, to_gram, partial, sms, st, what)) != DL_OK) return status;
-        p.a = p.b = {gram, l.s_pitch, l.s_plane, false};
+        // b S + c S^2 = c S (S + b / c I); where b / c is too large for a pair, b S is added up in the epilogue
+        PairEpilogue e = {};
+        e.pitch = l.s_pitch;
+        e.plane = l.s_plane;
+        e.scale = once;
+        e.symmetric = true;
+        const bool in_one = fabsf(b) <= 8.f * fabsf(c) && c != 0.f;
+        e.out = gram;
+        e.shifted = in_one ? shifted : nullptr;
+        e.shift = in_one ? b / c * kPairScale : 0.f;
+        if (c == 0.f) {   // the cubic iteration: M comes straight out of this product
+            e.scale = b * once;
+            e.diagonal = light ? 0.f : a * kPairScale;
+        }
+        if ((status = launch_planes(p, l.gram, e, partial, sms, st, what)) != DL_OK) return status;
+        if (c != 0.f) {
+            p.a = {gram, l.s_pitch, l.s_plane, false};
+            p.b = {in_one ? shifted : gram, l.s_pitch, l.s_plane, false};
+            p.k = l.side;
+            p.planes = 2;
+            e.out = poly;
+            e.shifted = nullptr;
+            e.more = in_one ? nullptr : gram;
+            e.factor = b;
+            e.scale = c * once;
+            e.diagonal = light ? 0.f : a * kPairScale;
+            if ((status = launch_planes(p, l.square, e, partial, sms, st, what)) != DL_OK) return status;
+        }
+        const Operand m = {c != 0.f ? poly : gram, l.s_pitch, l.s_plane, false};
         p.k = l.side;
-        p.planes = 2;
-        const PairEpilogue to_poly = {poly, gram, l.s_pitch, l.s_plane, c * once, b, light ? 0.f : a * kPairScale, true};
-        if ((status = launch_planes(p, l.square, to_poly, partial, sms, st, what)) != DL_OK) return status;
-        const Operand m = {poly, l.s_pitch, l.s_plane, false};
         p.a = l.tall ? Operand{x, l.x_pitch, l.x_plane, false} : m;
         p.b = l.tall ? m : Operand{x, l.x_pitch, l.x_plane, true};
         p.m = rows;
@@ -331,18 +379,24 @@ static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64
         p.planes = light ? 1 : 2;
         const uint16_t *more = light ? x : nullptr;
         if (i + 1 < steps) {
-            const PairEpilogue to_next = {next, more, l.x_pitch, l.x_plane, once, a, 0.f, false};
+            PairEpilogue to_next = {};
+            to_next.more = more;
+            to_next.pitch = l.x_pitch;
+            to_next.plane = l.x_plane;
+            to_next.scale = once;
+            to_next.factor = a;
+            to_next.out = next;
             status = launch_planes(p, l.product, to_next, partial, sms, st, what);
         } else {
-            OrthogonalEpilogue e = last;
-            e.all = all;
-            e.cols = cols;
-            e.more = more;
-            e.pitch = l.x_pitch;
-            e.plane = l.x_plane;
-            e.scale = twice;
-            e.factor = a * once;
-            status = launch_planes(p, l.product, e, partial, sms, st, what);
+            OrthogonalEpilogue to_end = last;
+            to_end.all = all;
+            to_end.cols = cols;
+            to_end.more = more;
+            to_end.pitch = l.x_pitch;
+            to_end.plane = l.x_plane;
+            to_end.scale = twice;
+            to_end.factor = a * once;
+            status = launch_planes(p, l.product, to_end, partial, sms, st, what);
         }
         if (status != DL_OK) return status;
         uint16_t *done = x;

@@ -91,7 +91,7 @@ def test_batches_steps_and_coefficients(rows, cols):
     assert whole.shape == (2, 3, rows, cols)
     one = D.ops.orthogonalize(g[4])
     assert far(whole.view(6, rows, cols)[4], one) <= 2 * bound(torch.float32, cols)   # other splits, other sums
-    for steps, coefficients in [(1, DEFAULT), (2, (1.5, -0.5, 0.0)), (3, [(3.0, -3.2, 1.2), (2.0, -1.5, 0.5), (1.5, -0.5, 0.0)]), (12, (1.5, -0.5, 0.0))]:
+    for steps, coefficients in [(1, DEFAULT), (2, (1.5, -0.5, 0.0)), (3, [(3.0, -3.2, 1.2), (2.0, -1.5, 0.5), (1.5, -0.5, 0.0)]), (12, (1.5, -0.5, 0.0)), (6, (1.6, -0.7, 0.02))]:
         got = D.ops.orthogonalize(g, steps=steps, coefficients=coefficients)
         want = definition(g, steps, coefficients)
         for z in range(6):
