@@ -20,6 +20,18 @@ __device__ __forceinline__ T from_float(float v) {
     else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
     else return __float2bfloat16_rn(v);
 }
+// Two 16-bit values, packed: conversions of two values at a time run at several times the rate of single ones.
+template <class T>
+__device__ __forceinline__ uint32_t two_of(float a, float b) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
 // 64 bytes of neighbouring values, and value j of them.
 struct Units {
     uint4 u[4];
@@ -48,8 +60,7 @@ __device__ __forceinline__ void store_rows(uint8_t *slot, int lane, const float 
     } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const T lo = from_float<T>(v[2 * j]), hi = from_float<T>(v[2 * j + 1]);
-            w[j] = (uint32_t)*reinterpret_cast<const uint16_t *>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t *>(&hi) << 16;
+            w[j] = two_of<T>(v[2 * j], v[2 * j + 1]);
         }
     }
     slot_row(slot, lane, w);

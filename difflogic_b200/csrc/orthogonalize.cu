@@ -91,12 +91,12 @@ normalise_kernel(const Matrices all, int64_t rows, int64_t cols, const double *_
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = update_of(m[j], v[j], all.nesterov);
         }
-        uint16_t hi[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) split_pair(v[j] * scale, hi[j], lo[j]);
+        uint2 hi, lo;
+        split_two(v[0] * scale, v[1] * scale, hi.x, lo.x);
+        split_two(v[2] * scale, v[3] * scale, hi.y, lo.y);
         uint16_t *to = x + 2 * z * plane + row * pitch + col;
-        *reinterpret_cast<ushort4 *>(to) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<ushort4 *>(to + plane) = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+        *reinterpret_cast<uint2 *>(to) = hi;
+        *reinterpret_cast<uint2 *>(to + plane) = lo;
     }
 }
 
@@ -196,13 +196,6 @@ struct PairEpilogue {
             __syncwarp();
             store(stage, lane, p, shifted, nullptr, p.row, col, p.m, p.n);
         }
-    }
-    static __device__ __forceinline__ void split_two(float a, float b, uint32_t &hi, uint32_t &lo) {
-        uint16_t h[2], l[2];
-        split_pair(a, h[0], l[0]);
-        split_pair(b, h[1], l[1]);
-        hi = (uint32_t)h[0] | (uint32_t)h[1] << 16;
-        lo = (uint32_t)l[0] | (uint32_t)l[1] << 16;
     }
 };
 
