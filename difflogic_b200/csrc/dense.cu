@@ -50,26 +50,38 @@ __device__ __forceinline__ float value_of(const Units &from, int j) {
 }
 
 // 32 rows of values, a row in each lane, to where they lie in memory: rows `pitch` values apart, those from m on and columns from n on
-// left out.
+// left out.  whole: rows lie and end on 16-byte units; else a lane stores a value and a warp the 64 bytes of one row or two at a time.
 template <class T>
-__device__ __forceinline__ void store_rows(uint8_t *slot, int lane, const float (&v)[64 / sizeof(T)], T *to, int64_t pitch, int row, int col, int m, int n) {
+__device__ __forceinline__ void store_rows(uint8_t *slot, int lane, const float (&v)[64 / sizeof(T)], T *to, int64_t pitch, int row, int col, int m, int n,
+                                           bool whole) {
     uint32_t w[16];
-    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            w[j] = two_of<T>(v[2 * j], v[2 * j + 1]);
-        }
+    for (int j = 0; j < 16; ++j) {
+        if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(v[j]);
+        else w[j] = two_of<T>(v[2 * j], v[2 * j + 1]);
     }
     slot_row(slot, lane, w);
     __syncwarp();
-    const int r = row + lane / 4, c = col + lane % 4 * (16 / (int)sizeof(T));
-    T *at = to + r * pitch + c;
+    if (whole) {
+        const int r = row + lane / 4, c = col + lane % 4 * (16 / (int)sizeof(T));
+        T *at = to + r * pitch + c;
+        uint4 u[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (r + 8 * i < m && c < n) *reinterpret_cast<uint4 *>(at + 8 * i * pitch) = *slot_unit(slot, lane, i);
+        for (int i = 0; i < 4; ++i) u[i] = *slot_unit(slot, lane, i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (r + 8 * i < m && c < n) *reinterpret_cast<uint4 *>(at + 8 * i * pitch) = u[i];
+    } else {
+        constexpr int kRow = 64 / sizeof(T), kAtOnce = 32 / kRow;   // values of a row, rows that 32 lanes take
+        const int mine = lane / kRow, c = lane % kRow;
+        T *at = to + (row + mine) * pitch + col + c;
+#pragma unroll 8
+        for (int r = mine; r < 32; r += kAtOnce, at += kAtOnce * pitch) {
+            const T value = *reinterpret_cast<const T *>(slot + r * 64 + ((c * (int)sizeof(T) / 16 ^ (r / 2 % 4)) << 4) + c * (int)sizeof(T) % 16);
+            if (row + r < m && col + c < n) *at = value;
+        }
+    }
+    __syncwarp();
 }
 
 template <class T>
@@ -78,7 +90,8 @@ struct DenseEpilogue {
     static constexpr int kColumns = 64 / sizeof(T);   // 64 bytes
     using Slope = typename std::conditional<sizeof(T) == 4, float, __half>::type;
     DenseOutput o;
-    bool whole;    // rows of y and slope lie and end on 16-byte units, and those of the residual
+    bool whole;            // rows of y and slope lie and end on 16-byte units
+    bool residual_whole;   // those of the residual too
     bool bias_wide;
 
     struct Place {
@@ -86,19 +99,24 @@ struct DenseEpilogue {
     };
     __device__ __forceinline__ Place begin(const Tile &, const MatmulShape &s, int row, int col, int) const { return {row, col, s.m, s.n}; }
 
+    struct Ahead {
+        uint4 u[4];   // of the residual, as slot_unit's
+    };
+    __device__ __forceinline__ void fetch(const Place &p, int across, int lane, Ahead &a) const {
+        if (!residual_whole) return;
+        const int r = p.row + lane / 4, c = p.col + across + lane % 4 * (16 / (int)sizeof(T));
+        const T *from = reinterpret_cast<const T *>(o.residual) + r * o.residual_row + c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            a.u[i] = r + 8 * i < p.m && c < p.n ? *reinterpret_cast<const uint4 *>(from + 8 * i * o.residual_row) : make_uint4(0, 0, 0, 0);
+    }
+
     template <bool SLOPE>
-    __device__ __forceinline__ void tile_piece(const Place &p, int across, const float (&v)[kColumns], uint8_t *stage, int lane) const {
+    __device__ __forceinline__ void rows(const Place &p, int across, const float (&v)[kColumns], const Ahead &a, uint8_t *stage, int lane) const {
         const T *bias = reinterpret_cast<const T *>(o.bias), *residual = reinterpret_cast<const T *>(o.residual);
         const int row = p.row + lane, col = p.col + across;
         const bool there = row < p.m;
         constexpr int kUnit = 16 / sizeof(T);   // values of 16 bytes
-        Units more;
-        if (residual != nullptr) {
-            const T *from = residual + row * o.residual_row + col;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                more.u[j] = there && col + (j + 1) * kUnit <= p.n ? *reinterpret_cast<const uint4 *>(from + j * kUnit) : make_uint4(0, 0, 0, 0);
-        }
         float z[kColumns], d[kColumns];
         if (bias == nullptr || o.rows_are_features) {
             const float b = bias != nullptr && there ? to_float(bias[row]) : 0.f;
@@ -116,92 +134,70 @@ struct DenseEpilogue {
         }
         activate<SLOPE>(z, d, o.act);
         if (residual != nullptr) {
+            if (residual_whole) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *slot_unit(stage, lane, i) = a.u[i];
+            } else {
+                constexpr int kRow = 64 / sizeof(T), kAtOnce = 32 / kRow;   // as store_rows'
+                const int mine = lane / kRow, c = lane % kRow;
+#pragma unroll 8
+                for (int r = mine; r < 32; r += kAtOnce)
+                    *reinterpret_cast<T *>(stage + r * 64 + ((c * (int)sizeof(T) / 16 ^ (r / 2 % 4)) << 4) + c * (int)sizeof(T) % 16) =
+                        p.row + r < p.m && col + c < p.n ? residual[(p.row + r) * o.residual_row + (col + c) * o.residual_col] : from_float<T>(0.f);
+            }
+            __syncwarp();
+            Units more;
+            slot_read_row(stage, lane, more.u);
+            __syncwarp();
 #pragma unroll
             for (int j = 0; j < kColumns; ++j) z[j] += value_of<T>(more, j);
         }
-        // The slots take turns: who writes one has met all others behind their reading of it.
-        T *y = reinterpret_cast<T *>(o.y);
+        store_rows(stage, lane, z, reinterpret_cast<T *>(o.y), o.y_pitch, p.row, col, p.m, p.n, whole);
         if (SLOPE) {
-            store_rows(stage, lane, z, y, o.y_pitch, p.row, col, p.m, p.n);
             if (sizeof(T) != 4) {
 #pragma unroll
                 for (int j = 0; j < kColumns; ++j) d[j] *= kSlopeScale;
             }
-            store_rows(stage + kSlotBytes, lane, d, reinterpret_cast<Slope *>(o.slope), o.y_pitch, p.row, col, p.m, p.n);
-        } else {
-            if (across == 0) __syncwarp();   // the last share may have ended on this slot
-            store_rows(stage + across / kColumns % 2 * kSlotBytes, lane, z, y, o.y_pitch, p.row, col, p.m, p.n);
+            store_rows(stage, lane, d, reinterpret_cast<Slope *>(o.slope), o.y_pitch, p.row, col, p.m, p.n, whole);
         }
     }
 
-    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], uint8_t *stage, int lane) const {
-        if (p.row >= p.m) return;
-        if (whole) {
-            if (o.slope != nullptr) tile_piece<true>(p, across, v, stage, lane);
-            else tile_piece<false>(p, across, v, stage, lane);
-            return;
-        }
-        // results whose rows are off the 16-byte units, or that lie the other way: neighbouring lanes have neighbouring rows
+    // Results that lie the other way: neighbouring lanes have neighbouring values.
+    template <bool SLOPE>
+    __device__ __forceinline__ void columns(const Place &p, int across, const float (&v)[kColumns], int lane) const {
         const T *bias = reinterpret_cast<const T *>(o.bias), *residual = reinterpret_cast<const T *>(o.residual);
-        T *y = reinterpret_cast<T *>(o.y);
-        Slope *slope = reinterpret_cast<Slope *>(o.slope);
-        constexpr float kScale = sizeof(T) == 4 ? 1.f : kSlopeScale;
-        const bool by_rows = o.rows_are_features == o.feature_major;
-#pragma unroll 1
-        for (int part = 0; part < kColumns; part += kPieceColumns) {
-            float t[kPieceColumns], d[kPieceColumns];
+        const int row = p.row + lane, col = p.col + across, left = p.n - col;
+        if (row >= p.m) return;
+        const float row_bias = bias != nullptr && o.rows_are_features ? to_float(bias[row]) : 0.f;
+        float z[kColumns], d[kColumns];
 #pragma unroll
-            for (int j = 0; j < kPieceColumns; ++j) t[j] = kColumns == kPieceColumns || part == 0 ? v[j] : v[kColumns - kPieceColumns + j];
-            if (!by_rows) {
-                const int row = p.row + lane, col = p.col + across + part, left = p.n - col;
-                if (row >= p.m) continue;
-                const float row_bias = bias != nullptr && o.rows_are_features ? to_float(bias[row]) : 0.f;
+        for (int j = 0; j < kColumns; ++j)
+            z[j] = v[j] + (bias != nullptr && !o.rows_are_features && j < left ? to_float(bias[col + j]) : row_bias);
+        activate<SLOPE>(z, d, o.act);
+        if (residual != nullptr) {
+            const T *from = residual + row * o.residual_row + col * o.residual_col;
 #pragma unroll
-                for (int j = 0; j < kPieceColumns; ++j)
-                    t[j] += bias != nullptr && !o.rows_are_features && j < left ? to_float(bias[col + j]) : row_bias;
-                activate<true>(t, d, o.act);
-                if (residual != nullptr) {
-                    const T *from = residual + row * o.residual_row + col * o.residual_col;
+            for (int j = 0; j < kColumns; ++j)
+                if (j < left) z[j] += to_float(from[j * o.residual_col]);
+        }
+        T *y = reinterpret_cast<T *>(o.y) + col * o.y_pitch + row;
+        Slope *slope = reinterpret_cast<Slope *>(o.slope) + col * o.y_pitch + row;
 #pragma unroll
-                    for (int j = 0; j < kPieceColumns; ++j)
-                        if (j < left) t[j] += to_float(from[j * o.residual_col]);
-                }
-                const int64_t at = col * o.y_pitch + row;
-#pragma unroll
-                for (int j = 0; j < kPieceColumns; ++j) {
-                    if (j >= left) continue;
-                    y[at + j * o.y_pitch] = from_float<T>(t[j]);
-                    if (slope != nullptr) slope[at + j * o.y_pitch] = from_float<Slope>(d[j] * kScale);
-                }
-                continue;
-            }
-            float q[4][4];
-            piece_quads(stage, lane, t, q);
-            const int col = p.col + across + part + lane % 4 * 4, left = p.n - col;
-            if (left <= 0) continue;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = p.row + lane / 4 + 8 * i;
-                if (row >= p.m) continue;
-                float e[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (bias != nullptr && j < left) q[i][j] += to_float(bias[o.rows_are_features ? row : col + j]);
-                activate<true>(q[i], e, o.act);
-                if (residual != nullptr) {
-                    const T *from = residual + row * o.residual_row + col * o.residual_col;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (j < left) q[i][j] += to_float(from[j * o.residual_col]);
-                }
-                const int64_t at = row * o.y_pitch + col;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j >= left) continue;
-                    y[at + j] = from_float<T>(q[i][j]);
-                    if (slope != nullptr) slope[at + j] = from_float<Slope>(e[j] * kScale);
-                }
-            }
+        for (int j = 0; j < kColumns; ++j) {
+            if (j >= left) continue;
+            y[j * o.y_pitch] = from_float<T>(z[j]);
+            if (SLOPE) slope[j * o.y_pitch] = from_float<Slope>(d[j] * (sizeof(T) == 4 ? 1.f : kSlopeScale));
+        }
+    }
+
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], const Ahead &a, uint8_t *stage, int lane) const {
+        if (p.row >= p.m) return;
+        if (o.rows_are_features == o.feature_major) {
+            if (o.slope != nullptr) rows<true>(p, across, v, a, stage, lane);
+            else rows<false>(p, across, v, a, stage, lane);
+        } else {
+            if (o.slope != nullptr) columns<true>(p, across, v, lane);
+            else columns<false>(p, across, v, lane);
         }
     }
 };
@@ -218,28 +214,10 @@ struct PlainEpilogue {
         int row, col, m, n;   // of the warp's first value
     };
     __device__ __forceinline__ Place begin(const Tile &, const MatmulShape &s, int row, int col, int) const { return {row, col, s.m, s.n}; }
-    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], uint8_t *stage, int lane) const {
-        if (p.row >= p.m) return;
-        if (whole) {
-            if (across == 0) __syncwarp();   // as DenseEpilogue's
-            store_rows(stage + across / kColumns % 2 * kSlotBytes, lane, v, out, pitch, p.row, p.col + across, p.m, p.n);
-            return;
-        }
-#pragma unroll 1
-        for (int part = 0; part < kColumns; part += kPieceColumns) {
-            float t[kPieceColumns], q[4][4];
-#pragma unroll
-            for (int j = 0; j < kPieceColumns; ++j) t[j] = kColumns == kPieceColumns || part == 0 ? v[j] : v[kColumns - kPieceColumns + j];
-            piece_quads(stage, lane, t, q);
-            const int col = p.col + across + part + lane % 4 * 4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = p.row + lane / 4 + 8 * i;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (row < p.m && col + j < p.n) out[row * pitch + col + j] = from_float<T>(q[i][j]);
-            }
-        }
+    using Ahead = NothingAhead;
+    __device__ __forceinline__ void fetch(const Place &, int, int, Ahead &) const {}
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], const Ahead &, uint8_t *stage, int lane) const {
+        if (p.row < p.m) store_rows(stage, lane, v, out, pitch, p.row, p.col + across, p.m, p.n, whole);
     }
 };
 
@@ -391,9 +369,9 @@ static int launch_layer(const Product &p, const MatmulPlan &plan, const DenseOut
     DenseEpilogue<T> e = {};
     e.o = o;
     e.bias_wide = aligned_to(o.bias, 16);
-    e.whole = o.rows_are_features == o.feature_major && whole_units<T>(o.y, p.n) && whole_units<T>(o.y, o.y_pitch) &&
-              (o.slope == nullptr || aligned_to(o.slope, 16)) &&
-              (o.residual == nullptr || (o.residual_col == 1 && whole_units<T>(o.residual, o.residual_row)));
+    e.whole = whole_units<T>(o.y, p.n) && whole_units<T>(o.y, o.y_pitch) && (o.slope == nullptr || aligned_to(o.slope, 16));
+    e.residual_whole = o.residual != nullptr && o.rows_are_features == o.feature_major && o.residual_col == 1 && whole_units<T>(o.residual, p.n) &&
+                       whole_units<T>(o.residual, o.residual_row);
     return launch_product<PLANES>(p, plan, e, partial, sms, st, what);
 }
 

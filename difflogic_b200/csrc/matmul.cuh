@@ -73,7 +73,10 @@ constexpr int kSlotBytes = 2048;     // 32 rows of 64 bytes
 constexpr int kStageBytes = 2 * kSlotBytes;   // shared memory of an epilogue warp
 
 // An epilogue takes pieces of 32 rows (lane = row) and kColumns columns from registers: `begin` says where the first piece of a warp's
-// share of a tile lies (row, col: of its first value), `piece` takes the one `across` columns further.
+// share of a tile lies (row, col: of its first value), `piece` takes the one `across` columns further.  What it has to read for that
+// `fetch` asks for beforehand -- the first one's while the products are still running, the others' a piece ahead: a read takes 3000
+// clocks when all SMs read at a time.
+struct NothingAhead {};
 //
 // Results leave by way of shared memory in tiles of 32 rows of 64 bytes, a slot each: written as the lanes have them, rows or columns as
 // rows, and read back with 8 rows of four lanes at a time, so that a warp's store is of eight whole 64-byte rows.  The swizzle puts the
@@ -348,8 +351,13 @@ const int col = t.col + (int)rank * Config::kOwnColumns;
             const int first = t.split * s.steps_per_split, last = min(s.k_steps, first + s.steps_per_split);
             const int row0 = t.row + (int)rank * kMatmulRows + quarter * 32;
             const auto place = epilogue.begin(t, s, row0, t.col + from, lane);
+            typename Epilogue::Ahead ahead;
+            epilogue.fetch(place, 0, lane, ahead);
             const auto finish = [&](const float (&v)[kSpan], int across) {
-                if (t.col + from + across < s.n || Epilogue::kWholeTiles) epilogue.piece(place, across, v, mine, lane);
+                if (t.col + from + across >= s.n && !Epilogue::kWholeTiles) return;
+                const typename Epilogue::Ahead now = ahead;
+                if (across + kSpan < kShare) epilogue.fetch(place, across + kSpan, lane, ahead);
+                epilogue.piece(place, across, v, now, mine, lane);
             };
             float kept[kKeep ? kShare : 1];
 #pragma unroll
@@ -449,7 +457,9 @@ struct StorePartial {
         const int piece = (row - t.row) / 32 + (col - t.col) / kPieceColumns * (tile_rows / 32);
         return {reinterpret_cast<float4 *>(out + tile * tile_rows * columns) + piece * (8 * kPieceColumns) + lane};
     }
-    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], uint8_t *, int) const {
+    using Ahead = NothingAhead;
+    __device__ __forceinline__ void fetch(const Place &, int, int, Ahead &) const {}
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], const Ahead &, uint8_t *, int) const {
         float4 *to = p.to + across / kPieceColumns * (tile_rows / 32) * (8 * kPieceColumns);
 #pragma unroll
         for (int c = 0; c < kPieceColumns; c += 4) to[c * 8] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
@@ -474,6 +484,9 @@ matmul_join_kernel(const float *__restrict__ partial, const MatmulShape s, const
         const float4 *from = reinterpret_cast<const float4 *>(partial + tile * ROWS * COLUMNS) +
                              (piece % kDown + piece / kDown * (kTake / kPieceColumns) * kDown) * (8 * kPieceColumns) + lane;
         const int64_t split = tiles * ROWS * COLUMNS / 4;
+        const auto place = epilogue.begin(t, s, row, col, lane);
+        typename Epilogue::Ahead ahead;
+        epilogue.fetch(place, 0, lane, ahead);
         float v[kTake] = {};
         for (int sp = 0; sp < s.splits; ++sp, from += split) {
 #pragma unroll
@@ -482,7 +495,7 @@ matmul_join_kernel(const float *__restrict__ partial, const MatmulShape s, const
                 v[c] += f.x; v[c + 1] += f.y; v[c + 2] += f.z; v[c + 3] += f.w;
             }
         }
-        epilogue.piece(epilogue.begin(t, s, row, col, lane), 0, v, s_stage[warp], lane);
+        epilogue.piece(place, 0, v, ahead, s_stage[warp], lane);
     }
 }
 #endif  // __CUDACC__

@@ -136,19 +136,33 @@ struct PairEpilogue {
         }
         __syncwarp();
     }
-    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], uint8_t *stage, int lane) const {
+    struct Ahead {
+        uint4 hi[4], lo[4];   // of `more`, as slot_unit's
+    };
+    __device__ __forceinline__ void fetch(const Place &p, int across, int lane, Ahead &a) const {
+        if (more == nullptr) return;
+        const int r = p.row + lane / 4, c = p.col + across + lane % 4 * 8;
+        const uint16_t *from = more + p.matrix + r * pitch + c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool there = r + 8 * i < p.m && c < p.n;
+            a.hi[i] = there ? *reinterpret_cast<const uint4 *>(from + 8 * i * pitch) : make_uint4(0, 0, 0, 0);
+            a.lo[i] = there ? *reinterpret_cast<const uint4 *>(from + 8 * i * pitch + plane) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], const Ahead &a, uint8_t *stage, int lane) const {
         const int col = p.col + across, below = p.row / kMatmulRows - col / kMatmulRows, row = p.row + lane;
         if (p.row >= p.m || (symmetric && below < 0)) return;
         const bool on_diagonal = p.row < col + kColumns && col < p.row + 32;
         uint32_t hi[16], lo[16];
+        float w[kColumns];
+#pragma unroll
+        for (int j = 0; j < kColumns; ++j) w[j] = v[j] * scale;
         if (more != nullptr) {
-            const int r = p.row + lane / 4, c = col + lane % 4 * 8;
-            const int64_t at = p.matrix + r * pitch + c;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool there = r + 8 * i < p.m && c < p.n;
-                *slot_unit(stage, lane, i) = there ? *reinterpret_cast<const uint4 *>(more + at + 8 * i * pitch) : make_uint4(0, 0, 0, 0);
-                *slot_unit(stage + kSlotBytes, lane, i) = there ? *reinterpret_cast<const uint4 *>(more + at + 8 * i * pitch + plane) : make_uint4(0, 0, 0, 0);
+                *slot_unit(stage, lane, i) = a.hi[i];
+                *slot_unit(stage + kSlotBytes, lane, i) = a.lo[i];
             }
             __syncwarp();
             uint4 h[4], l[4];
@@ -156,25 +170,20 @@ struct PairEpilogue {
             slot_read_row(stage + kSlotBytes, lane, l);
             __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                hi[4 * j] = h[j].x; hi[4 * j + 1] = h[j].y; hi[4 * j + 2] = h[j].z; hi[4 * j + 3] = h[j].w;
-                lo[4 * j] = l[j].x; lo[4 * j + 1] = l[j].y; lo[4 * j + 2] = l[j].z; lo[4 * j + 3] = l[j].w;
+            for (int j = 0; j < 16; ++j) {
+                const uint32_t x[4] = {h[j / 4].x, h[j / 4].y, h[j / 4].z, h[j / 4].w}, y[4] = {l[j / 4].x, l[j / 4].y, l[j / 4].z, l[j / 4].w};
+                const float2 up = __half22float2(*reinterpret_cast<const __half2 *>(&x[j % 4])), down = __half22float2(*reinterpret_cast<const __half2 *>(&y[j % 4]));
+                w[2 * j] += factor * (up.x + down.x);
+                w[2 * j + 1] += factor * (up.y + down.y);
             }
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                split_two(v[2 * j] * scale + factor * join_pair((uint16_t)hi[j], (uint16_t)lo[j]) + (diagonal != 0.f && row == col + 2 * j ? diagonal : 0.f),
-                          v[2 * j + 1] * scale + factor * join_pair((uint16_t)(hi[j] >> 16), (uint16_t)(lo[j] >> 16)) +
-                              (diagonal != 0.f && row == col + 2 * j + 1 ? diagonal : 0.f),
-                          hi[j], lo[j]);
-        } else if (diagonal != 0.f && on_diagonal) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                split_two(v[2 * j] * scale + (row == col + 2 * j ? diagonal : 0.f), v[2 * j + 1] * scale + (row == col + 2 * j + 1 ? diagonal : 0.f), hi[j],
-                          lo[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) split_two(v[2 * j] * scale, v[2 * j + 1] * scale, hi[j], lo[j]);
         }
+        if (on_diagonal && diagonal != 0.f) {
+#pragma unroll
+            for (int j = 0; j < kColumns; ++j)
+                if (row == col + j) w[j] += diagonal;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) split_two(w[2 * j], w[2 * j + 1], hi[j], lo[j]);
         slot_row(stage, lane, hi);
         slot_row(stage + kSlotBytes, lane, lo);
         __syncwarp();
@@ -189,8 +198,10 @@ struct PairEpilogue {
             store(stage, lane, p, out, shifted, col, p.row, p.n, p.m);
         } else if (shifted != nullptr && on_diagonal) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                split_two(v[2 * j] * scale + (row == col + 2 * j ? shift : 0.f), v[2 * j + 1] * scale + (row == col + 2 * j + 1 ? shift : 0.f), hi[j], lo[j]);
+            for (int j = 0; j < kColumns; ++j)
+                if (row == col + j) w[j] += shift;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) split_two(w[2 * j], w[2 * j + 1], hi[j], lo[j]);
             slot_row(stage, lane, hi);
             slot_row(stage + kSlotBytes, lane, lo);
             __syncwarp();
@@ -220,24 +231,35 @@ struct OrthogonalEpilogue {
         const int64_t at = r * cols + c;
         return {r, c, s.m, s.n, out == nullptr ? at : at + t.matrix * s.m * cols, 2 * t.matrix * plane, out == nullptr ? all.weight[t.matrix] : nullptr};
     }
-    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], uint8_t *stage, int lane) const {
-        float q[4][4], w[4][4];
+    struct Ahead {
+        ushort4 hi[4], lo[4];   // of `more`
+        float w[4][4];          // of the weights
+    };
+    __device__ __forceinline__ void fetch(const Place &p, int across, int, Ahead &a) const {
+        const int left = p.n - p.col - across;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (p.row + 8 * i >= p.m || left <= 0) continue;
+            if (p.weight != nullptr) load4(p.weight, p.at + across + 8 * i * cols, kFloat32, left < 4 ? left : 4, a.w[i]);
+            if (more != nullptr) {
+                const uint16_t *from = more + p.matrix + (p.row + 8 * i) * pitch + p.col + across;
+                a.hi[i] = *reinterpret_cast<const ushort4 *>(from);
+                a.lo[i] = *reinterpret_cast<const ushort4 *>(from + plane);
+            }
+        }
+    }
+    __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], const Ahead &a, uint8_t *stage, int lane) const {
+        float q[4][4];
         piece_quads(stage, lane, v, q);
         const int left = p.n - p.col - across;
         if (left <= 0) return;
-        if (p.weight != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (p.row + 8 * i < p.m) load4(p.weight, p.at + across + 8 * i * cols, kFloat32, left < 4 ? left : 4, w[i]);
-        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (p.row + 8 * i >= p.m) continue;
 #pragma unroll
             for (int j = 0; j < 4; ++j) q[i][j] *= scale;
             if (more != nullptr) {
-                const uint16_t *from = more + p.matrix + (p.row + 8 * i) * pitch + p.col + across;
-                const ushort4 hi = *reinterpret_cast<const ushort4 *>(from), lo = *reinterpret_cast<const ushort4 *>(from + plane);
+                const ushort4 hi = a.hi[i], lo = a.lo[i];
                 q[i][0] += factor * join_pair(hi.x, lo.x);
                 q[i][1] += factor * join_pair(hi.y, lo.y);
                 q[i][2] += factor * join_pair(hi.z, lo.z);
@@ -245,7 +267,7 @@ struct OrthogonalEpilogue {
             }
             if (p.weight != nullptr) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) q[i][j] = w[i][j] * decay - rate * q[i][j];
+                for (int j = 0; j < 4; ++j) q[i][j] = a.w[i][j] * decay - rate * q[i][j];
                 store4(p.weight, p.at + across + 8 * i * cols, kFloat32, left < 4 ? left : 4, q[i]);
             } else {
                 store4(out, p.at + across + 8 * i * cols, all.type, left < 4 ? left : 4, q[i]);
