@@ -101,15 +101,14 @@ normalise_kernel(const Matrices all, int64_t rows, int64_t cols, const double *_
 }
 
 // Results of the iteration as pairs: v = scale * sum (+ factor * the pair in `more`) (+ diagonal on the diagonal).  Of a symmetric result
-// the blocks of 128 x 128 below the diagonal are stored on both sides, those above it not looked at.  `shifted`: a second result,
-// v + shift on the diagonal and v elsewhere.
+// the blocks of 128 x 128 below the diagonal are stored on both sides, those above it not looked at.
 struct PairEpilogue {
     static constexpr bool kWholeTiles = false;
     static constexpr int kColumns = 32;
-    uint16_t *out, *shifted;   // null: no second result
+    uint16_t *out;
     const uint16_t *more;      // null: none
-    int64_t pitch, plane;      // of all three; rows are padded to whole units, whose last values are written too and read by nothing
-    float scale, factor, diagonal, shift;
+    int64_t pitch, plane;      // of both; rows are padded to whole units, whose last values are written too and read by nothing
+    float scale, factor, diagonal;
     bool symmetric;
     struct Place {
         int row, col, m, n;    // of the warp's first value
@@ -118,21 +117,21 @@ struct PairEpilogue {
     __device__ __forceinline__ Place begin(const Tile &t, const MatmulShape &s, int row, int col, int) const {
         return {row, col, s.m, s.n, 2 * t.matrix * plane};
     }
-    // The slots' rows -- high and low halves -- to rows row .. of the result(s), columns col .., of which those below `rows`, `cols` are there.
-    __device__ __forceinline__ void store(uint8_t *stage, int lane, const Place &p, uint16_t *to, uint16_t *as_well, int row, int col, int rows,
-                                          int cols) const {
+    // The slots' rows -- high and low halves -- to rows row .. of the result, columns col .., of which those below `rows`, `cols` are there.
+    __device__ __forceinline__ void store(uint8_t *stage, int lane, const Place &p, int row, int col, int rows, int cols) const {
         const int r = row + lane / 4, c = col + lane % 4 * 8;
-        const int64_t at = p.matrix + r * pitch + c;
+        uint16_t *to = out + p.matrix + r * pitch + c;
+        uint4 hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            hi[i] = *slot_unit(stage, lane, i);
+            lo[i] = *slot_unit(stage + kSlotBytes, lane, i);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (r + 8 * i >= rows || c >= cols) continue;
-            const uint4 hi = *slot_unit(stage, lane, i), lo = *slot_unit(stage + kSlotBytes, lane, i);
-            *reinterpret_cast<uint4 *>(to + at + 8 * i * pitch) = hi;
-            *reinterpret_cast<uint4 *>(to + at + 8 * i * pitch + plane) = lo;
-            if (as_well != nullptr) {
-                *reinterpret_cast<uint4 *>(as_well + at + 8 * i * pitch) = hi;
-                *reinterpret_cast<uint4 *>(as_well + at + 8 * i * pitch + plane) = lo;
-            }
+            *reinterpret_cast<uint4 *>(to + 8 * i * pitch) = hi[i];
+            *reinterpret_cast<uint4 *>(to + 8 * i * pitch + plane) = lo[i];
         }
         __syncwarp();
     }
@@ -153,7 +152,6 @@ struct PairEpilogue {
     __device__ __forceinline__ void piece(const Place &p, int across, const float (&v)[kColumns], const Ahead &a, uint8_t *stage, int lane) const {
         const int col = p.col + across, below = p.row / kMatmulRows - col / kMatmulRows, row = p.row + lane;
         if (p.row >= p.m || (symmetric && below < 0)) return;
-        const bool on_diagonal = p.row < col + kColumns && col < p.row + 32;
         uint32_t hi[16], lo[16];
         float w[kColumns];
 #pragma unroll
@@ -177,7 +175,7 @@ struct PairEpilogue {
                 w[2 * j + 1] += factor * (up.y + down.y);
             }
         }
-        if (on_diagonal && diagonal != 0.f) {
+        if (diagonal != 0.f && p.row < col + kColumns && col < p.row + 32) {
 #pragma unroll
             for (int j = 0; j < kColumns; ++j)
                 if (row == col + j) w[j] += diagonal;
@@ -187,7 +185,7 @@ struct PairEpilogue {
         slot_row(stage, lane, hi);
         slot_row(stage + kSlotBytes, lane, lo);
         __syncwarp();
-        store(stage, lane, p, out, on_diagonal ? nullptr : shifted, p.row, col, p.m, p.n);
+        store(stage, lane, p, p.row, col, p.m, p.n);
         if (symmetric && below > 0) {   // columns as rows
 #pragma unroll
             for (int j = 0; j < kColumns; ++j) {
@@ -195,17 +193,7 @@ struct PairEpilogue {
                 slot_column(stage + kSlotBytes, lane, j, (uint16_t)(lo[j / 2] >> (j % 2 * 16)));
             }
             __syncwarp();
-            store(stage, lane, p, out, shifted, col, p.row, p.n, p.m);
-        } else if (shifted != nullptr && on_diagonal) {
-#pragma unroll
-            for (int j = 0; j < kColumns; ++j)
-                if (row == col + j) w[j] += shift;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) split_two(w[2 * j], w[2 * j + 1], hi[j], lo[j]);
-            slot_row(stage, lane, hi);
-            slot_row(stage + kSlotBytes, lane, lo);
-            __syncwarp();
-            store(stage, lane, p, shifted, nullptr, p.row, col, p.m, p.n);
+            store(stage, lane, p, col, p.row, p.n, p.m);
         }
     }
 };
@@ -288,7 +276,7 @@ struct OrthogonalLayout {
     int parts;
     MatmulPlan gram, square, product;
     int64_t x_bytes, s_bytes, norm_bytes, partial_bytes;
-    int64_t total() const { return 2 * x_bytes + 3 * s_bytes + norm_bytes + partial_bytes; }
+    int64_t total() const { return 2 * x_bytes + 2 * s_bytes + norm_bytes + partial_bytes; }
 };
 
 static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t cols, bool light, int sms) {
@@ -313,7 +301,8 @@ static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t c
 }
 
 // steps times: S = X^T X (X X^T where X is wide), M = b S + c S^2, X = a X + X M (M X).  `last` takes the last product.
-// b S + c S^2 is one product, of S with S + b / c I, which the first product stores beside S.
+// b S is added up in the epilogue of c S^2, which reads S beside its products; S stored a second time with b / c on its diagonal, so that
+// one product gave both, costs more in stores than it saves: 4 x 1024 x 1024 bf16 347 us for 304.
 //
 // Results of 22 bits (fp32, fp16): every product is one of pairs, and a X comes out of the product too, as the diagonal of M, since
 // the pair of a X would have to be read again.  bf16 results have 8 bits, and the steps need no more than this: S from the first planes
@@ -332,8 +321,7 @@ static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64
         return p;
     };
     uint16_t *x = reinterpret_cast<uint16_t *>(take(l.x_bytes)), *next = reinterpret_cast<uint16_t *>(take(l.x_bytes));
-    uint16_t *gram = reinterpret_cast<uint16_t *>(take(l.s_bytes)), *shifted = reinterpret_cast<uint16_t *>(take(l.s_bytes)),
-             *poly = reinterpret_cast<uint16_t *>(take(l.s_bytes));
+    uint16_t *gram = reinterpret_cast<uint16_t *>(take(l.s_bytes)), *poly = reinterpret_cast<uint16_t *>(take(l.s_bytes));
     double *norms = reinterpret_cast<double *>(take(l.norm_bytes));
     float *partial = reinterpret_cast<float *>(at);
     int status;
@@ -356,29 +344,23 @@ static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64
         p.k = l.tall ? rows : cols;
         p.symmetric = true;
         p.planes = light ? 1 : 2;
-        // b S + c S^2 = c S (S + b / c I); where b / c is too large for a pair, b S is added up in the epilogue
         PairEpilogue e = {};
         e.pitch = l.s_pitch;
         e.plane = l.s_plane;
         e.scale = once;
         e.symmetric = true;
-        const bool in_one = fabsf(b) <= 8.f * fabsf(c) && c != 0.f;
         e.out = gram;
-        e.shifted = in_one ? shifted : nullptr;
-        e.shift = in_one ? b / c * kPairScale : 0.f;
         if (c == 0.f) {   // the cubic iteration: M comes straight out of this product
             e.scale = b * once;
             e.diagonal = light ? 0.f : a * kPairScale;
         }
         if ((status = launch_planes(p, l.gram, e, partial, sms, st, what)) != DL_OK) return status;
         if (c != 0.f) {
-            p.a = {gram, l.s_pitch, l.s_plane, false};
-            p.b = {in_one ? shifted : gram, l.s_pitch, l.s_plane, false};
+            p.a = p.b = {gram, l.s_pitch, l.s_plane, false};
             p.k = l.side;
             p.planes = 2;
             e.out = poly;
-            e.shifted = nullptr;
-            e.more = in_one ? nullptr : gram;
+            e.more = gram;
             e.factor = b;
             e.scale = c * once;
             e.diagonal = light ? 0.f : a * kPairScale;
