@@ -26,6 +26,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "difflogic_b200.h"
@@ -460,6 +461,61 @@ PyObject *dense(PyObject *, PyObject *const *args, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
+// -- orthogonalised updates ---------------------------------------------------------------------------------------------------------
+// What ops.muon_step does once it has its numbers: checks, addresses, workspace and launch, 2 us for 15 tensors that take the interpreter 15.
+
+// The tensor of item i where it is one, float32, contiguous, two-dimensional and on `device`; else null.
+const Tensor *matrix_at(PyObject *list, Py_ssize_t i, const c10::Device &device) {
+    PyObject *o = PyList_GET_ITEM(list, i);
+    if (!ordinary(o)) return nullptr;
+    const Tensor &t = THPVariable_Unpack(o);
+    return plain(t, at::kFloat, 2, device) && t.is_contiguous() ? &t : nullptr;
+}
+
+// muon_step(weights, grads, momenta, lr, momentum, nesterov, weight_decay, steps, address of the coefficients, eps) -> True, or None
+PyObject *muon_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    if (count != 10) {
+        PyErr_SetString(PyExc_TypeError, "muon_step: ten arguments");
+        return nullptr;
+    }
+    for (int i = 0; i < 3; ++i)
+        if (!PyList_Check(args[i]) || PyList_GET_SIZE(args[i]) != PyList_GET_SIZE(args[0])) Py_RETURN_NONE;
+    const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+    if (n == 0 || !ordinary(PyList_GET_ITEM(args[0], 0))) Py_RETURN_NONE;
+    const c10::Device device = THPVariable_Unpack(PyList_GET_ITEM(args[0], 0)).device();
+    if (!device.is_cuda()) Py_RETURN_NONE;
+    std::vector<int64_t> table, written;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const Tensor *w = matrix_at(args[0], i, device), *g = matrix_at(args[1], i, device), *m = matrix_at(args[2], i, device);
+        if (w == nullptr || g == nullptr || m == nullptr || w->sizes() != g->sizes() || w->sizes() != m->sizes()) Py_RETURN_NONE;
+        if (w->numel() == 0) continue;
+        for (const Tensor *t : {w, g, m}) table.push_back((int64_t)t->data_ptr());
+        table.push_back(w->size(0));
+        table.push_back(w->size(1));
+        written.push_back((int64_t)w->data_ptr());
+        written.push_back((int64_t)m->data_ptr());
+    }
+    std::sort(written.begin(), written.end());
+    if (table.empty() || std::adjacent_find(written.begin(), written.end()) != written.end()) Py_RETURN_NONE;
+    const double lr = PyFloat_AsDouble(args[3]), momentum = PyFloat_AsDouble(args[4]), decay = PyFloat_AsDouble(args[6]), eps = PyFloat_AsDouble(args[9]);
+    const int nesterov = PyObject_IsTrue(args[5]);
+    const long steps = PyLong_AsLong(args[7]);
+    const float *coefficients = reinterpret_cast<const float *>(PyLong_AsUnsignedLongLong(args[8]));
+    if (PyErr_Occurred()) return nullptr;
+    if (observed()) Py_RETURN_NONE;
+    const Tensor &first = THPVariable_Unpack(PyList_GET_ITEM(args[0], 0));
+    {
+        const WithoutGil nogil;
+        const c10::cuda::CUDAGuard guard(device);
+        const int64_t matrices = (int64_t)table.size() / 5;
+        const Tensor work = bytes(dl_muon_workspace_bytes(table.data(), matrices), first);
+        check(dl_muon_step_f32(table.data(), matrices, lr, momentum, nesterov, decay, (int)steps, coefficients, eps, pointer(work), stream_of(first)));
+    }
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject *launches(PyObject *, PyObject *) { return PyLong_FromLongLong(g_launches.load()); }
 
 // connect(dict of difflogic.py)
@@ -476,6 +532,7 @@ PyObject *connect(PyObject *, PyObject *dict) {
 PyMethodDef kMethods[] = {{"layer", (PyCFunction)(void *)layer, METH_FASTCALL, nullptr},
                           {"group_sum", (PyCFunction)(void *)group_sum, METH_FASTCALL, nullptr},
                           {"dense", (PyCFunction)(void *)dense, METH_FASTCALL, nullptr},
+                          {"muon_step", (PyCFunction)(void *)muon_step, METH_FASTCALL, nullptr},
                           {"launches", launches, METH_NOARGS, nullptr},
                           {"connect", connect, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};

@@ -13,14 +13,17 @@
 
 namespace dl {
 
-constexpr int kGramThreads = 256, kGramWarps = kGramThreads / 32;
+constexpr int kGramThreads = 512, kGramWarps = kGramThreads / 32;   // of a block that takes the steps
+constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32;      // of one that adds S up
 constexpr int kGramSums = 3 * 64;        // three 8 x 8 blocks of S: even-even, even-odd and odd-odd columns
-constexpr int kGramParts = 64;           // at most, of a matrix
+constexpr int kGramParts = 128;          // at most, of a matrix
 
 struct GramBlocks {
     GramJob job;
-    int64_t strip;                       // rows of a block, a multiple of 32
-    int first[GramJob::kMost + 1];       // block of every matrix (batch: of the first one)
+    struct {
+        int64_t strip;                   // rows of a block
+        int first[GramJob::kMost + 1];   // block of every matrix (batch: of the first one)
+    } sums, rows;
     double scale_eps;
     int steps;
     float coefficients[3 * kMostSteps];
@@ -31,28 +34,29 @@ __device__ __forceinline__ void multiply64(double (&d)[2], double a, double b) {
 }
 
 struct GramPlace {
-    int matrix, part, parts, sums;       // entry; strip of it, of how many; its first sum
-    int64_t base, rows;                  // first value, rows
+    int matrix, sums, parts;             // entry; its first sum, and how many
+    int64_t base, first, last;           // first value; rows of the block
 };
-__device__ __forceinline__ GramPlace gram_place(const GramBlocks &g, int block) {
+template <class Cut>
+__device__ __forceinline__ GramPlace gram_place(const GramBlocks &g, const Cut &cut, int block) {
     GramPlace p;
+    p.matrix = 0;
+    p.base = 0;
+    p.sums = 0;
     if (g.job.count == 1) {
-        p.matrix = 0;
-        p.parts = g.first[1];
-        const int z = block / p.parts;
-        p.part = block - z * p.parts;
-        p.rows = g.job.matrix[0].rows;
-        p.base = z * p.rows * g.job.cols;
-        p.sums = z * p.parts;
+        const int z = block / cut.first[1];
+        block -= z * cut.first[1];
+        p.base = z * g.job.matrix[0].rows * g.job.cols;
+        p.sums = z * g.sums.first[1];
     } else {
-        p.matrix = 0;
-        while (block >= g.first[p.matrix + 1]) ++p.matrix;
-        p.parts = g.first[p.matrix + 1] - g.first[p.matrix];
-        p.part = block - g.first[p.matrix];
-        p.rows = g.job.matrix[p.matrix].rows;
-        p.base = 0;
-        p.sums = g.first[p.matrix];
+        while (block >= cut.first[p.matrix + 1]) ++p.matrix;
+        block -= cut.first[p.matrix];
+        p.sums = g.sums.first[p.matrix];
     }
+    p.parts = g.sums.first[p.matrix + 1] - g.sums.first[p.matrix];
+    const int64_t rows = g.job.matrix[p.matrix].rows;
+    p.first = block * cut.strip;
+    p.last = p.first + cut.strip < rows ? p.first + cut.strip : rows;
     return p;
 }
 
@@ -74,19 +78,19 @@ __device__ __forceinline__ void load_row(const void *p, int64_t row_at, int col,
     }
 }
 
-__global__ void __launch_bounds__(kGramThreads)
+__global__ void __launch_bounds__(kSumThreads, 3)
 gram_sums_kernel(const __grid_constant__ GramBlocks g, double *__restrict__ sums) {
-    __shared__ double s_sum[kGramWarps][kGramSums];
+    __shared__ double s_sum[kSumWarps][kGramSums];
     grid_dependency_wait();
     grid_dependents_launch();
-    const GramPlace p = gram_place(g, blockIdx.x);
+    const GramPlace p = gram_place(g, g.sums, blockIdx.x);
     const GramMatrix &m = g.job.matrix[p.matrix];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, cols = g.job.cols, type = g.job.type, col = lane / 4 * 2;
-    const int64_t first = p.part * g.strip, last = first + g.strip < p.rows ? first + g.strip : p.rows;
+    const int64_t first = p.first, last = p.last;
     // lane l: row l % 4, columns 2 (l / 4) and the one after it, which makes its value both the A and the B of a block of S
     double even[2] = {0, 0}, mixed[2] = {0, 0}, odd[2] = {0, 0};
     constexpr int kAhead = 8;   // rows of four at a time
-    for (int64_t row = first + warp * 4 * kAhead; row < last; row += kGramWarps * 4 * kAhead) {
+    for (int64_t row = first + warp * 4 * kAhead; row < last; row += kSumWarps * 4 * kAhead) {
         float v[kAhead][2], o[kAhead][2];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
@@ -133,7 +137,7 @@ gram_sums_kernel(const __grid_constant__ GramBlocks g, double *__restrict__ sums
     if (threadIdx.x < kGramSums) {
         double r = 0;
 #pragma unroll
-        for (int w = 0; w < kGramWarps; ++w) r += s_sum[w][threadIdx.x];
+        for (int w = 0; w < kSumWarps; ++w) r += s_sum[w][threadIdx.x];
         sums[(int64_t)blockIdx.x * kGramSums + threadIdx.x] = r;
     }
 }
@@ -141,12 +145,18 @@ gram_sums_kernel(const __grid_constant__ GramBlocks g, double *__restrict__ sums
 constexpr int kSquarePitch = 18;   // doubles of a row of a 16 x 16 matrix
 using Square = double[kGramColumns][kSquarePitch];
 
-// One 8 x 8 block of A B.
+// One 8 x 8 block of A B, in two chains: an instruction takes 40 clocks until its sum can be added to.
 __device__ __forceinline__ void square_block(const Square &a, const Square &b, int block, int lane, double (&d)[2]) {
     const int down = block / 2 * 8, across = block % 2 * 8;
+    double e[2] = {0, 0};
     d[0] = d[1] = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) multiply64(d, a[down + lane / 4][4 * k + lane % 4], b[4 * k + lane % 4][across + lane / 4]);
+    for (int k = 0; k < 2; ++k) {
+        multiply64(d, a[down + lane / 4][4 * k + lane % 4], b[4 * k + lane % 4][across + lane / 4]);
+        multiply64(e, a[down + lane / 4][4 * k + 8 + lane % 4], b[4 * k + 8 + lane % 4][across + lane / 4]);
+    }
+    d[0] += e[0];
+    d[1] += e[1];
 }
 
 struct GramShared {
@@ -160,14 +170,22 @@ __device__ __forceinline__ const Square &take_steps(GramShared &s, const GramBlo
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     {
         double r[kGramSums / 32] = {};
-        for (int i = warp; i < parts; i += kGramWarps) {
+        constexpr int kMost = kGramParts / kGramWarps;   // of a warp, all asked for at a time
+        double2 d[kMost][kGramSums / 64];
+#pragma unroll
+        for (int i = 0; i < kMost; ++i)
 #pragma unroll
             for (int j = 0; j < kGramSums / 64; ++j) {
-                const double2 d = *reinterpret_cast<const double2 *>(sums + (int64_t)i * kGramSums + j * 64 + lane * 2);
-                r[2 * j] += d.x;
-                r[2 * j + 1] += d.y;
+                const int part = warp + i * kGramWarps;
+                d[i][j] = part < parts ? *reinterpret_cast<const double2 *>(sums + (int64_t)part * kGramSums + j * 64 + lane * 2) : make_double2(0, 0);
             }
-        }
+#pragma unroll
+        for (int i = 0; i < kMost; ++i)
+#pragma unroll
+            for (int j = 0; j < kGramSums / 64; ++j) {
+                r[2 * j] += d[i][j].x;
+                r[2 * j + 1] += d[i][j].y;
+            }
 #pragma unroll
         for (int j = 0; j < kGramSums / 64; ++j) {
             s.part[warp][j * 64 + lane * 2] = r[2 * j];
@@ -185,11 +203,14 @@ __device__ __forceinline__ const Square &take_steps(GramShared &s, const GramBlo
         if (kind == 2) s.s[2 * i + 1][2 * j + 1] = r;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        double trace = 0;
-        for (int i = 0; i < kGramColumns; ++i) trace += s.s[i][i];
-        const double norm = sqrt(trace);
-        s.scale = norm > g.scale_eps || norm != norm ? 1 / norm : 1 / g.scale_eps;
+    if (warp == 0) {
+        double trace = lane < kGramColumns ? s.s[lane][lane] : 0;
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) trace += __shfl_xor_sync(0xffffffffu, trace, off);
+        if (lane == 0) {
+            const double norm = sqrt(trace);
+            s.scale = norm > g.scale_eps || norm != norm ? 1 / norm : 1 / g.scale_eps;
+        }
     }
     __syncthreads();
     const double scale = s.scale;
@@ -215,7 +236,7 @@ __device__ __forceinline__ const Square &take_steps(GramShared &s, const GramBlo
             s.product[(i + 1) % 2][row][col + 1] = d[1];
         }
         if (i + 1 < g.steps) {
-            if (warp >= 4) {
+            if (warp >= 4 && warp < 8) {
                 square_block(s.s, s.m, block, lane, d);
                 s.moved[row][col] = d[0];
                 s.moved[row][col + 1] = d[1];
@@ -232,48 +253,53 @@ __device__ __forceinline__ const Square &take_steps(GramShared &s, const GramBlo
     return s.product[g.steps % 2];
 }
 
-__global__ void __launch_bounds__(kGramThreads)
+__global__ void __launch_bounds__(kGramThreads, 1)
 gram_apply_kernel(const __grid_constant__ GramBlocks g, const double *__restrict__ sums) {
     __shared__ GramShared s;
     grid_dependency_wait();
     grid_dependents_launch();
-    const GramPlace p = gram_place(g, blockIdx.x);
+    const GramPlace p = gram_place(g, g.rows, blockIdx.x);
     const GramMatrix &m = g.job.matrix[p.matrix];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, cols = g.job.cols, type = g.job.type;
-    const int64_t first = p.part * g.strip, last = first + g.strip < p.rows ? first + g.strip : p.rows;
+    const int64_t first = p.first, last = p.last;
     // a warp takes 8 rows at a time: lane l reads columns 4 (l % 4) .. + 3 of row l / 4 (which order the columns are summed in is
     // free) and has columns 2 (l % 4), + 1, + 8 and + 9 of the result
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 2;
     const int from = lane % 4 * 4, to = lane % 4 * 2;
-    float v[kAhead][4], o[kAhead][4], w[kAhead][2][2];
-    const auto fetch = [&](int64_t row) {
+    struct Rows {
+        float v[kAhead][4], o[kAhead][4], w[kAhead][2][2];
+    };
+    const auto fetch = [&](Rows &b, int64_t row) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int64_t r = row + i * 8 + lane / 4, at = p.base + r * cols;
-            load_row<4>(m.g, at, from, cols, type, r < last, v[i]);
-            if (m.momentum != nullptr) load_row<4>(m.momentum, at, from, cols, kFloat32, r < last, o[i]);
+            load_row<4>(m.g, at, from, cols, type, r < last, b.v[i]);
+            if (m.momentum != nullptr) load_row<4>(m.momentum, at, from, cols, kFloat32, r < last, b.o[i]);
             if (g.job.update) {
-                load_row<2>(m.out, at, to, cols, kFloat32, r < last, w[i][0]);
-                load_row<2>(m.out, at, to + 8, cols, kFloat32, r < last, w[i][1]);
+                load_row<2>(m.out, at, to, cols, kFloat32, r < last, b.w[i][0]);
+                load_row<2>(m.out, at, to + 8, cols, kFloat32, r < last, b.w[i][1]);
             }
         }
     };
+    constexpr int kStride = kGramWarps * 8 * kAhead;
+    Rows one, two;   // while one is worked on, the other is on its way
     int64_t row = first + warp * 8 * kAhead;
-    fetch(row);
+    fetch(one, row);
+    fetch(two, row + kStride);
     const Square &product = take_steps(s, g, sums + (int64_t)p.sums * kGramSums, p.parts);
     double factor[2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int k = 0; k < 4; ++k) factor[h][k] = product[from + k][8 * h + lane / 4];
-    for (; row < last; row += kGramWarps * 8 * kAhead) {
+    const auto apply = [&](const Rows &b, int64_t row) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int64_t r = row + i * 8 + lane / 4, at = p.base + r * cols;
             double d[2][2] = {};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const double x = m.momentum != nullptr ? update_of(o[i][k], v[i][k], g.job.nesterov) : v[i][k];
+                const double x = m.momentum != nullptr ? update_of(b.o[i][k], b.v[i][k], g.job.nesterov) : b.v[i][k];
                 multiply64(d[0], x, factor[0][k]);
                 multiply64(d[1], x, factor[1][k]);
             }
@@ -282,7 +308,7 @@ gram_apply_kernel(const __grid_constant__ GramBlocks g, const double *__restrict
             for (int h = 0; h < 2; ++h) {
                 float out[2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) out[j] = g.job.update ? w[i][h][j] * g.job.decay - m.rate * (float)d[h][j] : (float)d[h][j];
+                for (int j = 0; j < 2; ++j) out[j] = g.job.update ? b.w[i][h][j] * g.job.decay - m.rate * (float)d[h][j] : (float)d[h][j];
                 const int col = to + 8 * h;
                 if (type == kFloat32) {
                     float *at_out = reinterpret_cast<float *>(m.out) + at + col;
@@ -299,21 +325,26 @@ gram_apply_kernel(const __grid_constant__ GramBlocks g, const double *__restrict
                 }
             }
         }
-        const int64_t next = row + kGramWarps * 8 * kAhead;
-        if (next < last) fetch(next);
+        __syncwarp();
+    };
+    for (; row < last; row += 2 * kStride) {
+        apply(one, row);
+        if (row + 2 * kStride < last) fetch(one, row + 2 * kStride);
+        if (row + kStride >= last) break;
+        apply(two, row + kStride);
+        if (row + 3 * kStride < last) fetch(two, row + 3 * kStride);
     }
 }
 
-// Two blocks to an SM over all matrices, at most kGramParts to a matrix; a multiple of 32 rows each.
-static int64_t gram_strip(int64_t rows, int64_t most_rows, int sms) {
-    int64_t strip = ceil_div(rows, 2 * sms);
-    if (strip < ceil_div(most_rows, kGramParts)) strip = ceil_div(most_rows, kGramParts);
-    return ceil_div(strip < 1 ? 1 : strip, 32) * 32;
+// Sums: three blocks to an SM over all matrices, 256 rows at a time, at most kGramParts to a matrix.
+static int64_t sum_strip(int64_t rows, int64_t most_rows, int sms) {
+    const int64_t each = ceil_div(rows, 3 * sms), least = ceil_div(most_rows, kGramParts);
+    return ceil_div(each > least ? each : least, 256) * 256;
 }
 
 int64_t gram_workspace_bytes(int64_t matrices, int64_t rows, int sms) {
-    // a strip is at least rows / (2 sms) of all rows: that many whole ones, and one more for each matrix
-    return (2 * sms + matrices) * (int64_t)kGramSums * (int64_t)sizeof(double);
+    // a strip has at least rows / (3 sms) of all rows: that many whole ones, and one more for each matrix
+    return (3 * sms + matrices) * (int64_t)kGramSums * (int64_t)sizeof(double);
 }
 
 int launch_gram_steps(const GramJob &job, int steps, const float *coefficients, double eps, double *workspace, int sms, cudaStream_t st,
@@ -329,13 +360,16 @@ int launch_gram_steps(const GramJob &job, int steps, const float *coefficients, 
         if (job.matrix[i].rows > most) most = job.matrix[i].rows;
     }
     const int64_t batch = job.count == 1 ? job.batch : 1;
-    g.strip = gram_strip(rows * batch, most, sms);
-    for (int i = 0; i < job.count; ++i) g.first[i + 1] = g.first[i] + (int)ceil_div(job.matrix[i].rows, g.strip);
-    const int64_t blocks = g.first[job.count] * batch;
-    launch_dependent(true, gram_sums_kernel, dim3((unsigned)blocks), dim3(kGramThreads), 0, st, g, workspace);
+    g.sums.strip = sum_strip(rows * batch, most, sms);
+    g.rows.strip = ceil_div(ceil_div(rows * batch, sms), 32) * 32;   // a block to an SM, as each takes the steps
+    for (int i = 0; i < job.count; ++i) {
+        g.sums.first[i + 1] = g.sums.first[i] + (int)ceil_div(job.matrix[i].rows, g.sums.strip);
+        g.rows.first[i + 1] = g.rows.first[i] + (int)ceil_div(job.matrix[i].rows, g.rows.strip);
+    }
+    launch_dependent(true, gram_sums_kernel, dim3((unsigned)(g.sums.first[job.count] * batch)), dim3(kSumThreads), 0, st, g, workspace);
     int status = launch_status(what);
     if (status != DL_OK) return status;
-    launch_dependent(true, gram_apply_kernel, dim3((unsigned)blocks), dim3(kGramThreads), 0, st, g, (const double *)workspace);
+    launch_dependent(true, gram_apply_kernel, dim3((unsigned)(g.rows.first[job.count] * batch)), dim3(kGramThreads), 0, st, g, (const double *)workspace);
     return launch_status(what);
 }
 

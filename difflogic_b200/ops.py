@@ -980,7 +980,7 @@ def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
         raise ValueError("orthogonalize: a matrix or a batch of them, got %d dimensions" % x.dim())
     if not 0 < eps < math.inf:
         raise ValueError("orthogonalize: eps must be positive, got %r" % (eps,))
-    table = _newton_schulz(_coefficients(coefficients), steps)
+    table = _newton_schulz(coefficients if coefficients is NEWTON_SCHULZ else _coefficients(coefficients), steps)
     x = x.detach().contiguous()
     out = torch.empty_like(x)
     rows, cols = x.shape[-2:]
@@ -1004,11 +1004,17 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     if not len(weights) == len(grads) == len(momenta):
         raise ValueError("muon_step: %d weights, %d gradients, %d momenta" % (len(weights), len(grads), len(momenta)))
-    table = _newton_schulz(_coefficients(coefficients), steps)
+    table = _newton_schulz(coefficients if coefficients is NEWTON_SCHULZ else _coefficients(coefficients), steps)
     if not (0 <= momentum < 1 and lr >= 0 and weight_decay >= 0 and 0 < eps < math.inf):
         raise ValueError("muon_step: needs 0 <= momentum < 1, lr >= 0, weight_decay >= 0 and eps > 0, got %r, %r, %r, %r" % (momentum, lr, weight_decay, eps))
     if not weights:
         return
+    from .optim import count_update
+    if weights[0].is_cuda and N.nodes().muon_step(weights, grads, momenta, float(lr), float(momentum), nesterov, float(weight_decay), steps,
+                                                  ctypes.addressof(table), float(eps)):
+        count_update(weights)
+        return
+    # what is not of the ordinary form
     entries, written = [], set()
     device = weights[0].device
     for w, g, m in zip(weights, grads, momenta):
@@ -1033,5 +1039,4 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
     with N.on_device(weights[0]):
         work = torch.empty(lib.dl_muon_workspace_bytes(entries, count), dtype=torch.uint8, device=device)
         N.check(lib.dl_muon_step_f32(entries, count, lr, momentum, nesterov, weight_decay, steps, table, eps, work.data_ptr(), N.stream_of(weights[0])))
-    from .optim import count_update
     count_update(weights)
