@@ -60,24 +60,37 @@ __device__ __forceinline__ GramPlace gram_place(const GramBlocks &g, const Cut &
     return p;
 }
 
-// N neighbouring values of a row of `cols`; those behind its end are zero.
-template <int N>
-__device__ __forceinline__ void load_row(const void *p, int64_t row_at, int col, int cols, int type, bool there, float (&v)[N]) {
-    if (there && type == kFloat32 && col + N <= cols && cols % N == 0 && (reinterpret_cast<uintptr_t>(p) & (4 * N - 1)) == 0) {
-        const float *at = reinterpret_cast<const float *>(p) + row_at + col;
-        if constexpr (N == 4) {
-            const float4 f = *reinterpret_cast<const float4 *>(at);
-            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-        } else {
-            const float2 f = *reinterpret_cast<const float2 *>(at);
-            v[0] = f.x; v[1] = f.y;
-        }
+// N neighbouring values of row `row` of `cols`; a row that is not there reads as the last one.  WHOLE: rows of 16 fp32 values on 16-byte
+// units, else values one by one, zeros behind the end of a row.
+template <bool WHOLE, int N>
+__device__ __forceinline__ void load_row(const void *p, int64_t base, int64_t row, int64_t last, int col, int cols, int type, float (&v)[N]) {
+    const int64_t at = base + (row < last ? row : last - 1) * (WHOLE ? kGramColumns : cols) + col;
+    if constexpr (WHOLE && N == 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + at);
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else if constexpr (WHOLE) {
+        const float2 f = *reinterpret_cast<const float2 *>(reinterpret_cast<const float *>(p) + at);
+        v[0] = f.x; v[1] = f.y;
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = there && col + j < cols ? load_as_float(p, row_at + col + j, type) : 0.f;
+        for (int j = 0; j < N; ++j) v[j] = col + j < cols ? load_as_float(p, at + j, type) : 0.f;
+    }
+}
+template <bool WHOLE>
+__device__ __forceinline__ void store_two(void *p, int64_t at, int col, int cols, int type, float a, float b) {
+    if constexpr (WHOLE) {
+        *reinterpret_cast<float2 *>(reinterpret_cast<float *>(p) + at) = make_float2(a, b);
+    } else if (type == kFloat32) {
+        if (col < cols) reinterpret_cast<float *>(p)[at] = a;
+        if (col + 1 < cols) reinterpret_cast<float *>(p)[at + 1] = b;
+    } else {
+        if (col < cols) reinterpret_cast<uint16_t *>(p)[at] = to_16bit(a, type);
+        if (col + 1 < cols) reinterpret_cast<uint16_t *>(p)[at + 1] = to_16bit(b, type);
     }
 }
 
+// UPDATE: of momenta, of weights.
+template <bool WHOLE, bool UPDATE>
 __global__ void __launch_bounds__(kSumThreads, 3)
 gram_sums_kernel(const __grid_constant__ GramBlocks g, double *__restrict__ sums) {
     __shared__ double s_sum[kSumWarps][kGramSums];
@@ -95,32 +108,22 @@ gram_sums_kernel(const __grid_constant__ GramBlocks g, double *__restrict__ sums
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int64_t r = row + i * 4 + lane % 4;
-            load_row<2>(m.g, p.base + r * cols, col, cols, type, r < last, v[i]);
-            if (m.momentum != nullptr) load_row<2>(m.momentum, p.base + r * cols, col, cols, kFloat32, r < last, o[i]);
+            load_row<WHOLE>(m.g, p.base, r, last, col, cols, type, v[i]);
+            if (UPDATE) load_row<WHOLE>(m.momentum, p.base, r, last, col, cols, kFloat32, o[i]);
         }
-        if (m.momentum != nullptr) {
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int64_t r = row + i * 4 + lane % 4;
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t r = row + i * 4 + lane % 4;
+            const bool there = r < last;
+            if (UPDATE) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     o[i][j] = new_momentum(o[i][j], v[i][j], g.job.keep);
                     v[i][j] = update_of(o[i][j], v[i][j], g.job.nesterov);
                 }
-                float *to = m.momentum + p.base + r * cols + col;
-                if (r < last) {
-                    if (cols % 2 == 0 && col < cols && (reinterpret_cast<uintptr_t>(to) & 7) == 0) {
-                        *reinterpret_cast<float2 *>(to) = make_float2(o[i][0], o[i][1]);
-                    } else {
-                        if (col < cols) to[0] = o[i][0];
-                        if (col + 1 < cols) to[1] = o[i][1];
-                    }
-                }
+                if (there) store_two<WHOLE>(m.momentum, p.base + r * (WHOLE ? kGramColumns : cols) + col, col, cols, kFloat32, o[i][0], o[i][1]);
             }
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const double a = v[i][0], b = v[i][1];
+            const double a = there ? v[i][0] : 0.f, b = there ? v[i][1] : 0.f;
             multiply64(even, a, a);
             multiply64(mixed, a, b);
             multiply64(odd, b, b);
@@ -253,6 +256,7 @@ __device__ __forceinline__ const Square &take_steps(GramShared &s, const GramBlo
     return s.product[g.steps % 2];
 }
 
+template <bool WHOLE, bool UPDATE>
 __global__ void __launch_bounds__(kGramThreads, 1)
 gram_apply_kernel(const __grid_constant__ GramBlocks g, const double *__restrict__ sums) {
     __shared__ GramShared s;
@@ -272,12 +276,12 @@ gram_apply_kernel(const __grid_constant__ GramBlocks g, const double *__restrict
     const auto fetch = [&](Rows &b, int64_t row) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int64_t r = row + i * 8 + lane / 4, at = p.base + r * cols;
-            load_row<4>(m.g, at, from, cols, type, r < last, b.v[i]);
-            if (m.momentum != nullptr) load_row<4>(m.momentum, at, from, cols, kFloat32, r < last, b.o[i]);
-            if (g.job.update) {
-                load_row<2>(m.out, at, to, cols, kFloat32, r < last, b.w[i][0]);
-                load_row<2>(m.out, at, to + 8, cols, kFloat32, r < last, b.w[i][1]);
+            const int64_t r = row + i * 8 + lane / 4;
+            load_row<WHOLE>(m.g, p.base, r, last, from, cols, type, b.v[i]);
+            if (UPDATE) {
+                load_row<WHOLE>(m.momentum, p.base, r, last, from, cols, kFloat32, b.o[i]);
+                load_row<WHOLE>(m.out, p.base, r, last, to, cols, kFloat32, b.w[i][0]);
+                load_row<WHOLE>(m.out, p.base, r, last, to + 8, cols, kFloat32, b.w[i][1]);
             }
         }
     };
@@ -295,11 +299,11 @@ gram_apply_kernel(const __grid_constant__ GramBlocks g, const double *__restrict
     const auto apply = [&](const Rows &b, int64_t row) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int64_t r = row + i * 8 + lane / 4, at = p.base + r * cols;
+            const int64_t r = row + i * 8 + lane / 4;
             double d[2][2] = {};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const double x = m.momentum != nullptr ? update_of(b.o[i][k], b.v[i][k], g.job.nesterov) : b.v[i][k];
+                const double x = UPDATE ? update_of(b.o[i][k], b.v[i][k], g.job.nesterov) : b.v[i][k];
                 multiply64(d[0], x, factor[0][k]);
                 multiply64(d[1], x, factor[1][k]);
             }
@@ -308,21 +312,9 @@ gram_apply_kernel(const __grid_constant__ GramBlocks g, const double *__restrict
             for (int h = 0; h < 2; ++h) {
                 float out[2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) out[j] = g.job.update ? b.w[i][h][j] * g.job.decay - m.rate * (float)d[h][j] : (float)d[h][j];
+                for (int j = 0; j < 2; ++j) out[j] = UPDATE ? b.w[i][h][j] * g.job.decay - m.rate * (float)d[h][j] : (float)d[h][j];
                 const int col = to + 8 * h;
-                if (type == kFloat32) {
-                    float *at_out = reinterpret_cast<float *>(m.out) + at + col;
-                    if (cols % 2 == 0 && col < cols && (reinterpret_cast<uintptr_t>(at_out) & 7) == 0) {
-                        *reinterpret_cast<float2 *>(at_out) = make_float2(out[0], out[1]);
-                        continue;
-                    }
-                    if (col < cols) at_out[0] = out[0];
-                    if (col + 1 < cols) at_out[1] = out[1];
-                } else {
-                    uint16_t *at_out = reinterpret_cast<uint16_t *>(m.out) + at + col;
-                    if (col < cols) at_out[0] = to_16bit(out[0], type);
-                    if (col + 1 < cols) at_out[1] = to_16bit(out[1], type);
-                }
+                store_two<WHOLE>(m.out, p.base + r * (WHOLE ? kGramColumns : cols) + col, col, cols, UPDATE ? kFloat32 : type, out[0], out[1]);
             }
         }
         __syncwarp();
@@ -361,15 +353,30 @@ int launch_gram_steps(const GramJob &job, int steps, const float *coefficients, 
     }
     const int64_t batch = job.count == 1 ? job.batch : 1;
     g.sums.strip = sum_strip(rows * batch, most, sms);
-    g.rows.strip = ceil_div(ceil_div(rows * batch, sms), 32) * 32;   // a block to an SM, as each takes the steps
+    // a block to an SM, as each takes the steps; not one more than there are, which would run alone
+    const auto blocks_of = [&](int64_t strip) {
+        int64_t n = 0;
+        for (int i = 0; i < job.count; ++i) n += ceil_div(job.matrix[i].rows, strip);
+        return n * batch;
+    };
+    g.rows.strip = ceil_div(ceil_div(rows * batch, sms), 32) * 32;
+    while (blocks_of(g.rows.strip) > sms && g.rows.strip < most) g.rows.strip += 32;
     for (int i = 0; i < job.count; ++i) {
         g.sums.first[i + 1] = g.sums.first[i] + (int)ceil_div(job.matrix[i].rows, g.sums.strip);
         g.rows.first[i + 1] = g.rows.first[i] + (int)ceil_div(job.matrix[i].rows, g.rows.strip);
     }
-    launch_dependent(true, gram_sums_kernel, dim3((unsigned)(g.sums.first[job.count] * batch)), dim3(kSumThreads), 0, st, g, workspace);
-    int status = launch_status(what);
-    if (status != DL_OK) return status;
-    launch_dependent(true, gram_apply_kernel, dim3((unsigned)(g.rows.first[job.count] * batch)), dim3(kGramThreads), 0, st, g, (const double *)workspace);
+    bool whole = job.cols == kGramColumns && job.type == kFloat32;
+    for (int i = 0; i < job.count; ++i)
+        whole = whole && aligned_to(job.matrix[i].g, 16) && aligned_to(job.matrix[i].momentum, 16) && aligned_to(job.matrix[i].out, 16);
+    const dim3 sums((unsigned)(g.sums.first[job.count] * batch)), blocks((unsigned)(g.rows.first[job.count] * batch));
+    const auto launch = [&](auto sums_kernel, auto apply_kernel) {
+        launch_dependent(true, sums_kernel, sums, dim3(kSumThreads), 0, st, g, workspace);
+        launch_dependent(true, apply_kernel, blocks, dim3(kGramThreads), 0, st, g, (const double *)workspace);
+    };
+    if (whole && job.update) launch(gram_sums_kernel<true, true>, gram_apply_kernel<true, true>);
+    else if (whole) launch(gram_sums_kernel<true, false>, gram_apply_kernel<true, false>);
+    else if (job.update) launch(gram_sums_kernel<false, true>, gram_apply_kernel<false, true>);
+    else launch(gram_sums_kernel<false, false>, gram_apply_kernel<false, false>);
     return launch_status(what);
 }
 
