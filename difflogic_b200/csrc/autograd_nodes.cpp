@@ -516,6 +516,37 @@ PyObject *muon_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
+// orthogonalize(x, steps, address of the coefficients, eps) -> the result, or None
+PyObject *orthogonalize(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    if (count != 4) {
+        PyErr_SetString(PyExc_TypeError, "orthogonalize: four arguments");
+        return nullptr;
+    }
+    if (!ordinary(args[0])) Py_RETURN_NONE;
+    const Tensor &x = THPVariable_Unpack(args[0]);
+    const at::ScalarType type = x.scalar_type();
+    if ((type != at::kFloat && type != at::kBFloat16 && type != at::kHalf) || x.dim() < 2 || x.numel() == 0 || !plain(x, type, x.dim(), x.device()) ||
+        !x.is_contiguous() || observed() || x._fw_grad(0).defined())
+        Py_RETURN_NONE;
+    const long steps = PyLong_AsLong(args[1]);
+    const float *coefficients = reinterpret_cast<const float *>(PyLong_AsUnsignedLongLong(args[2]));
+    const double eps = PyFloat_AsDouble(args[3]);
+    if (PyErr_Occurred()) return nullptr;
+    Tensor out;
+    {
+        const WithoutGil nogil;
+        const c10::cuda::CUDAGuard guard(x.device());
+        const at::NoGradGuard no_grad;
+        out = at::empty_like(x, x.options().requires_grad(false));
+        const int64_t rows = x.size(-2), cols = x.size(-1), batch = x.numel() / (rows * cols);
+        const Tensor work = bytes(dl_orthogonalize_workspace_bytes(batch, rows, cols, kind_of(type)), x);
+        check(dl_orthogonalize(x.data_ptr(), out.data_ptr(), batch, rows, cols, kind_of(type), (int)steps, coefficients, eps, pointer(work), stream_of(x)));
+    }
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject *launches(PyObject *, PyObject *) { return PyLong_FromLongLong(g_launches.load()); }
 
 // connect(dict of difflogic.py)
@@ -533,6 +564,7 @@ PyMethodDef kMethods[] = {{"layer", (PyCFunction)(void *)layer, METH_FASTCALL, n
                           {"group_sum", (PyCFunction)(void *)group_sum, METH_FASTCALL, nullptr},
                           {"dense", (PyCFunction)(void *)dense, METH_FASTCALL, nullptr},
                           {"muon_step", (PyCFunction)(void *)muon_step, METH_FASTCALL, nullptr},
+                          {"orthogonalize", (PyCFunction)(void *)orthogonalize, METH_FASTCALL, nullptr},
                           {"launches", launches, METH_NOARGS, nullptr},
                           {"connect", connect, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};

@@ -249,63 +249,111 @@ lay_out_kernel(const void *__restrict__ src, int64_t rows, int64_t cols, int64_t
 }
 
 // gz = gy * slope into planes (none where the gradient of y can be used as it is: dst null), and the sums of its columns (sum_rows: of
-// its rows) over a strip of rows.  A block takes 128 columns (32 lanes of 4) and a strip; 8 row groups.
+// its rows) over a strip of rows.  A block takes 32 lanes x 16 bytes of columns and a strip, 8 rows at a time, four of each warp on their
+// way.  WHOLE: rows lie and end on 16-byte units.
+template <class T>
+constexpr int kGradientColumns = 32 * 16 / (int)sizeof(T);
+
+template <class T, bool WHOLE>
 __global__ void __launch_bounds__(kThreads)
-pre_gradient_kernel(const void *__restrict__ gy, const void *__restrict__ slope, int64_t rows, int64_t cols, int type,
-                    uint16_t *__restrict__ dst, int64_t dst_pitch, int64_t plane, int64_t strip, float *__restrict__ partial, int sum_rows) {
-    __shared__ float s_sum[kThreads / 32][128];
+pre_gradient_kernel(const T *__restrict__ gy, const void *__restrict__ slope, int64_t rows, int64_t cols, uint16_t *__restrict__ dst,
+                    int64_t dst_pitch, int64_t plane, int64_t strip, float *__restrict__ partial, int sum_rows) {
+    using Slope = typename std::conditional<sizeof(T) == 4, float, __half>::type;
+    constexpr int kValues = 16 / sizeof(T), kAhead = 4, kGroups = kThreads / 32;
+    __shared__ float s_sum[kGroups][kGradientColumns<T>];
     grid_dependency_wait();
     grid_dependents_launch();
     const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
-    const int64_t col = (int64_t)blockIdx.x * 128 + lane * 4, first = (int64_t)blockIdx.y * strip, last = first + strip < rows ? first + strip : rows;
-    const int valid = (int)(cols - col < 4 ? cols - col : 4);
-    float total[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t row = first + group; row < last; row += kThreads / 32) {
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (valid > 0) {
-            load4(gy, row * cols + col, type, valid, v);
-            if (slope != nullptr) {
-                float d[4];
-                load4(slope, row * cols + col, type == kFloat32 ? kFloat32 : kFloat16, valid, d);
-                const float scale = type == kFloat32 ? 1.f : 1.f / kSlopeScale;
+    const int64_t col = (int64_t)blockIdx.x * kGradientColumns<T> + lane * kValues, first = (int64_t)blockIdx.y * strip,
+                  last = first + strip < rows ? first + strip : rows;
+    const int left = (int)(cols - col < kValues ? cols - col : kValues);
+    const Slope *slopes = reinterpret_cast<const Slope *>(slope);
+    float total[kValues] = {};
+    struct __align__(16) Pack {
+        T v[kValues];
+    };
+    struct __align__(16) SlopePack {
+        Slope v[kValues];
+    };
+    for (int64_t row = first + group; row < last; row += kGroups * kAhead) {
+        float v[kAhead][kValues];
+        if constexpr (WHOLE) {
+            Pack g[kAhead];
+            SlopePack d[kAhead];
+            const bool there = left > 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] *= d[j] * scale;
+            for (int i = 0; i < kAhead; ++i) {
+                const int64_t r = row + i * kGroups < last ? row + i * kGroups : last - 1, at = r * cols + (there ? col : 0);
+                g[i] = *reinterpret_cast<const Pack *>(gy + at);
+                if (slope != nullptr) d[i] = *reinterpret_cast<const SlopePack *>(slopes + at);
             }
-            if (dst != nullptr) {
-                const int64_t to = row * dst_pitch + col;
-                uint16_t p[3][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (type == kFloat32) split_triple(v[j], p[0][j], p[1][j], p[2][j]);
-                    else p[0][j] = to_16bit(v[j], type);
+            for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+                for (int j = 0; j < kValues; ++j) {
+                    v[i][j] = there && row + i * kGroups < last ? to_float(g[i].v[j]) : 0.f;
+                    if (slope != nullptr) v[i][j] *= to_float(d[i].v[j]) * (sizeof(T) == 4 ? 1.f : 1.f / kSlopeScale);
                 }
-                *reinterpret_cast<ushort4 *>(dst + to) = make_ushort4(p[0][0], p[0][1], p[0][2], p[0][3]);
-                if (type == kFloat32) {
-                    *reinterpret_cast<ushort4 *>(dst + plane + to) = make_ushort4(p[1][0], p[1][1], p[1][2], p[1][3]);
-                    *reinterpret_cast<ushort4 *>(dst + 2 * plane + to) = make_ushort4(p[2][0], p[2][1], p[2][2], p[2][3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+                for (int j = 0; j < kValues; ++j) {
+                    const int64_t r = row + i * kGroups, at = r * cols + col + j;
+                    v[i][j] = r < last && j < left ? to_float(gy[at]) : 0.f;
+                    if (slope != nullptr && r < last && j < left) v[i][j] *= to_float(slopes[at]) * (sizeof(T) == 4 ? 1.f : 1.f / kSlopeScale);
                 }
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t r = row + i * kGroups;
+            if (dst != nullptr && r < last && left > 0) {   // planes' rows are padded: a whole unit may be written
+                uint16_t *to = dst + r * dst_pitch + col;
+                if constexpr (sizeof(T) == 4) {
+                    uint16_t p[3][4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) split_triple(v[i][j], p[0][j], p[1][j], p[2][j]);
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+                        *reinterpret_cast<ushort4 *>(to + q * plane) = make_ushort4(p[q][0], p[q][1], p[q][2], p[q][3]);
+                } else {
+                    *reinterpret_cast<uint4 *>(to) = make_uint4(two_of<T>(v[i][0], v[i][1]), two_of<T>(v[i][2], v[i][3]), two_of<T>(v[i][4], v[i][5]),
+                                                                two_of<T>(v[i][6], v[i][7]));
+                }
+            }
+            float r_sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < kValues; ++j) {
+                total[j] += v[i][j];
+                r_sum += v[i][j];
+            }
+            if (partial != nullptr && sum_rows) {   // the features are rows: this row's share of the block's samples
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) r_sum += __shfl_xor_sync(0xffffffffu, r_sum, off);
+                if (lane == 0 && r < last) partial[(int64_t)blockIdx.x * rows + r] = r_sum;
             }
         }
-        if (partial != nullptr && sum_rows) {   // the features are rows: this row's share of 128 samples
-            float r = v[0] + v[1] + v[2] + v[3];
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) r += __shfl_xor_sync(0xffffffffu, r, off);
-            if (lane == 0) partial[(int64_t)blockIdx.x * rows + row] = r;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) total[j] += v[j];
     }
     if (partial == nullptr || sum_rows) return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s_sum[group][lane * 4 + j] = total[j];
+    for (int j = 0; j < kValues; ++j) s_sum[group][lane * kValues + j] = total[j];
     __syncthreads();
-    const int64_t c = (int64_t)blockIdx.x * 128 + threadIdx.x;
-    if (threadIdx.x < 128 && c < cols) {
-        float r = 0.f;
+    if (threadIdx.x >= kGradientColumns<T>) return;
+    const int64_t c = (int64_t)blockIdx.x * kGradientColumns<T> + threadIdx.x;
+    if (c >= cols) return;
+    float r = 0.f;
 #pragma unroll
-        for (int g = 0; g < kThreads / 32; ++g) r += s_sum[g][threadIdx.x];
-        partial[blockIdx.y * cols + c] = r;
-    }
+    for (int g = 0; g < kGroups; ++g) r += s_sum[g][threadIdx.x];
+    partial[blockIdx.y * cols + c] = r;
+}
+
+template <class T>
+static void launch_pre_gradient(const void *gy, const void *slope, int64_t rows, int64_t cols, uint16_t *dst, int64_t dst_pitch, int64_t plane,
+                                int64_t strips, int64_t strip, float *partial, int sum_rows, cudaStream_t st) {
+    const dim3 grid((unsigned)ceil_div(cols, kGradientColumns<T>), (unsigned)strips);
+    const bool whole = aligned_to(gy, 16) && aligned_to(slope, 16) && cols * sizeof(T) % 16 == 0;
+    launch_dependent(true, whole ? pre_gradient_kernel<T, true> : pre_gradient_kernel<T, false>, grid, dim3(kThreads), 0, st,
+                     reinterpret_cast<const T *>(gy), slope, rows, cols, dst, dst_pitch, plane, strip, partial, sum_rows);
 }
 
 // Adds the partial sums up, in their order.
@@ -384,10 +432,12 @@ static MatmulPlan plan_forward(int64_t batch, int64_t inner, int64_t outer, bool
                                                   : plan_matmul(batch, outer, inner, 1, planes, false, sms);
 }
 
+static int gradient_columns(int type) { return type == kFloat32 ? kGradientColumns<float> : kGradientColumns<__half>; }
+
 // Strips of rows of a pre-activation gradient, enough for whole SMs.
-static int64_t strips_of(int64_t rows, int64_t cols, int sms, int64_t *strip) {
-    int64_t strips = ceil_div(4 * sms, ceil_div(cols, 128));
-    if (strips > ceil_div(rows, 8)) strips = ceil_div(rows, 8);
+static int64_t strips_of(int64_t rows, int64_t cols, int type, int sms, int64_t *strip) {
+    int64_t strips = ceil_div(4 * sms, ceil_div(cols, gradient_columns(type)));
+    if (strips > ceil_div(rows, 32)) strips = ceil_div(rows, 32);
     if (strips > 65535) strips = 65535;
     *strip = ceil_div(rows, strips);
     return ceil_div(rows, *strip);
@@ -500,8 +550,8 @@ static DenseBackward plan_backward(const DenseLayout &l, int64_t batch, int64_t 
     b.g_pitch = padded(b.g_cols);
     b.g_plane = b.g_rows * b.g_pitch;
     b.g_bytes = b.lay_gz ? padded_bytes(b.planes * b.g_plane * 2) : 0;
-    b.strips = strips_of(b.g_rows, b.g_cols, sms, &b.strip);
-    b.parts = g_feature_major ? ceil_div(b.g_cols, 128) : b.strips;
+    b.strips = strips_of(b.g_rows, b.g_cols, type, sms, &b.strip);
+    b.parts = g_feature_major ? ceil_div(b.g_cols, gradient_columns(type)) : b.strips;
     b.bias_bytes = padded_bytes(b.parts * outer * 4);
     b.to_x = plan_matmul(batch, inner, outer, 1, b.planes, false, sms);
     b.to_w = plan_matmul(outer, inner, batch, 1, b.planes, false, sms);
@@ -550,9 +600,8 @@ extern "C" DL_API int dl_dense_backward(const void *gy, int g_feature_major, con
         w_planes = to;
     }
     if (b.lay_gz || gb) {
-        launch_dependent(true, pre_gradient_kernel, dim3((unsigned)ceil_div(b.g_cols, 128), (unsigned)b.strips), dim3(kThreads), 0, st, gy, slope,
-                         b.g_rows, b.g_cols, type, b.lay_gz ? gz : (uint16_t *)nullptr, b.g_pitch, b.g_plane, b.strip, gb ? sums : (float *)nullptr,
-                         g_feature_major);
+        const auto launch = type == kFloat32 ? launch_pre_gradient<float> : type == kBFloat16 ? launch_pre_gradient<__nv_bfloat16> : launch_pre_gradient<__half>;
+        launch(gy, slope, b.g_rows, b.g_cols, b.lay_gz ? gz : nullptr, b.g_pitch, b.g_plane, b.strips, b.strip, gb ? sums : nullptr, g_feature_major, st);
         if ((status = launch_status(what)) != DL_OK) return status;
     }
     if (gb) {

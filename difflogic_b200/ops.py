@@ -981,6 +981,10 @@ def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     if not 0 < eps < math.inf:
         raise ValueError("orthogonalize: eps must be positive, got %r" % (eps,))
     table = _newton_schulz(coefficients if coefficients is NEWTON_SCHULZ else _coefficients(coefficients), steps)
+    out = N.nodes().orthogonalize(x, steps, ctypes.addressof(table), float(eps))
+    if out is not None:
+        return out
+    # what is not of the ordinary form
     x = x.detach().contiguous()
     out = torch.empty_like(x)
     rows, cols = x.shape[-2:]
