@@ -324,7 +324,7 @@ DenseOut dense_forward(const Tensor &x, const Tensor &w, const Tensor &bias, con
     const auto options = x.options().requires_grad(false);
     DenseOut o;
     o.y = feature_major ? at::empty_strided({batch, outer}, {1, batch}, options) : at::empty({batch, outer}, options);
-    if (want_slope && act != DL_ACT_NONE) o.slope = at::empty({batch * outer}, options.dtype(kind == 0 ? at::kFloat : at::kHalf));
+    if (want_slope && act != DL_ACT_NONE) o.slope = at::empty({batch * outer}, options.dtype(x.scalar_type() == at::kBFloat16 ? at::kHalf : at::kFloat));
     o.x = readable(x);
     int64_t sizes[3];
     dl_dense_forward_sizes(o.x.t.data_ptr(), o.x.pitch, o.x.feature_major, w.data_ptr(), batch, inner, outer, feature_major, kind, sizes);

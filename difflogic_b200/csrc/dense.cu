@@ -49,6 +49,12 @@ __device__ __forceinline__ float value_of(const Units &from, int j) {
     }
 }
 
+// How the derivatives of a layer of T are kept.
+template <class T>
+using SlopeOf = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __half, float>::type;
+template <class T>
+constexpr float kScaleOf = std::is_same<T, __nv_bfloat16>::value ? kSlopeScale : 1.f;
+
 // 32 rows of values, a row in each lane, to where they lie in memory: rows `pitch` values apart, those from m on and columns from n on
 // left out.  whole: rows lie and end on 16-byte units; else a lane stores a value and a warp the 64 bytes of one row or two at a time.
 template <class T>
@@ -88,7 +94,7 @@ template <class T>
 struct DenseEpilogue {
     static constexpr bool kWholeTiles = false;
     static constexpr int kColumns = 64 / sizeof(T);   // 64 bytes
-    using Slope = typename std::conditional<sizeof(T) == 4, float, __half>::type;
+    using Slope = SlopeOf<T>;
     DenseOutput o;
     bool whole;            // rows of y and slope lie and end on 16-byte units
     bool residual_whole;   // those of the residual too
@@ -154,11 +160,14 @@ struct DenseEpilogue {
         }
         store_rows(stage, lane, z, reinterpret_cast<T *>(o.y), o.y_pitch, p.row, col, p.m, p.n, whole);
         if (SLOPE) {
-            if (sizeof(T) != 4) {
+            constexpr int kAtOnce = 64 / sizeof(Slope);   // fp16 layers: two pieces
 #pragma unroll
-                for (int j = 0; j < kColumns; ++j) d[j] *= kSlopeScale;
+            for (int c = 0; c < kColumns; c += kAtOnce) {
+                float part[kAtOnce];
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) part[j] = d[c + j] * kScaleOf<T>;
+                store_rows(stage, lane, part, reinterpret_cast<Slope *>(o.slope), o.y_pitch, p.row, col + c, p.m, p.n, whole);
             }
-            store_rows(stage, lane, d, reinterpret_cast<Slope *>(o.slope), o.y_pitch, p.row, col, p.m, p.n, whole);
         }
     }
 
@@ -186,7 +195,7 @@ struct DenseEpilogue {
         for (int j = 0; j < kColumns; ++j) {
             if (j >= left) continue;
             y[j * o.y_pitch] = from_float<T>(z[j]);
-            if (SLOPE) slope[j * o.y_pitch] = from_float<Slope>(d[j] * (sizeof(T) == 4 ? 1.f : kSlopeScale));
+            if (SLOPE) slope[j * o.y_pitch] = from_float<Slope>(d[j] * kScaleOf<T>);
         }
     }
 
@@ -258,7 +267,7 @@ template <class T, bool WHOLE>
 __global__ void __launch_bounds__(kThreads)
 pre_gradient_kernel(const T *__restrict__ gy, const void *__restrict__ slope, int64_t rows, int64_t cols, uint16_t *__restrict__ dst,
                     int64_t dst_pitch, int64_t plane, int64_t strip, float *__restrict__ partial, int sum_rows) {
-    using Slope = typename std::conditional<sizeof(T) == 4, float, __half>::type;
+    using Slope = SlopeOf<T>;
     constexpr int kValues = 16 / sizeof(T), kAhead = 4, kGroups = kThreads / 32;
     __shared__ float s_sum[kGroups][kGradientColumns<T>];
     grid_dependency_wait();
@@ -292,7 +301,7 @@ pre_gradient_kernel(const T *__restrict__ gy, const void *__restrict__ slope, in
 #pragma unroll
                 for (int j = 0; j < kValues; ++j) {
                     v[i][j] = there && row + i * kGroups < last ? to_float(g[i].v[j]) : 0.f;
-                    if (slope != nullptr) v[i][j] *= to_float(d[i].v[j]) * (sizeof(T) == 4 ? 1.f : 1.f / kSlopeScale);
+                    if (slope != nullptr) v[i][j] *= to_float(d[i].v[j]) * (1.f / kScaleOf<T>);
                 }
         } else {
 #pragma unroll
@@ -301,7 +310,7 @@ pre_gradient_kernel(const T *__restrict__ gy, const void *__restrict__ slope, in
                 for (int j = 0; j < kValues; ++j) {
                     const int64_t r = row + i * kGroups, at = r * cols + col + j;
                     v[i][j] = r < last && j < left ? to_float(gy[at]) : 0.f;
-                    if (slope != nullptr && r < last && j < left) v[i][j] *= to_float(slopes[at]) * (sizeof(T) == 4 ? 1.f : 1.f / kSlopeScale);
+                    if (slope != nullptr && r < last && j < left) v[i][j] *= to_float(slopes[at]) * (1.f / kScaleOf<T>);
                 }
         }
 #pragma unroll

@@ -6,8 +6,8 @@ feature-major layout that logic layers read -- or makes the fully connected netw
 
 * bf16 and fp16 layers multiply their values as they are, fp32 layers three bf16 planes of each value, which is as exact as 32-bit
   arithmetic; all sums are 32-bit, results are rounded once;
-* the backward pass multiplies the incoming gradient with the kept derivative of the activation (fp32, or fp16 times 2^14 where the
-  layer's type has 16 bits) and rounds the product to the layer's type before the two matrix products.
+* the backward pass multiplies the incoming gradient with the kept derivative of the activation (fp32, or for bf16
+  layers fp16 times 2^14) and rounds the product to the layer's type before the two matrix products.
 
 `implementation='python'` is the pure-torch definition of the same layer and runs anywhere.
 """
@@ -46,7 +46,7 @@ def _forward(x, w, bias, residual, act, feature_major, want_slope):
     y = torch.empty_strided((batch, outer), (1, batch) if feature_major else (outer, 1), dtype=x.dtype, device=x.device)
     slope = None
     if want_slope and act:
-        slope = torch.empty(batch * outer, dtype=torch.float32 if kind == 0 else torch.float16, device=x.device)
+        slope = torch.empty(batch * outer, dtype=torch.float16 if x.dtype == torch.bfloat16 else torch.float32, device=x.device)
     if batch == 0:
         return y, slope, x, None, None
     x, pitch, x_feature = _layout(x)

@@ -560,7 +560,7 @@ DL_API int dl_backward_w_announce_f32(const float *x, const int64_t *a, const in
  *
  * x [batch][inner] with rows x_pitch values apart, or, x_feature_major, [inner][batch]; w [outer][inner] contiguous; bias [outer] and
  * residual may be NULL, residual's strides in values.  y [batch][outer] or, y_feature_major, [outer][batch], contiguous.  slope (NULL:
- * not wanted): act' in y's layout, fp32, or for 16-bit types fp16 times 2^14.  x_planes, w_planes, workspace: sizes[0 .. 2] bytes of
+ * not wanted): act' in y's layout, fp32, or for bf16 fp16 times 2^14.  x_planes, w_planes, workspace: sizes[0 .. 2] bytes of
  * dl_dense_forward_sizes, 16-byte aligned; what is laid out in the planes serves the backward pass.
  *
  *   gz = gy * slope;  gx = gz w [batch][inner],  gw = gz^T x [outer][inner],  gb = sum of gz over the batch

@@ -51,10 +51,10 @@ def check(x, w, b, r, act, feature_major=False, gy=None, columns=None):
     grads = dict(zip([n for n, v in zip("xwbr", (x, w, b, r)) if v is not None], torch.autograd.grad(y, leaves, gy)))
     G = gy.double()
     gz = G * slope
-    # the slope: its own roundings, those of z (second derivatives stay below 1.13), 11 bits where it is kept in fp16; gz rounded once
-    kept = (2.0 ** -11 if t != torch.float32 else 0) + 2.0 ** -20
+    # the slope: its own roundings, those of z (second derivatives stay below 1.13), 11 bits where bf16 layers keep it in fp16; gz rounded once
+    kept = (2.0 ** -11 if t == torch.bfloat16 else 0) + 2.0 ** -20
     jump = (z.abs() <= 2 * z_off).double() if act == "relu" else 0     # either side of relu's corner
-    gz_off = G.abs() * (1.13 * z_off + kept * slope.abs() + 4e-12 + jump) + 2.0 ** -22 * G.abs() * (act is not None)
+    gz_off = G.abs() * (1.13 * z_off + kept * slope.abs() + (4e-12 if t == torch.bfloat16 else 0) + jump) + 2.0 ** -22 * G.abs() * (act is not None)
     in_product = gz_off + half * (gz.abs() + gz_off) + smallest
     want_g = {"x": gz @ W, "w": gz.t() @ X, "b": gz.sum(0)}
     offs = {"x": in_product @ W.abs() + product_error(W.shape[0]) * (gz.abs() @ W.abs()),
