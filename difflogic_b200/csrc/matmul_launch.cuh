@@ -1,6 +1,8 @@
 // Launching the matrix products of matmul.cuh.
 #pragma once
 
+#include <atomic>
+
 #include "matmul.cuh"
 #include "matmul_plan.h"
 
@@ -34,7 +36,15 @@ static int launch_tiles(const MatmulShape &shape, const CUtensorMap &a, const CU
                         cudaStream_t st, const char *what) {
     using Config = MatmulConfig<PLANES, COLUMNS, PAIR>;
     auto kernel = matmul_kernel<PLANES, COLUMNS, PAIR, Epilogue>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Config::kSharedBytes) != cudaSuccess) return launch_status(what);
+    // once for each kernel and device: the call takes the host longer than the rest of a launch
+    static std::atomic<uint64_t> allowed{0};
+    int device = 0;
+    cudaGetDevice(&device);
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if ((allowed.load(std::memory_order_relaxed) & bit) == 0) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Config::kSharedBytes) != cudaSuccess) return launch_status(what);
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
     const int64_t ctas = PAIR ? 2 * (int64_t)shape.tiles : shape.tiles, most = PAIR ? sms / 2 * 2 : sms;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(ctas < most ? ctas : most));
