@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <string>
 
 #include "difflogic_b200.h"
 
@@ -50,7 +51,9 @@ std::atomic<long long> g_launches{0};  // kernels launched from here, as _native
 PyObject *g_module_dict = nullptr;     // difflogic.py's: `_backward_w_stream` and `_backward_of_node`
 
 void check(int status) {
-    TORCH_CHECK(status == DL_OK, "difflogic_b200 (status ", status, "): ", dl_last_error_string());
+    // one string: a number in the message would go through a stream, and a compiler that brings its own C++ library links one here whose
+    // locale is not PyTorch's (the process ended there instead of raising)
+    TORCH_CHECK(status == DL_OK, "difflogic_b200 (status " + std::to_string(status) + "): " + dl_last_error_string());
     ++g_launches;
 }
 

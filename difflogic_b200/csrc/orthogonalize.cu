@@ -1,6 +1,10 @@
 // Newton-Schulz steps on matrices by the matrix products of matmul.cuh, the Muon step made of them, and their entry points.
 #include <math.h>
 
+#include <algorithm>
+#include <exception>
+#include <vector>
+
 #include "gram_steps.h"
 #include "matmul_launch.cuh"
 
@@ -507,6 +511,29 @@ static int64_t rows_of(const GramJob &job) {
     return rows * job.batch;
 }
 
+// Whether what is written, weights and momenta, shares no memory with anything else of the table; gradients may share theirs.
+static bool disjoint(const int64_t *table, int64_t count) {
+    struct Range {
+        int64_t first, last;
+        bool written;
+    };
+    std::vector<Range> all;   // may throw
+    all.reserve(3 * count);
+    for (int64_t i = 0; i < count; ++i) {
+        const int64_t *t = table + 5 * i, size = t[3] * t[4] * 4;
+        if (size == 0) continue;
+        for (int j = 0; j < 3; ++j) all.push_back({t[j], t[j] + size, j != 1});
+    }
+    std::sort(all.begin(), all.end(), [](const Range &a, const Range &b) { return a.first < b.first; });
+    int64_t any = 0, written = 0;   // where what came so far ends
+    for (const Range &r : all) {
+        if (r.first < (r.written ? any : written)) return false;
+        any = std::max(any, r.last);
+        if (r.written) written = std::max(written, r.last);
+    }
+    return true;
+}
+
 }  // namespace dl
 
 extern "C" DL_API int64_t dl_muon_workspace_bytes(const int64_t *table, int64_t count) {
@@ -542,6 +569,11 @@ extern "C" DL_API int dl_muon_step_f32(const int64_t *table, int64_t count, doub
         DL_REQUIRE((t[0] | t[1] | t[2]) % 4 == 0, DL_ERR_INVALID_ARG, "%s: misaligned matrix", what);
     }
     if (count == 0) return DL_OK;
+    try {
+        DL_REQUIRE(disjoint(table, count), DL_ERR_INVALID_ARG, "%s: a weight or momentum shares memory with another matrix", what);
+    } catch (const std::exception &) {
+        return fail(DL_ERR_INVALID_ARG, "%s: no memory on the host for %lld matrices", what, (long long)count);
+    }
     DL_REQUIRE(workspace && aligned_to(workspace, 16), DL_ERR_INVALID_ARG, "%s: the workspace is missing or not 16-byte aligned", what);
     const int sms = current_sms();
     cudaStream_t st = as_stream(stream);

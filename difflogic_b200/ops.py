@@ -1004,7 +1004,7 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
         m += (1 - momentum) (g - m);  u = g + momentum (m - g) (nesterov) or m
         w = (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) orthogonalize(u)
     which is torch.optim.Muon's rule, in 32 bits.  weights, grads, momenta: lists of 2-D contiguous float32 tensors on one CUDA device, of
-    which no two weights or momenta share memory."""
+    which no weight or momentum shares memory with another tensor of the lists."""
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     if not len(weights) == len(grads) == len(momenta):
         raise ValueError("muon_step: %d weights, %d gradients, %d momenta" % (len(weights), len(grads), len(momenta)))

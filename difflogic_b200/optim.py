@@ -509,8 +509,8 @@ class FlatMuon(torch.optim.Optimizer):
                       of a matrix is lr sqrt(max(1, rows / cols))
     :param adam_lr, betas, adam_eps: of the vectors, which take no weight decay
 
-    The buffers have FlatAdam's layout: LogicLayer's backward writes into `flat_grad`, and TrainStep all-reduces pieces of it.  A parameter
-    without a gradient is left alone.  A step can be captured in a CUDA graph."""
+    The buffers have FlatAdam's layout: LogicLayer's backward writes into `flat_grad`, and TrainStep all-reduces pieces of it.  A matrix
+    without a gradient is left alone, and so are the vectors where none has one.  A step can be captured in a CUDA graph."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=None, eps=1e-7, ns_steps=5,
                  adam_lr=1e-3, betas=(0.9, 0.999), adam_eps=1e-8):
@@ -591,21 +591,20 @@ class FlatMuon(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         g = self.param_groups[0]
-        matrices = [p for p in self._matrices if p.grad is not None]
+        matrices, vectors = ([p for p in some if p.grad is not None] for some in (self._matrices, self._vectors))
+        if vectors and len(vectors) != len(self._vectors):
+            raise RuntimeError("FlatMuon: some vectors have a gradient and some have none; give those that are not trained requires_grad=False "
+                               "and leave them out")
         grads = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in matrices]
         ops.muon_step([p.data for p in matrices], grads, [self.state[p]['momentum_buffer'] for p in matrices], lr=g['lr'], momentum=g['momentum'],
                       nesterov=g['nesterov'], weight_decay=g['weight_decay'], steps=g['ns_steps'], coefficients=g['ns_coefficients'], eps=g['eps'])
         count_update(matrices)
-        vectors = [p for p in self._vectors if p.grad is not None]
         if vectors:
             # one kernel over the vectors' part of the flat buffers
             for p in vectors:
                 view = self.grad_view(p)
                 if p.grad.data_ptr() != view.data_ptr():
                     view.copy_(p.grad)
-            if len(vectors) != len(self._vectors):
-                raise RuntimeError("FlatMuon: some vectors have a gradient and some have none; give those that are not trained requires_grad=False "
-                                   "and leave them out")
             beta1, beta2 = g['betas']
             first = self._first_vector
             with N.on_device(self.flat_param):

@@ -592,7 +592,8 @@ DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, int64_t row
 
 /* One step of `count` fp32 matrices: momentum += (1 - mu)(g - momentum); u = g + mu (momentum - g) (nesterov) or momentum;
  * w = (1 - lr decay) w - lr sqrt(max(1, rows / cols)) X, X the orthogonalised u.  table (on the host): {w, g, momentum, rows, cols} of
- * every matrix, device addresses as integers; no two may share memory.  Matrices of up to 16 columns take two kernels all together, the
+ * every matrix, device addresses as integers; no weight or momentum may share
+ * memory with anything else (refused).  Matrices of up to 16 columns take two kernels all together, the
  * others some for every shape. */
 DL_API int64_t dl_muon_workspace_bytes(const int64_t *table, int64_t count);
 DL_API int dl_muon_step_f32(const int64_t *table, int64_t count, double lr, double momentum, int nesterov, double weight_decay, int steps,

@@ -187,6 +187,31 @@ def test_muon_step_refuses():
         D.ops.muon_step([w, w], [w.clone()] * 2, [w.clone(), w.clone()], lr=0.1)
 
 
+@pytest.mark.parametrize("cols", [4, 40])
+def test_muon_step_refuses_shared_memory(cols):
+    memory = torch.randn(40, cols, device="cuda")
+    a, b, c, d, g = memory[:10], memory[5:15], memory[20:30], memory[30:], torch.randn(10, cols, device="cuda")
+    before = memory.clone()
+    for weights, grads, momenta in (([a, b], [g, g], [c, d]), ([a, c], [g, g], [d, b]), ([a], [b], [c]), ([a], [a], [c]), ([a], [g], [b]),
+                                    ([c], [memory[29:39]], [a])):
+        with pytest.raises((ValueError, RuntimeError), match="shares memory"):
+            D.ops.muon_step(weights, grads, momenta, lr=0.1)
+    assert torch.equal(memory, before)
+    D.ops.muon_step([a, c], [g, g], [memory[10:20], d], lr=0.1)     # neighbours, and one gradient for two
+    assert not torch.equal(memory[:10], before[:10]) and not torch.equal(memory[20:30], before[20:30])
+
+
+def test_flat_muon_refuses_before_it_updates():
+    model = torch.nn.Sequential(D.DenseLayer(8, 8), D.DenseLayer(8, 8))
+    optimizer = FlatMuon(model.parameters(), lr=0.1)
+    model(torch.randn(4, 8, device="cuda")).sum().backward()
+    model[1].bias.grad = None
+    before = optimizer.flat_param.clone(), optimizer.flat_momentum.clone()
+    with pytest.raises(RuntimeError, match="vectors"):
+        optimizer.step()
+    assert torch.equal(optimizer.flat_param, before[0]) and torch.equal(optimizer.flat_momentum, before[1])
+
+
 def network(seed=0):
     torch.manual_seed(seed)
     return torch.nn.Sequential(torch.nn.Flatten(), D.DenseLayer(48, 120, activation="silu"), D.DenseLayer(120, 200, feature_major=True),
