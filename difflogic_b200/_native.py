@@ -125,8 +125,8 @@ _launches = 0
 
 
 def launch_count():
-    """Number of kernel launches issued through check() or by the native autograd nodes so far (every checked entry point launches
-    one kernel)."""
+    """Number of entry points called through check() or by the native autograd nodes so far, each of which launches a kernel; those of
+    dense layers and orthogonalised updates, which launch several, count as one."""
     return _launches + (_nodes.launches() if _nodes is not None else 0)
 
 

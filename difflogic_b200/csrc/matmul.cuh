@@ -47,7 +47,7 @@ __device__ __forceinline__ void split_two(float a, float b, uint32_t &hi, uint32
 }
 __device__ __forceinline__ float join_pair(uint16_t hi, uint16_t lo) { return __half2float(__ushort_as_half(hi)) + __half2float(__ushort_as_half(lo)); }
 
-// The nearest bf16 at each step: exact for every fp32.  Infinities and NaN go into the first plane alone; values that would round to
+// The nearest bf16 at each step: exact for every fp32 from 2^-110 on.  Infinities and NaN go into the first plane alone; values that would round to
 // infinity are cut off.
 __device__ __forceinline__ void split_triple(float x, uint16_t &hi, uint16_t &mid, uint16_t &lo) {
     const uint32_t bits = __float_as_uint(x);
@@ -241,7 +241,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 #pragma unroll 1
                     for (int p = 0; p < PLANES; ++p) {
                         const int z = t.matrix * s.planes_z + p;
-const int row = t.row + (int)rank * kMatmulRows;
+                        const int row = t.row + (int)rank * kMatmulRows;
                         if (!s.a_mn) {
                             tile_load<PAIR>(at, &map_a, k, row, z, bar);
                         } else {
@@ -253,7 +253,7 @@ const int row = t.row + (int)rank * kMatmulRows;
 #pragma unroll 1
                     for (int p = 0; p < PLANES; ++p) {
                         const int z = t.matrix * s.planes_z + p;
-const int col = t.col + (int)rank * Config::kOwnColumns;
+                        const int col = t.col + (int)rank * Config::kOwnColumns;
                         if (!s.b_mn) {
                             tile_load<PAIR>(at, &map_b, k, col, z, bar);
                         } else {

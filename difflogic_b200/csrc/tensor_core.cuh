@@ -110,13 +110,6 @@ __device__ __forceinline__ void tensor_read32(uint32_t address, uint32_t (&v)[32
           "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(address));
 }
-__device__ __forceinline__ void tensor_read16(uint32_t address, uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(address));
-}
 __device__ __forceinline__ void tensor_read_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Descriptor of an operand in shared memory, 128-byte swizzle.  K-major: rows of 128 bytes, 8-row groups every 1024 bytes, 16 values
