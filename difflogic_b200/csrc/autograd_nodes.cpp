@@ -17,6 +17,7 @@
 #include <ATen/ops/empty_strided.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -408,6 +409,17 @@ struct DenseNode : torch::autograd::Function<DenseNode> {
     }
 };
 
+// A backward pass that is captured may not reach another stream's work.  A leaf of a graph that lives has its accumulator on the stream
+// that the graph was made on, a pass captured on another stream would wait for that one, and the process ends: refused here instead.
+void refuse_older_graph(const Tensor &t) {
+    if (!t.defined() || !t.is_leaf() || !t.requires_grad()) return;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (accumulator == nullptr) return;
+    const auto stream = accumulator->stream();
+    TORCH_CHECK(!stream || *stream == c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap(),
+                "difflogic_b200: dense is captured while a graph of the same tensors, made on another stream, is alive; delete its outputs before the capture");
+}
+
 // dense(x, weight, bias | None, residual | None, activation, feature_major) -> output, or None
 PyObject *dense(PyObject *, PyObject *const *args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
@@ -455,6 +467,8 @@ PyObject *dense(PyObject *, PyObject *const *args, Py_ssize_t count) {
         }
         const bool graph = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (bias.defined() && bias.requires_grad()) ||
                                                           (residual.defined() && residual.requires_grad()));
+        if (graph && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+            for (const Tensor &t : {x, w, bias, residual}) refuse_older_graph(t);
         const auto given = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
         y = graph ? DenseNode::apply(x, w, given(bias), given(residual), (int64_t)act, (bool)feature_major)
                   : dense_forward(x, w, bias, residual, (int)act, feature_major, false).y;

@@ -9,6 +9,12 @@
 // (measured: 6e-7 after 800, 1.2e-6 after 2000, where 32-bit sums of rounded steps have 2e-7 and 4e-7).  So the sums of planes are
 // taken out of tensor memory every steps_per_sum steps and added up in the epilogue's registers, and the small products have a sum
 // of their own.
+//
+// What bounds it.  Large products: the tensor cores.  8192 x 4096 x 4096 bf16 with the epilogue of a dense layer 207 us, 1330 TFLOP/s (a
+// library's plain product, 4096 values a side and more, has 1627 in a burst); 4096 x 4096 x 4096 of pairs 336 us, three products each:
+// 1230 TFLOP/s.  Pairs of SMs share a tile of 256 x 256 there, since a step's copies of 128 x 128 take as long as its products (60 bytes
+// a clock and SM).  Products of a few tiles per SM: their latency, about 5 us until the sums of the first steps are there and 5 to 10 us
+// of epilogue that no next tile hides; 1024 x 1024 x 1024 of pairs 20 us.
 #pragma once
 
 #include "matmul_values.cuh"
@@ -72,11 +78,12 @@ constexpr int kPieceColumns = 16;    // columns of which sums are kept together 
 constexpr int kSlotBytes = 2048;     // 32 rows of 64 bytes
 constexpr int kStageBytes = 2 * kSlotBytes;   // shared memory of an epilogue warp
 
+struct NothingAhead {};
+
 // An epilogue takes pieces of 32 rows (lane = row) and kColumns columns from registers: `begin` says where the first piece of a warp's
 // share of a tile lies (row, col: of its first value), `piece` takes the one `across` columns further.  What it has to read for that
 // `fetch` asks for beforehand -- the first one's while the products are still running, the others' a piece ahead: a read takes 3000
 // clocks when all SMs read at a time.
-struct NothingAhead {};
 //
 // Results leave by way of shared memory in tiles of 32 rows of 64 bytes, a slot each: written as the lanes have them, rows or columns as
 // rows, and read back with 8 rows of four lanes at a time, so that a warp's store is of eight whole 64-byte rows.  The swizzle puts the

@@ -281,3 +281,27 @@ def test_layer_feeds_logic_layers_without_a_copy():
     for p, q in zip(model.parameters(), reference.parameters()):
         # the framework's own bound for gradients through logic layers
         assert (p.grad.cpu().double() - q.grad).abs().max().item() <= 1e-4 * q.grad.abs().max().item()
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    x, w, b = torch.randn(40, 16, device="cuda"), torch.randn(24, 16, device="cuda", requires_grad=True), torch.randn(24, device="cuda", requires_grad=True)
+    gy = torch.randn(40, 24, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            want = torch.autograd.grad(D.dense(x, w, b, activation="relu"), (w, b), gy)
+    torch.cuda.current_stream().wait_stream(side)
+    alive = D.dense(x, w, b, activation="relu")
+    with pytest.raises(RuntimeError, match="alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            D.dense(x, w, b, activation="relu")
+    with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+        D.dense(x, w, b)                      # no graph of its own
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = torch.autograd.grad(D.dense(x, w, b, activation="relu"), (w, b), gy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
