@@ -221,7 +221,7 @@ struct OrthogonalEpilogue {
     __device__ __forceinline__ Place begin(const Tile &t, const MatmulShape &s, int row, int col, int lane) const {
         const int r = row + lane / 4, c = col + lane % 4 * 4;
         const int64_t at = r * cols + c;
-        return {r, c, s.m, s.n, out == nullptr ? at : at + t.matrix * s.m * cols, 2 * t.matrix * plane, out == nullptr ? all.weight[t.matrix] : nullptr};
+        return {r, c, s.m, s.n, out == nullptr ? at : at + (int64_t)t.matrix * s.m * cols, 2 * t.matrix * plane, out == nullptr ? all.weight[t.matrix] : nullptr};
     }
     struct Ahead {
         ushort4 hi[4], lo[4];   // of `more`

@@ -136,3 +136,27 @@ def test_workspaces_follow_the_sizes(rows, cols, k, batch, kind):
             assert 0 <= sizes[2] <= 64 << 20
             assert lib.dl_orthogonalize_workspace_bytes(batch, rows, cols, kind) > 0
             assert lib.dl_dense_backward_workspace_bytes(16, 0, 1, 16, k, 0, 16, 1, 1, rows, k, cols, kind) > 0
+
+
+def test_gradients_outside_the_flat_buffer_are_reduced_in_it():
+    """A dense layer's gradient is a tensor of its own: before a bucket of the flat buffer is reduced, it moves into its slice."""
+    from difflogic_b200.training import TrainStep
+    flat = torch.zeros(12)
+    inside, outside = torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(2, 4))
+
+    class Optimizer:
+        def grad_view(self, p):
+            return flat[:4] if p is inside else flat[4:].view(2, 4)
+
+    step = TrainStep.__new__(TrainStep)
+    step._on_gpu, step.optimizer = True, Optimizer()
+    step._bucket_of, step._bucket_slices, step._pending = {inside: 0, outside: 0}, [flat], [2]
+    reduced = []
+    step._launch_all_reduce = lambda t: reduced.append(t.clone())
+    flat[:4] = 1
+    inside.grad, outside.grad = flat[:4], torch.arange(8.).view(2, 4)
+    step._reduce_when_ready(outside)
+    assert not reduced and outside.grad.data_ptr() == flat[4:].data_ptr()
+    step._reduce_when_ready(inside)
+    assert inside.grad.data_ptr() == flat.data_ptr()
+    assert len(reduced) == 1 and reduced[0].tolist() == [1, 1, 1, 1, 0, 1, 2, 3, 4, 5, 6, 7]

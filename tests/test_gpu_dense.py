@@ -305,3 +305,27 @@ def test_capture_beside_an_eager_graph_is_refused():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+def whole_numbers(*size):
+    """-1, 0 and 1: sums of products are exact, and so is what they round to."""
+    return torch.empty(*size, dtype=torch.bfloat16, device="cuda").random_(-1, 2).requires_grad_()
+
+
+@pytest.mark.parametrize("rows, inner, cols", [(70000, 16, 33000), (66000, 33000, 24), (3, 33000, 66000)])
+def test_offsets_behind_32_bits(rows, inner, cols):
+    torch.manual_seed(5)
+    x, w, b, r = whole_numbers(rows, inner), whole_numbers(cols, inner), whole_numbers(cols), whole_numbers(rows, cols)
+    gy = whole_numbers(rows, cols).detach()
+    y = D.dense(x, w, b, residual=r, activation="relu")
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), gy)
+    last = slice(-min(rows, 300), None), slice(-40, None)
+    with torch.no_grad():
+        z = x[last[0]].double() @ w.double().t() + b.double()
+        assert torch.equal(y[last[0]], (z.clamp(min=0) + r[last[0]].double()).bfloat16())
+        gz = gy[last[0]].double() * (z > 0)
+        assert torch.equal(gx[last[0]], (gz @ w.double()).bfloat16())
+        del z, gz
+        z = torch.cat([part.double() @ w[last[1]].double().t() for part in x.split(4096)]) + b[last[1]].double()
+        gz = gy[:, last[1]].double() * (z > 0)
+        assert torch.equal(gw[last[1], -40:], (gz.t() @ x[:, -40:].double()).bfloat16()) and torch.equal(gb[last[1]], gz.sum(0).bfloat16())

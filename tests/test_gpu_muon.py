@@ -316,3 +316,24 @@ def test_flat_muon_state():
     opt.zero_grad()
     opt.step()
     assert all(torch.equal(p, q) for p, q in zip(model.parameters(), frozen))
+
+
+def test_offsets_behind_32_bits():
+    rows, last = 140_000_000, slice(-1000, None)
+    torch.manual_seed(6)
+    w, g = torch.randn(rows, 16, device="cuda"), torch.randn(rows, 16, device="cuda")
+    m, before = torch.zeros_like(g), w[last].double()
+    gram = sum(part.double().t() @ part.double() for part in g.split(4_000_000))
+    norm = gram.trace().sqrt()
+    s, p = gram / norm ** 2, torch.eye(16, dtype=torch.float64, device="cuda")
+    for _ in range(5):
+        a, b, c = DEFAULT
+        step = a * torch.eye(16, dtype=torch.float64, device="cuda") + b * s + c * s @ s
+        p, s = p @ step, step @ s @ step
+    want = g[last].double() / norm @ p
+    assert far(D.ops.orthogonalize(g)[last], want) <= bound(torch.float32, 16)
+    lr = 1.0
+    D.ops.muon_step([w], [g], [m], lr=lr, momentum=0.5, nesterov=False)
+    update = (before - w[last].double()) / (lr * math.sqrt(rows / 16))
+    # the difference of two roundings of the weight (2^-24 of up to 6), over a rate of 3000 and entries of 1e-4
+    assert far(m[last], 0.5 * g[last].double()) <= 2.0 ** -24 and far(update, want) <= bound(torch.float32, 16) + 2 * 2.0 ** -24 * 6 / 3000 / 8e-5
