@@ -409,15 +409,16 @@ struct DenseNode : torch::autograd::Function<DenseNode> {
     }
 };
 
-// A backward pass that is captured may not reach another stream's work.  A leaf of a graph that lives has its accumulator on the stream
-// that the graph was made on, a pass captured on another stream would wait for that one, and the process ends: refused here instead.
+// A leaf of a graph that lives has its accumulator on the stream that the graph was made on, and a captured backward pass brings that
+// stream into the capture.  The default stream cannot be brought in, and the process ends: refused here instead.
 void refuse_older_graph(const Tensor &t) {
     if (!t.defined() || !t.is_leaf() || !t.requires_grad()) return;
     const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
     if (accumulator == nullptr) return;
     const auto stream = accumulator->stream();
-    TORCH_CHECK(!stream || *stream == c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap(),
-                "difflogic_b200: dense is captured while a graph of the same tensors, made on another stream, is alive; delete its outputs before the capture");
+    TORCH_CHECK(!stream || *stream != c10::cuda::getDefaultCUDAStream(t.device().index()).unwrap(),
+                "difflogic_b200: dense is captured while a graph of the same tensors, made on the default stream, is alive; delete its outputs before the "
+                "capture");
 }
 
 // dense(x, weight, bias | None, residual | None, activation, feature_major) -> output, or None

@@ -134,8 +134,8 @@ def dense(x, weight, bias=None, residual=None, activation=None, feature_major=Fa
     x `[..., in]`, weight `[out, in]`, bias `[out]`, residual `[..., out]`, all of one type (float32, bfloat16 or float16) on one CUDA
     device; activation: None, 'relu', 'sigmoid', 'silu' or 'gelu' (the exact one).  x may be a transposed view, as logic layers return
     them.  An infinite float32
-    operand makes the results it enters infinite or undefined.  A call that a CUDA graph captures needs earlier graphs of its leaves, made
-    on other streams, gone (their outputs deleted).  feature_major: a 2-D result lies in memory as `[out, batch]` (same values, other strides), which a LogicLayer reads without a
+    operand makes the results it enters infinite or undefined.  A call that a CUDA graph captures is refused while an
+    earlier graph of its leaves, made on the default stream, is alive.  feature_major: a 2-D result lies in memory as `[out, batch]` (same values, other strides), which a LogicLayer reads without a
     copy."""
     act = ACTIVATIONS.get(activation, -1)
     if act >= 0 and x.is_cuda:

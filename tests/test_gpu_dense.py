@@ -307,6 +307,27 @@ def test_capture_beside_an_eager_graph_is_refused():
     assert all(torch.equal(p, q) for p, q in zip(want, got))
 
 
+def test_capture_beside_a_warm_up_on_another_stream():
+    x, w = torch.randn(40, 16, device="cuda"), torch.randn(24, 16, device="cuda", requires_grad=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            w.grad = None
+            loss = D.dense(x, w, activation="silu").sum()
+            loss.backward()
+    torch.cuda.current_stream().wait_stream(side)
+    want = w.grad.clone()
+    w.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):        # on a stream of its own, `loss` alive
+        D.dense(x, w, activation="silu").sum().backward()
+    w.grad.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(w.grad, want) and bool(torch.isfinite(loss.detach()))
+
+
 def whole_numbers(*size):
     """-1, 0 and 1: sums of products are exact, and so is what they round to."""
     return torch.empty(*size, dtype=torch.bfloat16, device="cuda").random_(-1, 2).requires_grad_()
