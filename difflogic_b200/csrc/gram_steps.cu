@@ -152,7 +152,7 @@ gram_sums_kernel(const __grid_constant__ GramBlocks g, double *__restrict__ sums
 constexpr int kSquarePitch = 18;   // doubles of a row of a 16 x 16 matrix
 using Square = double[kGramColumns][kSquarePitch];
 
-// One 8 x 8 block of A B, in two chains: an instruction takes 40 clocks until its sum can be added to.
+// One 8 x 8 block of A B, in two chains: an instruction takes about 30 clocks until its sum can be added to.
 __device__ __forceinline__ void square_block(const Square &a, const Square &b, int block, int lane, double (&d)[2]) {
     const int down = block / 2 * 8, across = block % 2 * 8;
     double e[2] = {0, 0};
