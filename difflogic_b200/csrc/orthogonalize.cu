@@ -304,6 +304,34 @@ static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t c
     return l;
 }
 
+// How far a step's polynomials go.  Singular values of X start in [0, 1]; a step takes those of [0, reach] to |a s + b s^3 + c s^5|, which
+// as a continuous image of an interval with 0 in it is the interval up to the largest one: at the end or where the derivative is zero.
+static double largest_value(double a, double b, double c, double reach) {
+    double most = fabs(reach * (a + reach * reach * (b + reach * reach * c)));
+    const double root = 9 * b * b - 20 * a * c;
+    if (root >= 0)   // of a + 3 b u + 5 c u^2, u = s^2
+        for (const double down : {-3 * b + sqrt(root), -3 * b - sqrt(root)}) {
+            const double u = c != 0 ? down / (10 * c) : b != 0 ? -a / (3 * b) : 0;
+            if (u > 0 && u < reach * reach) most = std::max(most, fabs(sqrt(u) * (a + u * (b + u * c))));
+        }
+    return most;
+}
+// The largest of |a + b u + c u^2| over the same values, u = s^2: the norm of M.
+static double largest_factor(double a, double b, double c, double reach) {
+    const double end = reach * reach, u = c != 0 ? -b / (2 * c) : 0;
+    double most = std::max(fabs(a), fabs(a + end * (b + end * c)));
+    if (u > 0 && u < end) most = std::max(most, fabs(a + u * (b + u * c)));
+    return most;
+}
+constexpr double kMostReach = 8.01;   // X itself is kept times 2^12: fp16 ends at 16 of that
+// Pairs of a matrix of this norm are kept as many times smaller, a power of two, so that its entries, no larger than the norm, stay below 16
+// with some room for what is rounded on the way.  1 for coefficients that keep values near 1.
+static float kept_smaller(double norm) {
+    float by = 1.f;
+    while (norm / by > 12) by *= 2;
+    return by;
+}
+
 // steps times: S = X^T X (X X^T where X is wide), M = b S + c S^2, X = a X + X M (M X).  `last` takes the last product.
 // b S is added up in the epilogue of c S^2, which reads S beside its products; S stored a second time with b / c on its diagonal, so that
 // one product gave both, costs more in stores than it saves: 4 x 1024 x 1024 bf16 347 us for 304.
@@ -341,8 +369,11 @@ static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64
     p.planes_z = 2;
     p.exact = !light;
     const float once = 1.f / kPairScale, twice = once * once;
+    double reach = 1;
     for (int i = 0; i < steps; ++i) {
         const float a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
+        const float gram_by = kept_smaller(reach * reach), poly_by = kept_smaller(largest_factor(light ? 0.f : a, b, c, reach));
+        reach = largest_value(a, b, c, reach);
         p.a = p.b = {x, l.x_pitch, l.x_plane, l.tall};
         p.m = p.n = l.side;
         p.k = l.tall ? rows : cols;
@@ -351,12 +382,12 @@ static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64
         PairEpilogue e = {};
         e.pitch = l.s_pitch;
         e.plane = l.s_plane;
-        e.scale = once;
+        e.scale = once / gram_by;
         e.symmetric = true;
         e.out = gram;
         if (c == 0.f) {   // the cubic iteration: M comes straight out of this product
-            e.scale = b * once;
-            e.diagonal = light ? 0.f : a * kPairScale;
+            e.scale = b * once / poly_by;
+            e.diagonal = light ? 0.f : a * kPairScale / poly_by;
         }
         if ((status = launch_planes(p, l.gram, e, partial, sms, st, what)) != DL_OK) return status;
         if (c != 0.f) {
@@ -365,9 +396,9 @@ static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64
             p.planes = 2;
             e.out = poly;
             e.more = gram;
-            e.factor = b;
-            e.scale = c * once;
-            e.diagonal = light ? 0.f : a * kPairScale;
+            e.factor = b * (gram_by / poly_by);
+            e.scale = c * once * (gram_by * gram_by / poly_by);
+            e.diagonal = light ? 0.f : a * kPairScale / poly_by;
             if ((status = launch_planes(p, l.square, e, partial, sms, st, what)) != DL_OK) return status;
         }
         const Operand m = {c != 0.f ? poly : gram, l.s_pitch, l.s_plane, false};
@@ -384,7 +415,7 @@ static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64
             to_next.more = more;
             to_next.pitch = l.x_pitch;
             to_next.plane = l.x_plane;
-            to_next.scale = once;
+            to_next.scale = once * poly_by;
             to_next.factor = a;
             to_next.out = next;
             status = launch_planes(p, l.product, to_next, partial, sms, st, what);
@@ -395,7 +426,7 @@ static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64
             to_end.more = more;
             to_end.pitch = l.x_pitch;
             to_end.plane = l.x_plane;
-            to_end.scale = twice;
+            to_end.scale = twice * poly_by;
             to_end.factor = a * once;
             status = launch_planes(p, l.product, to_end, partial, sms, st, what);
         }
@@ -423,6 +454,13 @@ extern "C" DL_API int64_t dl_orthogonalize_workspace_bytes(int64_t batch, int64_
 static int check_steps(int steps, const float *coefficients, double eps, const char *what) {
     DL_REQUIRE(steps >= 1 && steps <= kMostSteps && coefficients, DL_ERR_INVALID_ARG, "%s: needs 1 to %d steps and their coefficients", what, kMostSteps);
     DL_REQUIRE(eps > 0, DL_ERR_INVALID_ARG, "%s: eps must be positive", what);
+    double reach = 1;
+    for (int i = 0; i < steps; ++i) {
+        const float *at = coefficients + 3 * i;
+        for (int j = 0; j < 3; ++j) DL_REQUIRE(fabsf(at[j]) <= 64, DL_ERR_INVALID_ARG, "%s: a coefficient of more than 64", what);
+        reach = largest_value(at[0], at[1], at[2], reach);
+        DL_REQUIRE(reach <= kMostReach, DL_ERR_INVALID_ARG, "%s: with these coefficients singular values do not stay near 1", what);
+    }
     return DL_OK;
 }
 

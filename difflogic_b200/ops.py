@@ -12,7 +12,6 @@ import ctypes
 import functools
 import math
 
-import numpy as np
 import torch
 
 from . import _native as N
@@ -943,6 +942,17 @@ _FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)   # makes every singular value about 1 in five steps
 
 
+def _largest_value(a, b, c, reach):
+    """The largest of |a s + b s^3 + c s^5| for s in [0, reach]: at the end, or where the derivative is zero."""
+    candidates, root = [reach], 9 * b * b - 20 * a * c
+    if c == 0:
+        roots = [-a / (3 * b)] if b != 0 else []
+    else:
+        roots = [(-3 * b + sign * math.sqrt(root)) / (10 * c) for sign in (1, -1)] if root >= 0 else []
+    candidates += [math.sqrt(u) for u in roots if 0 < u < reach * reach]
+    return max(abs(s * (a + s * s * (b + s * s * c))) for s in candidates)
+
+
 @functools.lru_cache(maxsize=64)
 def _newton_schulz(coefficients, steps):
     """The coefficients of every step as the library takes them.  A singular value s becomes a s + b s^3 + c s^5; the iterates are kept
@@ -952,11 +962,11 @@ def _newton_schulz(coefficients, steps):
     sets = coefficients if isinstance(coefficients[0], tuple) else (coefficients,) * steps
     if len(sets) != steps or any(len(s) != 3 for s in sets):
         raise ValueError("orthogonalize: three coefficients, or three for each of the %d steps" % steps)
-    values = np.linspace(0.0, 1.0, 4097)
+    reach = 1.0     # what [0, 1] has become is [0, reach]
     for a, b, c in sets:
-        squares = values * values
-        values = np.abs(values * (a + squares * (b + c * squares)))
-        if not values.max() <= 8.0 or not max(abs(a), abs(b), abs(c)) <= 64.0:     # undefined ones too
+        fits = max(abs(a), abs(b), abs(c)) <= 64.0 and not any(map(math.isnan, (a, b, c)))
+        reach = _largest_value(a, b, c, reach) if fits else math.inf
+        if not reach <= 8.0 * (1 + 1e-6):
             raise ValueError("orthogonalize: with these coefficients the iteration does not stay near 1")
     return (ctypes.c_float * (3 * steps))(*[v for s in sets for v in s])
 
@@ -970,7 +980,8 @@ def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     in the Frobenius norm, then `steps` times X <- a X + b (X X^T) X + c (X X^T)^2 X.
 
     x: `[..., rows, cols]` float32, bfloat16 or float16 on a CUDA device, every matrix on its own; the result has x's type.
-    coefficients: (a, b, c), or one such triple for each step.  The products run on the tensor cores with operands of 22 bits
+    coefficients: (a, b, c), or one such triple for each step, with which singular values from [0, 1] stay at 8 or below (errors grow by
+    the slopes of a s + b s^3 + c s^5 from step to step).  The products run on the tensor cores with operands of 22 bits
     (bfloat16: 11, which leaves the result less far off than its own rounding does).  An entry
     that is infinite or undefined makes its whole matrix undefined."""
     N.require_cuda(x)

@@ -585,7 +585,9 @@ DL_API int dl_dense_backward(const void *gy, int g_feature_major, const void *sl
 /* X = G / max(|G|_F, eps), then for each step with its (a, b, c) in `coefficients` (steps x 3, on the host)
  *   X <- a X + b (X X^T) X + c (X X^T)^2 X
  * for `batch` contiguous matrices rows x cols; out in G's type.  The iterates are kept to 22 bits (fp16 pairs times 2^12: values up to
- * 16), sums in 32 bits; bf16 matrices are multiplied with 11 bits, which leaves the result less far off than its rounding does. */
+ * 16; Gram matrices and polynomials that go further are kept a power of two smaller), sums in 32 bits; bf16 matrices are multiplied with
+ * 11 bits, which leaves the result less far off than its rounding does.  Coefficients of more than 64 are refused, and those with which
+ * singular values from [0, 1] grow past 8 on the way. */
 DL_API int64_t dl_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int type);
 DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, int64_t rows, int64_t cols, int type, int steps,
                             const float *coefficients, double eps, void *workspace, void *stream);

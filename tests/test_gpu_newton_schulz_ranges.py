@@ -1,0 +1,79 @@
+"""Newton-Schulz steps whose Gram matrices and polynomials are far from 1: everything that is kept between products has to fit its 16-bit
+planes for all coefficients that are accepted."""
+import math
+
+import pytest
+import torch
+
+import difflogic_b200 as D
+
+pytestmark = pytest.mark.gpu
+
+# polynomials with a past 16, with values between 4 and 8 on the way (their squares pass 16), with b s^2 + c s^4 past 16, cubic ones
+COEFFICIENTS = [((20.0, -60.0, 48.0),), ((20.0, -60.0, 45.0),), ((20.0, -40.0, 20.0),), ((16.5, -16.5, 0.0),),
+                ((6.0, 0.0, 0.0), (0.2, -0.01, 0.0001)), ((5.0, 0.0, 0.0), (0.3, -0.001, 0.00001)), ((8.0, 0.0, 0.0), (1.0, 0.0, 0.0)),
+                ((8.0, 0.0, 0.0), (0.5, -0.015, 0.0), (1.5, -0.1, 0.002)), ((24.0, -60.0, 44.0), (0.1, 0.0, 0.0))]
+
+
+def steps_and_bound(g, coefficients, unit, eps=1e-7):
+    """The definition in 64 bits, and how far off (Frobenius norm) iterates may be whose planes are `unit` off, relative to each value.
+
+    With X off by E, p(X) is off by max |p'| E: p acts on the singular values.  A step adds what it rounds itself: S = X X^T from planes that
+    are a unit off, summed in 32 bits (2^-23 every 16 values) and stored (a unit, no less than half the smallest 16-bit number over 2^12,
+    times the power of two that S and M are kept smaller by, 64 at most); M = a + b S + c S^2 likewise, S^2 of pairs; M X likewise."""
+    x = g.double()
+    x = x / x.square().sum().sqrt().clamp(min=eps)
+    x = x if x.shape[0] <= x.shape[1] else x.mT
+    side = x.shape[0]
+    F, top = (lambda v: v.norm().item()), (lambda v: torch.linalg.matrix_norm(v, 2).item())
+    acc = lambda k: (k / 16 + 8) * 2.0 ** -23  # noqa: E731
+    pair = 2.0 ** -22
+    least = 2.0 ** -25 / 4096 * 64
+    off = unit * F(x) + least * math.sqrt(x.numel())
+    for a, b, c in coefficients:
+        s = x @ x.mT
+        m = a * torch.eye(side, dtype=torch.float64, device=x.device) + b * s + c * s @ s
+        s_off = (2 * unit + acc(x.shape[1])) * F(x) ** 2 + pair * F(s) + least * side
+        m_off = (abs(b) + 2 * abs(c) * top(s)) * s_off + abs(c) * (2 * pair + acc(side)) * F(s) ** 2 + pair * F(m) + least * side
+        own = top(x) * m_off + (2 * unit + acc(side)) * F(m) * F(x) + least * math.sqrt(x.numel())
+        reach = top(x) * 1.01
+        slopes = torch.linspace(0, reach, 4001, dtype=torch.float64)
+        slope = (a + 3 * b * slopes ** 2 + 5 * c * slopes ** 4).abs().max().item()
+        x = m @ x
+        off = slope * off + own + pair * F(x)
+    return (x if g.shape[0] <= g.shape[1] else x.mT), off
+
+
+def matrix(kind, rows, cols):
+    gen = torch.Generator().manual_seed(rows + cols)
+    if kind == "one direction":
+        return torch.randn(rows, 1, generator=gen) @ torch.randn(1, cols, generator=gen)
+    return torch.randn(rows, cols, generator=gen)
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["noise", "one direction"])
+@pytest.mark.parametrize("coefficients", COEFFICIENTS)
+@pytest.mark.parametrize("rows, cols", [(1, 17), (64, 40), (40, 64), (300, 130)])
+def test_all_accepted_coefficients_fit(rows, cols, coefficients, kind, t):
+    g = matrix(kind, rows, cols).to(t).cuda()
+    got = D.ops.orthogonalize(g, steps=len(coefficients), coefficients=coefficients)
+    want, off = steps_and_bound(g, coefficients, 2.0 ** -11 if t == torch.bfloat16 else 2.0 ** -22)
+    half = torch.finfo(t).eps / 2
+    assert bool(torch.isfinite(got).all())
+    assert (got.double() - want).norm().item() <= off + half * (want.norm().item() + off) + 2.0 ** -25 * math.sqrt(g.numel())
+
+
+def test_gate_weights_and_dense_weights_take_the_same_step():
+    """The same matrix with columns of zeros behind it: once up to 16 columns, in 64 bits, once in planes."""
+    coefficients = ((20.0, -60.0, 48.0),)
+    gen = torch.Generator().manual_seed(3)
+    narrow = torch.randn(200, 16, generator=gen).cuda()
+    wide = torch.cat([narrow, torch.zeros(200, 8, device="cuda")], 1)
+    weights, momenta = [torch.zeros_like(narrow), torch.zeros_like(wide)], [torch.zeros_like(narrow), torch.zeros_like(wide)]
+    D.ops.muon_step(weights, [narrow, wide], momenta, lr=1.0, steps=1, coefficients=coefficients)
+    want, off = steps_and_bound(narrow, coefficients, 2.0 ** -22)
+    rate = math.sqrt(200 / 16), math.sqrt(200 / 24)
+    for w, r in zip(weights, rate):
+        assert bool(torch.isfinite(w).all())
+        assert (w[:, :16].double() / -r - want).norm().item() <= 2 * off + 2.0 ** -22 * want.norm().item()

@@ -1,0 +1,61 @@
+"""Which coefficients of Newton-Schulz steps are accepted: those that keep singular values at 8 or below, wherever they were on the way."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import difflogic_b200 as D
+from difflogic_b200 import _native as N
+
+
+def largest(coefficients, points=200001):
+    """Over a grid that is laid anew over what the step before has reached."""
+    reach = 1.0
+    for a, b, c in coefficients:
+        s = np.linspace(0, reach, points)
+        reach = np.abs(s * (a + s * s * (b + s * s * c))).max()
+    return reach
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_the_largest_value_is_found(seed):
+    rng = np.random.default_rng(seed)
+    sets = [tuple(rng.uniform(-1, 1, 3) * 10.0 ** rng.uniform(-1, 1.5)) for _ in range(3)]
+    if seed % 4 == 0:
+        sets = [(a, b, 0.0) for a, b, c in sets]
+    reach = 1.0
+    for s in sets:
+        reach = min(D.ops._largest_value(*s, reach), 50.0)
+    got, grid = 1.0, 1.0
+    for s in sets:
+        got = D.ops._largest_value(*s, got)
+        grid = largest([s], 20001) if grid == 1.0 else np.abs(np.polyval([s[2], 0, s[1], 0, s[0], 0], np.linspace(0, grid, 20001))).max()
+        assert abs(got - grid) <= 1e-5 * grid + 1e-12
+        got = grid = min(got, 50.0)
+
+
+@pytest.mark.parametrize("coefficients, fits", [(((20.0, -60.0, 48.0),), True), (((8.0, 0.0, 0.0),), True), (((8.1, 0.0, 0.0),), False),
+                                                (((8.0, 0.0, 0.0), (1.0, 0.0, 0.0)), True), (((8.0, 0.0, 0.0), (1.01, 0.0, 0.0)), False),
+                                                (((64.0, -64.0, 0.0),), False), (((24.0, -60.0, 44.0),), True), (((-8.0, 0.0, 0.0),), True),
+                                                # between the images of a grid over [0, 1] the second step's peak would be missed
+                                                (((8.0, 0.0, 0.0), (0.0, 0.0, -0.001)), False)])
+def test_coefficients_at_the_edge(coefficients, fits):
+    assert (largest(coefficients) <= 8.0 + 1e-6) == fits
+    steps, lib = len(coefficients), N.lib()
+    table = (ctypes.c_float * (3 * steps))(*[v for s in coefficients for v in s])
+    status = lib.dl_orthogonalize(None, None, 0, 4, 4, 0, steps, table, 1e-7, None, None)
+    assert lib.dl_muon_step_f32(None, 0, 0.1, 0.9, 1, 0.0, steps, table, 1e-7, None, None) == status
+    if fits:
+        assert status == N.DL_OK and list(D.ops._newton_schulz(coefficients, steps)) == list(table)
+    else:
+        assert status == N.DL_ERR_INVALID_ARG and "singular values" in N.last_error()
+        with pytest.raises(ValueError, match="near 1"):
+            D.ops._newton_schulz(coefficients, steps)
+
+
+def test_the_library_refuses_what_is_not_a_number():
+    for bad in ((float("nan"), 0.0, 0.0), (1.0, float("inf"), 0.0), (1.0, 0.0, -65.0)):
+        table = (ctypes.c_float * 3)(*bad)
+        assert N.lib().dl_orthogonalize(None, None, 0, 4, 4, 0, 1, table, 1e-7, None, None) == N.DL_ERR_INVALID_ARG
+        with pytest.raises(ValueError, match="near 1"):
+            D.ops._newton_schulz(bad, 1)
