@@ -61,11 +61,11 @@ square_sums_kernel(const Matrices all, int64_t count, double *__restrict__ parti
     }
 }
 
-// X = G / max(|G|, eps) as pairs.
+// X = G / max(|G|, eps) as pairs.  Norms whose inverse times 2^12 is no ordinary fp32 number take two factors, the first a power of two.
 __global__ void __launch_bounds__(kThreads)
 normalise_kernel(const Matrices all, int64_t rows, int64_t cols, const double *__restrict__ partial, int parts, double eps,
                  uint16_t *__restrict__ x, int64_t pitch, int64_t plane) {
-    __shared__ float s_scale;
+    __shared__ float s_first, s_scale;
     grid_dependency_wait();
     grid_dependents_launch();
     const int64_t z = blockIdx.y, base = all.stride * z;
@@ -77,12 +77,15 @@ normalise_kernel(const Matrices all, int64_t rows, int64_t cols, const double *_
         for (int i = threadIdx.x; i < parts; i += 32) sum += partial[z * parts + i];
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        const double norm = sqrt(sum);
-        // a norm that is not finite (an infinite or undefined entry) makes the whole result undefined
-        if (threadIdx.x == 0) s_scale = norm <= 1.7e308 ? (float)((double)kPairScale / (norm > eps ? norm : eps)) : __int_as_float(0x7fc00000);
+        const double norm = sqrt(sum), by = norm > eps ? norm : eps;
+        if (threadIdx.x == 0) {
+            s_first = by < 0x1p-64 ? 0x1p100f : by > 0x1p100 ? 0x1p-60f : 1.f;
+            // a norm that is not finite (an infinite or undefined entry) makes the whole result undefined
+            s_scale = norm <= 1.7e308 ? (float)((double)kPairScale / (by * s_first)) : __int_as_float(0x7fc00000);
+        }
     }
     __syncthreads();
-    const float scale = s_scale;
+    const float first = s_first, scale = s_scale;
     const int64_t quads = (cols + 3) / 4, total = rows * quads;
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
         const int64_t row = i / quads, col = (i - row * quads) * 4, at = base + row * cols + col;
@@ -96,8 +99,8 @@ normalise_kernel(const Matrices all, int64_t rows, int64_t cols, const double *_
             for (int j = 0; j < 4; ++j) v[j] = update_of(m[j], v[j], all.nesterov);
         }
         uint2 hi, lo;
-        split_two(v[0] * scale, v[1] * scale, hi.x, lo.x);
-        split_two(v[2] * scale, v[3] * scale, hi.y, lo.y);
+        split_two(v[0] * first * scale, v[1] * first * scale, hi.x, lo.x);
+        split_two(v[2] * first * scale, v[3] * first * scale, hi.y, lo.y);
         uint16_t *to = x + 2 * z * plane + row * pitch + col;
         *reinterpret_cast<uint2 *>(to) = hi;
         *reinterpret_cast<uint2 *>(to + plane) = lo;
@@ -442,6 +445,10 @@ static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64
 
 using namespace dl;
 
+// The smallest norm of a matrix that is not zero is 1.4e-45: any eps far below that is the same one, and the scales that it leads to, and
+// their squares, are finite.
+static double usable_eps(double eps) { return eps > 1e-60 ? eps : 1e-60; }
+
 // Matrices of so few columns stay as they are: their Gram matrix is iterated instead (gram_steps.cu).
 static bool few_columns(int64_t cols) { return cols <= kGramColumns; }
 
@@ -482,7 +489,7 @@ extern "C" DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, 
         job.matrix[0] = {g, nullptr, out, rows, 0.f};
         job.cols = (int)cols;
         job.type = type;
-        return launch_gram_steps(job, steps, coefficients, eps, reinterpret_cast<double *>(workspace), current_sms(), as_stream(stream), what);
+        return launch_gram_steps(job, steps, coefficients, usable_eps(eps), reinterpret_cast<double *>(workspace), current_sms(), as_stream(stream), what);
     }
     Matrices all = {};
     all.g[0] = g;
@@ -490,7 +497,7 @@ extern "C" DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, 
     all.type = type;
     OrthogonalEpilogue last = {};
     last.out = out;
-    return orthogonalise(all, batch, rows, cols, steps, coefficients, eps, last, reinterpret_cast<uint8_t *>(workspace), current_sms(),
+    return orthogonalise(all, batch, rows, cols, steps, coefficients, usable_eps(eps), last, reinterpret_cast<uint8_t *>(workspace), current_sms(),
                          as_stream(stream), what);
 }
 
@@ -627,7 +634,7 @@ extern "C" DL_API int dl_muon_step_f32(const int64_t *table, int64_t count, doub
             job.nesterov = toward;
             job.decay = decay;
             for (int i = 0; i < job.count; ++i) job.matrix[i].rate = rate(job.matrix[i].rows, job.cols);
-            return launch_gram_steps(job, steps, coefficients, eps, reinterpret_cast<double *>(workspace), sms, st, what);
+            return launch_gram_steps(job, steps, coefficients, usable_eps(eps), reinterpret_cast<double *>(workspace), sms, st, what);
         },
         [&](Matrices &all, int64_t batch, int64_t rows, int64_t cols) {
             all.type = kFloat32;
@@ -636,6 +643,6 @@ extern "C" DL_API int dl_muon_step_f32(const int64_t *table, int64_t count, doub
             OrthogonalEpilogue last = {};
             last.decay = decay;
             last.rate = rate(rows, cols);
-            return orthogonalise(all, batch, rows, cols, steps, coefficients, eps, last, reinterpret_cast<uint8_t *>(workspace), sms, st, what);
+            return orthogonalise(all, batch, rows, cols, steps, coefficients, usable_eps(eps), last, reinterpret_cast<uint8_t *>(workspace), sms, st, what);
         });
 }

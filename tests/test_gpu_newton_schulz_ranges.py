@@ -1,5 +1,5 @@
 """Newton-Schulz steps whose Gram matrices and polynomials are far from 1: everything that is kept between products has to fit its 16-bit
-planes for all coefficients that are accepted."""
+planes for all coefficients that are accepted, and so have the scales for all eps and sizes of values."""
 import math
 
 import pytest
@@ -77,3 +77,28 @@ def test_gate_weights_and_dense_weights_take_the_same_step():
     for w, r in zip(weights, rate):
         assert bool(torch.isfinite(w).all())
         assert (w[:, :16].double() / -r - want).norm().item() <= 2 * off + 2.0 ** -22 * want.norm().item()
+
+
+@pytest.mark.parametrize("rows, cols", [(60, 16), (60, 40), (40, 90), (5, 7)])
+@pytest.mark.parametrize("eps", [1e-30, 1e-36, 1e-44, 1e-160, 5e-324])
+def test_any_eps(rows, cols, eps):
+    assert not D.ops.orthogonalize(torch.zeros(rows, cols, device="cuda"), eps=eps).any()
+    g = matrix("noise", rows, cols).cuda()
+    got = D.ops.orthogonalize(torch.stack([g, torch.zeros_like(g), g]), eps=eps)
+    assert not got[1].any() and torch.equal(got[0], got[2])
+    want, off = steps_and_bound(g, [D.ops.NEWTON_SCHULZ] * 5, 2.0 ** -22)
+    assert (got[0].double() - want).norm().item() <= off + 2.0 ** -23 * want.norm().item()
+    w, m = torch.ones(rows, cols, device="cuda"), torch.zeros(rows, cols, device="cuda")
+    D.ops.muon_step([w], [torch.zeros_like(w)], [m], lr=0.1, eps=eps)
+    assert torch.equal(w, torch.ones_like(w))
+
+
+@pytest.mark.parametrize("rows, cols", [(60, 16), (60, 40), (40, 90)])
+@pytest.mark.parametrize("size", [2.0 ** -140, 2.0 ** -126, 2.0 ** -100, 2.0 ** 100, 2.0 ** 125])
+def test_the_smallest_and_the_largest_matrices(rows, cols, size):
+    """Brought to norm 1, a matrix is what it was before all its entries were multiplied with a power of two."""
+    g = (matrix("noise", rows, cols) * size).cuda()      # rounded to what is left of 24 bits down there
+    assert bool(torch.isfinite(g).all())
+    got = D.ops.orthogonalize(g, eps=1e-60)
+    want, off = steps_and_bound(g, [D.ops.NEWTON_SCHULZ] * 5, 2.0 ** -22, eps=1e-60)
+    assert (got.double() - want).norm().item() <= off + 2.0 ** -23 * want.norm().item()
