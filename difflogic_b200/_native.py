@@ -110,6 +110,8 @@ SIGNATURES = {
     "dl_dense_forward_sizes": (None, [_ptr, _i64, _int, _ptr, _i64, _i64, _i64, _int, _int, _ptr]),
     "dl_dense_forward": (_int, [_ptr, _i64, _int, _ptr, _ptr, _ptr, _i64, _i64, _int, _ptr, _int, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64,
                                 _int, _ptr]),
+    "dl_dense_planes_bytes": (_i64, [_i64, _i64, _int]),
+    "dl_dense_lay_out": (_int, [_ptr, _i64, _i64, _i64, _int, _ptr, _ptr]),
     "dl_dense_backward_workspace_bytes": (_i64, [_ptr, _int, _int, _ptr, _i64, _int, _ptr, _int, _int, _i64, _i64, _i64, _int]),
     "dl_dense_backward": (_int, [_ptr, _int, _ptr, _ptr, _i64, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _int, _ptr]),
     "dl_orthogonalize_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),

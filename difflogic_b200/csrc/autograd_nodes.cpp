@@ -341,14 +341,31 @@ DenseOut dense_forward(const Tensor &x, const Tensor &w, const Tensor &bias, con
     return o;
 }
 
+// The planes of an operand, as its products read them.
+Tensor lay_out(const Matrix &m) {
+    const int64_t rows = m.t.size(m.feature_major), cols = m.t.size(!m.feature_major);
+    const int kind = kind_of(m.t.scalar_type());
+    const Tensor planes = bytes(dl_dense_planes_bytes(rows, cols, kind), m.t);
+    check(dl_dense_lay_out(m.t.data_ptr(), rows, cols, m.pitch, kind, planes.data_ptr(), stream_of(m.t)));
+    return planes;
+}
+
 struct DenseNode : torch::autograd::Function<DenseNode> {
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const std::optional<Tensor> &b, const std::optional<Tensor> &r,
                           int64_t act, bool feature_major) {
         const Tensor bias = b.value_or(Tensor()), residual = r.value_or(Tensor());
-        const DenseOut o = dense_forward(x, w, bias, residual, (int)act, feature_major, true);
+        DenseOut o = dense_forward(x, w, bias, residual, (int)act, feature_major, true);
         ctx->set_materialize_grads(false);
+        bool keep_x = !o.x_planes.defined(), keep_w = !o.w_planes.defined();
+        if (x.scalar_type() == at::kFloat && keep_w) {
+            // Few samples.  An optimizer's kernels may change fp32 parameters before the backward pass, without autograd's version counters: it
+            // gets the values that were read here, laid out now as it would do itself.
+            if (w.requires_grad()) o.x_planes = lay_out(o.x);
+            if (x.requires_grad()) o.w_planes = lay_out({w, w.size(1), false});
+            keep_x = keep_w = false;
+        }
         // what was laid out for the product serves the backward pass too, in place of the tensor itself
-        ctx->save_for_backward({o.x_planes.defined() ? Tensor() : o.x.t, o.w_planes.defined() ? Tensor() : w, o.x_planes, o.w_planes, o.slope});
+        ctx->save_for_backward({keep_x ? o.x.t : Tensor(), keep_w ? w : Tensor(), o.x_planes, o.w_planes, o.slope});
         ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(0), x.size(1), w.size(0), o.x.pitch, o.x.feature_major, feature_major, b.has_value(), r.has_value()};
         // their alignment decided what was laid out
         ctx->saved_data["at"] = std::vector<int64_t>{(int64_t)o.x.t.data_ptr(), (int64_t)w.data_ptr()};

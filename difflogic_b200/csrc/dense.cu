@@ -481,6 +481,20 @@ extern "C" DL_API void dl_dense_forward_sizes(const void *x, int64_t x_pitch, in
     sizes[2] = plan_forward(batch, inner, outer, y_feature_major != 0, l.planes, current_sms()).partial_bytes;
 }
 
+extern "C" DL_API int64_t dl_dense_planes_bytes(int64_t rows, int64_t cols, int type) {
+    if (rows <= 0 || cols <= 0) return 0;
+    return padded_bytes((type == kFloat32 ? 3 : 1) * rows * padded(cols) * 2);
+}
+
+extern "C" DL_API int dl_dense_lay_out(const void *src, int64_t rows, int64_t cols, int64_t pitch, int type, void *planes, void *stream) {
+    const char *what = "dl_dense_lay_out";
+    int status;
+    if (!dense_sizes(0, rows, cols, type, what, &status)) return status;
+    DL_REQUIRE(src && planes && aligned_to(planes, 16), DL_ERR_INVALID_ARG, "%s: null pointer or planes that are not 16-byte aligned", what);
+    DL_REQUIRE(pitch >= cols, DL_ERR_INVALID_ARG, "%s: rows overlap", what);
+    return lay_out(src, rows, cols, pitch, type, planes, padded(cols), rows * padded(cols), current_sms(), as_stream(stream), what);
+}
+
 extern "C" DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_feature_major, const void *w, const void *bias, const void *residual,
                                        int64_t residual_batch, int64_t residual_feature, int act, void *y, int y_feature_major, void *slope,
                                        void *x_planes, void *w_planes, void *workspace, int64_t batch, int64_t inner, int64_t outer, int type,

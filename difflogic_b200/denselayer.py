@@ -62,14 +62,31 @@ def _forward(x, w, bias, residual, act, feature_major, want_slope):
     return y, slope, x, x_planes, w_planes
 
 
+def _lay_out(t, pitch, feature_major):
+    """The planes of an operand, as its products read them."""
+    rows, cols = reversed(t.shape) if feature_major else t.shape
+    lib, kind = N.lib(), TYPES[t.dtype]
+    with N.on_device(t):
+        planes = _bytes(lib.dl_dense_planes_bytes(rows, cols, kind), t)
+        N.check(lib.dl_dense_lay_out(t.data_ptr(), rows, cols, pitch, kind, planes.data_ptr(), N.stream_of(t)))
+    return planes
+
+
 class DenseFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, act, feature_major):
         ctx.set_materialize_grads(False)
         y, slope, read, x_planes, w_planes = _forward(x, w, bias, residual, act, feature_major, True)
-        # what was laid out for the product serves the backward pass too, in place of the tensor itself
-        ctx.save_for_backward(read if x_planes is None else None, w if w_planes is None else None, x_planes, w_planes, slope)
         _, ctx.pitch, ctx.x_feature = _layout(read)
+        keep_x, keep_w = x_planes is None, w_planes is None
+        if x.dtype == torch.float32 and keep_w and x.shape[0] > 0:
+            # Few samples.  An optimizer's kernels may change fp32 parameters before the backward pass, without autograd's version counters:
+            # it gets the values that were read here, laid out now as it would do itself.
+            x_planes = _lay_out(read, ctx.pitch, ctx.x_feature) if ctx.needs_input_grad[1] else None
+            w_planes = _lay_out(w, w.shape[1], False) if ctx.needs_input_grad[0] else None
+            keep_x = keep_w = False
+        # what was laid out for the product serves the backward pass too, in place of the tensor itself
+        ctx.save_for_backward(read if keep_x else None, w if keep_w else None, x_planes, w_planes, slope)
         ctx.x_ptr, ctx.w_ptr = read.data_ptr(), w.data_ptr()     # their alignment decided what was laid out
         ctx.sizes = (x.shape[0], x.shape[1], w.shape[0])
         ctx.has_bias, ctx.feature_major, ctx.act = bias is not None, feature_major, act

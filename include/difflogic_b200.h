@@ -567,6 +567,8 @@ DL_API int dl_backward_w_announce_f32(const float *x, const int64_t *a, const in
  *
  * gy contiguous in y's layout or the other one, slope (NULL: no activation) in gy's; gx, gw, gb NULL: not wanted.  x_planes, w_planes:
  * those of the forward pass, or NULL: then x and w are there, and the workspace has room for them (lay_x, lay_w: asked for with NULL).
+ * dl_dense_lay_out makes them where the forward pass did without (few samples), for operands that may change before the backward pass:
+ * rows x cols values as they lie in memory, rows `pitch` apart (x_feature_major: rows are features), dl_dense_planes_bytes bytes.
  * ---------------------------------------------------------------------------------------- */
 enum { DL_ACT_NONE = 0, DL_ACT_RELU = 1, DL_ACT_SIGMOID = 2, DL_ACT_SILU = 3, DL_ACT_GELU = 4 };
 DL_API void dl_dense_forward_sizes(const void *x, int64_t x_pitch, int x_feature_major, const void *w, int64_t batch, int64_t inner,
@@ -575,6 +577,8 @@ DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_feature_major,
                             int64_t residual_batch, int64_t residual_feature, int act, void *y, int y_feature_major, void *slope,
                             void *x_planes, void *w_planes, void *workspace, int64_t batch, int64_t inner, int64_t outer, int type,
                             void *stream);
+DL_API int64_t dl_dense_planes_bytes(int64_t rows, int64_t cols, int type);
+DL_API int dl_dense_lay_out(const void *src, int64_t rows, int64_t cols, int64_t pitch, int type, void *planes, void *stream);
 DL_API int64_t dl_dense_backward_workspace_bytes(const void *gy, int g_feature_major, int has_slope, const void *x, int64_t x_pitch,
                                                  int x_feature_major, const void *w, int lay_x, int lay_w, int64_t batch, int64_t inner,
                                                  int64_t outer, int type);
