@@ -547,6 +547,12 @@ PyObject *muon_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
         const Tensor work = bytes(dl_muon_workspace_bytes(table.data(), matrices), first);
         check(dl_muon_step_f32(table.data(), matrices, lr, momentum, nesterov, decay, (int)steps, coefficients, eps, pointer(work), stream_of(first)));
     }
+    // in place, for whoever has kept these for a backward pass; tensors of inference mode have no counters
+    for (Py_ssize_t i = 0; i < n; ++i)
+        for (int j : {0, 2}) {
+            const Tensor &t = THPVariable_Unpack(PyList_GET_ITEM(args[j], i));
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+        }
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
 }

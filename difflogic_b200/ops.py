@@ -1014,7 +1014,8 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
     """One step of the Muon optimizer on matrices, in place: for every weight w with its gradient g and momentum buffer m
         m += (1 - momentum) (g - m);  u = g + momentum (m - g) (nesterov) or m
         w = (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) orthogonalize(u)
-    which is torch.optim.Muon's rule, in 32 bits.  weights, grads, momenta: lists of 2-D contiguous float32 tensors on one CUDA device, of
+    which is torch.optim.Muon's rule, in 32 bits.  For autograd weights and momenta have changed in place: what was computed from them
+    before and needs them for its gradient cannot be differentiated any more.  weights, grads, momenta: lists of 2-D contiguous float32 tensors on one CUDA device, of
     which no weight or momentum shares memory with another tensor of the lists."""
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     if not len(weights) == len(grads) == len(momenta):
@@ -1054,4 +1055,7 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
     with N.on_device(weights[0]):
         work = torch.empty(lib.dl_muon_workspace_bytes(entries, count), dtype=torch.uint8, device=device)
         N.check(lib.dl_muon_step_f32(entries, count, lr, momentum, nesterov, weight_decay, steps, table, eps, work.data_ptr(), N.stream_of(weights[0])))
+    for t in weights + momenta:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
     count_update(weights)

@@ -1,4 +1,5 @@
-"""Optimizer steps between a forward and a backward pass: gradients of dense layers are those of the weights that the forward pass read."""
+"""Optimizer steps between a forward and a backward pass: gradients of dense layers are those of the weights that the forward pass read, and
+what a step changes in place counts as changed for autograd where it was called on tensors of anybody's graph."""
 import pytest
 import torch
 
@@ -34,3 +35,36 @@ def test_gradients_are_those_of_the_weights_that_were_read(rows, optimizer, way,
     assert all(torch.equal(p, q) for p, q in zip(want, got))
     again = torch.autograd.grad(y, leaves, gy)
     assert all(torch.equal(p, q) for p, q in zip(want, again))
+
+
+@pytest.mark.parametrize("way", ["native", "python"])
+def test_muon_step_is_in_place_for_autograd(way):
+    class Weight(torch.nn.Parameter):      # not what the native call takes
+        pass
+
+    torch.manual_seed(0)
+    w, x = torch.randn(8, 20, device="cuda"), torch.randn(5, 20, device="cuda", requires_grad=True)
+    w = torch.nn.Parameter(w) if way == "native" else Weight(w)
+    g, m = torch.randn(8, 20, device="cuda"), torch.zeros(8, 20, device="cuda")
+    y = torch.nn.functional.linear(x, w)
+    versions = w._version, g._version, m._version
+    D.ops.muon_step([w], [g], [m], lr=0.1)
+    assert (w._version, g._version, m._version) == (versions[0] + 1, versions[1], versions[2] + 1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    D.dense(x, w).sum().backward()         # the weights as they are now
+    assert torch.allclose(x.grad, w.detach().sum(0).expand(5, 20), rtol=1e-5, atol=1e-5)
+    with torch.inference_mode():
+        state = [torch.randn(8, 20, device="cuda") for _ in range(3)]
+        D.ops.muon_step(state[:1], state[1:2], state[2:], lr=0.1)      # these have no counters
+
+
+def test_an_optimizers_step_leaves_version_counters_alone():
+    model = torch.nn.Sequential(D.DenseLayer(20, 30), D.LogicLayer(30, 40), D.GroupSum(4))
+    opt = FlatMuon(model.parameters(), lr=0.1)
+    versions = [p._version for p in model.parameters()]
+    loss = model(torch.randn(40, 20, device="cuda")).sum()
+    loss.backward(retain_graph=True)
+    opt.step()
+    assert versions == [p._version for p in model.parameters()]
+    loss.backward()
