@@ -4,8 +4,9 @@ A logic network reads values between 0 and 1.  `DenseLayer` learns them -- an en
 feature-major layout that logic layers read -- or makes the fully connected networks that the reference compares with
 (experiments/main_baseline.py).  With `implementation='cuda'` it runs on csrc/dense.cu:
 
-* bf16 and fp16 layers multiply their values as they are, fp32 layers three bf16 planes of each value, which is as exact as 32-bit
-  arithmetic; all sums are 32-bit, results are rounded once;
+* bf16 and fp16 layers multiply their values as they are, fp32 layers three bf16 planes of each value, all 24 bits, or in the forward pass
+  of up to 32 samples two parts of 11 bits (a product is then up to 2^-21 off, of either sign): results are no further off than those of
+  32-bit arithmetic; all sums are 32-bit, results are rounded once;
 * the backward pass multiplies the incoming gradient with the kept derivative of the activation (fp32, or for bf16
   layers fp16 times 2^14) and rounds the product to the layer's type before the two matrix products.
 
