@@ -22,6 +22,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -427,15 +428,33 @@ struct DenseNode : torch::autograd::Function<DenseNode> {
 };
 
 // A leaf of a graph that lives has its accumulator on the stream that the graph was made on, and a captured backward pass brings that
-// stream into the capture.  The default stream cannot be brought in, and the process ends: refused here instead.
+// stream into the capture.  The default stream cannot be brought in, and the process ends: refused here instead.  t is a leaf, or made of
+// one by operations on it alone (views, reshaping, copies).
 void refuse_older_graph(const Tensor &t) {
-    if (!t.defined() || !t.is_leaf() || !t.requires_grad()) return;
-    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
-    if (accumulator == nullptr) return;
-    const auto stream = accumulator->stream();
+    if (!t.defined() || !t.requires_grad()) return;
+    std::shared_ptr<torch::autograd::Node> node = t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn();
+    while (node != nullptr && dynamic_cast<torch::autograd::AccumulateGrad *>(node.get()) == nullptr)
+        node = node->num_outputs() == 1 ? node->next_edge(0).function : nullptr;
+    if (node == nullptr) return;
+    const auto stream = node->stream();
     TORCH_CHECK(!stream || *stream != c10::cuda::getDefaultCUDAStream(t.device().index()).unwrap(),
                 "difflogic_b200: dense is captured while a graph of the same tensors, made on the default stream, is alive; delete its outputs before the "
                 "capture");
+}
+bool capturing() { return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; }
+
+// refuse_older_graphs(x, weight, bias | None, residual | None): for calls that take the Python functions
+PyObject *refuse_older_graphs(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        if (!THPVariable_Check(args[i])) continue;
+        const Tensor &t = THPVariable_Unpack(args[i]);
+        if (!t.is_cuda()) continue;
+        const c10::cuda::CUDAGuard guard(t.device());
+        if (capturing()) refuse_older_graph(t);
+    }
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
 }
 
 // dense(x, weight, bias | None, residual | None, activation, feature_major) -> output, or None
@@ -479,14 +498,14 @@ PyObject *dense(PyObject *, PyObject *const *args, Py_ssize_t count) {
     {
         const WithoutGil nogil;
         const c10::cuda::CUDAGuard guard(device);
+        const bool graph = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (bias.defined() && bias.requires_grad()) ||
+                                                          (residual.defined() && residual.requires_grad()));
+        if (graph && capturing())
+            for (const Tensor &t : {x, w, bias, residual}) refuse_older_graph(t);
         if (x.dim() != 2) {
             x = x.reshape({-1, x.size(-1)});
             if (residual.defined()) residual = residual.reshape({-1, outer});
         }
-        const bool graph = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (bias.defined() && bias.requires_grad()) ||
-                                                          (residual.defined() && residual.requires_grad()));
-        if (graph && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
-            for (const Tensor &t : {x, w, bias, residual}) refuse_older_graph(t);
         const auto given = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
         y = graph ? DenseNode::apply(x, w, given(bias), given(residual), (int64_t)act, (bool)feature_major)
                   : dense_forward(x, w, bias, residual, (int)act, feature_major, false).y;
@@ -604,6 +623,7 @@ PyObject *connect(PyObject *, PyObject *dict) {
 PyMethodDef kMethods[] = {{"layer", (PyCFunction)(void *)layer, METH_FASTCALL, nullptr},
                           {"group_sum", (PyCFunction)(void *)group_sum, METH_FASTCALL, nullptr},
                           {"dense", (PyCFunction)(void *)dense, METH_FASTCALL, nullptr},
+                          {"refuse_older_graphs", (PyCFunction)(void *)refuse_older_graphs, METH_FASTCALL, nullptr},
                           {"muon_step", (PyCFunction)(void *)muon_step, METH_FASTCALL, nullptr},
                           {"orthogonalize", (PyCFunction)(void *)orthogonalize, METH_FASTCALL, nullptr},
                           {"launches", launches, METH_NOARGS, nullptr},

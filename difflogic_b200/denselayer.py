@@ -151,10 +151,10 @@ def dense(x, weight, bias=None, residual=None, activation=None, feature_major=Fa
 
     x `[..., in]`, weight `[out, in]`, bias `[out]`, residual `[..., out]`, all of one type (float32, bfloat16 or float16) on one CUDA
     device; activation: None, 'relu', 'sigmoid', 'silu' or 'gelu' (the exact one).  x may be a transposed view, as logic layers return
-    them.  An infinite float32
-    operand makes the results it enters infinite or undefined.  A call that a CUDA graph captures is refused while an
-    earlier graph of its leaves, made on the default stream, is alive.  feature_major: a 2-D result lies in memory as `[out, batch]` (same values, other strides), which a LogicLayer reads without a
-    copy."""
+    them.  An infinite float32 operand makes the results it enters infinite or undefined.  A call that a CUDA graph captures is refused
+    while an earlier graph, made on the default stream, is alive that has one of these tensors as a leaf, or the leaf that one of them is a
+    view, reshape or copy of.  feature_major: a 2-D result lies in memory as `[out, batch]` (same values, other strides), which a LogicLayer
+    reads without a copy."""
     act = ACTIVATIONS.get(activation, -1)
     if act >= 0 and x.is_cuda:
         # the native node; None for a call that is not of the ordinary form
@@ -168,12 +168,15 @@ def dense(x, weight, bias=None, residual=None, activation=None, feature_major=Fa
     if feature_major and x.dim() != 2:
         raise ValueError("dense: feature_major needs a 2-D x, got %d dimensions" % x.dim())
     lead, outer = x.shape[:-1], weight.shape[0]
+    graph = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
+    if graph:
+        N.nodes().refuse_older_graphs(x, weight, bias, residual)
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
         residual = None if residual is None else residual.reshape(-1, outer)
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if graph:
         y = DenseFunction.apply(x, weight, bias, residual, act, bool(feature_major))
     else:
         y = _forward(x, weight, bias, residual, act, bool(feature_major), False)[0]
