@@ -107,6 +107,7 @@ SIGNATURES = {
     "dl_backward_w_announce_f32": (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _int, _int, _int, _ptr,
                                           _ptr, _ptr, _int, _int, _ptr]),
     "dl_adam_step_f32": (_int, [_ptr, _ptr, _ptr, _ptr, _i64, _f32, _f32, _f32, _f32, _f32, _ptr, _ptr]),
+    "dl_matmul_choice": (_int, []),
     "dl_dense_forward_sizes": (None, [_ptr, _i64, _int, _ptr, _i64, _i64, _i64, _int, _int, _ptr]),
     "dl_dense_forward": (_int, [_ptr, _i64, _int, _ptr, _ptr, _ptr, _i64, _i64, _int, _ptr, _int, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64,
                                 _int, _ptr]),

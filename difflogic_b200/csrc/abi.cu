@@ -85,6 +85,9 @@ extern "C" DL_API int dl_set_tuning(int key, int value) {
     return DL_OK;
 }
 
+extern "C" DL_API int dl_matmul_choice(void) {
+    return (dl::tuning(DL_TUNE_MATMUL_COLUMNS) & 0x3ff) << 8 | (dl::tuning(DL_TUNE_MATMUL_SPLITS) & 0xfff) << 18;
+}
 extern "C" DL_API int dl_get_tuning(int key) { return key >= 0 && key < DL_TUNE_COUNT ? dl::tuning(key) : -1; }
 
 extern "C" DL_API int dl_coefs_f32(const float *w, int w_mode, float *coef, int64_t n_out, void *stream) {

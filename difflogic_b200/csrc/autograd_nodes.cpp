@@ -325,7 +325,7 @@ struct DenseOut {
 };
 DenseOut dense_forward(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &residual, int act, bool feature_major, bool want_slope) {
     const int64_t batch = x.size(0), inner = x.size(1), outer = w.size(0);
-    const int kind = kind_of(x.scalar_type());
+    const int kind = kind_of(x.scalar_type()) | dl_matmul_choice();
     const auto options = x.options().requires_grad(false);
     DenseOut o;
     o.y = feature_major ? at::empty_strided({batch, outer}, {1, batch}, options) : at::empty({batch, outer}, options);
@@ -406,7 +406,7 @@ struct DenseNode : torch::autograd::Function<DenseNode> {
             if (want_b) out[2] = at::empty({outer}, options);
             const Matrix read = x.defined() ? readable(x) : Matrix{Tensor(), pitch, (bool)sizes[4]};
             const void *px = x.defined() ? x.data_ptr() : (const void *)at[0], *pw = w.defined() ? w.data_ptr() : (const void *)at[1];
-            const int kind = kind_of(gy.scalar_type());
+            const int kind = kind_of(gy.scalar_type()) | dl_matmul_choice();
             const Tensor work = bytes(dl_dense_backward_workspace_bytes(g.data_ptr(), feature_major, slope.defined(), px, read.pitch, read.feature_major,
                                                                         pw, want_w && !x_planes.defined(), want_x && !w_planes.defined(), batch, inner,
                                                                         outer, kind),
@@ -600,8 +600,9 @@ PyObject *orthogonalize(PyObject *, PyObject *const *args, Py_ssize_t count) {
         const at::NoGradGuard no_grad;
         out = at::empty_like(x, x.options().requires_grad(false));
         const int64_t rows = x.size(-2), cols = x.size(-1), batch = x.numel() / (rows * cols);
-        const Tensor work = bytes(dl_orthogonalize_workspace_bytes(batch, rows, cols, kind_of(type)), x);
-        check(dl_orthogonalize(x.data_ptr(), out.data_ptr(), batch, rows, cols, kind_of(type), (int)steps, coefficients, eps, pointer(work), stream_of(x)));
+        const int kind = kind_of(type) | dl_matmul_choice();
+        const Tensor work = bytes(dl_orthogonalize_workspace_bytes(batch, rows, cols, kind), x);
+        check(dl_orthogonalize(x.data_ptr(), out.data_ptr(), batch, rows, cols, kind, (int)steps, coefficients, eps, pointer(work), stream_of(x)));
     }
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS

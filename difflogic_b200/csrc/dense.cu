@@ -442,9 +442,9 @@ static int launch_layer(const Product &p, const MatmulPlan &plan, const DenseOut
 // neighbouring lanes; but few samples fill half of a tile's 64 columns rather than half of its 128 rows.
 static bool features_as_rows(int64_t batch, bool feature_major) { return feature_major || batch <= 64; }
 
-static MatmulPlan plan_forward(int64_t batch, int64_t inner, int64_t outer, bool feature_major, int planes, int sms) {
-    return features_as_rows(batch, feature_major) ? plan_matmul(outer, batch, inner, 1, planes, false, sms)
-                                                  : plan_matmul(batch, outer, inner, 1, planes, false, sms);
+static MatmulPlan plan_forward(int64_t batch, int64_t inner, int64_t outer, bool feature_major, int planes, int sms, int choice) {
+    return features_as_rows(batch, feature_major) ? plan_matmul(outer, batch, inner, 1, planes, false, sms, choice)
+                                                  : plan_matmul(batch, outer, inner, 1, planes, false, sms, choice);
 }
 
 static int gradient_columns(int type) { return type == kFloat32 ? kGradientColumns<float> : kGradientColumns<__half>; }
@@ -473,12 +473,13 @@ using namespace dl;
 
 extern "C" DL_API void dl_dense_forward_sizes(const void *x, int64_t x_pitch, int x_feature_major, const void *w, int64_t batch, int64_t inner,
                                              int64_t outer, int y_feature_major, int type, int64_t *sizes) {
+    const int choice = matmul_choice(&type);
     sizes[0] = sizes[1] = sizes[2] = 0;
     if (batch <= 0 || inner <= 0 || outer <= 0 || dense_rows_applicable(batch, type)) return;
     const DenseLayout l = dense_layout(batch, inner, outer, x_pitch, x_feature_major != 0, type, x, w);
     sizes[0] = l.x_bytes;
     sizes[1] = l.w_bytes;
-    sizes[2] = plan_forward(batch, inner, outer, y_feature_major != 0, l.planes, current_sms()).partial_bytes;
+    sizes[2] = plan_forward(batch, inner, outer, y_feature_major != 0, l.planes, current_sms(), choice).partial_bytes;
 }
 
 extern "C" DL_API int64_t dl_dense_planes_bytes(int64_t rows, int64_t cols, int type) {
@@ -500,6 +501,7 @@ extern "C" DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_fea
                                        void *x_planes, void *w_planes, void *workspace, int64_t batch, int64_t inner, int64_t outer, int type,
                                        void *stream) {
     const char *what = "dl_dense_forward";
+    const int choice = matmul_choice(&type);
     int status;
     if (!dense_sizes(batch, inner, outer, type, what, &status)) return status;
     DL_REQUIRE(act >= DL_ACT_NONE && act <= DL_ACT_GELU, DL_ERR_INVALID_ARG, "%s: unknown activation %d", what, act);
@@ -514,7 +516,7 @@ extern "C" DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_fea
                                y_feature_major != 0};
         return launch_dense_rows(x, x_pitch, x_feature_major != 0, w, e, batch, inner, outer, type, sms, st);
     }
-    const MatmulPlan plan = plan_forward(batch, inner, outer, y_feature_major != 0, l.planes, sms);
+    const MatmulPlan plan = plan_forward(batch, inner, outer, y_feature_major != 0, l.planes, sms, choice);
     DL_REQUIRE((!l.lay_x || x_planes) && (!l.lay_w || w_planes) && (plan.partial_bytes == 0 || workspace), DL_ERR_INVALID_ARG,
                "%s: a workspace is missing", what);
     DL_REQUIRE(aligned_to(x_planes, 16) && aligned_to(w_planes, 16) && aligned_to(workspace, 16), DL_ERR_INVALID_ARG,
@@ -570,7 +572,7 @@ struct DenseBackward {
 };
 
 static DenseBackward plan_backward(const DenseLayout &l, int64_t batch, int64_t inner, int64_t outer, bool g_feature_major, int type, bool act,
-                                   const void *gy, bool lay_x, bool lay_w, int sms) {
+                                   const void *gy, bool lay_x, bool lay_w, int sms, int choice) {
     DenseBackward b = {};
     b.planes = type == kFloat32 ? 3 : 1;
     b.g_rows = g_feature_major ? outer : batch;
@@ -582,8 +584,8 @@ static DenseBackward plan_backward(const DenseLayout &l, int64_t batch, int64_t 
     b.strips = strips_of(b.g_rows, b.g_cols, type, sms, &b.strip);
     b.parts = g_feature_major ? ceil_div(b.g_cols, gradient_columns(type)) : b.strips;
     b.bias_bytes = padded_bytes(b.parts * outer * 4);
-    b.to_x = plan_matmul(batch, inner, outer, 1, b.planes, false, sms);
-    b.to_w = plan_matmul(outer, inner, batch, 1, b.planes, false, sms);
+    b.to_x = plan_matmul(batch, inner, outer, 1, b.planes, false, sms, choice);
+    b.to_w = plan_matmul(outer, inner, batch, 1, b.planes, false, sms, choice);
     b.partial_bytes = padded_bytes(b.to_x.partial_bytes > b.to_w.partial_bytes ? b.to_x.partial_bytes : b.to_w.partial_bytes);
     b.x_bytes = lay_x ? l.x_bytes : 0;
     b.w_bytes = lay_w ? l.w_bytes : 0;
@@ -595,15 +597,17 @@ static DenseBackward plan_backward(const DenseLayout &l, int64_t batch, int64_t 
 extern "C" DL_API int64_t dl_dense_backward_workspace_bytes(const void *gy, int g_feature_major, int has_slope, const void *x, int64_t x_pitch,
                                                             int x_feature_major, const void *w, int lay_x, int lay_w, int64_t batch, int64_t inner,
                                                             int64_t outer, int type) {
+    const int choice = matmul_choice(&type);
     if (batch <= 0 || inner <= 0 || outer <= 0) return 0;
     const DenseLayout l = dense_layout(batch, inner, outer, x_pitch, x_feature_major != 0, type, x, w);
-    return plan_backward(l, batch, inner, outer, g_feature_major != 0, type, has_slope != 0, gy, lay_x != 0, lay_w != 0, current_sms()).total();
+    return plan_backward(l, batch, inner, outer, g_feature_major != 0, type, has_slope != 0, gy, lay_x != 0, lay_w != 0, current_sms(), choice).total();
 }
 
 extern "C" DL_API int dl_dense_backward(const void *gy, int g_feature_major, const void *slope, const void *x, int64_t x_pitch, int x_feature_major,
                                         const void *w, const void *x_planes, const void *w_planes, void *gx, void *gw, void *gb, void *workspace,
                                         int64_t batch, int64_t inner, int64_t outer, int type, void *stream) {
     const char *what = "dl_dense_backward";
+    const int choice = matmul_choice(&type);
     int status;
     if (!dense_sizes(batch, inner, outer, type, what, &status)) return status;
     DL_REQUIRE(batch > 0, DL_ERR_INVALID_ARG, "%s: empty batch", what);
@@ -612,7 +616,7 @@ extern "C" DL_API int dl_dense_backward(const void *gy, int g_feature_major, con
     const int sms = current_sms();
     const DenseLayout l = dense_layout(batch, inner, outer, x_pitch, x_feature_major != 0, type, x, w);
     const bool lay_x = gw && l.lay_x && !x_planes, lay_w = gx && l.lay_w && !w_planes;
-    const DenseBackward b = plan_backward(l, batch, inner, outer, g_feature_major != 0, type, slope != nullptr, gy, lay_x, lay_w, sms);
+    const DenseBackward b = plan_backward(l, batch, inner, outer, g_feature_major != 0, type, slope != nullptr, gy, lay_x, lay_w, sms, choice);
     DL_REQUIRE((!lay_x || x) && (!lay_w || w), DL_ERR_INVALID_ARG, "%s: null pointer", what);
     cudaStream_t st = as_stream(stream);
     uint8_t *at = reinterpret_cast<uint8_t *>(workspace);

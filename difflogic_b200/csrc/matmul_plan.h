@@ -5,6 +5,14 @@
 
 namespace dl {
 
+// What a caller wants of a plan (dl_matmul_choice), in the bits of a type above the lowest eight.  The plan depends on nothing but the
+// arguments of a call, so that the one that asks for a workspace and the one that uses it make the same.
+static inline int matmul_choice(int *type) {
+    const int choice = *type >> 8;
+    *type &= 0xff;
+    return choice;
+}
+
 struct MatmulPlan {
     int columns;            // of a tile: 64 or 128, or 256 with two CTAs to a tile of 256 rows
     bool pair;
@@ -28,12 +36,12 @@ static inline int64_t tiles_of(int64_t m, int64_t n, int64_t rows, int64_t colum
 // clocks; a pair's 256 x 256 128); its copies, 60 bytes a clock; shared memory, which the products read and the copies write, 125 bytes a
 // clock.  A tile ends with its epilogue, which the next tile's steps hide, the last one's do not; a join of splits costs a launch and
 // moves the sums once more.  The cheapest of the tile widths and splits is taken.
-static inline MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, int64_t batch, int planes, bool symmetric, int sms) {
+static inline MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, int64_t batch, int planes, bool symmetric, int sms, int choice) {
     MatmulPlan best = {};
     double best_clocks = 0;
     const int64_t steps = ceil_div(k, 64);
     const int products = planes == 1 ? 1 : planes == 2 ? 3 : 6;
-    const int only_columns = tuning(DL_TUNE_MATMUL_COLUMNS), only_splits = tuning(DL_TUNE_MATMUL_SPLITS);
+    const int wanted = choice & 0x3ff, only_columns = wanted == 64 || wanted == 128 || wanted == 256 ? wanted : 0, only_splits = choice >> 10;
     for (int columns = 64; columns <= 256; columns *= 2) {
         const bool pair = columns == 256;
         if (only_columns > 0 ? columns != only_columns : columns > 64 && n <= columns / 2) continue;

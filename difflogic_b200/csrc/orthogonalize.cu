@@ -286,7 +286,7 @@ struct OrthogonalLayout {
     int64_t total() const { return 2 * x_bytes + 2 * s_bytes + norm_bytes + partial_bytes; }
 };
 
-static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t cols, bool light, int sms) {
+static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t cols, bool light, int sms, int choice) {
     OrthogonalLayout l = {};
     l.tall = rows >= cols;
     l.side = l.tall ? cols : rows;
@@ -295,9 +295,9 @@ static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t c
     l.s_pitch = padded(l.side);
     l.s_plane = l.side * l.s_pitch;
     l.parts = (int)(ceil_div(rows * cols, 4 * kThreads * 4) < 2 * sms ? ceil_div(rows * cols, 4 * kThreads * 4) : 2 * sms);
-    l.gram = plan_matmul(l.side, l.side, l.tall ? rows : cols, batch, light ? 1 : 2, true, sms);
-    l.square = plan_matmul(l.side, l.side, l.side, batch, 2, true, sms);
-    l.product = plan_matmul(rows, cols, l.side, batch, light ? 1 : 2, false, sms);
+    l.gram = plan_matmul(l.side, l.side, l.tall ? rows : cols, batch, light ? 1 : 2, true, sms, choice);
+    l.square = plan_matmul(l.side, l.side, l.side, batch, 2, true, sms, choice);
+    l.product = plan_matmul(rows, cols, l.side, batch, light ? 1 : 2, false, sms, choice);
     l.x_bytes = padded_bytes(batch * 2 * l.x_plane * 2);
     l.s_bytes = padded_bytes(batch * 2 * l.s_plane * 2);
     l.norm_bytes = padded_bytes(batch * l.parts * 8);
@@ -346,9 +346,9 @@ static float kept_smaller(double norm) {
 // of X in a product with a I + b S + c S^2 grows by a factor of a in every step along directions of small singular values, 4e-2 in the
 // end where X has few large ones; M alone is next to nothing along those.  All together 1.6e-3, half the products.
 static int orthogonalise(const Matrices &all, int64_t batch, int64_t rows, int64_t cols, int steps, const float *coefficients, double eps,
-                         const OrthogonalEpilogue &last, uint8_t *workspace, int sms, cudaStream_t st, const char *what) {
+                         const OrthogonalEpilogue &last, uint8_t *workspace, int sms, int choice, cudaStream_t st, const char *what) {
     const bool light = all.type == kBFloat16;
-    const OrthogonalLayout l = orthogonal_layout(batch, rows, cols, light, sms);
+    const OrthogonalLayout l = orthogonal_layout(batch, rows, cols, light, sms, choice);
     uint8_t *at = workspace;
     const auto take = [&](int64_t bytes) {
         uint8_t *p = at;
@@ -453,9 +453,10 @@ static double usable_eps(double eps) { return eps > 1e-60 ? eps : 1e-60; }
 static bool few_columns(int64_t cols) { return cols <= kGramColumns; }
 
 extern "C" DL_API int64_t dl_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int type) {
+    const int choice = matmul_choice(&type);
     if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
     if (few_columns(cols)) return gram_workspace_bytes(batch, batch * rows, current_sms());
-    return orthogonal_layout(batch, rows, cols, type == kBFloat16, current_sms()).total();
+    return orthogonal_layout(batch, rows, cols, type == kBFloat16, current_sms(), choice).total();
 }
 
 static int check_steps(int steps, const float *coefficients, double eps, const char *what) {
@@ -474,6 +475,7 @@ static int check_steps(int steps, const float *coefficients, double eps, const c
 extern "C" DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, int64_t rows, int64_t cols, int type, int steps,
                                        const float *coefficients, double eps, void *workspace, void *stream) {
     const char *what = "dl_orthogonalize";
+    const int choice = matmul_choice(&type);
     DL_REQUIRE(batch >= 0 && rows >= 0 && cols >= 0 && rows <= INT32_MAX / 2 && cols <= INT32_MAX / 2, DL_ERR_INVALID_ARG, "%s: bad size", what);
     DL_REQUIRE(batch <= 65535, DL_ERR_TOO_LARGE, "%s: more than 65535 matrices", what);
     DL_REQUIRE(type >= kFloat32 && type <= kFloat16, DL_ERR_INVALID_ARG, "%s: unknown type %d", what, type);
@@ -498,7 +500,7 @@ extern "C" DL_API int dl_orthogonalize(const void *g, void *out, int64_t batch, 
     OrthogonalEpilogue last = {};
     last.out = out;
     return orthogonalise(all, batch, rows, cols, steps, coefficients, usable_eps(eps), last, reinterpret_cast<uint8_t *>(workspace), current_sms(),
-                         as_stream(stream), what);
+                         choice, as_stream(stream), what);
 }
 
 // One step: the matrices of few columns together, then those of one shape after the other.
@@ -594,7 +596,7 @@ extern "C" DL_API int64_t dl_muon_workspace_bytes(const int64_t *table, int64_t 
             return DL_OK;
         },
         [&](Matrices &, int64_t batch, int64_t rows, int64_t cols) {
-            const int64_t bytes = orthogonal_layout(batch, rows, cols, false, sms).total();
+            const int64_t bytes = orthogonal_layout(batch, rows, cols, false, sms, 0).total();
             if (bytes > most) most = bytes;
             return DL_OK;
         });
@@ -643,6 +645,6 @@ extern "C" DL_API int dl_muon_step_f32(const int64_t *table, int64_t count, doub
             OrthogonalEpilogue last = {};
             last.decay = decay;
             last.rate = rate(rows, cols);
-            return orthogonalise(all, batch, rows, cols, steps, coefficients, usable_eps(eps), last, reinterpret_cast<uint8_t *>(workspace), sms, st, what);
+            return orthogonalise(all, batch, rows, cols, steps, coefficients, usable_eps(eps), last, reinterpret_cast<uint8_t *>(workspace), sms, 0, st, what);
         });
 }

@@ -52,6 +52,7 @@ def _forward(x, w, bias, residual, act, feature_major, want_slope):
         return y, slope, x, None, None
     x, pitch, x_feature = _layout(x)
     lib = N.lib()
+    kind |= lib.dl_matmul_choice()
     with N.on_device(x):
         px, pw = x.data_ptr(), w.data_ptr()
         sizes = (ctypes.c_int64 * 3)()
@@ -118,7 +119,8 @@ class DenseFunction(torch.autograd.Function):
                 if slope is not None and feature != ctx.feature_major and batch > 1 and outer > 1:
                     feature = ctx.feature_major
                     g = gy.t().contiguous().t() if feature else gy.contiguous()
-                lib, kind = N.lib(), TYPES[gy.dtype]
+                lib = N.lib()
+                kind = TYPES[gy.dtype] | lib.dl_matmul_choice()
                 with N.on_device(gy):
                     px, pw = x.data_ptr() if x is not None else ctx.x_ptr, w.data_ptr() if w is not None else ctx.w_ptr
                     work = _bytes(lib.dl_dense_backward_workspace_bytes(g.data_ptr(), feature, slope is not None, px, ctx.pitch, ctx.x_feature, pw,

@@ -1003,9 +1003,10 @@ def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
         return out
     batch = x.numel() // (rows * cols)
     lib = N.lib()
+    kind = _FLOAT_TYPES[x.dtype] | lib.dl_matmul_choice()
     with N.on_device(x):
-        work = torch.empty(lib.dl_orthogonalize_workspace_bytes(batch, rows, cols, _FLOAT_TYPES[x.dtype]), dtype=torch.uint8, device=x.device)
-        N.check(lib.dl_orthogonalize(x.data_ptr(), out.data_ptr(), batch, rows, cols, _FLOAT_TYPES[x.dtype], steps, table, eps, work.data_ptr(),
+        work = torch.empty(lib.dl_orthogonalize_workspace_bytes(batch, rows, cols, kind), dtype=torch.uint8, device=x.device)
+        N.check(lib.dl_orthogonalize(x.data_ptr(), out.data_ptr(), batch, rows, cols, kind, steps, table, eps, work.data_ptr(),
                                      N.stream_of(x)))
     return out
 

@@ -75,8 +75,8 @@ enum {
     DL_TUNE_FUSED_CLUSTER = 5,      /* dl_eval_groupbitsum: CTAs per class, 2, 4 or 8                            */
     DL_TUNE_FORWARD_KERNEL = 6,     /* dl_forward_f32: 1 = register kernel, 2 = staged (bulk-copy) kernel        */
     DL_TUNE_WALK_KERNEL = 7,        /* dl_backward_walk_f32: 1 = register kernel, 2 = staged kernel where it can  */
-    DL_TUNE_MATMUL_COLUMNS = 8,     /* matrix products: columns of a tile, 64, 128 or 256                          */
-    DL_TUNE_MATMUL_SPLITS = 9,      /* matrix products: pieces that the sum is cut into, as far as it goes       */
+    DL_TUNE_MATMUL_COLUMNS = 8,     /* dl_matmul_choice: columns of a tile, 64, 128 or 256                         */
+    DL_TUNE_MATMUL_SPLITS = 9,      /* dl_matmul_choice: pieces that the sum is cut into, as far as it goes      */
     DL_TUNE_COUNT = 10
 };
 DL_API int dl_set_tuning(int key, int value);
@@ -553,7 +553,8 @@ DL_API int dl_backward_w_announce_f32(const float *x, const int64_t *a, const in
  * Dense layers beside the logic layers, and the orthogonalised updates of their weights.  (The reference's own dense layers are
  * torch.nn.Linear and its activations, experiments/main_baseline.py; it has no kernels for them.)
  *
- * type: 0 fp32, 1 bf16, 2 fp16.  Sums are 32-bit.  fp32 operands are multiplied as three bf16 planes, all 24 bits; up to 32 samples as two
+ * type: 0 fp32, 1 bf16, 2 fp16, and what dl_matmul_choice returns, the same for a call and the question for its workspace.  Sums are 32-bit.
+ * fp32 operands are multiplied as three bf16 planes, all 24 bits; up to 32 samples as two
  * values of 11 bits, which leaves a product up to 2^-21 off, of either sign, and results no further off than sums of rounded 32-bit steps.
  * An infinite operand makes the results it enters infinite or undefined.
  *
@@ -572,6 +573,9 @@ DL_API int dl_backward_w_announce_f32(const float *x, const int64_t *a, const in
  * rows x cols values as they lie in memory, rows `pitch` apart (x_feature_major: rows are features), dl_dense_planes_bytes bytes.
  * ---------------------------------------------------------------------------------------- */
 enum { DL_ACT_NONE = 0, DL_ACT_RELU = 1, DL_ACT_SIGMOID = 2, DL_ACT_SILU = 3, DL_ACT_GELU = 4 };
+/* DL_TUNE_MATMUL_* as bits of a type, 0 where they are not set: asked for once for a call and its workspace, which then agree whoever sets the
+ * switches meanwhile. */
+DL_API int dl_matmul_choice(void);
 DL_API void dl_dense_forward_sizes(const void *x, int64_t x_pitch, int x_feature_major, const void *w, int64_t batch, int64_t inner,
                                    int64_t outer, int y_feature_major, int type, int64_t *sizes);
 DL_API int dl_dense_forward(const void *x, int64_t x_pitch, int x_feature_major, const void *w, const void *bias, const void *residual,
