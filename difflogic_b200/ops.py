@@ -953,7 +953,7 @@ def _largest_value(a, b, c, reach):
     return max(abs(s * (a + s * s * (b + s * s * c))) for s in candidates)
 
 
-@functools.lru_cache(maxsize=64)
+@functools.lru_cache(maxsize=64, typed=True)
 def _newton_schulz(coefficients, steps):
     """The coefficients of every step as the library takes them.  A singular value s becomes a s + b s^3 + c s^5; the iterates are kept
     as numbers of up to 16, so coefficients that let values from [0, 1] grow past 8 on the way are refused."""

@@ -59,3 +59,13 @@ def test_the_library_refuses_what_is_not_a_number():
         assert N.lib().dl_orthogonalize(None, None, 0, 4, 4, 0, 1, table, 1e-7, None, None) == N.DL_ERR_INVALID_ARG
         with pytest.raises(ValueError, match="near 1"):
             D.ops._newton_schulz(bad, 1)
+
+
+def test_what_was_refused_once_is_refused_after_a_call_that_equals_it():
+    """1, 1.0 and True are one key of a table that does not look at types."""
+    for steps in (1, 2):
+        table = D.ops._newton_schulz((1.5, -0.5, 0.0), steps)
+        assert D.ops._newton_schulz((1.5, -0.5, 0.0), steps) is table
+        for wrong in (float(steps), True) if steps == 1 else (float(steps),):
+            with pytest.raises(ValueError, match="whole number"):
+                D.ops._newton_schulz((1.5, -0.5, 0.0), wrong)
