@@ -8,6 +8,6 @@ from .difflogic import LogicLayer, GroupSum
 from .packbitstensor import PackBitsTensor
 from .compiled_model import CompiledLogicNet
 from .denselayer import DenseLayer, dense
-from . import functional, ops
+from . import functional, ops, optim, training
 
-__all__ = ["LogicLayer", "GroupSum", "PackBitsTensor", "CompiledLogicNet", "DenseLayer", "dense", "functional", "ops"]
+__all__ = ["LogicLayer", "GroupSum", "PackBitsTensor", "CompiledLogicNet", "DenseLayer", "dense", "functional", "ops", "optim", "training"]
