@@ -242,7 +242,8 @@ static void launch_outputs(const RowsJob &j, const DenseOutput &e, int sms, cuda
 
 template <int NT>
 static void launch_samples(const RowsJob &j, const DenseOutput &e, bool whole, int sms, cudaStream_t st) {
-    if (j.type == kFloat32) whole ? launch_outputs<NT, true, true>(j, e, sms, st) : launch_outputs<NT, true, false>(j, e, sms, st);
+    if constexpr (NT == 4) whole ? launch_outputs<NT, true, true>(j, e, sms, st) : launch_outputs<NT, true, false>(j, e, sms, st);   // fp32 alone
+    else if (j.type == kFloat32) whole ? launch_outputs<NT, true, true>(j, e, sms, st) : launch_outputs<NT, true, false>(j, e, sms, st);
     else whole ? launch_outputs<NT, false, true>(j, e, sms, st) : launch_outputs<NT, false, false>(j, e, sms, st);
 }
 
