@@ -149,7 +149,7 @@ def _check(x, weight, bias, residual, activation):
 
 
 def dense(x, weight, bias=None, residual=None, activation=None, feature_major=False):
-    """act(x weight^T + bias) + residual, differentiable once.
+    """act(x weight^T + bias) + residual, differentiable once and not in forward mode.
 
     x `[..., in]`, weight `[out, in]`, bias `[out]`, residual `[..., out]`, all of one type (float32, bfloat16 or float16) on one CUDA
     device; activation: None, 'relu', 'sigmoid', 'silu' or 'gelu' (the exact one).  x may be a transposed view, as logic layers return
@@ -178,7 +178,8 @@ def dense(x, weight, bias=None, residual=None, activation=None, feature_major=Fa
         residual = None if residual is None else residual.reshape(-1, outer)
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    if graph:
+    # apply() refuses forward mode, which there is no derivative for
+    if graph or any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in (x, weight, bias, residual)):
         y = DenseFunction.apply(x, weight, bias, residual, act, bool(feature_major))
     else:
         y = _forward(x, weight, bias, residual, act, bool(feature_major), False)[0]

@@ -979,11 +979,13 @@ def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     """The nearest matrix to x with singular values near 1, by Newton-Schulz steps (the update of the Muon optimizer): X = x / max(|x|, eps)
     in the Frobenius norm, then `steps` times X <- a X + b (X X^T) X + c (X X^T)^2 X.
 
-    x: `[..., rows, cols]` float32, bfloat16 or float16 on a CUDA device, every matrix on its own; the result has x's type.
+    x: `[..., rows, cols]` float32, bfloat16 or float16 on a CUDA device, every matrix on its own; the result has x's type and, as all of
+    this module's, no part in x's graph: no gradient goes through it.  Entries that X would have below 2^-36, of matrices far smaller than
+    eps, count as zero where there are more than 16 columns.
     coefficients: (a, b, c), or one such triple for each step, with which singular values from [0, 1] stay at 8 or below (errors grow by
-    the slopes of a s + b s^3 + c s^5 from step to step).  The products run on the tensor cores with operands of 22 bits
-    (bfloat16: 11, which leaves the result less far off than its own rounding does).  An entry
-    that is infinite or undefined makes its whole matrix undefined."""
+    the slopes of a s + b s^3 + c s^5 from step to step).  The products run on the tensor cores with operands of 22 bits (bfloat16: 11,
+    which leaves the result less far off than its own rounding does), those of up to 16 columns in 64 bits.  An entry that is infinite or
+    undefined makes its whole matrix undefined."""
     N.require_cuda(x)
     if x.dtype not in _FLOAT_TYPES:
         raise ValueError("orthogonalize: float32, bfloat16 or float16, got %s" % x.dtype)
