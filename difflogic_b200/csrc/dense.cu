@@ -1,7 +1,7 @@
 // Dense layers: y = act(x w^T + bias) + residual and its gradients, by the matrix products of matmul.cuh; what lays out their operands,
 // and the entry points.
 //
-// Forward and backward pass of 8192 samples, 4096 -> 4096, bf16, SiLU and residual: 816 us = 1010 TFLOP/s, of which the forward product
+// Forward and backward pass of 8192 samples, 4096 -> 4096, bf16, SiLU and residual: 804 us = 1026 TFLOP/s, of which the forward product
 // 244 us (its epilogue reads the residual and writes y and the derivative, which the next tile's products do not all hide), the
 // pre-activation's gradient 34 (memory), the input's 198 and the weight's 220.  Small layers are bound by their chain of eight kernels of
 // 5 to 20 us, and by the host: 1001 samples, 783 -> 2001, fp16, 90 us from Python and 68 in a captured graph; 128 samples, 784 -> 8000,

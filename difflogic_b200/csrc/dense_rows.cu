@@ -4,7 +4,7 @@
 // memory.  The products go to the warp-wide matrix instructions (16 outputs x 8 samples), which take their operands from registers, so
 // that w goes from memory straight into them: fp32 values are split there, where the tensor cores' tiles would have them laid out in three planes
 // in memory first, four times the bytes of w; and no tile of 64 columns waits for samples that are not there.
-// 4096 -> 16000, 8 samples, fp32: 54 us, 4.8 TB/s; 784 -> 16000: 15 us, 3.4 TB/s, bound by the latency of reads of which a block has 4
+// 4096 -> 16000, 8 samples, fp32: 51 us, 5.2 TB/s; 784 -> 16000: 15 us, 3.4 TB/s, bound by the latency of reads of which a block has 4
 // a thread under way; 2048 -> 2048, one sample, bf16: 5 us, a launch and two waits for memory.
 // The order in which k is summed is free: a lane reads 16 neighbouring bytes of its rows of w and of x, and what the instruction calls
 // columns t and t + 4 (fp32) are neighbours in memory.
@@ -225,8 +225,10 @@ dense_rows_kernel(const __grid_constant__ RowsJob j, const DenseOutput output) {
     }
 }
 
-// This way / the tensor cores' way, us: fp32 784 -> 16000, 16 samples: 18 / 54, 32: 37 / 54; 2048 -> 2048: 12 / 26, 15 / 26; bf16 784 -> 16000,
-// 8: 9.6 / 11.2, 16: 12.7 / 11.2, 32: 29 / 12.4; 2048 -> 2048, 16: 7.0 / 9.0; rows off the 16-byte units, 783 -> 2001, 16: 7.0 / 13.3.
+// This way / the tensor cores' way (one sample more), us: fp32 784 -> 16000, 16 samples: 18 / 51, 32: 32 / 51; 2048 -> 2048: 12 / 25, 15 / 25;
+// 784 -> 256, 32: 6.5 / 14; bf16 784 -> 16000, 8: 9.0 / 11, 16: 12.3 / 10.5; 2048 -> 2048, 16: 7.0 / 9.6; rows off the 16-byte units, 783 -> 2001,
+// 16: 8.2 / 14.  Not so where few outputs and a long sum leave most SMs without a block, which the rule does not look at: fp32 16000 -> 10,
+// 8: 30 / 23, 32: 80 / 23; 4096 -> 100, 8: 12 / 17, 32: 26 / 17.
 bool dense_rows_applicable(int64_t batch, int type) { return batch <= (type == kFloat32 ? 32 : 16); }
 
 template <int NT, bool FULL, bool WHOLE>

@@ -1,4 +1,4 @@
-// The 5th-generation tensor cores (tcgen05) and tiled asynchronous copies, as the matrix products in matmul.cu use them.
+// The 5th-generation tensor cores (tcgen05) and tiled asynchronous copies, as the matrix products in matmul.cuh use them.
 //
 // One thread issues the products: both operands lie in shared memory as tiles of 64 values x 64 rows (8 KB) in the 128-byte swizzle that
 // the tiled copy writes, the 32-bit accumulator of 128 rows lies in tensor memory, one lane per row and one column per value.  A tile's
