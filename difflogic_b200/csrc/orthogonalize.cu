@@ -312,11 +312,11 @@ static OrthogonalLayout orthogonal_layout(int64_t batch, int64_t rows, int64_t c
 static double largest_value(double a, double b, double c, double reach) {
     double most = fabs(reach * (a + reach * reach * (b + reach * reach * c)));
     const double root = 9 * b * b - 20 * a * c;
-    if (root >= 0)   // of a + 3 b u + 5 c u^2, u = s^2
-        for (const double down : {-3 * b + sqrt(root), -3 * b - sqrt(root)}) {
-            const double u = c != 0 ? down / (10 * c) : b != 0 ? -a / (3 * b) : 0;
+    if (root >= 0) {   // the roots of a + 3 b u + 5 c u^2, u = s^2, without a difference of near equals where c is small
+        const double q = -(3 * b + copysign(sqrt(root), b)) / 2;
+        for (const double u : {q / (5 * c), a / q})
             if (u > 0 && u < reach * reach) most = std::max(most, fabs(sqrt(u) * (a + u * (b + u * c))));
-        }
+    }
     return most;
 }
 // The largest of |a + b u + c u^2| over the same values, u = s^2: the norm of M.

@@ -944,11 +944,10 @@ NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)   # makes every singular value about 1
 
 def _largest_value(a, b, c, reach):
     """The largest of |a s + b s^3 + c s^5| for s in [0, reach]: at the end, or where the derivative is zero."""
-    candidates, root = [reach], 9 * b * b - 20 * a * c
-    if c == 0:
-        roots = [-a / (3 * b)] if b != 0 else []
-    else:
-        roots = [(-3 * b + sign * math.sqrt(root)) / (10 * c) for sign in (1, -1)] if root >= 0 else []
+    candidates, root, roots = [reach], 9 * b * b - 20 * a * c, []
+    if root >= 0:   # of a + 3 b u + 5 c u^2, u = s^2, without a difference of near equals where c is small
+        q = -(3 * b + math.copysign(math.sqrt(root), b)) / 2
+        roots = ([q / (5 * c)] if c != 0 else []) + ([a / q] if q != 0 else [])
     candidates += [math.sqrt(u) for u in roots if 0 < u < reach * reach]
     return max(abs(s * (a + s * s * (b + s * s * c))) for s in candidates)
 
@@ -962,6 +961,7 @@ def _newton_schulz(coefficients, steps):
     sets = coefficients if isinstance(coefficients[0], tuple) else (coefficients,) * steps
     if len(sets) != steps or any(len(s) != 3 for s in sets):
         raise ValueError("orthogonalize: three coefficients, or three for each of the %d steps" % steps)
+    sets = [tuple(ctypes.c_float(v).value for v in s) for s in sets]    # as the library has them, which looks at them once more
     reach = 1.0     # what [0, 1] has become is [0, reach]
     for a, b, c in sets:
         fits = max(abs(a), abs(b), abs(c)) <= 64.0 and not any(map(math.isnan, (a, b, c)))

@@ -69,3 +69,17 @@ def test_what_was_refused_once_is_refused_after_a_call_that_equals_it():
         for wrong in (float(steps), True) if steps == 1 else (float(steps),):
             with pytest.raises(ValueError, match="whole number"):
                 D.ops._newton_schulz((1.5, -0.5, 0.0), wrong)
+
+
+@pytest.mark.parametrize("c", [0.0, 1e-8, -1e-8, 1e-15, -1e-15, 1e-20, -1e-20, 1e-36, 1e-45])
+@pytest.mark.parametrize("b", [-60.0, -20.0])
+def test_small_coefficients_hide_no_peak(b, c):
+    """The peak of a s + b s^3 beside a last coefficient that is next to nothing."""
+    a = -b
+    peak = a * 2 / 3 / 3 ** 0.5
+    assert D.ops._largest_value(a, b, c, 1.0) == pytest.approx(peak, rel=1e-6)
+    table = (ctypes.c_float * 3)(a, b, c)
+    status = N.lib().dl_orthogonalize(None, None, 0, 4, 4, 0, 1, table, 1e-7, None, None)
+    assert (status == N.DL_OK) == (peak <= 8)
+    assert D.ops._largest_value(0.0, 0.0, c, 1.0) == abs(c) and D.ops._largest_value(a, 0.0, 0.0, 1.0) == a
+    assert D.ops._largest_value(0.0, b, 0.0, 1.0) == -b and D.ops._largest_value(0.0, b, c, 1.0) == pytest.approx(-b, rel=1e-6)
