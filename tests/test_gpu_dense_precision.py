@@ -128,3 +128,23 @@ def test_inputs_that_are_not_finite(rows):
         y = D.dense(x, bad)
         keep = [j for j in range(24) if j != i]
         assert not torch.isfinite(y[:, i]).any() and torch.equal(y[:, keep], clean[:, keep])
+
+
+@pytest.mark.parametrize("act", [None, "relu", "sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("rows", [10, 40])
+def test_activations_far_out_of_planes(act, rows):
+    """Pre-activations where exponentials overflow and planes are cut off, one input and a weight of 1: limits, not undefined values.  An
+    activation and its derivative cost a few roundings in 32 bits, relative to values of at most 1.13 |z|; sigmoids' derivatives s (1 - s) lose
+    what 1 - s rounds away, 2^-24."""
+    z = torch.tensor([torch.finfo(torch.float32).max, torch.finfo(torch.float32).min, 3e38, -3e38, -1e4, -100.0, -20.0, -0.0, 20.0, 1e4])
+    x, w = z.repeat(rows // 10).cuda().view(-1, 1).requires_grad_(), torch.ones(1, 1, device="cuda")
+    y = D.dense(x, w, activation=act)
+    g, = torch.autograd.grad(y, x, torch.ones_like(y))
+    v = x.detach().double()
+    s, phi = torch.sigmoid(v), torch.special.ndtr(v)
+    density = torch.exp(-v * v / 2) / math.sqrt(2 * math.pi)
+    far = v.abs() > 1e3                       # infinity times zero
+    want, slope = {None: (v, torch.ones_like(v)), "relu": (v.clamp(min=0), (v > 0).double()), "sigmoid": (s, s * (1 - s)),
+                   "silu": (v * s, s + torch.where(far, 0, v * s * (1 - s))), "gelu": (v * phi, phi + torch.where(far, 0, v * density))}[act]
+    assert bool(torch.isfinite(y).all() & torch.isfinite(g).all())
+    assert bool(((y.double() - want).abs() <= 2.0 ** -19 * want.abs() + 1e-6).all()) and bool(((g.double() - slope).abs() <= 2.0 ** -19 * slope + 2e-6).all())

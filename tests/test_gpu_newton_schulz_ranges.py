@@ -102,3 +102,19 @@ def test_the_smallest_and_the_largest_matrices(rows, cols, size):
     got = D.ops.orthogonalize(g, eps=1e-60)
     want, off = steps_and_bound(g, [D.ops.NEWTON_SCHULZ] * 5, 2.0 ** -22, eps=1e-60)
     assert (got.double() - want).norm().item() <= off + 2.0 ** -23 * want.norm().item()
+
+
+def test_an_optimizer_of_steep_steps():
+    """One list of coefficients for gate weights and dense weights: the products of both stay finite, and their sizes are those of the steps."""
+    torch.manual_seed(0)
+    model = torch.nn.Sequential(D.DenseLayer(30, 50), D.LogicLayer(50, 80), D.GroupSum(4))
+    opt = D.optim.FlatMuon(model.parameters(), lr=0.01, weight_decay=0.0, ns_coefficients=(20.0, -60.0, 48.0), ns_steps=1)
+    before = [p.detach().clone() for p in model.parameters() if p.dim() == 2]
+    model(torch.rand(64, 30, device="cuda")).square().mean().backward()
+    grads = [p.grad.clone() for p in model.parameters() if p.dim() == 2]
+    opt.step()
+    for p, old, g in zip((p for p in model.parameters() if p.dim() == 2), before, grads):
+        want, off = steps_and_bound(g * 0.0975, ((20.0, -60.0, 48.0),), 2.0 ** -22)     # (1 - mu) g and nesterov: a multiple of g
+        rate = 0.01 * math.sqrt(max(1.0, p.shape[0] / p.shape[1]))
+        moved = (old.double() - p.detach().double()) / rate
+        assert (moved - want).norm().item() <= 2 * off + 2.0 ** -22 * want.norm().item() + 2 * 2.0 ** -24 * (old.norm() + p.norm()).item() / rate

@@ -68,3 +68,32 @@ def test_an_optimizers_step_leaves_version_counters_alone():
     opt.step()
     assert versions == [p._version for p in model.parameters()]
     loss.backward()
+
+
+@pytest.mark.parametrize("rows", [1, 8, 32, 33])
+def test_captured_steps_read_the_weights_of_their_replay(rows):
+    """What a backward pass reads is laid out anew in every replay."""
+    torch.manual_seed(rows)
+    x, w, b = (torch.randn(*s, device="cuda", requires_grad=True) for s in ((rows, 24), (40, 24), (40,)))
+    gy = torch.randn(rows, 40, device="cuda")
+    run = lambda: torch.autograd.grad(D.dense(x, w, b, activation="gelu"), (x, w, b), gy)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, results = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results.append(run())
+        graphs.append(graph)
+    momenta = [torch.zeros_like(x), torch.zeros_like(w)]
+    for _ in range(3):
+        D.ops.muon_step([x, w], [torch.randn_like(x), torch.randn_like(w)], momenta, lr=0.1)
+        want = run()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for got in results:
+            assert all(torch.equal(p, q) for p, q in zip(want, got))
