@@ -553,10 +553,10 @@ DL_API int dl_backward_w_announce_f32(const float *x, const int64_t *a, const in
  * Dense layers beside the logic layers, and the orthogonalised updates of their weights.  (The reference's own dense layers are
  * torch.nn.Linear and its activations, experiments/main_baseline.py; it has no kernels for them.)
  *
- * type: 0 fp32, 1 bf16, 2 fp16, and what dl_matmul_choice returns, the same for a call and the question for its workspace.  Sums are 32-bit.
- * fp32 operands are multiplied as three bf16 planes, all 24 bits; up to 32 samples as two
- * values of 11 bits, which leaves a product up to 2^-21 off, of either sign, and results no further off than sums of rounded 32-bit steps.
- * An infinite operand makes the results it enters infinite or undefined.
+ * type: 0 fp32, 1 bf16, 2 fp16, and what dl_matmul_choice returns, the same for a call and the question for its workspace.  Sums are
+ * 32-bit.  fp32 operands are multiplied as three bf16 planes, all 24 bits; in the forward pass of up to 32 samples as two values of 11 bits,
+ * which leaves a product up to 2^-21 off, of either sign, and results no further off than sums of rounded 32-bit steps.  An infinite
+ * operand makes the results it enters infinite or undefined.
  *
  *   y = act(x w^T + bias) + residual
  *
